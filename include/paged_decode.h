@@ -44,6 +44,8 @@ extern "C" {
 /* Device error word bits (pd_device_error). */
 #define PD_DEVERR_WAIT_TIMEOUT 1u  /* an mbarrier wait exceeded its time limit          */
 #define PD_DEVERR_APPEND_RANGE 2u  /* append skipped a slot / block id outside the pool  */
+#define PD_DEVERR_ROPE_RANGE 4u    /* a position outside the cos/sin tables              */
+#define PD_DEVERR_COPY_RANGE 8u    /* a page copy skipped a block id outside the pool    */
 
 /* Human-readable name of a status code (static storage). */
 const char* pd_status_string(int status);
@@ -309,6 +311,88 @@ int pd_kv_append_table_rope(void* k_pool, void* v_pool, int64_t n_blocks, int32_
                             int32_t src_dtype, int32_t batch, int32_t n_kv_head, int32_t head_dim,
                             const void* rope_cos, const void* rope_sin, int64_t rope_stride,
                             int32_t rotary_dim, void* stream);
+
+/* ---------------------------------------------------------------- head norms with rotation
+ *
+ * pd_qk_norm_rope -- the model's q_norm / k_norm (RMS norm of each head row) and
+ * apply_rotary_emb_partial (model/layers.py:59-117, 200-211) in one launch: for a head row x with
+ * weight w, y = x / sqrt(mean(x^2) + eps) * w, then the GPT-NeoX rotation of y's first rotary_dim
+ * elements by row positions[t] of the cos / sin tables (rotary_dim / 2 entries each), all in fp32
+ * with one rounding at the end. q (n_tokens, n_head, D) and k (n_tokens, n_kv_head, D) may be
+ * views of one fused projection (token and head strides, unit last stride) and may be normalised
+ * in place (q_out = q). positions: int32 or int64 (PD_SLOT_I32 / PD_SLOT_I64), or NULL for 0, 1,
+ * 2, ... A position outside [0, n_pos) gives a row of zeros and PD_DEVERR_ROPE_RANGE. q, k,
+ * weights, tables and outputs share one dtype. head_dim 2..256, rotary_dim even, 0..head_dim. */
+int pd_qk_norm_rope(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, void* q_out,
+                    int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh, const void* q_weight,
+                    const void* k_weight, const void* rope_cos, const void* rope_sin, int64_t cos_stride,
+                    int64_t sin_stride, int64_t n_pos, const void* positions, int32_t pos_dtype, int64_t n_tokens,
+                    int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t rotary_dim, float eps, int32_t dtype,
+                    void* stream);
+
+/* ---------------------------------------------------------------- 4-bit pages
+ *
+ * A pool of 4-bit pages is bytes (n_blocks, n_kv_head, block_size / 16, 18 * head_dim), contiguous
+ * and 16-byte aligned. The last dimension is one kv head's record of 16 tokens, W = min(D, 128):
+ *   K codes   8 D bytes  [D / W][16 tokens][W / 2]      a byte: element 2 j low, 2 j + 1 high
+ *   K scales    D bytes  [D / W][16 tokens][W / 16]     e4m3, one for 16 neighbouring elements
+ *   V codes   8 D bytes  [2][D / 16 groups][8 tokens][8]
+ *   V scales    D bytes  [2][D / 16 groups][8 tokens]
+ * A code is e2m1 (0 .5 1 1.5 2 3 4 6 and a sign bit); an element stands for code * scale *
+ * units[kv][head], units (2, n_kv_head) fp32 powers of two on the device (NULL: all 1). 4.5 bits
+ * an element. head_dim 64, 128 or 256, block_size a power of two >= 16 (PD_ERR_UNSUPPORTED
+ * otherwise). The reference has no quantised cache.
+ *
+ * pd_fp4_write_slots quantises token i of k / v (n_tokens, n_kv_head, D; strides of token and
+ * head, unit last) into flat slot slot_ids[i] (pd_kv_append_slots' slots): scale = e4m3(max |x /
+ * unit| / 6), code = e2m1(x / unit / scale), both to nearest with ties to even, saturating; NaN
+ * counts as zero. pd_fp4_write_table takes row b's slot from its block table and position, as
+ * pd_kv_append_table does. pd_fp4_read_slots writes the values back as dst_dtype (exact for units
+ * of 1 in 16 bits; rounded to nearest where the type's range ends). Slots outside the pool are
+ * skipped (read: zeros) and flagged with PD_DEVERR_APPEND_RANGE. */
+int pd_fp4_write_slots(void* pages, int64_t n_blocks, int32_t block_size, const void* slot_ids, int32_t slot_dtype,
+                       const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                       const float* units, int32_t src_dtype, int64_t n_tokens, int32_t n_kv_head, int32_t head_dim,
+                       void* stream);
+int pd_fp4_write_table(void* pages, int64_t n_blocks, int32_t block_size, const int32_t* block_table,
+                       int64_t bt_stride, int32_t max_blocks, const int64_t* pos, const void* k,
+                       const int64_t* k_strides, const void* v, const int64_t* v_strides, const float* units,
+                       int32_t src_dtype, int32_t batch, int32_t n_kv_head, int32_t head_dim, void* stream);
+int pd_fp4_read_slots(const void* pages, int64_t n_blocks, int32_t block_size, const void* slot_ids,
+                      int32_t slot_dtype, void* k, const int64_t* k_strides, void* v, const int64_t* v_strides,
+                      const float* units, int32_t dst_dtype, int64_t n_tokens, int32_t n_kv_head, int32_t head_dim,
+                      void* stream);
+
+/* pd_fp4_decode is pd_decode over 4-bit pages, pd_fp4_prefill is pd_prefill over them (same
+ * arguments, masks and conventions): q and out fp16 or bf16, any number of q heads per kv head;
+ * total_q is the packed tensors' token count, which offsets in cu_seqlens_q never pass.
+ * A block id outside the pool reads zeros. workspace: pd_fp4_workspace_bytes(head_dim) bytes of
+ * device memory, 256-byte aligned, ZERO-FILLED before its first launch (every launch leaves its
+ * counters at zero again); two launches that may run concurrently must not share one. */
+size_t pd_fp4_workspace_bytes(int32_t head_dim);
+int pd_fp4_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* pages, int64_t n_blocks, int32_t block_size,
+                  const float* units, const int32_t* block_table, int64_t bt_stride, int32_t max_blocks,
+                  const int32_t* seqlen, void* out, int64_t o_sb, int64_t o_sh, int32_t batch, int32_t n_head,
+                  int32_t n_kv_head, int32_t head_dim, int32_t dtype, float scale_log2, void* workspace,
+                  size_t workspace_bytes, void* stream);
+int pd_fp4_prefill(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, const void* pages, int64_t n_blocks, int32_t block_size,
+                   const float* units, const int32_t* block_table, int64_t bt_stride, int32_t max_blocks,
+                   const int32_t* cu_seqlens_q, const int32_t* seqlen_k, void* out, int64_t o_st, int64_t o_sh,
+                   int32_t batch, int32_t max_seqlen_q, int32_t n_head, int32_t n_kv_head, int32_t head_dim,
+                   int32_t dtype, float scale_log2, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- page copies
+ *
+ * pd_block_copy -- block dst[i] takes the bytes of block src[i] in each of n_pools pools
+ * (n_blocks blocks of block_bytes contiguous bytes each; pools is a host array), and, with a
+ * block_table (table_rows, table_cols) of row stride bt_stride, every entry e in [0, n_blocks)
+ * becomes remap[e]. One launch for up to 128 pools. Destinations are distinct and none is also a
+ * source. Pairs with an id outside the pool are skipped and flagged with PD_DEVERR_COPY_RANGE.
+ * src and dst are device vectors, int32 or int64 (id_dtype). No reference counterpart (its block
+ * manager neither shares nor moves blocks). */
+int pd_block_copy(void* const* pools, int32_t n_pools, int64_t n_blocks, int64_t block_bytes, const void* src,
+                  const void* dst, int32_t id_dtype, int64_t n_pairs, int32_t* block_table, int64_t table_rows,
+                  int64_t table_cols, int64_t bt_stride, const int32_t* remap, void* stream);
 
 /* ---------------------------------------------------------------- tuning / introspection
  * Launch shape of the decode kernel: warps per CTA, pipeline stages per warp, CTAs per SM

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import argparse
 import os
+import re
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -36,6 +37,11 @@ SOURCES = [
     "pd_decode_mma_f16.cu",
     "pd_prefill.cu",
     "pd_prefill_tc.cu",
+    "pd_ops_api.cu",
+    "pd_norm_rope.cu",
+    "pd_fp4_rows.cu",
+    "pd_fp4_attend.cu",
+    "pd_block_copy.cu",
 ]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -57,6 +63,18 @@ def _nvcc() -> str:
     return str(path) if path.exists() else "nvcc"
 
 
+def _headers(src: Path, seen: set[Path] | None = None) -> set[Path]:
+    """The repository's headers that ``src`` includes, directly or through another."""
+    seen = set() if seen is None else seen
+    for name in re.findall(r'^#include "([^"]+)"', src.read_text(), flags=re.M):
+        for folder in (CSRC, INCLUDE):
+            header = folder / name
+            if header.exists() and header not in seen:
+                seen.add(header)
+                _headers(header, seen)
+    return seen
+
+
 def _stale(target: Path, deps: list[Path]) -> bool:
     if not target.exists():
         return True
@@ -67,7 +85,6 @@ def _stale(target: Path, deps: list[Path]) -> bool:
 def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False) -> Path:
     """Compile and link the library; returns its path. Raises on a compiler error."""
     BUILD.mkdir(exist_ok=True)
-    headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [INCLUDE / "paged_decode.h"]
     nvcc = _nvcc()
     objects = []
     jobs = []
@@ -75,7 +92,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
         src = CSRC / name
         obj = BUILD / (Path(name).stem + ".o")
         objects.append(obj)
-        if force or _stale(obj, [src, *headers]):
+        if force or _stale(obj, [src, *_headers(src)]):
             cmd = [nvcc, *ARCH, *NVCC_FLAGS, "-c", str(src), "-o", str(obj)]
             if ptxas_verbose:
                 cmd[1:1] = ["-Xptxas", "-v"]

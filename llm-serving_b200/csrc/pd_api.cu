@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "paged_decode.h"
+#include "pd_api_internal.h"
 #include "pd_internal.h"
 
 namespace pd {
@@ -571,6 +572,27 @@ int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache
 }
 
 }  // namespace
+
+// What the other entry-point files share with this one (pd_internal.h).
+int api_cuda_fail(cudaError_t e, const char* where) { return cuda_fail(e, where); }
+
+int api_message(int status, const char* text) {
+  snprintf(g_last_error, sizeof(g_last_error), "%s", text);
+  return status;
+}
+
+void api_count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+
+unsigned long long api_wait_limit_ns() { return g_wait_limit_ns.load(std::memory_order_relaxed); }
+
+int api_device(int* sms, unsigned** err) {
+  int dev = 0;
+  if (current_device(&dev) != PD_OK) return PD_ERR_CUDA;
+  *sms = sm_count(dev);
+  *err = error_word(dev);
+  return *sms > 0 && *err != nullptr ? PD_OK : PD_ERR_CUDA;
+}
+
 }  // namespace pd
 
 using namespace pd;

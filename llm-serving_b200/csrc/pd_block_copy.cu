@@ -1,0 +1,82 @@
+// pd_block_copy.cu -- pages copied from block to block in every layer's pools, with the block
+// tables renumbered in the same launch (sm_100a).
+//
+// For each pool tensor and each pair i, block dst[i] takes the bytes of block src[i]; then every
+// table entry e in [0, n_blocks) becomes remap[e]. What a fork (its last, partly filled page), a
+// copy on write and a compaction need. No destination is also a source and destinations are
+// distinct (the block manager's plans guarantee both), so the copies are independent and one
+// launch does them all.
+//
+// Bound by memory: every byte is read and written once. A block is cut into 8 KB pieces, one CTA
+// of 256 threads with two 16-byte loads in flight per thread for each; the pieces of all pairs and
+// all pools form one grid.
+#include "pd_block_copy.cuh"
+#include "pd_internal.h"
+
+namespace pd {
+
+namespace {
+
+__device__ __forceinline__ int64_t block_id(const BlockCopyParams& p, const void* ids, int64_t i) {
+  return p.ids_i64 ? reinterpret_cast<const int64_t*>(ids)[i] : int64_t(reinterpret_cast<const int32_t*>(ids)[i]);
+}
+
+__global__ void __launch_bounds__(256) pd_block_copy_kernel(const __grid_constant__ BlockCopyParams p) {
+  const int64_t pieces = (p.block_bytes + COPY_PIECE - 1) / COPY_PIECE;
+  const int64_t per_pool = p.n_pairs * pieces;
+  const int64_t total = per_pool * p.n_pools;
+  for (int64_t it = blockIdx.x; it < total; it += gridDim.x) {
+    const int pool = int(it / per_pool);
+    const int64_t rem = it - pool * per_pool;
+    const int64_t pair = rem / pieces;
+    const int64_t from = block_id(p, p.src, pair), to = block_id(p, p.dst, pair);
+    if (from < 0 || from >= p.n_blocks || to < 0 || to >= p.n_blocks) {
+      if (threadIdx.x == 0) atomicOr(p.err, DEVERR_COPY_RANGE);
+      continue;
+    }
+    const int64_t begin = (rem - pair * pieces) * COPY_PIECE;
+    const int64_t end = begin + COPY_PIECE < p.block_bytes ? begin + COPY_PIECE : p.block_bytes;
+    const unsigned char* s = p.pools[pool] + from * p.block_bytes;
+    unsigned char* d = p.pools[pool] + to * p.block_bytes;
+    if (p.vec16) {
+      uint4 r[COPY_PIECE / 4096];
+#pragma unroll
+      for (int j = 0; j < COPY_PIECE / 4096; ++j) {
+        const int64_t o = begin + (j * 256 + threadIdx.x) * 16;
+        if (o < end) r[j] = __ldcs(reinterpret_cast<const uint4*>(s + o));
+      }
+#pragma unroll
+      for (int j = 0; j < COPY_PIECE / 4096; ++j) {
+        const int64_t o = begin + (j * 256 + threadIdx.x) * 16;
+        if (o < end) __stcs(reinterpret_cast<uint4*>(d + o), r[j]);
+      }
+    } else {
+      for (int64_t o = begin + threadIdx.x; o < end; o += 256) d[o] = s[o];
+    }
+  }
+  if (p.table != nullptr) {
+    const int64_t entries = p.table_rows * p.table_cols;
+    for (int64_t i = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; i < entries;
+         i += int64_t(gridDim.x) * blockDim.x) {
+      const int64_t row = i / p.table_cols;
+      int32_t* e = p.table + row * p.table_st + (i - row * p.table_cols);
+      const int32_t b = *e;
+      if (b >= 0 && b < p.n_blocks) *e = p.remap[b];
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_block_copy(const BlockCopyParams& p, int sms, cudaStream_t stream) {
+  const int64_t pieces = (p.block_bytes + COPY_PIECE - 1) / COPY_PIECE;
+  const int64_t entries = p.table != nullptr ? p.table_rows * p.table_cols : 0;
+  int64_t blocks = p.n_pairs * pieces * p.n_pools;
+  if (blocks < (entries + 255) / 256) blocks = (entries + 255) / 256;
+  if (blocks == 0) return cudaSuccess;
+  if (blocks > int64_t(sms) * 64) blocks = int64_t(sms) * 64;
+  pd_block_copy_kernel<<<unsigned(blocks), 256, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace pd

@@ -99,6 +99,12 @@ class PagedPool:
         self.flush()
         return self._values
 
+    def block_tensors(self) -> list[torch.Tensor]:
+        """Every tensor that holds blocks of the pool (K and V of every layer), after
+        :meth:`flush`: what ``serve.block_copy.copy_blocks`` moves pages in."""
+        self.flush()
+        return [*self._keys, *self._values]
+
     def flush(self) -> None:
         """Launch the decode-step append that ``PagedKV.write`` recorded, if any, on the
         stream it was recorded on. Afterwards the pools hold every written token."""
