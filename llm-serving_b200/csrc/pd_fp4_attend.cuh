@@ -25,17 +25,22 @@
 //  * tokens past the row are masked to P = 0 and their V scales to 0, so whatever bytes a page
 //    holds there (a NaN scale included) never reaches the sums.
 //
-// Work split: the (row, kv head, column block, record) sequence is cut into equal runs, one per
-// warp, so every SM streams the same number of bytes whatever the lengths. Each warp prefetches
-// its run through a ring of records in shared memory (cp.async, no barrier shared with other
-// warps). A unit (row, kv head, column block) cut between warps leaves partial (m, l, acc) pieces:
-// the CTA joins its own in shared memory; a unit cut between CTAs goes through the workspace and
-// the last CTA to arrive joins it, in piece order whoever arrives last, so results do not depend
-// on timing. Nothing waits: a CTA that is not last leaves.
+// Work split: the (row, kv head, column block, tile) sequence is cut into equal runs, one per
+// CTA and in it one per warp, so every SM streams the same number of bytes whatever the lengths.
+// Each warp prefetches its run through its own ring of tiles (two records, 32 keys) in shared
+// memory by bulk copies of 18 D bytes per record, or of both where they share a page: no lane
+// but one spends instructions on it, and no warp waits for another's data. A unit (row, kv head, column block) cut between warps leaves partial (m, l,
+// acc) pieces that the CTA joins in shared memory; a unit cut between CTAs goes through the
+// workspace and the last CTA to arrive joins it, in piece order whoever arrives last, so results
+// do not depend on timing, and a CTA that is not last leaves. Where there are no more units than
+// CTAs and a CTA can take a unit in a few tiles per warp, each unit gets one CTA: the join
+// between CTAs (some 3 us of fences and arrivals) would cost more than it spreads.
 #pragma once
 
 #include "pd_fp4.cuh"
 #include "pd_internal.h"
+
+#include <type_traits>
 
 namespace pd {
 
@@ -43,15 +48,34 @@ namespace fp4 {
 
 constexpr int MAX_ROWS = 1024;  // rows of one launch (their prefix sums are in shared memory)
 constexpr int COLS = 8;         // columns of a unit
+constexpr int TILE = 2 * FP4_TILE;  // keys of a warp's step: two records
+// Tiles per warp up to which a unit is one CTA's (when there are no more units than CTAs).
+constexpr int WHOLE_TILES = 4;
+// A running maximum below every score: finite, so that exp2(score - maximum) needs no special case
+// for columns that have seen no key (their scores are -inf).
+constexpr float NO_MAX = -3.0e38f;
+// The running maximum moves only when a score passes it by more than 2^HEADROOM: rescaling the
+// accumulators is then rare, and P stays below 2^8, which fp16 holds as exactly as smaller values.
+constexpr float HEADROOM = 8.f;
 
 // Floats of one CTA-level partial: m and l of 8 columns, then 8 x D accumulators.
 __host__ __device__ constexpr int partial_floats(int d) { return 2 * COLS + COLS * d; }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
-  const int n = live ? 16 : 0;  // 0: fills with zeros, reads nothing
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+// Bulk copy of `bytes` (a multiple of 16) into shared memory, counted on the mbarrier; the source
+// is read once, so its lines are the first to leave the L2.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar, uint64_t pol) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar), "l"(pol)
+      : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {  // 2^x, 2 ulp, subnormal results flushed to zero
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 r;
@@ -118,8 +142,10 @@ struct Worker {
   uint32_t qb[KS][2];
   float o[MT][4];
   float m_run[2], l_run[2];
+  float bar[2];  // m_run + HEADROOM: the scores that move the maximum
   float mul[2];  // score multiplier of columns 2c, 2c + 1
   int lim[2];    // their last visible key
+  int open_lim;  // keys up to this one are visible to every live column
 
   __device__ __forceinline__ void init(int lane_) {
     lane = lane_;
@@ -168,18 +194,18 @@ struct Worker {
       mul[j] = __shfl_sync(FULL_MASK, down, (2 * c + j) * 4) * (p.scale_log2 * unit);
       const int col = first + 2 * c + j;
       lim[j] = col < cols ? r.lk - r.chunk + col / p.group : -1;
-      m_run[j] = -INFINITY;
+      m_run[j] = bar[j] = NO_MAX;
       l_run[j] = 0.f;
     }
+    open_lim = r.lk - r.chunk + first / p.group;  // columns are in token order: the first sees least
 #pragma unroll
     for (int m = 0; m < MT; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
   }
 
-  // One record at shared address `a`; its first token is key `t0`, `rows` of its tokens exist.
-  __device__ __forceinline__ void tile(uint32_t a, int t0, int rows) {
-    float acc[2][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[0][i] = acc[1][i] = 0.f;
+  // q . k of the 16 tokens of the record at shared address `a`: acc[0], acc[1] token g of columns 2c,
+  // 2c + 1; acc[2], acc[3] token g + 8.
+  __device__ __forceinline__ void scores(uint32_t a, float (&acc)[4]) const {
+    acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
 #pragma unroll
     for (int b = 0; b < BLK; ++b) {
       alignas(16) uint32_t w0[KSB / 2], w1[KSB / 2];  // codes of tokens g and g + 8
@@ -212,50 +238,25 @@ struct Worker {
           y[i] = hmul2_bits(y[i], s1[u >> 1]);
         }
         const int ks = b * KSB + 2 * u;
-        X::m16n8k16(acc[0], x[0], y[0], x[1], y[1], qb[ks][0], qb[ks][1]);
-        X::m16n8k16(acc[1], x[2], y[2], x[3], y[3], qb[ks + 1][0], qb[ks + 1][1]);
+        X::m16n8k16(acc, x[0], y[0], x[1], y[1], qb[ks][0], qb[ks][1]);
+        X::m16n8k16(acc, x[2], y[2], x[3], y[3], qb[ks + 1][0], qb[ks + 1][1]);
       }
     }
-    float s[4];
-    bool exceeds = false;
+  }
+
+  // O^T += V^T P^T of the record at `a`, P as its fragment pair (pb0: tokens 0 .. 7, pb1: 8 .. 15);
+  // its tokens from `rows` on count as zeros.
+  template <int PARTS>
+  __device__ __forceinline__ void values(uint32_t a, const uint32_t (&pb0)[PARTS], const uint32_t (&pb1)[PARTS],
+                                         int rows) {
+    // scales of tokens 2c, 2c + 1 and 2c + 8, 2c + 9; zero past the row
+    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+    if (rows < FP4_TILE) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = i & 1, t = t0 + g + 8 * (i >> 1);
-      s[i] = t <= lim[j] ? (acc[0][i] + acc[1][i]) * mul[j] : -INFINITY;
-      exceeds |= s[i] > m_run[j];
-    }
-    if (__any_sync(FULL_MASK, exceeds)) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float t = fmaxf(s[j], s[2 + j]);
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) t = fmaxf(t, __shfl_xor_sync(FULL_MASK, t, off));
-        t = fmaxf(t, m_run[j]);
-        const float alpha = t == -INFINITY ? 1.f : exp2f(m_run[j] - t);
-        m_run[j] = t;
-        l_run[j] *= alpha;
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          o[m][j] *= alpha;
-          o[m][2 + j] *= alpha;
-        }
+      for (int hi = 0; hi < 2; ++hi) {
+        const int t = 8 * hi + 2 * c;
+        keep[hi] = (t < rows ? 0x0000ffffu : 0u) | (t + 1 < rows ? 0xffff0000u : 0u);
       }
-    }
-    float pr[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = i & 1;
-      pr[i] = s[i] == -INFINITY ? 0.f : exp2f(s[i] - m_run[j]);
-      l_run[j] += pr[i];
-    }
-    const uint32_t pb0 = movmatrix_trans(Elem<__half>::pack2(pr[0], pr[1]));
-    const uint32_t pb1 = movmatrix_trans(Elem<__half>::pack2(pr[2], pr[3]));
-    // V scales of tokens 2c, 2c + 1 and 2c + 8, 2c + 9; zero past the row
-    uint32_t keep[2];
-#pragma unroll
-    for (int hi = 0; hi < 2; ++hi) {
-      const int t = 8 * hi + 2 * c;
-      keep[hi] = (t < rows ? 0x0000ffffu : 0u) | (t + 1 < rows ? 0xffff0000u : 0u);
     }
 #pragma unroll
     for (int b = 0; b < BLK; ++b) {
@@ -293,8 +294,72 @@ struct Worker {
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          X::m16n8k16(o[b * 8 + u * 4 + i], even[0][i], odd[0][i], even[1][i], odd[1][i], pb0, pb1);
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part)
+            X::m16n8k16(o[b * 8 + u * 4 + i], even[0][i], odd[0][i], even[1][i], odd[1][i], pb0[part], pb1[part]);
       }
+    }
+  }
+
+  // A tile of two records at shared address `a`: keys t0 .. t0 + 31, of which `rows` exist. Two
+  // records share the maximum's test, the wait and the copy of a tile, and give the scheduler
+  // two independent chains.
+  __device__ __forceinline__ void tile(uint32_t a, int t0, int rows) {
+    float sc[8];
+    // both records whatever `rows`: what an absent one holds is masked below
+    scores(a, *reinterpret_cast<float(*)[4]>(sc));
+    scores(a + fp4_record_bytes(D), *reinterpret_cast<float(*)[4]>(sc + 4));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sc[i] *= mul[i & 1];
+    if (t0 + 2 * FP4_TILE - 1 > open_lim) {  // some column's last key, or the row's, is in this tile
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        sc[i] = t0 + (i >> 2) * FP4_TILE + 8 * ((i >> 1) & 1) + g <= lim[i & 1] ? sc[i] : -INFINITY;
+    }
+    float top[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) top[j] = fmaxf(fmaxf(sc[j], sc[2 + j]), fmaxf(sc[4 + j], sc[6 + j]));
+    if (__any_sync(FULL_MASK, top[0] > bar[0] || top[1] > bar[1])) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float t = top[j];
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) t = fmaxf(t, __shfl_xor_sync(FULL_MASK, t, off));
+        t = fmaxf(t, m_run[j]);
+        const float alpha = ex2(m_run[j] - t);
+        m_run[j] = t;
+        bar[j] = t + HEADROOM;
+        l_run[j] *= alpha;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          o[m][j] *= alpha;
+          o[m][2 + j] *= alpha;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      sc[i] = ex2(sc[i] - m_run[i & 1]);
+      l_run[i & 1] += sc[i];
+    }
+    // P is one fp16 operand for bf16 outputs (2^-12 is an eighth of their half ulp) and a hi + lo pair
+    // for fp16 outputs, whose rounding is no coarser than fp16 P's
+    constexpr int PARTS = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      uint32_t pb[2][PARTS];
+#pragma unroll
+      for (int hi = 0; hi < 2; ++hi) {
+        const float p0 = sc[4 * r + 2 * hi], p1 = sc[4 * r + 2 * hi + 1];
+        const uint32_t whole = Elem<__half>::pack2(p0, p1);
+        pb[hi][0] = movmatrix_trans(whole);
+        if constexpr (PARTS == 2) {
+          float f[2];
+          Elem<__half>::unpack2(whole, f);
+          pb[hi][1] = movmatrix_trans(Elem<__half>::pack2(p0 - f[0], p1 - f[1]));
+        }
+      }
+      values<PARTS>(a + r * fp4_record_bytes(D), pb[0], pb[1], rows - r * FP4_TILE);
     }
   }
 
@@ -357,7 +422,7 @@ struct Worker {
   }
 };
 
-// A partial unit of this CTA: records [t0, t1) of unit `unit` (kv head, column block) of row b.
+// A partial unit of this CTA: tiles [t0, t1) of unit `unit` (kv head, column block) of row b.
 struct Piece {
   int row, unit, t0, t1;  // row < 0: none
 };
@@ -365,13 +430,12 @@ struct Piece {
 // Joins `n` pieces' four elements of column col: ml(i) is piece i's (m, l) block, acc(i) its elements.
 template <typename Ml, typename Acc>
 __device__ __forceinline__ void join4(int n, int col, Ml ml, Acc acc, float (&x)[4], float& m, float& l) {
-  m = -INFINITY;
+  m = NO_MAX;
   for (int i = 0; i < n; ++i) m = fmaxf(m, ml(i)[col]);
   l = 0.f;
   x[0] = x[1] = x[2] = x[3] = 0.f;
-  if (m == -INFINITY) return;
   for (int i = 0; i < n; ++i) {
-    const float f = exp2f(ml(i)[col] - m);
+    const float f = ex2(ml(i)[col] - m);
     const float4 v = acc(i);
     l = fmaf(f, ml(i)[COLS + col], l);
     x[0] = fmaf(f, v.x, x[0]);
@@ -391,78 +455,107 @@ __device__ __forceinline__ void store_out4(const Fp4AttendParams& p, const Row& 
       make_uint2(Elem<T>::pack2(x[0] * inv, x[1] * inv), Elem<T>::pack2(x[2] * inv, x[3] * inv));
 }
 
-// Shared memory: [prefix int64 (rows + 1) | records and units per row | pieces | piece (m, l) |
-// piece accumulators (2 NW x cols x D) | rings (NW x stages x record)].
+// Shared memory: [stage barriers (NW x stages) | prefix int64 (rows + 1) | tiles and units per row |
+// pieces | piece (m, l) | leading pieces' accumulators (NW x cols x D) | rings (NW x stages x 2
+// records)]. A warp's trailing piece is its last work: its accumulators take the warp's ring, which
+// holds 18 D x 2 bytes a stage and so at least the 32 D of eight columns.
 struct Smem {
-  int rows_off, piece_off, ml_off, acc_off, ring_off, bytes;
+  int pre_off, rows_off, piece_off, ml_off, acc_off, ring_off, bytes;
 };
 
 __host__ __device__ inline Smem smem_layout(int batch, int nw, int cols, int d, int stages) {
   Smem s;
-  s.rows_off = (batch + 1) * 8;
+  s.pre_off = nw * stages * 8;
+  s.rows_off = s.pre_off + (batch + 1) * 8;
   s.piece_off = (s.rows_off + batch * 8 + 15) & ~15;
   s.ml_off = s.piece_off + 2 * nw * int(sizeof(Piece));
   s.acc_off = s.ml_off + 2 * nw * 2 * COLS * 4;
-  s.ring_off = (s.acc_off + 2 * nw * cols * d * 4 + 127) & ~127;
-  s.bytes = s.ring_off + nw * stages * fp4_record_bytes(d);
+  s.ring_off = (s.acc_off + nw * cols * d * 4 + 127) & ~127;
+  s.bytes = s.ring_off + nw * stages * 2 * fp4_record_bytes(d);
   return s;
 }
 
+// A position in the tile sequence: tile `tile` of unit `unit` (kv head, column block) of row b.
+struct Cursor {
+  int b, unit, tile, tiles, units;
+};
+
 template <typename T, int D, int NW>
 __global__ void __launch_bounds__(NW * 32, 1)
-    pd_fp4_attend_kernel(const __grid_constant__ Fp4AttendParams p, int stages, int max_cols, int min_records) {
+    pd_fp4_attend_kernel(const __grid_constant__ Fp4AttendParams p, int stages, int max_cols, int min_tiles) {
   constexpr int REC = fp4_record_bytes(D);
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ long long warp_sums[NW];
+  __shared__ long long warp_sums[2][NW];
   __shared__ unsigned last_flags[2];
   const Smem L = smem_layout(p.batch, NW, max_cols, D, stages);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  long long* pre = reinterpret_cast<long long*>(smem);
-  int2* rows = reinterpret_cast<int2*>(smem + L.rows_off);  // (records, units) per row
+  long long* pre = reinterpret_cast<long long*>(smem + L.pre_off);
+  int2* rows = reinterpret_cast<int2*>(smem + L.rows_off);  // (tiles, units) per row
   Piece* pieces = reinterpret_cast<Piece*>(smem + L.piece_off);
   float* piece_ml = reinterpret_cast<float*>(smem + L.ml_off);
-  float* piece_acc = reinterpret_cast<float*>(smem + L.acc_off);
+  auto piece_acc = [&](int slot) -> float* {  // slot 2 w: warp w's leading piece, 2 w + 1: its trailing one
+    return slot & 1 ? reinterpret_cast<float*>(smem + L.ring_off) + size_t(slot >> 1) * stages * (2 * REC / 4)
+                    : reinterpret_cast<float*>(smem + L.acc_off) + size_t(slot >> 1) * max_cols * D;
+  };
+  const uint32_t bars = smem_addr(smem) + uint32_t(warp * stages) * 8u;
 
-  // ---- records of every row, and their prefix sums
+  // ---- tiles of every row, their prefix sums, the unit count and the longest row
+  long long total, units_total;
+  int longest;
   {
+    if (lane < stages) mbar_init(bars + lane * 8u, 1);
+    fence_barrier_init();
     const int per = (p.batch + NW * 32 - 1) / (NW * 32);
     const int b0 = tid * per;
-    long long sum = 0;
+    long long sum = 0, usum = 0;
+    int most = 0;
     for (int b = b0; b < b0 + per && b < p.batch; ++b) {
       const Row r = row_of(p, b);
-      const int records = r.lk > FP4_TILE ? (r.lk + FP4_TILE - 1) / FP4_TILE : 1;
+      const int tiles = r.lk > TILE ? (r.lk + TILE - 1) / TILE : 1;
       const int units = p.n_kv_head * ((r.sq * p.group + COLS - 1) / COLS);
-      rows[b] = make_int2(records, units);
-      sum += (long long)records * units;
+      rows[b] = make_int2(tiles, units);
+      sum += (long long)tiles * units;
+      usum += units;
+      most = units > 0 && tiles > most ? tiles : most;
     }
     long long incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long up = __shfl_up_sync(FULL_MASK, incl, o);
       if (lane >= o) incl += up;
+      usum += __shfl_xor_sync(FULL_MASK, usum, o);
+      most = max(most, __shfl_xor_sync(FULL_MASK, most, o));
     }
-    if (lane == 31) warp_sums[warp] = incl;
+    if (lane == 31) {
+      warp_sums[0][warp] = incl;
+      warp_sums[1][warp] = (usum << 31) | most;  // both below 2^31
+    }
     if (tid < 2 * NW) pieces[tid].row = -1;
     __syncthreads();
     long long at = incl - sum;
-    for (int w = 0; w < warp; ++w) at += warp_sums[w];
+    total = units_total = 0;
+    longest = 0;
+    for (int w = 0; w < NW; ++w) {
+      if (w < warp) at += warp_sums[0][w];
+      total += warp_sums[0][w];
+      units_total += warp_sums[1][w] >> 31;
+      longest = max(longest, int(warp_sums[1][w] & 0x7fffffff));
+    }
     for (int b = b0; b < b0 + per && b < p.batch; ++b) {
       pre[b] = at;
       at += (long long)rows[b].x * rows[b].y;
-      if (b == p.batch - 1) pre[p.batch] = at;
     }
+    if (tid == 0) pre[p.batch] = total;
     __syncthreads();
   }
-  const long long total = pre[p.batch];
   if (total == 0) return;
-  // Warps with work: all of them, unless that leaves a warp fewer than min_records.
-  const long long all = (long long)gridDim.x * NW;
-  long long active = (total + min_records - 1) / min_records;
-  active = active < all ? active : all;
-  const long long me = (long long)blockIdx.x * NW + warp;
-  if ((long long)blockIdx.x * NW >= active) return;
-  auto begin_of = [&](long long w) -> long long { return w >= active ? total : w * total / active; };
-  auto find_row = [&](long long f) -> int {  // last b with pre[b] <= f that has work
+
+  // ---- this CTA's run [c0, c1) and this warp's part of it
+  const bool whole = units_total <= gridDim.x && longest <= WHOLE_TILES * NW;
+  long long ctas = whole ? units_total : (total + NW * min_tiles - 1) / (NW * min_tiles);
+  ctas = ctas < gridDim.x ? ctas : gridDim.x;
+  if (blockIdx.x >= ctas) return;
+  auto find_row = [&](long long f) -> int {  // last b with pre[b] <= f: the row of tile f
     int lo = 0, hi = p.batch - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -470,115 +563,166 @@ __global__ void __launch_bounds__(NW * 32, 1)
     }
     return lo;
   };
+  long long c0, c1;
+  if (whole) {  // the blockIdx-th unit
+    int b = 0, u = int(blockIdx.x);
+    while (u >= rows[b].y) u -= rows[b++].y;
+    c0 = pre[b] + (long long)u * rows[b].x;
+    c1 = c0 + rows[b].x;
+  } else {
+    c0 = blockIdx.x * total / ctas;
+    c1 = (blockIdx.x + 1) * total / ctas;
+  }
+  const int in_cta = int(c1 - c0);
+  const int warps = min(NW, (in_cta + min_tiles - 1) / min_tiles);
+  const long long f0 = c0 + (long long)in_cta * min(warp, warps) / warps;
+  const int count = warp < warps ? int(c0 + (long long)in_cta * (warp + 1) / warps - f0) : 0;
 
-  const long long f0 = begin_of(me), f1 = begin_of(me + 1);
-  const int count = int(f1 - f0);
   if (count > 0) {
-    const uint32_t ring = smem_addr(smem + L.ring_off) + uint32_t(warp * stages) * REC;
-    const int tpb_mask = (1 << p.log2_tpb) - 1;
-    // Lookup cursor: the record whose block id is being fetched; one record ahead of the copies.
-    struct Cursor {
-      int b, unit, rec, records, units;
-    };
-    auto place = [&](Cursor& k, long long f) {
-      k.b = find_row(f);
-      const long long r = f - pre[k.b];
-      k.records = rows[k.b].x;
-      k.units = rows[k.b].y;
-      k.unit = int(r / k.records);
-      k.rec = int(r - (long long)k.unit * k.records);
-    };
-    auto step = [&](Cursor& k) {
-      if (++k.rec < k.records) return;
-      k.rec = 0;
+    constexpr uint32_t STAGE = 2 * REC;
+    const uint32_t ring = smem_addr(smem + L.ring_off) + uint32_t(warp * stages) * STAGE;
+    const uint64_t policy = l2_policy_evict_first();
+    auto step_unit = [&](Cursor& k) {  // to the next unit's first tile
+      k.tile = 0;
       if (++k.unit < k.units) return;
       k.unit = 0;
       do ++k.b; while (k.b < p.batch && rows[k.b].y == 0);
       if (k.b < p.batch) {
-        k.records = rows[k.b].x;
+        k.tiles = rows[k.b].x;
         k.units = rows[k.b].y;
       }
     };
-    Cursor look, at;
-    place(look, f0);
-    at = look;
-    int next_blk = -1, next_sub = 0;
-    int looked = 0;
-    auto lookup = [&]() {
-      if (looked >= count) return;
-      const int page = look.rec >> p.log2_tpb;
-      const int cbs = look.units / p.n_kv_head;
-      next_sub = ((look.unit / cbs) << p.log2_tpb) + (look.rec & tpb_mask);
-      next_blk = page < p.max_blocks ? __ldg(p.table + int64_t(look.b) * p.bt_stride + page) : -1;
-      ++looked;
-      step(look);
+    Cursor at;
+    at.b = find_row(f0);
+    {
+      const long long r = f0 - pre[at.b];
+      at.tiles = rows[at.b].x;
+      at.units = rows[at.b].y;
+      at.unit = int(r / at.tiles);
+      at.tile = int(r - (long long)at.unit * at.tiles);
+    }
+
+    // ---- prefetch: tile `ahead`, its blocks from a window of 32 block ids held by the lanes, the
+    // next 32 already loading. A window starts at a tile's first page, so a tile's two pages
+    // (block_size 16) are always in one window.
+    Cursor ahead = at;
+    int win = 0, win_next = 0, win_page = 0, last_page = 0, records = 0;
+    const unsigned char* head_pages = nullptr;  // this head's first record of block 0
+    auto entry = [&](int page) -> int {
+      return page <= last_page ? __ldg(p.table + int64_t(ahead.b) * p.bt_stride + page) : -1;
     };
-    lookup();
+    auto open_ahead = [&]() {
+      const int h = ahead.unit / (ahead.units / p.n_kv_head);
+      head_pages = p.pages + (int64_t(h) << p.log2_tpb) * REC;
+      records = (row_of(p, ahead.b).lk + FP4_TILE - 1) / FP4_TILE;
+      last_page = min(((records + (1 << p.log2_tpb) - 1) >> p.log2_tpb), p.max_blocks) - 1;
+      win_page = (2 * ahead.tile) >> p.log2_tpb;
+      win = entry(win_page + lane);
+      win_next = entry(win_page + 32 + lane);
+    };
+    open_ahead();
+    const uint32_t block_stride = uint32_t(p.n_kv_head << p.log2_tpb) * REC;
     int issued = 0;
+    uint32_t fill = 0;  // stage of the next copy
     auto issue = [&]() {
-      if (issued < count) {
-        const bool live = next_blk >= 0 && next_blk < p.n_blocks;
-        const unsigned char* src =
-            p.pages + (((live ? int64_t(next_blk) : 0) * p.n_kv_head << p.log2_tpb) + next_sub) * REC;
-        const uint32_t dst = ring + uint32_t(issued % stages) * REC;
-        lookup();
-#pragma unroll
-        for (int i = 0; i < (REC / 16 + 31) / 32; ++i) {
-          const int ch = i * 32 + lane;
-          if (ch < REC / 16) cp_async16(dst + ch * 16, src + (live ? ch * 16 : 0), live);
-        }
-        ++issued;
+      if (issued == count) return;
+      const int rec = 2 * ahead.tile;
+      int page = (rec >> p.log2_tpb) - win_page;
+      if (page >= 32) {
+        win_page += 32;
+        page -= 32;
+        win = win_next;
+        win_next = entry(win_page + 32 + lane);
       }
-      cp_async_commit();
+      const uint32_t dst = ring + fill * STAGE, bar = bars + fill * 8u;
+      const int blk0 = __shfl_sync(FULL_MASK, win, page);
+      const int blk1 = p.log2_tpb == 0 ? __shfl_sync(FULL_MASK, win, (page + 1) & 31) : blk0;
+      const bool two = rec + 1 < records;
+      const bool live0 = blk0 >= 0 && blk0 < p.n_blocks, live1 = blk1 >= 0 && blk1 < p.n_blocks;
+      if (live0 && (live1 || !two)) {
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar, two ? STAGE : REC);
+          const unsigned char* src0 = head_pages + uint64_t(blk0) * block_stride;
+          if (p.log2_tpb == 0) {
+            bulk_load(dst, src0, REC, bar, policy);
+            if (two) bulk_load(dst + REC, head_pages + uint64_t(blk1) * block_stride, REC, bar, policy);
+          } else {  // both records in one page, one after the other
+            bulk_load(dst, src0 + (rec & ((1 << p.log2_tpb) - 1)) * REC, two ? STAGE : REC, bar, policy);
+          }
+        }
+      } else {  // a block outside the pool reads zeros
+        const int sub = rec & ((1 << p.log2_tpb) - 1);
+#pragma unroll 1
+        for (int r = 0; r < 2; ++r) {
+          const bool live = r == 0 ? live0 : live1;
+          const int in_page = p.log2_tpb == 0 ? 0 : sub + r;
+          const uint4* src = reinterpret_cast<const uint4*>(
+              head_pages + (live ? uint64_t(r == 0 ? blk0 : blk1) * block_stride + in_page * REC : 0));
+          for (int i = lane; i < REC / 16; i += 32) {
+            const uint4 v = live && (r == 0 || two) ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + r * REC + i * 16), "r"(v.x), "r"(v.y),
+                         "r"(v.z), "r"(v.w)
+                         : "memory");
+          }
+        }
+        fence_proxy_async_smem();  // a later bulk copy writes the same bytes
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+      }
+      fill = fill + 1 == uint32_t(stages) ? 0 : fill + 1;
+      ++issued;
+      if (++ahead.tile == ahead.tiles && issued < count) {
+        step_unit(ahead);
+        open_ahead();
+      }
     };
     for (int s = 0; s < stages - 1; ++s) issue();
 
     Worker<T, D> wk;
     wk.init(lane);
-    Row row{};
-    int h = 0, first = 0, t_begin = 0;
-    for (int n = 0; n < count; ++n) {
-      if (n == 0 || at.rec == 0) {  // a unit opens
-        row = row_of(p, at.b);
-        const int cbs = at.units / p.n_kv_head;
-        h = at.unit / cbs;
-        first = (at.unit - h * cbs) * COLS;
-        t_begin = at.rec;
-        wk.start(p, row, h, first);
-      }
-      // record n has landed once at most stages - 2 later groups are pending
-      switch (stages) {
-        case 2: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-        case 3: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-        case 4: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-        case 5: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-        default: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-      }
-      __syncwarp();  // every lane's bytes are in, and every lane is done with the stage refilled next
-      issue();
-      const int t0 = at.rec * FP4_TILE;
-      wk.tile(ring + uint32_t(n % stages) * REC, t0, row.lk - t0);
-      const bool unit_ends = at.rec + 1 == at.records;
-      if (unit_ends || n == count - 1) {
-        if (unit_ends && t_begin == 0) {
-          wk.finish(p, row, h, first);
-        } else {
-          const int slot = 2 * warp + (t_begin == 0 ? 1 : 0);
-          const int cols = min(COLS, row.sq * p.group - first);
-          wk.store_piece(piece_ml + slot * 2 * COLS, piece_acc + size_t(slot) * max_cols * D, cols);
-          if (lane == 0) {
-            Piece pc;
-            pc.row = at.b;
-            pc.unit = at.unit;
-            pc.t0 = t_begin;
-            pc.t1 = at.rec + 1;
-            pieces[slot] = pc;
-          }
+    uint32_t stage = 0, phase = 0;
+    int taken = 0;
+    bool ok = true;
+    for (int n = 0; n < count;) {
+      const Row row = row_of(p, at.b);
+      const int cbs = at.units / p.n_kv_head;
+      const int h = at.unit / cbs, first = (at.unit - h * cbs) * COLS;
+      const int begin = at.tile, end = min(at.tiles, at.tile + count - n);
+      wk.start(p, row, h, first);
+      for (int tile = begin; tile < end; ++tile) {
+        if (ok && !warp_wait_phase(bars + stage * 8u, phase, p.wait_ns)) {
+          ok = false;  // the rest of the run is left out; its pieces and arrivals still happen
+          if (lane == 0) atomicOr(p.err, DEVERR_WAIT_TIMEOUT);
+        }
+        if (!ok) continue;
+        __syncwarp();  // every lane is done with the stage that the next copy fills
+        issue();
+        wk.tile(ring + stage * STAGE, tile * TILE, row.lk - tile * TILE);
+        ++taken;
+        if (++stage == uint32_t(stages)) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
-      step(at);
+      n += end - begin;
+      if (begin == 0 && end == at.tiles) {
+        wk.finish(p, row, h, first);
+      } else {
+        const int slot = 2 * warp + (begin == 0 ? 1 : 0);
+        wk.store_piece(piece_ml + slot * 2 * COLS, piece_acc(slot), min(COLS, row.sq * p.group - first));
+        if (lane == 0) pieces[slot] = Piece{at.b, at.unit, begin, end};
+      }
+      if (n < count) step_unit(at);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!ok) {  // never leave with a copy in flight: stages in the order of their copies
+      for (; taken < issued; ++taken) {
+        warp_wait_phase(bars + stage * 8u, phase, DRAIN_LIMIT_NS);
+        if (++stage == uint32_t(stages)) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
   }
 
   // ---- joins within the CTA
@@ -595,24 +739,22 @@ __global__ void __launch_bounds__(NW * 32, 1)
   unsigned heads = __ballot_sync(FULL_MASK, opens);
   float* const cta_part = p.partials + size_t(blockIdx.x) * 2 * partial_floats(D);
   int task = 0;
-  bool cut[2] = {false, false};
-  Piece cut_piece[2] = {};
+  int cut0 = -1, cut1 = -1;  // first piece of the unit cut at the CTA's front, and at its back
   while (heads) {
     const int s0 = __ffs(heads) - 1;
     heads &= heads - 1;
     const unsigned upto = heads ? (1u << (__ffs(heads) - 1)) - 1u : 0xffffffffu;
     const unsigned members = valid & upto & ~((1u << s0) - 1u);
-    const int s1 = 31 - __clz(members);
-    const Piece a = pieces[s0], z = pieces[s1];
-    const bool complete = a.t0 == 0 && z.t1 == rows[a.row].x;
+    const Piece a = pieces[s0];
+    const int2 rw = rows[a.row];
+    const bool complete = a.t0 == 0 && pieces[31 - __clz(members)].t1 == rw.x;
     const Row r = row_of(p, a.row);
-    const int cbs = rows[a.row].y / p.n_kv_head;
+    const int cbs = rw.y / p.n_kv_head;
     const int h = a.unit / cbs, first = (a.unit - h * cbs) * COLS;
     const int cols = min(COLS, r.sq * p.group - first);
     const int slot = a.t0 > 0 ? 0 : 1;
     if (!complete) {
-      cut[slot] = true;
-      cut_piece[slot] = a;
+      if (slot == 0) cut0 = s0; else cut1 = s0;
     }
     const float unit = p.units != nullptr ? __ldg(p.units + p.n_kv_head + h) : 1.f;
     const int n = __popc(members);
@@ -625,8 +767,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
       // after the first piece, each further one is the next warp's leading piece
       auto index = [&](int i) -> int { return i == 0 ? s0 : 2 * ((s0 >> 1) + i); };
       join4(n, col, [&](int i) { return piece_ml + index(i) * 2 * COLS; },
-            [&](int i) { return *reinterpret_cast<const float4*>(piece_acc + size_t(index(i)) * max_cols * D + e); }, x,
-            m, l);
+            [&](int i) { return *reinterpret_cast<const float4*>(piece_acc(index(i)) + e); }, x, m, l);
       if (complete) {
         store_out4<T>(p, r, h, first + col, e - col * D, unit, x, l);
       } else {
@@ -639,43 +780,39 @@ __global__ void __launch_bounds__(NW * 32, 1)
       }
     }
   }
-  if (!cut[0] && !cut[1]) return;  // uniform
+  if (cut0 < 0 && cut1 < 0) return;  // uniform
 
   // ---- joins between CTAs: the last one to arrive at a unit joins its partials, in CTA order
   __threadfence();
   __syncthreads();
-  int cta0[2] = {0, 0}, n_cta[2] = {0, 0};
-#pragma unroll
+#pragma unroll 1
   for (int s = 0; s < 2; ++s) {
-    if (!cut[s]) continue;
-    const long long u0 = pre[cut_piece[s].row] + (long long)cut_piece[s].unit * rows[cut_piece[s].row].x;
-    const long long u1 = u0 + rows[cut_piece[s].row].x - 1;
-    // the warp of record f: the largest w with w * total / active <= f
-    cta0[s] = int((((u0 + 1) * active + total - 1) / total - 1) / NW);
-    n_cta[s] = int((((u1 + 1) * active + total - 1) / total - 1) / NW) - cta0[s] + 1;
+    const int at = s == 0 ? cut0 : cut1;
+    if (at < 0) continue;
+    const Piece a = pieces[at];
+    const int2 rw = rows[a.row];
+    const long long u0 = pre[a.row] + (long long)a.unit * rw.x, u1 = u0 + rw.x - 1;
+    // the CTA of tile f: the largest c with c * total / ctas <= f
+    const int cta0 = int(((u0 + 1) * ctas + total - 1) / total - 1);
+    const int n = int(((u1 + 1) * ctas + total - 1) / total - 1) - cta0 + 1;
     if (tid == 0) {
-      const unsigned old = atomicAdd(p.counters + cta0[s], 1u);
-      last_flags[s] = old == unsigned(n_cta[s] - 1);
-      if (last_flags[s]) p.counters[cta0[s]] = 0u;  // zero again for the next launch
+      const unsigned old = atomicAdd(p.counters + cta0, 1u);
+      last_flags[s] = old == unsigned(n - 1);
+      if (last_flags[s]) p.counters[cta0] = 0u;  // zero again for the next launch
+      __threadfence();
     }
-  }
-  __threadfence();
-  __syncthreads();
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    if (!cut[s] || !last_flags[s]) continue;
-    const Piece a = cut_piece[s];
+    __syncthreads();
+    if (!last_flags[s]) continue;
     const Row r = row_of(p, a.row);
-    const int cbs = rows[a.row].y / p.n_kv_head;
+    const int cbs = rw.y / p.n_kv_head;
     const int h = a.unit / cbs, first = (a.unit - h * cbs) * COLS;
     const int cols = min(COLS, r.sq * p.group - first);
     const float unit = p.units != nullptr ? __ldg(p.units + p.n_kv_head + h) : 1.f;
-    const int n = n_cta[s];
     for (int e = tid * 4; e < cols * D; e += NW * 128) {
       const int col = e / D;
       float x[4], m, l;
       auto part = [&](int i) -> const float* {  // the first CTA's is its unit that goes on, the others' their first
-        return p.partials + (size_t(cta0[s] + i) * 2 + (i == 0 ? 1 : 0)) * partial_floats(D);
+        return p.partials + (size_t(cta0 + i) * 2 + (i == 0 ? 1 : 0)) * partial_floats(D);
       };
       join4(n, col, part,
             [&](int i) { return __ldcg(reinterpret_cast<const float4*>(part(i) + 2 * COLS + e)); }, x, m, l);
