@@ -6,6 +6,9 @@ binds it with ctypes (``model/_native.py``). Every translation unit is compiled 
 CUDA runtime, so the .so only needs the driver (``libcuda.so.1``) at run time and can be
 loaded (not used) on a host without a GPU.
 
+The Python binding of the newer operators, ``pd_ops.so``, is compiled beside it with g++ against
+torch's headers; it calls the library through addresses it is handed and links to nothing of it.
+
 Usage: ``python llm-serving_b200/build.py [--force] [--verbose]``. The output lands next to
 this file and is rebuilt only when a source is newer than it.
 """
@@ -25,6 +28,9 @@ CSRC = HERE / "csrc"
 INCLUDE = HERE.parent / "include"
 BUILD = HERE / "_build"
 LIB = HERE / "libpaged_decode.so"
+#: The Python binding of the newer operators (csrc/py_ops.cpp): a CPython extension over torch's
+#: C++ API that calls the library's C ABI. Compiled by the host compiler, no device code.
+OPS = HERE / "pd_ops.so"
 
 SOURCES = [
     "pd_api.cu",
@@ -82,6 +88,21 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(dep.stat().st_mtime > mtime for dep in deps)
 
 
+def _ops_command() -> list[str]:
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    includes = [INCLUDE, CSRC, root / "include", root / "include/torch/csrc/api/include",
+                sysconfig.get_paths()["include"], Path(cuda) / "include"]
+    libs = ["torch_python", "torch", "torch_cpu", "torch_cuda", "c10", "c10_cuda"]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+            *[f"-I{p}" for p in includes], str(CSRC / "py_ops.cpp"), "-o", str(OPS), f"-L{root / 'lib'}",
+            *[f"-l{name}" for name in libs]]
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False) -> Path:
     """Compile and link the library; returns its path. Raises on a compiler error."""
     BUILD.mkdir(exist_ok=True)
@@ -97,6 +118,10 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
             if ptxas_verbose:
                 cmd[1:1] = ["-Xptxas", "-v"]
             jobs.append(cmd)
+    ops_source = CSRC / "py_ops.cpp"
+    compile_jobs = len(jobs)
+    if force or _stale(OPS, [ops_source, *_headers(ops_source)]):
+        jobs.append(_ops_command())
 
     def run(cmd):
         if verbose:
@@ -109,9 +134,9 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
             if proc.returncode != 0 or verbose or ptxas_verbose:
                 sys.stderr.write(proc.stdout + proc.stderr)
             if proc.returncode != 0:
-                raise RuntimeError(f"nvcc failed ({proc.returncode}): {' '.join(cmd)}")
+                raise RuntimeError(f"{Path(cmd[0]).name} failed ({proc.returncode}): {' '.join(cmd)}")
 
-    if force or jobs or _stale(LIB, objects):
+    if force or compile_jobs or _stale(LIB, objects):
         cmd = [nvcc, *ARCH, "-shared", "-cudart", "static", "-o", str(LIB), *map(str, objects)]
         if verbose:
             print(" ".join(cmd), flush=True)

@@ -10,6 +10,7 @@ the library cannot be loaded, :data:`AVAILABLE` is False and every caller raises
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import math
 from pathlib import Path
 
@@ -181,6 +182,32 @@ lib, LOAD_ERROR = _load()
 AVAILABLE: bool = lib is not None
 
 
+OPS_PATH = LIB_PATH.parent / "pd_ops.so"
+
+
+def _load_ops():
+    """The binding of the newer operators (csrc/py_ops.cpp), bound to the library loaded above."""
+    if lib is None:
+        return None, LOAD_ERROR
+    if not OPS_PATH.exists():
+        return None, f"{OPS_PATH} is missing; run `python llm-serving_b200/build.py`"
+    try:
+        spec = importlib.util.spec_from_file_location("pd_ops", OPS_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind({name: ctypes.cast(getattr(lib, name), _c_ptr).value for name in _SIGNATURES}, check)
+    except ImportError as exc:  # pragma: no cover - depends on the host
+        return None, f"could not load {OPS_PATH}: {exc}"
+    return module, None
+
+
+def require_ops():
+    """The operators' binding; RuntimeError where it or the library is missing."""
+    if ops is None:
+        raise RuntimeError(f"the sm_100a operators are not available: {OPS_ERROR}")
+    return ops
+
+
 def require() -> ctypes.CDLL:
     if lib is None:
         raise RuntimeError(f"the sm_100a paged-decode library is not available: {LOAD_ERROR}")
@@ -212,26 +239,6 @@ def check(status: int, what: str) -> None:
 
 def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
-
-
-class _NoGuard:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_NO_GUARD = _NoGuard()
-
-
-def device_guard(device: torch.device):
-    """``torch.cuda.device(device)``, or nothing where that device is current already (the guard
-    itself costs about a microsecond of every call)."""
-    index = device.index
-    if index is None or index == torch.cuda.current_device():
-        return _NO_GUARD
-    return torch.cuda.device(device)
 
 
 def strides3(t: torch.Tensor):
@@ -416,107 +423,6 @@ def append_table(k_pool, v_pool, block_table, pos, k, v, rope=None) -> None:
     check(status, "pd_kv_append_table_rope")
 
 
-def qk_norm_rope(q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions, rotary_dim, eps) -> None:
-    """One pd_qk_norm_rope launch on the current stream. Tensors are already validated."""
-    tokens, heads, d = q.shape
-    status = require().pd_qk_norm_rope(
-        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-        q_out.data_ptr(), q_out.stride(0), q_out.stride(1), k_out.data_ptr(), k_out.stride(0), k_out.stride(1),
-        q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.stride(0), sin.stride(0),
-        cos.shape[0], 0 if positions is None else positions.data_ptr(),
-        PD_SLOT_I32 if positions is not None and positions.dtype == torch.int32 else PD_SLOT_I64,
-        tokens, heads, k.shape[1], d, rotary_dim, eps, _DTYPES[q.dtype], stream_handle(q.device),
-    )
-    if status:
-        check(status, "pd_qk_norm_rope")
-
-
-def strides2(t: torch.Tensor):
-    """The (token, head) element strides of a 3-D row tensor as int64[2]."""
-    return (_c_i64 * 2)(t.stride(0), t.stride(1))
-
-
-def _page_geometry(pages: torch.Tensor) -> tuple[int, int, int, int]:
-    """(n_blocks, block_size, n_kv_head, head_dim) of a 4-bit pool tensor."""
-    n_blocks, hkv, records, record = pages.shape
-    return n_blocks, records * 16, hkv, record // 18
-
-
-def fp4_write_slots(pages, slot_ids, k, v, units) -> None:
-    n_blocks, bs, hkv, d = _page_geometry(pages)
-    status = require().pd_fp4_write_slots(
-        pages.data_ptr(), n_blocks, bs, slot_ids.data_ptr(),
-        PD_SLOT_I64 if slot_ids.dtype == torch.int64 else PD_SLOT_I32, k.data_ptr(), strides2(k), v.data_ptr(),
-        strides2(v), 0 if units is None else units.data_ptr(), _DTYPES[k.dtype], k.shape[0], hkv, d,
-        stream_handle(pages.device))
-    if status:
-        check(status, "pd_fp4_write_slots")
-
-
-def fp4_write_table(pages, block_table, pos, k, v, units) -> None:
-    n_blocks, bs, hkv, d = _page_geometry(pages)
-    status = require().pd_fp4_write_table(
-        pages.data_ptr(), n_blocks, bs, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-        pos.data_ptr(), k.data_ptr(), strides2(k), v.data_ptr(), strides2(v),
-        0 if units is None else units.data_ptr(), _DTYPES[k.dtype], k.shape[0], hkv, d, stream_handle(pages.device))
-    if status:
-        check(status, "pd_fp4_write_table")
-
-
-def fp4_read_slots(pages, slot_ids, k, v, units) -> None:
-    n_blocks, bs, hkv, d = _page_geometry(pages)
-    status = require().pd_fp4_read_slots(
-        pages.data_ptr(), n_blocks, bs, slot_ids.data_ptr(),
-        PD_SLOT_I64 if slot_ids.dtype == torch.int64 else PD_SLOT_I32, k.data_ptr(), strides2(k), v.data_ptr(),
-        strides2(v), 0 if units is None else units.data_ptr(), _DTYPES[k.dtype], k.shape[0], hkv, d,
-        stream_handle(pages.device))
-    if status:
-        check(status, "pd_fp4_read_slots")
-
-
-def fp4_workspace_bytes(head_dim: int) -> int:
-    return int(require().pd_fp4_workspace_bytes(head_dim))
-
-
-def fp4_decode(q, pages, block_table, seqlen, out, units, scale_log2, workspace, stream) -> None:
-    n_blocks, bs, hkv, d = _page_geometry(pages)
-    status = require().pd_fp4_decode(
-        q.data_ptr(), q.stride(0), q.stride(1), pages.data_ptr(), n_blocks, bs,
-        0 if units is None else units.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-        block_table.shape[1], seqlen.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), q.shape[0], q.shape[1],
-        hkv, d, _DTYPES[q.dtype], scale_log2, workspace.data_ptr(), workspace.numel(), stream)
-    if status:
-        check(status, "pd_fp4_decode")
-
-
-def fp4_prefill(q, pages, block_table, cu_seqlens_q, seqlen_k, max_seqlen_q, out, units, scale_log2, workspace,
-                stream) -> None:
-    n_blocks, bs, hkv, d = _page_geometry(pages)
-    status = require().pd_fp4_prefill(
-        q.data_ptr(), q.shape[0], q.stride(0), q.stride(1), pages.data_ptr(), n_blocks, bs,
-        0 if units is None else units.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-        block_table.shape[1], cu_seqlens_q.data_ptr(), seqlen_k.data_ptr(), out.data_ptr(), out.stride(0),
-        out.stride(1), seqlen_k.shape[0], max_seqlen_q, q.shape[1], hkv, d, _DTYPES[q.dtype], scale_log2,
-        workspace.data_ptr(), workspace.numel(), stream)
-    if status:
-        check(status, "pd_fp4_prefill")
-
-
-def block_copy(pools, src, dst, block_table, remap) -> None:
-    """One pd_block_copy call: ``pools`` are equal contiguous tensors with blocks first."""
-    first = pools[0]
-    ptrs = (_c_ptr * len(pools))(*[t.data_ptr() for t in pools])
-    rows, cols = (0, 0) if block_table is None else block_table.shape
-    status = require().pd_block_copy(
-        ptrs, len(pools), first.shape[0], first.numel() // first.shape[0] * first.element_size(), src.data_ptr(), dst.data_ptr(),
-        PD_SLOT_I64 if src.dtype == torch.int64 else PD_SLOT_I32, src.shape[0],
-        0 if block_table is None else block_table.data_ptr(), rows, cols,
-        0 if block_table is None else max(block_table.stride(0), cols), 0 if remap is None else remap.data_ptr(),
-        stream_handle(first.device))
-    if status:
-        check(status, "pd_block_copy")
-
-
 class NativePlan:
     """Owner of one ``pd_plan`` handle (host memory); destroyed with the object."""
 
@@ -587,3 +493,6 @@ class NativePlan:
 
 def default_scale(head_dim: int) -> float:
     return 1.0 / math.sqrt(head_dim)
+
+
+ops, OPS_ERROR = _load_ops()

@@ -29,19 +29,14 @@ import math
 import torch
 
 from model import _native
-from model.paged import PagedKV, PagedPool, _positive, _same_device, _unit_last_stride
-from model.triton_decode import _LOG2E, _pow2, _raise_first, _require_backend, _require_cuda_tensors
+from model.paged import PagedKV, PagedPool, _positive
+from model.triton_decode import _pow2, _raise_first
 
-__all__ = ["Fp4KV", "Fp4Pool", "fp4_pages", "paged_decode_fp4", "paged_prefill_fp4", "read_slots_fp4",
+__all__ = ["Fp4KV", "Fp4Pool", "fp4_pages", "fp4_workspace", "paged_decode_fp4", "paged_prefill_fp4", "read_slots_fp4",
            "write_slots_fp4"]
 
 _HEAD_DIMS = (64, 128, 256)
 _QUERY_DTYPES = (torch.float16, torch.bfloat16)
-_ROW_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
-
-#: Per (device, stream) workspace of the one-shot calls: zero-filled once, left at zero by every launch.
-_WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
-
 
 def _pool_rules(block_size, head_dim):
     yield not _pow2(block_size) or block_size < 16, lambda: (
@@ -58,34 +53,10 @@ def fp4_pages(n_blocks: int, block_size: int, n_kv_head: int, head_dim: int, *, 
     return torch.zeros(n_blocks, n_kv_head, block_size // 16, 18 * head_dim, dtype=torch.uint8, device=device)
 
 
-def _pages_rules(pages, units):
-    yield pages.dim() != 4 or pages.dtype != torch.uint8, lambda: (
-        "pages must be uint8 (n_blocks, H_kv, block_size / 16, 18 * head_dim), got "
-        f"{tuple(pages.shape)} {pages.dtype}")
-    yield pages.shape[3] not in (18 * 64, 18 * 128, 18 * 256) or not _pow2(pages.shape[2]) or pages.shape[1] < 1, lambda: (
-        f"pages of shape {tuple(pages.shape)} are not 4-bit pages of head_dim 64, 128 or 256")
-    yield not pages.is_contiguous() or pages.data_ptr() % 16 != 0, lambda: (
-        "pages must be contiguous and 16-byte aligned")
-    if units is not None:
-        yield units.dtype != torch.float32 or tuple(units.shape) != (2, pages.shape[1]), lambda: (
-            f"units must be float32 (2, {pages.shape[1]}), got {tuple(units.shape)} {units.dtype}")
-        yield units.device != pages.device or not units.is_contiguous(), lambda: (
-            f"units must be contiguous on {pages.device}")
-
-
-def _rows_rules(pages, slot_ids, k, v):
-    hkv, d = pages.shape[1], pages.shape[3] // 18
-    yield k.dim() != 3 or tuple(k.shape[1:]) != (hkv, d), lambda: (
-        f"k/v must be (n, {hkv}, {d}) for these pages, got {tuple(k.shape)} / {tuple(v.shape)}")
-    yield k.shape != v.shape, lambda: f"k/v shapes differ: {tuple(k.shape)} vs {tuple(v.shape)}"
-    yield k.dtype not in _ROW_DTYPES or v.dtype != k.dtype, lambda: (
-        f"k/v must share one dtype of fp32, fp16 or bf16, got {k.dtype} / {v.dtype}")
-    yield slot_ids.dim() != 1 or slot_ids.numel() != k.shape[0], lambda: (
-        f"slot_ids must be 1-D with one entry per token ({k.shape[0]}), got {tuple(slot_ids.shape)}")
-    yield slot_ids.dtype not in (torch.int32, torch.int64), lambda: (
-        f"slot_ids must be an integer tensor, got {slot_ids.dtype}")
-    yield any(t.device != pages.device for t in (slot_ids, k, v)), lambda: (
-        f"slot_ids, k and v must be on {pages.device}")
+def fp4_workspace(like: torch.Tensor) -> torch.Tensor:
+    """A workspace of its own for attention calls that may run beside others, on ``like``'s device:
+    zero-filled once, and left at zero by every call."""
+    return _native.require_ops().fp4_workspace(like)
 
 
 def write_slots_fp4(pages, slot_ids, k, v, *, units=None) -> None:
@@ -97,91 +68,13 @@ def write_slots_fp4(pages, slot_ids, k, v, *, units=None) -> None:
     the powers of two that K's and V's elements are counted in (``None``: 1). Values beyond
     ``6 * 448`` units saturate and NaN counts as zero.
     """
-    _require_backend()
-    _require_cuda_tensors((("pages", pages),))
-    _raise_first(_pages_rules(pages, units))
-    _raise_first(_rows_rules(pages, slot_ids, k, v))
-    if k.shape[0] == 0:
-        return
-    with _native.device_guard(pages.device):
-        _native.fp4_write_slots(pages, slot_ids.contiguous(), _unit_last_stride(k), _unit_last_stride(v), units)
+    (_native.ops or _native.require_ops()).fp4_write_slots(pages, slot_ids, k, v, units)
 
 
 def read_slots_fp4(pages, slot_ids, dtype=torch.bfloat16, *, units=None):
     """``(k, v)``, each ``(n, H_kv, D)`` in ``dtype``: the values that flat slots ``slot_ids`` hold, one
     launch. A slot outside the pool reads zeros and sets ``_native.DEVERR_APPEND_RANGE``."""
-    _require_backend()
-    _require_cuda_tensors((("pages", pages),))
-    _raise_first(_pages_rules(pages, units))
-    n, hkv, d = slot_ids.numel(), pages.shape[1], pages.shape[3] // 18
-    k, v = torch.empty((2, n, hkv, d), dtype=dtype, device=pages.device)
-    _raise_first(_rows_rules(pages, slot_ids, k, v))
-    if n:
-        with _native.device_guard(pages.device):
-            _native.fp4_read_slots(pages, slot_ids.contiguous(), k, v, units)
-    return k, v
-
-
-def _new_workspace(device) -> torch.Tensor:
-    return torch.zeros(_native.fp4_workspace_bytes(256), dtype=torch.uint8, device=device)
-
-
-def _workspace(device: torch.device, stream: int) -> torch.Tensor:
-    key = (device.index, stream)
-    ws = _WORKSPACES.get(key)
-    if ws is None:
-        ws = _new_workspace(device)
-        if torch.cuda.is_current_stream_capturing():
-            return ws  # its zero fill is a node of the graph, so it belongs to the graph alone
-        _WORKSPACES[key] = ws
-    return ws
-
-
-def _attend_rules(q, pages, block_table, rows, lengths):
-    yield q.dim() != 3, lambda: f"q must be (tokens, H, D), got shape {tuple(q.shape)}"
-    yield q.dtype not in _QUERY_DTYPES, lambda: f"q dtype must be fp16 or bf16, got {q.dtype}"
-    yield q.shape[2] * 18 != pages.shape[3], lambda: (
-        f"q head_dim {q.shape[2]} != pages head_dim {pages.shape[3] // 18}")
-    yield q.shape[1] < 1 or q.shape[1] % pages.shape[1] != 0, lambda: (
-        f"n_head ({q.shape[1]}) must be a multiple of n_kv_head ({pages.shape[1]})")
-    yield block_table.dim() != 2 or block_table.shape[0] != rows, lambda: (
-        f"block_table must be ({rows}, max_blocks), got shape {tuple(block_table.shape)}")
-    yield block_table.dtype != torch.int32, lambda: f"block_table must be int32, got {block_table.dtype}"
-    for name, t, shape in lengths:
-        yield tuple(t.shape) != shape, lambda name=name, t=t, shape=shape: (
-            f"{name} must be {shape}, got {tuple(t.shape)}")
-        yield t.dtype not in (torch.int32, torch.int64), lambda name=name, t=t: (
-            f"{name} must be int32 or int64, got {t.dtype}")
-    yield any(t.device != q.device for t in (pages, block_table, *(t for _, t, _ in lengths))), lambda: (
-        f"pages, block_table and the lengths must be on {q.device} like q")
-
-
-def _int32(t: torch.Tensor) -> torch.Tensor:
-    if t.dtype != torch.int32:
-        t = t.to(torch.int32)
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _kernel_rows(q: torch.Tensor) -> torch.Tensor:
-    """q with a unit last stride and 16-byte aligned rows (a copy where it is not so already)."""
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
-        return q if q.data_ptr() % 16 == 0 else q.clone()
-    return q
-
-
-def _kernel_table(block_table: torch.Tensor) -> torch.Tensor:
-    if block_table.shape[1] and (block_table.stride(1) != 1 or block_table.stride(0) < block_table.shape[1]):
-        return block_table.contiguous()
-    return block_table
-
-
-def _output(q, out):
-    if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {tuple(q.shape)} {q.dtype} tensor on {q.device}")
-    return out
+    return (_native.ops or _native.require_ops()).fp4_read_slots(pages, slot_ids, dtype, units)
 
 
 def paged_decode_fp4(q, pages, block_table, seqlen, *, units=None, scale: float | None = None, out=None,
@@ -190,26 +83,12 @@ def paged_decode_fp4(q, pages, block_table, seqlen, *, units=None, scale: float 
 
     ``q`` ``(B, H, D)`` fp16 or bf16; ``block_table`` int32 ``(B, max_blocks)``, of whose row ``b`` only
     the first ``ceil(seqlen[b] / block_size)`` entries matter; ``seqlen`` ``(B,)`` int32 (int64 is
-    cast). Returns ``(B, H, D)`` in ``q.dtype``. ``workspace`` (optional) is a zero-filled uint8 tensor
-    of ``_native.fp4_workspace_bytes(256)`` bytes that no concurrent launch uses; without it the
-    calls of one stream share one.
+    cast). Returns ``(B, H, D)`` in ``q.dtype``. ``workspace`` (optional) is a tensor of
+    :func:`fp4_workspace` that no concurrent launch uses; without it the calls of one stream
+    share one.
     """
-    _require_backend()
-    _require_cuda_tensors((("q", q), ("pages", pages)))
-    _raise_first(_pages_rules(pages, units))
-    batch = q.shape[0]
-    _raise_first(_attend_rules(q, pages, block_table, batch, (("seqlen", seqlen, (batch,)),)))
-    out = _output(q, out)
-    if batch == 0:
-        return out
-    if scale is None:
-        scale = 1.0 / math.sqrt(q.shape[2])
-    with _native.device_guard(q.device):
-        stream = _native.stream_handle(q.device)
-        ws = _workspace(q.device, stream) if workspace is None else workspace
-        _native.fp4_decode(_kernel_rows(q), pages, _kernel_table(block_table), _int32(seqlen), out, units,
-                           scale * _LOG2E, ws, stream)
-    return out
+    ops = _native.ops or _native.require_ops()
+    return ops.fp4_decode(q, pages, block_table, seqlen, units, scale, out, workspace)
 
 
 def paged_prefill_fp4(q, pages, block_table, cu_seqlens_q, seqlen_k, max_seqlen_q: int, *, units=None,
@@ -222,24 +101,8 @@ def paged_prefill_fp4(q, pages, block_table, cu_seqlens_q, seqlen_k, max_seqlen_
     chunk; tokens of a longer one past it are left unwritten. ``workspace`` as in
     :func:`paged_decode_fp4`.
     """
-    _require_backend()
-    _require_cuda_tensors((("q", q), ("pages", pages)))
-    _raise_first(_pages_rules(pages, units))
-    batch = seqlen_k.shape[0] if seqlen_k.dim() == 1 else -1
-    _raise_first(_attend_rules(q, pages, block_table, batch, (
-        ("seqlen_k", seqlen_k, (batch,)), ("cu_seqlens_q", cu_seqlens_q, (batch + 1,)))))
-    out = _output(q, out)
-    max_seqlen_q = int(max_seqlen_q)
-    if batch == 0 or q.shape[0] == 0 or max_seqlen_q <= 0:
-        return out
-    if scale is None:
-        scale = 1.0 / math.sqrt(q.shape[2])
-    with _native.device_guard(q.device):
-        stream = _native.stream_handle(q.device)
-        ws = _workspace(q.device, stream) if workspace is None else workspace
-        _native.fp4_prefill(_kernel_rows(q), pages, _kernel_table(block_table), _int32(cu_seqlens_q), _int32(seqlen_k),
-                            max_seqlen_q, out, units, scale * _LOG2E, ws, stream)
-    return out
+    ops = _native.ops or _native.require_ops()
+    return ops.fp4_prefill(q, pages, block_table, cu_seqlens_q, seqlen_k, max_seqlen_q, units, scale, out, workspace)
 
 
 class Fp4Pool(PagedPool):
@@ -336,8 +199,7 @@ class Fp4KV(PagedKV):
             raise TypeError(f"Fp4KV needs an Fp4Pool, got {type(pool).__name__}")
         super().__init__(pool, block_tables, lengths, rope_len=rope_len, seats=seats, n_head=n_head,
                          check_bounds=check_bounds, fuse_append=False)
-        with _native.device_guard(pool.pages[0].device):
-            self._fp4_workspace = _new_workspace(pool.pages[0].device)
+        self._fp4_workspace = fp4_workspace(pool.pages[0])
         self._scale = 1.0 / math.sqrt(self.head_dim)
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, *, rope=None) -> None:
@@ -346,10 +208,8 @@ class Fp4KV(PagedKV):
         super().write(layer, k, v)
 
     def _append_now(self, layer: int, k3: torch.Tensor, v3: torch.Tensor, rope=None) -> None:
-        with _native.device_guard(self.pool.pages[layer].device):
-            _native.fp4_write_table(self.pool.pages[layer], self._block_table_tensor, self.pos,
-                                    _unit_last_stride(k3), _unit_last_stride(v3.to(k3.dtype)),
-                                    self.pool.units[layer])
+        _native.require_ops().fp4_write_table(self.pool.pages[layer], self._block_table_tensor, self.pos, k3,
+                                              v3.to(k3.dtype), self.pool.units[layer])
 
     def attend(self, layer: int, q: torch.Tensor, *, dropout_p: float = 0.0,
                out: torch.Tensor | None = None) -> torch.Tensor:

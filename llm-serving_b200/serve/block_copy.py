@@ -10,33 +10,23 @@ from __future__ import annotations
 import torch
 
 from model import _native
-from model.triton_decode import _require_backend
 
 __all__ = ["copy_blocks"]
 
 
-def _ids(name: str, ids, device, n_blocks: int) -> torch.Tensor:
+def _ids(name: str, ids, pool: torch.Tensor) -> torch.Tensor:
+    """A device vector of block ids from Python ints (a tensor passes as it is)."""
     if isinstance(ids, torch.Tensor):
-        if ids.dim() != 1 or ids.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"{name} must be a 1-D int32 or int64 tensor, got {tuple(ids.shape)} {ids.dtype}")
-        if ids.device != device:
-            raise ValueError(f"{name} is on {ids.device} but the pools are on {device}")
-        return ids.contiguous()
+        return ids
     ids = list(ids)
     for i in ids:
         if isinstance(i, bool) or not isinstance(i, int):
             raise ValueError(f"{name} must hold ints, got {i!r}")
-        if not 0 <= i < n_blocks:
-            raise IndexError(f"{name}: block id {i} outside the pool's {n_blocks} blocks")
+        if not 0 <= i < pool.shape[0]:
+            raise IndexError(f"{name}: block id {i} outside the pool's {pool.shape[0]} blocks")
     if name == "dst" and len(set(ids)) != len(ids):
         raise ValueError("dst holds a block id twice")
-    return torch.tensor(ids, dtype=torch.int64, device=device)
-
-
-def _tensors(pools) -> list[torch.Tensor]:
-    if hasattr(pools, "block_tensors"):
-        return pools.block_tensors()
-    return [pools] if isinstance(pools, torch.Tensor) else list(pools)
+    return torch.tensor(ids, dtype=torch.int64, device=pool.device)
 
 
 def copy_blocks(pools, src, dst, *, block_table=None, remap=None) -> None:
@@ -51,36 +41,13 @@ def copy_blocks(pools, src, dst, *, block_table=None, remap=None) -> None:
     ``remap`` (int32 ``(n_blocks,)``), every table entry ``e`` inside the pool becomes ``remap[e]``
     in the same launch. Runs on the current stream.
     """
-    _require_backend()
-    tensors = _tensors(pools)
-    if not tensors:
-        raise ValueError("copy_blocks needs at least one pool")
-    first = tensors[0]
-    shape, dtype, device = first.shape, first.dtype, first.device
-    if not first.is_cuda:
-        raise RuntimeError(f"copy_blocks requires CUDA pools, got {device}; there is no CPU path.")
-    if first.dim() < 2 or first.numel() == 0:
-        raise ValueError(f"a pool needs (n_blocks, ...) elements, got {tuple(shape)}")
-    for t in tensors:
-        if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
-            raise ValueError(f"every pool must be a contiguous {tuple(shape)} {dtype} tensor on {device}")
-    n_blocks = shape[0]
-    src, dst = _ids("src", src, device, n_blocks), _ids("dst", dst, device, n_blocks)
-    if src.shape != dst.shape:
-        raise ValueError(f"src has {src.numel()} blocks and dst {dst.numel()}")
-    if src.dtype != dst.dtype:
-        src, dst = src.long(), dst.long()
-    if (block_table is None) != (remap is None):
-        raise ValueError("block_table and remap go together")
-    if block_table is not None:
-        if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.device != device:
-            raise ValueError(f"block_table must be an int32 (B, max_blocks) tensor on {device}")
-        if block_table.shape[1] > 1 and block_table.stride(1) != 1:
-            raise ValueError("block_table needs a unit column stride (it is renumbered in place)")
-        if block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]:
-            raise ValueError("block_table rows must not overlap (it is renumbered in place)")
-        if remap.dtype != torch.int32 or tuple(remap.shape) != (n_blocks,) or remap.device != device:
-            raise ValueError(f"remap must be an int32 ({n_blocks},) tensor on {device}")
-        remap = remap.contiguous()
-    with _native.device_guard(device):
-        _native.block_copy(tensors, src, dst, block_table, remap)
+    ops = _native.ops or _native.require_ops()
+    if hasattr(pools, "block_tensors"):
+        pools = pools.block_tensors()
+    elif not isinstance(pools, list):
+        pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
+    if not isinstance(src, torch.Tensor) or not isinstance(dst, torch.Tensor):
+        if not pools or not isinstance(pools[0], torch.Tensor) or pools[0].dim() == 0:
+            raise ValueError("copy_blocks needs at least one pool of (n_blocks, ...) elements")
+        src, dst = _ids("src", src, pools[0]), _ids("dst", dst, pools[0])
+    ops.block_copy(pools, src, dst, block_table, remap)
