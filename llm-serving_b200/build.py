@@ -47,6 +47,7 @@ SOURCES = [
     "pd_norm_rope.cu",
     "pd_fp4_rows.cu",
     "pd_fp4_attend.cu",
+    "pd_fp4_prefill.cu",
     "pd_block_copy.cu",
 ]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -146,6 +146,8 @@ struct Fp4AttendParams {
 // Launchers. sms: multiprocessors of the current device.
 cudaError_t launch_fp4_rows(const Fp4RowsParams& p, int dtype, bool read, bool vec, int sms, cudaStream_t stream);
 cudaError_t launch_fp4_attend(const Fp4AttendParams& p, int dtype, int head_dim, int sms, cudaStream_t stream);
+// The same for long chunks, on tcgen05 tiles (pd_fp4_prefill.cu); needs cu_q.
+cudaError_t launch_fp4_prefill(const Fp4AttendParams& p, int dtype, int head_dim, cudaStream_t stream);
 int fp4_max_rows();  // rows of one attention launch
 size_t fp4_counter_bytes(int sms);
 size_t fp4_workspace_bytes(int head_dim, int sms);

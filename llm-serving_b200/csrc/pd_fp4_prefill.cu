@@ -1,0 +1,585 @@
+// pd_fp4_prefill.cu -- causal attention of query chunks over 4-bit pages on the 5th-generation
+// tensor cores (tcgen05 / TMEM) for sm_100a: fp16 / bf16 queries, head_dim 64, 128 or 256, any group.
+//
+// The same function as pd_fp4_attend.cuh (out = softmax(q K^T scale) V over each query's visible
+// keys, fp32 softmax and accumulation) for chunks whose products outweigh the cache's bytes. A query
+// row is a (token, q head of the kv head's group) pair, token-major, so a group's heads share
+// every decoded K/V tile.
+//
+// How (one CTA = NQ blocks of 128 query rows of one row's chunk and one kv head):
+//  * 4 decoding warps turn the next KT keys of the 4-bit pages into fp16 tiles in shared memory:
+//    codes by the hardware conversion, times their scale by one packed multiply (exact: 2 by 4
+//    significant bits), stored in the 128-byte-swizzled layout the MMA reads (rows = keys, so K is
+//    K-major and V MN-major). Raw records are loaded into registers one tile ahead and block
+//    ids two, so no conversion waits on memory; units are dealt to lanes so that every 16-byte
+//    store of a quarter-warp meets eight different banks.
+//  * one thread issues the MMAs: S = Q K^T (M 128, N KT, K head_dim) into TMEM, and O += P V with P read
+//    from TMEM, where the softmax wrote it over the S it came from;
+//  * 4 softmax warps per block of query rows, one thread per row (TMEM lane = row): maximum over the
+//    row's scores, P = 2^(s - m) as fp16, and the fp32 sum; no exchange between threads. The maximum
+//    moves only when a tile passes it by 2^8, so rescaling O in TMEM is rare.
+//  With NQ = 2 the blocks alternate: while the softmax of one runs, the tensor cores do the other's
+//  P V and next S, and each decoded tile serves 256 rows. At head_dim 256 TMEM holds one block
+//  (O takes 256 of its 512 columns), which alternates between two S buffers instead.
+//  * q enters as fp16 with a power of two per row that puts its largest element near 2^13 (exact for
+//    every bf16 element within 2^-27 of the largest); P as fp16: 2^-12 relative on weights whose
+//    sum is kept unrounded, below half an ulp of the result.
+//  * Tokens past the row have P = 0, and their V is stored as zeros, so whatever bytes a page holds
+//    there never reach O.
+//  * Every wait is bounded; a role whose wait runs out records DEVERR_WAIT_TIMEOUT and raises the
+//    CTA's abort flag, every role then leaves its loop, the MMA thread waits for its MMAs and the CTA
+//    frees its TMEM and returns.
+#include "paged_decode.h"
+#include "pd_fp4.cuh"
+#include "pd_tcgen05.cuh"
+
+namespace pd {
+
+namespace {
+
+constexpr int ROWS = 128;        // query rows of a block (the MMA's M)
+constexpr float HEADROOM = 8.f;  // log2 headroom before the running maximum is moved
+
+template <int D>
+struct Cfg {
+  static constexpr int NQ = D <= 128 ? 2 : 1;     // blocks of query rows per CTA
+  static constexpr int KT = D <= 128 ? 128 : 64;  // keys per tile (the S MMA's N)
+  static constexpr int NSB = 2;                   // S/P buffers: one per block, or two of the one block
+  static constexpr int SOFTMAX_WARPS = 4 * NQ;
+  static constexpr int DECODE_WARPS = 4;
+  static constexpr int MMA_WARP = SOFTMAX_WARPS + DECODE_WARPS;
+  static constexpr int THREADS = (MMA_WARP + 1) * 32;
+  static constexpr int STAGES = 2;  // decoded tiles of K, and of V
+  static constexpr int Q_BYTES = ROWS * D * 2;
+  static constexpr int KV_BYTES = KT * D * 2;
+  static constexpr int O_COL = NSB * KT;
+  static constexpr int TMEM_COLS = 512;
+  static_assert(O_COL + NQ * D <= TMEM_COLS, "TMEM columns");
+  static constexpr int OFF_Q = 1024;  // barriers and flags before it
+  static constexpr int OFF_K = OFF_Q + NQ * Q_BYTES;
+  static constexpr int OFF_V = OFF_K + STAGES * KV_BYTES;
+  static constexpr int SMEM = OFF_V + STAGES * KV_BYTES + 1024;  // + run-time 1 KB alignment
+  static_assert(SMEM <= 232448, "shared memory per CTA");
+  // Units of 16 code bytes (32 elements): of K a token's 32 elements, of V 16 elements of two tokens.
+  static constexpr int UNITS = KT * D / 32;
+  static constexpr int PER_THREAD = UNITS / (DECODE_WARPS * 32);
+  static constexpr int PER_RECORD = D / 2;
+};
+
+// Barrier slots (8 bytes each) at the front of shared memory.
+struct Bars {
+  static constexpr int K_FULL = 0;   // [2] K tile stored: one arrival per decoding warp
+  static constexpr int V_FULL = 2;   // [2]
+  static constexpr int K_EMPTY = 4;  // [2] every S of the tile completed (commit)
+  static constexpr int V_EMPTY = 6;  // [2] every P V of the tile completed (commit)
+  static constexpr int S_FULL = 8;   // [2] S buffer written (commit)
+  static constexpr int P_FULL = 10;  // [2] P written over it, O rescaled: one arrival per softmax warp
+  static constexpr int O_DONE = 12;  // [2] P V that read the buffer completed (commit)
+  static constexpr int Q_FULL = 14;  // Q stored: one arrival per softmax warp
+  static constexpr int DRAIN = 15;
+  static constexpr int TMEM_SLOT = 160;  // byte offsets
+  static constexpr int ABORT = 168;
+};
+
+__device__ __forceinline__ bool thread_wait(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
+  if (limit_ns < TEST_LIMIT_NS) return false;
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = global_timer_ns();
+  for (unsigned it = 1;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 63u) == 0 && global_timer_ns() - t0 > limit_ns) return false;
+  }
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 16 columns of 32 bits: thread t of the warp writes lane taddr.lane + t.
+__device__ __forceinline__ void st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// Offset of 16-byte unit u of row r in a 128-byte-swizzled piece.
+__device__ __forceinline__ uint32_t sw128(int r, int u) { return uint32_t(r * 128 + ((u ^ (r & 7)) << 4)); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(const __grid_constant__ Fp4AttendParams p,
+                                                                           int blocks) {
+  using C = Cfg<D>;
+  using E = Elem<T>;
+  constexpr int REC = fp4_record_bytes(D);
+  constexpr int NQ = C::NQ, KT = C::KT;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t raw = smem_addr(smem_raw);
+  unsigned char* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  const uint32_t sbase = smem_addr(smem);
+  auto bar = [&](int slot) -> uint32_t { return sbase + uint32_t(slot) * 8u; };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Bars::ABORT);
+
+  if (warp == C::MMA_WARP) {
+    if (lane == 0) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(bar(Bars::K_FULL + i), C::DECODE_WARPS);
+        mbar_init(bar(Bars::V_FULL + i), C::DECODE_WARPS);
+        mbar_init(bar(Bars::K_EMPTY + i), 1);
+        mbar_init(bar(Bars::V_EMPTY + i), 1);
+        mbar_init(bar(Bars::S_FULL + i), 1);
+        mbar_init(bar(Bars::P_FULL + i), 4);
+        mbar_init(bar(Bars::O_DONE + i), 1);
+      }
+      mbar_init(bar(Bars::Q_FULL), C::SOFTMAX_WARPS);
+      mbar_init(bar(Bars::DRAIN), 1);
+      *abort_flag = 0;
+      fence_barrier_init();
+    }
+    __syncwarp();
+    tc::tmem_alloc(sbase + Bars::TMEM_SLOT, C::TMEM_COLS);
+    tc::tmem_relinquish();
+  }
+
+  // Query blocks slowest and last ones first: the causal tail has the most keys.
+  const int pairs = p.batch * p.n_kv_head;
+  const int b = int(blockIdx.x) % p.batch;
+  const int h = (int(blockIdx.x) / p.batch) % p.n_kv_head;
+  const int qblock = blocks - 1 - int(blockIdx.x) / pairs;
+  const int q_begin = min(max(__ldg(p.cu_q + b), 0), p.total_q);
+  const int chunk = max(min(max(__ldg(p.cu_q + b + 1), 0), p.total_q) - q_begin, 0);
+  const int sq = min(chunk, p.max_seqlen_q);
+  int lk = __ldg(p.seqlen + b);
+  lk = lk < 0 ? 0 : (lk > p.capacity ? p.capacity : lk);
+  const int rows = sq * p.group;
+  const int row0 = qblock * NQ * ROWS;  // first query row of the CTA
+  // keys that block q of the CTA needs: up to its last row's token
+  int kend[NQ], tiles[NQ], most = 0;
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const int r0 = row0 + q * ROWS;
+    const int last = min(r0 + ROWS, rows) - 1;
+    kend[q] = r0 < rows ? min(max(lk - chunk + last / p.group + 1, 0), lk) : 0;
+    tiles[q] = (kend[q] + KT - 1) / KT;
+    most = max(most, tiles[q]);
+  }
+
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + Bars::TMEM_SLOT);
+  auto k_addr = [&](int s) -> uint32_t { return sbase + uint32_t(C::OFF_K + s * C::KV_BYTES); };
+  auto v_addr = [&](int s) -> uint32_t { return sbase + uint32_t(C::OFF_V + s * C::KV_BYTES); };
+  auto fail = [&]() {
+    *abort_flag = 1;
+    atomicOr(p.err, DEVERR_WAIT_TIMEOUT);
+  };
+
+  if (row0 >= rows) {
+    // no query row
+  } else if (warp >= C::SOFTMAX_WARPS && warp < C::MMA_WARP) {
+    // ---------------------------------------------------------------- decoding warps
+    const int t = tid - C::SOFTMAX_WARPS * 32;  // 0 .. 127
+    constexpr int N = C::PER_THREAD;
+    const int32_t* trow = p.table + int64_t(b) * p.bt_stride;
+    const int tpb_mask = (1 << p.log2_tpb) - 1;
+    const int records = (lk + FP4_TILE - 1) / FP4_TILE;
+    const unsigned char* head = p.pages + (int64_t(h) << p.log2_tpb) * REC;
+    const uint32_t block_stride = uint32_t(p.n_kv_head << p.log2_tpb) * REC;
+    // Unit i of this thread is unit (i * 128 + t) of the tile: record first, so a warp reads
+    // consecutive bytes.
+    auto rec_of = [&](int tile, int i) -> int { return tile * (KT / 16) + (i * 128 + t) / C::PER_RECORD; };
+    auto block_of = [&](int tile, int i) -> int {
+      const int rec = rec_of(tile, i), page = rec >> p.log2_tpb;
+      return tile < most && rec < records && page < p.max_blocks ? __ldg(trow + page) : -1;
+    };
+    auto record_at = [&](int blk, int rec) -> const unsigned char* {
+      return blk >= 0 && blk < p.n_blocks ? head + uint64_t(blk) * block_stride + (rec & tpb_mask) * REC : nullptr;
+    };
+    const int u = t % C::PER_RECORD;  // unit inside a record (128 is a multiple of PER_RECORD)
+    // K unit: 16 bytes at 16 u of the record's codes, i.e. 32 elements of one token
+    constexpr int W = D < 128 ? D : 128, CH = W / 32;  // 16-byte chunks of a token in a block
+    const int k_blk = u / (16 * CH), k_tok = (u / CH) % 16, k_ch = u % CH;
+    const int k_el = k_blk * W + k_ch * 32;  // first element
+    const int k_scale_off = 8 * D + k_blk * W + k_tok * (W / 16) + k_ch * 2;
+    // V unit: 16 bytes at 16 u of the V codes: group v_gr of tokens v_tok, v_tok + 1
+    const int v_half = u / (D / 4), v_gr = (u / 4) % (D / 16), v_tok = v_half * 8 + (u % 4) * 2;
+    const int v_scale_off = 17 * D + v_half * (D / 2) + v_gr * 8 + (u % 4) * 2;
+
+    uint4 kraw[N], vraw[N];
+    uint32_t ksc[N], vsc[N];
+    int blk[N], blk_next[N];
+    auto load = [&](const int (&ids)[N], int tile, uint4 (&code)[N], uint32_t (&scale)[N], int code_off, int scale_off) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const unsigned char* r = record_at(ids[i], rec_of(tile, i));
+        code[i] = make_uint4(0u, 0u, 0u, 0u);
+        scale[i] = 0u;
+        if (r != nullptr) {
+          code[i] = __ldg(reinterpret_cast<const uint4*>(r + code_off));
+          scale[i] = __ldg(reinterpret_cast<const uint16_t*>(r + scale_off));
+        }
+      }
+    };
+    const int k_code_off = 16 * u, v_code_off = 9 * D + 16 * u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) blk[i] = block_of(0, i);
+    load(blk, 0, kraw, ksc, k_code_off, k_scale_off);
+    load(blk, 0, vraw, vsc, v_code_off, v_scale_off);
+#pragma unroll
+    for (int i = 0; i < N; ++i) blk[i] = block_of(1, i);
+    bool ok = true;
+    for (int j = 0; ok && j < most; ++j) {
+      if (__any_sync(FULL_MASK, *abort_flag != 0)) break;
+      const int s = j & 1;
+#pragma unroll
+      for (int i = 0; i < N; ++i) blk_next[i] = block_of(j + 2, i);
+      if (j >= 2 && !warp_wait_phase(bar(Bars::K_EMPTY + s), uint32_t((j / 2 - 1) & 1), p.wait_ns)) {
+        ok = false;
+        break;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int row = ((i * 128 + t) / C::PER_RECORD) * 16 + k_tok;
+        const uint32_t pair = e4m3x2_to_half2(ksc[i]);
+        const uint32_t s0 = __byte_perm(pair, 0, 0x1010), s1 = __byte_perm(pair, 0, 0x3232);
+        const uint32_t w[4] = {kraw[i].x, kraw[i].y, kraw[i].z, kraw[i].w};
+        const uint32_t piece = k_addr(s) + uint32_t((k_el >> 6) * (KT * 128));
+        const int u0 = (k_el & 63) >> 3;
+        // a quarter-warp's lanes are two tokens x four chunks (or four x two): rotating the order
+        // by the piece and the token makes their eight units different
+        const int turn = ((k_el >> 6) & 1) ^ ((k_tok & 1) << 1);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int e = q ^ turn;
+          uint32_t x[4];
+          const uint32_t word = e & 2 ? (e & 1 ? w[3] : w[2]) : (e & 1 ? w[1] : w[0]);
+          e2m1x8_to_half2x4(word, x);
+          const uint32_t sc = e & 2 ? s1 : s0;
+          sts128(piece + sw128(row, u0 + e), hmul2_bits(x[0], sc), hmul2_bits(x[1], sc), hmul2_bits(x[2], sc),
+                 hmul2_bits(x[3], sc));
+        }
+      }
+      load(blk, j + 1, kraw, ksc, k_code_off, k_scale_off);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(Bars::K_FULL + s));
+      if (j >= 2 && !warp_wait_phase(bar(Bars::V_EMPTY + s), uint32_t((j / 2 - 1) & 1), p.wait_ns)) {
+        ok = false;
+        break;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int row = ((i * 128 + t) / C::PER_RECORD) * 16 + v_tok;
+        const int key = j * KT + row;
+        uint32_t sc = e4m3x2_to_half2(vsc[i]);
+        sc &= (key < lk ? 0x0000ffffu : 0u) | (key + 1 < lk ? 0xffff0000u : 0u);  // zeros past the row
+        const uint32_t w[4] = {vraw[i].x, vraw[i].y, vraw[i].z, vraw[i].w};
+        const uint32_t piece = v_addr(s) + uint32_t((v_gr >> 2) * (KT * 128));
+        const int u0 = (v_gr & 3) * 2;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int e = q ^ (v_gr & 1);  // odd groups write their second unit first: no bank twice
+          const uint32_t word = e & 2 ? (e & 1 ? w[3] : w[2]) : (e & 1 ? w[1] : w[0]);
+          uint32_t x[4];
+          e2m1x8_to_half2x4(word, x);
+          const uint32_t f = e & 2 ? __byte_perm(sc, 0, 0x3232) : __byte_perm(sc, 0, 0x1010);
+          sts128(piece + sw128(row + (e >> 1), u0 + (e & 1)), hmul2_bits(x[0], f), hmul2_bits(x[1], f),
+                 hmul2_bits(x[2], f), hmul2_bits(x[3], f));
+        }
+      }
+      load(blk, j + 1, vraw, vsc, v_code_off, v_scale_off);
+#pragma unroll
+      for (int i = 0; i < N; ++i) blk[i] = blk_next[i];
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(Bars::V_FULL + s));
+    }
+    if (!ok && lane == 0) fail();
+  } else if (warp == C::MMA_WARP) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (lane == 0 && most > 0) {
+      constexpr uint32_t IDESC_S = tc::instr_desc_f16(false, ROWS, KT, false, false);
+      constexpr uint32_t IDESC_PV = tc::instr_desc_f16(false, ROWS, D, false, true);
+      bool ok = thread_wait(bar(Bars::Q_FULL), 0u, p.wait_ns);
+      const uint64_t q_desc = tc::smem_desc(sbase + C::OFF_Q, 16u, 1024u);
+      const uint64_t k_desc = tc::smem_desc(k_addr(0), 16u, 1024u);
+      const uint64_t v_desc = tc::smem_desc(v_addr(0), uint32_t(KT * 128), 1024u);
+      // S/P buffer of (block q, tile j) and the phase of that use on the buffer's barriers
+      auto buf = [&](int q, int j) -> int { return NQ == 2 ? q : j & 1; };
+      auto use = [&](int j) -> uint32_t { return NQ == 2 ? uint32_t(j) : uint32_t(j >> 1); };
+      // S of (q, j), once P V of the buffer's previous use has read its P
+      auto issue_s = [&](int q, int j) -> bool {
+        const int s = j & 1, sb = buf(q, j);
+        if (!thread_wait(bar(Bars::K_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns)) return false;
+        if (use(j) > 0 && !thread_wait(bar(Bars::O_DONE + sb), (use(j) - 1) & 1u, p.wait_ns)) return false;
+        tc::fence_after_sync();
+        const uint64_t a0 = q_desc + uint64_t((q * C::Q_BYTES) >> 4), b0 = k_desc + uint64_t((s * C::KV_BYTES) >> 4);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks)
+          tc::mma_f16_ss(tmem + uint32_t(sb * KT), a0 + uint64_t(((ks >> 2) * (ROWS * 128) + (ks & 3) * 32) >> 4),
+                         b0 + uint64_t(((ks >> 2) * (KT * 128) + (ks & 3) * 32) >> 4), IDESC_S, ks > 0);
+        tc::commit(bar(Bars::S_FULL + sb));
+        // the last block that uses this K tile frees it
+        if (q == NQ - 1 || j >= tiles[NQ - 1]) tc::commit(bar(Bars::K_EMPTY + s));
+        return true;
+      };
+      auto issue_pv = [&](int q, int j) -> bool {
+        const int s = j & 1, sb = buf(q, j);
+        if (!thread_wait(bar(Bars::P_FULL + sb), use(j) & 1u, p.wait_ns) ||
+            !thread_wait(bar(Bars::V_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns))
+          return false;
+        tc::fence_after_sync();
+        const uint64_t b0 = v_desc + uint64_t((s * C::KV_BYTES) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < KT / 16; ++kk)
+          tc::mma_f16_ts(tmem + uint32_t(C::O_COL + q * D), tmem + uint32_t(sb * KT + kk * 8),
+                         b0 + uint64_t((kk * 2048) >> 4), IDESC_PV, j > 0 || kk > 0);
+        tc::commit(bar(Bars::O_DONE + sb));
+        if (q == NQ - 1 || j >= tiles[NQ - 1]) tc::commit(bar(Bars::V_EMPTY + s));
+        return true;
+      };
+      if (NQ == 2) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+          if (ok && tiles[q] > 0) ok = issue_s(q, 0);
+        for (int j = 0; ok && j < most; ++j) {
+          if (*abort_flag) break;
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            if (ok && j < tiles[q]) ok = issue_pv(q, j);
+            if (ok && j + 1 < tiles[q]) ok = issue_s(q, j + 1);
+          }
+        }
+      } else {
+        if (ok) ok = issue_s(0, 0);
+        for (int j = 0; ok && j < most; ++j) {
+          if (*abort_flag) break;
+          if (j + 1 < most) ok = issue_s(0, j + 1);
+          if (ok) ok = issue_pv(0, j);
+        }
+      }
+      if (!ok) fail();
+      tc::commit(bar(Bars::DRAIN));  // never leave with an MMA in flight
+      thread_wait(bar(Bars::DRAIN), 0u, DRAIN_LIMIT_NS);
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax warps
+    const int q = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;  // row of the block = TMEM lane
+    const int n = row0 + q * ROWS + r;
+    const bool live = n < rows;
+    const int tok = live ? n / p.group : 0, hg = live ? n - tok * p.group : 0;
+    const int64_t hq = int64_t(h) * p.group + hg;
+    float down;  // 1 / the row's power of two
+    {
+      const T* src = reinterpret_cast<const T*>(p.q) + int64_t(q_begin + tok) * p.q_st + hq * p.q_sh;
+      float top = 0.f;
+      if (live) {
+#pragma unroll 4
+        for (int u = 0; u < D / 8; ++u) {
+          float x[8];
+          E::unpack(__ldg(reinterpret_cast<const uint4*>(src) + u), x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+        }
+      }
+      int e = int(__float_as_uint(top) >> 23);
+      e = e == 0 || e == 255 ? 140 : e;
+      const int shift = max(-100, min(100, 140 - e));
+      // a negative scale's sign goes into q, so that the score multiplier is never negative
+      const float up = copysignf(__uint_as_float(uint32_t(127 + shift) << 23), p.scale_log2);
+      down = __uint_as_float(uint32_t(127 - shift) << 23);
+#pragma unroll 4
+      for (int u = 0; u < D / 8; ++u) {
+        float x[8];
+        E::unpack(live ? __ldg(reinterpret_cast<const uint4*>(src) + u) : make_uint4(0u, 0u, 0u, 0u), x);
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = Elem<__half>::pack2(x[2 * i] * up, x[2 * i + 1] * up);
+        sts128(sbase + C::OFF_Q + uint32_t(q * C::Q_BYTES + (u >> 3) * (ROWS * 128)) + sw128(r, u & 7), w[0], w[1], w[2],
+               w[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(Bars::Q_FULL));
+    }
+    const float mul = fabsf(p.scale_log2) * (p.units != nullptr ? __ldg(p.units + h) : 1.f) * down;
+    const int lim = live ? lk - chunk + tok : lk - 1;  // last visible key; padding rows see any
+    const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t o_tmem = lane_base + uint32_t(C::O_COL + q * D);
+    float m_run = -3.0e38f, l_run = 0.f;
+    bool ok = true;
+    int mine = tiles[0];
+#pragma unroll
+    for (int i = 1; i < NQ; ++i) mine = q == i ? tiles[i] : mine;
+    for (int j = 0; j < mine; ++j) {
+      const int sb = NQ == 2 ? q : j & 1;
+      const uint32_t ph = (NQ == 2 ? uint32_t(j) : uint32_t(j >> 1)) & 1u;
+      if (__any_sync(FULL_MASK, *abort_flag != 0) || !warp_wait_phase(bar(Bars::S_FULL + sb), ph, p.wait_ns)) {
+        ok = false;
+        break;
+      }
+      tc::fence_after_sync();
+      const uint32_t s_tmem = lane_base + uint32_t(sb * KT);
+      const bool open = __all_sync(FULL_MASK, j * KT + KT - 1 <= lim);  // no key of the tile is hidden
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+      for (int c = 0; c < KT; c += 32) {
+        uint32_t x[32];
+        tc::ld_32x32b_x32(s_tmem + uint32_t(c), x);
+        tc::wait_ld();
+        if (open) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            top[i & 3] = fmaxf(top[i & 3], j * KT + c + i <= lim ? __uint_as_float(x[i]) : -INFINITY);
+        }
+      }
+      // mul > 0: the maximum of the products is the product of the maximum
+      const float tmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mul;
+      const bool move = tmax > m_run + HEADROOM || (m_run < -1.0e38f && tmax > m_run);
+      if (__any_sync(FULL_MASK, move)) {
+        const float alpha = move ? ex2(m_run - tmax) : 1.f;
+        if (move) m_run = tmax;
+        l_run *= alpha;
+        if (j > 0) {  // O *= alpha once P V of tile j - 1 has landed
+          const int pb = NQ == 2 ? q : (j - 1) & 1;
+          const uint32_t pp = (NQ == 2 ? uint32_t(j - 1) : uint32_t((j - 1) >> 1)) & 1u;
+          if (!warp_wait_phase(bar(Bars::O_DONE + pb), pp, p.wait_ns)) {
+            ok = false;
+            break;
+          }
+          tc::fence_after_sync();
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tc::ld_32x32b_x32(o_tmem + uint32_t(c), o);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tc::st_32x32b_x32(o_tmem + uint32_t(c), o);
+          }
+        }
+      }
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int c = 0; c < KT; c += 32) {
+        uint32_t x[32], w[16];
+        tc::ld_32x32b_x32(s_tmem + uint32_t(c), x);
+        tc::wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float a = fmaf(__uint_as_float(x[i]), mul, -m_run), d = fmaf(__uint_as_float(x[i + 1]), mul, -m_run);
+          if (!open) {
+            a = j * KT + c + i <= lim ? a : -INFINITY;
+            d = j * KT + c + i + 1 <= lim ? d : -INFINITY;
+          }
+          a = ex2(a);
+          d = ex2(d);
+          sum[(i >> 1) & 3] += a + d;
+          w[i >> 1] = Elem<__half>::pack2(a, d);
+        }
+        // 32 keys of P take 16 columns, all of them columns whose scores are already read
+        st_32x32b_x16(s_tmem + uint32_t(c / 2), w);
+      }
+      l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tc::wait_st();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(Bars::P_FULL + sb));
+    }
+    if (ok && mine > 0) {
+      const int lb = NQ == 2 ? q : (mine - 1) & 1;
+      const uint32_t lp = (NQ == 2 ? uint32_t(mine - 1) : uint32_t((mine - 1) >> 1)) & 1u;
+      ok = warp_wait_phase(bar(Bars::O_DONE + lb), lp, p.wait_ns);
+    }
+    if (!ok) {
+      if (lane == 0) fail();
+    } else {
+      tc::fence_after_sync();
+      const float unit = p.units != nullptr ? __ldg(p.units + p.n_kv_head + h) : 1.f;
+      const float inv = l_run > 0.f ? unit / l_run : 0.f;
+      T* dst = reinterpret_cast<T*>(p.out) + int64_t(q_begin + tok) * p.o_st + hq * p.o_sh;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        if (mine > 0) {
+          tc::ld_32x32b_x32(o_tmem + uint32_t(c), o);
+          tc::wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+        if (live) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = E::pack2(__uint_as_float(o[8 * u + 2 * i]) * inv, __uint_as_float(o[8 * u + 2 * i + 1]) * inv);
+            *reinterpret_cast<uint4*>(dst + c + 8 * u) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+    }
+  }
+
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == C::MMA_WARP) {
+    __syncwarp();
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+template <typename T, int D>
+cudaError_t launch_t(const Fp4AttendParams& p, cudaStream_t stream) {
+  using C = Cfg<D>;
+  auto fn = pd_fp4_prefill_kernel<T, D>;
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev >= 64 || !attr_set[dev]) {
+    err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (err != cudaSuccess) return err;
+    if (dev < 64) attr_set[dev] = true;
+  }
+  const int64_t rows = int64_t(p.max_seqlen_q) * p.group;
+  const int64_t blocks = (rows + C::NQ * ROWS - 1) / (C::NQ * ROWS);
+  const int64_t ctas = blocks * p.batch * p.n_kv_head;
+  if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+  fn<<<dim3(unsigned(ctas)), C::THREADS, C::SMEM, stream>>>(p, int(blocks));
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_d(const Fp4AttendParams& p, int head_dim, cudaStream_t stream) {
+  switch (head_dim) {
+    case 64: return launch_t<T, 64>(p, stream);
+    case 128: return launch_t<T, 128>(p, stream);
+    case 256: return launch_t<T, 256>(p, stream);
+  }
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+cudaError_t launch_fp4_prefill(const Fp4AttendParams& p, int dtype, int head_dim, cudaStream_t stream) {
+  return dtype == PD_BF16 ? launch_d<__nv_bfloat16>(p, head_dim, stream) : launch_d<__half>(p, head_dim, stream);
+}
+
+}  // namespace pd

@@ -55,6 +55,20 @@ int rows_common(Fp4RowsParams& p, int dtype, bool read, const int64_t* k_strides
                   read ? "4-bit read launch" : "4-bit write launch");
 }
 
+// Whether a chunk call runs on tcgen05 tiles. Per visible key, the warp kernel's time goes with the
+// 8-column units of query rows over the SMs (about A clocks for each at 32 keys), the tile
+// kernel's with the waves of its CTAs, one block of 256 (at head_dim 256: 128) query rows each
+// (about B clocks at 128 keys). Lengths stay on the device, but both times are proportional to
+// them, so the comparison needs only the counts the host has.
+bool use_tiles(int64_t total_q, int32_t max_seqlen_q, int32_t batch, int32_t n_kv_head, int32_t group,
+               int32_t head_dim, int sms) {
+  constexpr double A = 260.0 / 32, B = 2600.0 / 128;
+  const double units = double(n_kv_head) * (double(total_q) * group / 8 + 0.5 * batch);
+  const int64_t block = head_dim == 256 ? 128 : 256;
+  const int64_t ctas = int64_t(batch) * n_kv_head * ((int64_t(max_seqlen_q) * group + block - 1) / block);
+  return double((ctas + sms - 1) / sms) * B < units / sms * A;
+}
+
 int attend_common(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, const void* pages, int64_t n_blocks, int32_t block_size,
                   const float* units, const int32_t* block_table, int64_t bt_stride, int32_t max_blocks,
                   const int32_t* cu_q, int32_t max_seqlen_q, const int32_t* seqlen, void* out, int64_t o_st,
@@ -100,6 +114,7 @@ int attend_common(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, co
   p.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + fp4_counter_bytes(sms));
   p.err = err;
   p.wait_ns = api_wait_limit_ns();
+  const bool tiles = cu_q != nullptr && use_tiles(total_q, max_seqlen_q, batch, n_kv_head, p.group, head_dim, sms);
   for (int b0 = 0; b0 < batch; b0 += fp4_max_rows()) {
     p.batch = batch - b0 < fp4_max_rows() ? batch - b0 : fp4_max_rows();
     // a chunk's offsets are absolute, a decode step's row b is q row b
@@ -109,7 +124,8 @@ int attend_common(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, co
     p.cu_q = cu_q != nullptr ? cu_q + b0 : nullptr;
     p.seqlen = seqlen + b0;
     p.table = block_table != nullptr ? block_table + int64_t(b0) * bt_stride : nullptr;
-    st = launched(launch_fp4_attend(p, dtype, head_dim, sms, static_cast<cudaStream_t>(stream)),
+    const cudaStream_t on = static_cast<cudaStream_t>(stream);
+    st = launched(tiles ? launch_fp4_prefill(p, dtype, head_dim, on) : launch_fp4_attend(p, dtype, head_dim, sms, on),
                   "4-bit attention launch");
     if (st != PD_OK) return st;
   }
