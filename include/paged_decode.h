@@ -427,6 +427,12 @@ int pd_get_decode_mode(int32_t* mode, int32_t* shared_stages, int32_t* row_cost)
 int pd_set_prefill_mode(int32_t mode);
 int pd_get_prefill_mode(void);
 
+/* Kernel of pd_fp4_prefill for calls made afterwards: mode 0 (default) chooses by the counts of
+ * rows, query tokens and heads, 1 runs the warp-level mma.sync kernel (pd_fp4_decode's), 2 the
+ * tcgen05 tiles. All compute the same function; results agree within rounding. */
+int pd_set_fp4_prefill_mode(int32_t mode);
+int pd_get_fp4_prefill_mode(void);
+
 /* Time limit, in nanoseconds, of the kernels' waits on a pipeline stage (mbarrier) or on a
  * split item's arrival counter, for launches made afterwards (default 1 s; 0 restores it;
  * at most 10 s). A wait that runs out records PD_DEVERR_WAIT_TIMEOUT in the device error word,

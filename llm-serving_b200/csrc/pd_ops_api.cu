@@ -1,5 +1,7 @@
 // pd_ops_api.cu -- the extern "C" boundary of the head norm with rotation, the 4-bit pages and the
 // page copies (declared in include/paged_decode.h): argument checks on the host, then the launch.
+#include <atomic>
+
 #include "paged_decode.h"
 #include "pd_api_internal.h"
 #include "pd_block_copy.cuh"
@@ -9,6 +11,9 @@
 namespace pd {
 
 namespace {
+
+// Kernel of pd_fp4_prefill: 0 chooses, 1 warp kernel, 2 tcgen05 tiles.
+std::atomic<int> g_fp4_prefill_mode{0};
 
 bool valid_dtype(int dtype) { return dtype == PD_F32 || dtype == PD_F16 || dtype == PD_BF16; }
 int elem_size(int dtype) { return dtype == PD_F32 ? 4 : 2; }
@@ -114,7 +119,9 @@ int attend_common(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, co
   p.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + fp4_counter_bytes(sms));
   p.err = err;
   p.wait_ns = api_wait_limit_ns();
-  const bool tiles = cu_q != nullptr && use_tiles(total_q, max_seqlen_q, batch, n_kv_head, p.group, head_dim, sms);
+  const int mode = g_fp4_prefill_mode.load(std::memory_order_relaxed);
+  const bool tiles = cu_q != nullptr && (mode == 2 || (mode == 0 && use_tiles(total_q, max_seqlen_q, batch, n_kv_head,
+                                                                             p.group, head_dim, sms)));
   for (int b0 = 0; b0 < batch; b0 += fp4_max_rows()) {
     p.batch = batch - b0 < fp4_max_rows() ? batch - b0 : fp4_max_rows();
     // a chunk's offsets are absolute, a decode step's row b is q row b
@@ -285,6 +292,14 @@ int pd_fp4_prefill(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, c
                        cu_seqlens_q, max_seqlen_q, seqlen_k, out, o_st, o_sh, batch, n_head, n_kv_head, head_dim,
                        dtype, scale_log2, workspace, workspace_bytes, stream);
 }
+
+int pd_set_fp4_prefill_mode(int32_t mode) {
+  if (mode < 0 || mode > 2) return PD_ERR_INVALID;
+  g_fp4_prefill_mode.store(mode, std::memory_order_relaxed);
+  return PD_OK;
+}
+
+int pd_get_fp4_prefill_mode(void) { return g_fp4_prefill_mode.load(std::memory_order_relaxed); }
 
 int pd_block_copy(void* const* pools, int32_t n_pools, int64_t n_blocks, int64_t block_bytes, const void* src,
                   const void* dst, int32_t id_dtype, int64_t n_pairs, int32_t* block_table, int64_t table_rows,

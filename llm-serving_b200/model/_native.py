@@ -144,6 +144,8 @@ _SIGNATURES = {
          _c_ptr, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_float, _c_ptr, _c_size,
          _c_ptr],
     ),
+    "pd_set_fp4_prefill_mode": (ctypes.c_int, [_c_i32]),
+    "pd_get_fp4_prefill_mode": (ctypes.c_int, []),
     "pd_block_copy": (
         ctypes.c_int,
         [ctypes.POINTER(_c_ptr), _c_i32, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i32, _c_i64, _c_ptr, _c_i64,
@@ -297,6 +299,15 @@ def set_prefill_mode(mode: int) -> None:
 
 def get_prefill_mode() -> int:
     return int(require().pd_get_prefill_mode())
+
+
+def set_fp4_prefill_mode(mode: int) -> None:
+    """Kernel of chunks over 4-bit pages. 0: by the counts (default); 1: warp kernel; 2: tcgen05 tiles."""
+    check(require().pd_set_fp4_prefill_mode(int(mode)), "pd_set_fp4_prefill_mode")
+
+
+def get_fp4_prefill_mode() -> int:
+    return int(require().pd_get_fp4_prefill_mode())
 
 
 def set_wait_limit(limit_ns: int) -> None:
