@@ -76,14 +76,17 @@ __device__ __forceinline__ uint32_t float_to_e4m3(float x) {
   return uint32_t(r) & 0xffu;
 }
 
-// Two fp32 -> one code byte (a in the low nibble), to nearest even, saturating at 6.
-__device__ __forceinline__ uint32_t floats_to_e2m1x2(float a, float b) {
+// Eight fp32 -> four code bytes (lower element in the low nibble), to nearest even, saturating at 6.
+__device__ __forceinline__ uint32_t floats_to_e2m1x8(const float* f) {
   uint32_t r;
-  asm("{\n\t.reg .b8 t;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\t"
-      "cvt.u32.u8 %0, t;\n\t}"
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
       : "=r"(r)
-      : "f"(b), "f"(a));
+      : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
   return r;
 }
 

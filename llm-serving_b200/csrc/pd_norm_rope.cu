@@ -22,27 +22,29 @@ namespace {
 
 constexpr int NORM_HEADS = 4;  // heads in flight per lane group
 
-// 4 consecutive elements as fp32.
+// 4 consecutive elements as they are in memory: 8 bytes of 16-bit types, 16 of fp32.
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, float (&f)[4]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(p);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-  } else {
-    const uint2 r = *reinterpret_cast<const uint2*>(p);
+struct Four {
+  using Raw = uint2;
+  __device__ __forceinline__ static void unpack(const Raw& r, float (&f)[4]) {
     Elem<T>::unpack2(r.x, f);
     Elem<T>::unpack2(r.y, f + 2);
   }
-}
-
-template <typename T>
-__device__ __forceinline__ void store4(T* p, const float (&f)[4]) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-  } else {
-    *reinterpret_cast<uint2*>(p) = make_uint2(Elem<T>::pack2(f[0], f[1]), Elem<T>::pack2(f[2], f[3]));
+  __device__ __forceinline__ static Raw pack(const float (&f)[4]) {
+    return make_uint2(Elem<T>::pack2(f[0], f[1]), Elem<T>::pack2(f[2], f[3]));
   }
-}
+};
+template <>
+struct Four<float> {
+  using Raw = float4;
+  __device__ __forceinline__ static void unpack(const Raw& r, float (&f)[4]) {
+    f[0] = r.x;
+    f[1] = r.y;
+    f[2] = r.z;
+    f[3] = r.w;
+  }
+  __device__ __forceinline__ static Raw pack(const float (&f)[4]) { return make_float4(f[0], f[1], f[2], f[3]); }
+};
 
 __device__ __forceinline__ int64_t position_of(const NormRopeParams& p, int64_t t) {
   if (p.pos == nullptr) return t;
@@ -52,15 +54,19 @@ __device__ __forceinline__ int64_t position_of(const NormRopeParams& p, int64_t 
 
 // LANES = D / 8 lanes per head (8, 16 or 32). Lane l of a head holds elements e0 .. e0 + 3 and
 // e1 .. e1 + 3: a rotary pair block while 4 l < R / 2, two blocks of the passed-through rest after.
+// What is loaded stays packed until its head's turn: four heads in flight then cost 16 registers.
 template <typename T, int LANES>
-__global__ void __launch_bounds__(256) pd_norm_rope_kernel(const NormRopeParams p) {
+__global__ void __launch_bounds__(256, 4) pd_norm_rope_kernel(const NormRopeParams p) {
   constexpr int D = LANES * 8;
   constexpr int GROUPS = 32 / LANES;  // heads of a warp at once
+  using F = Four<T>;
+  using Raw = typename F::Raw;
   const int lane = threadIdx.x & 31;
   const int l = lane % LANES, grp = lane / LANES;
-  const int heads = p.n_head + p.n_kv_head;
-  const int per_warp = GROUPS * NORM_HEADS;
-  const int chunks = (heads + per_warp - 1) / per_warp;
+  constexpr int PER_WARP = GROUPS * NORM_HEADS;
+  // an item is a token and PER_WARP of its q heads, or of its k heads
+  const uint32_t q_chunks = (p.n_head + PER_WARP - 1) / PER_WARP, k_chunks = (p.n_kv_head + PER_WARP - 1) / PER_WARP;
+  const uint32_t chunks = q_chunks + k_chunks;
   const int64_t items = p.n_tokens * chunks;
   const int half = p.rotary_dim >> 1;
   const bool rot = 4 * l < half;
@@ -68,56 +74,70 @@ __global__ void __launch_bounds__(256) pd_norm_rope_kernel(const NormRopeParams 
   const int e1 = rot ? half + 4 * l : e0 + 4;
   for (int64_t it = int64_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); it < items;
        it += int64_t(gridDim.x) * (blockDim.x >> 5)) {
-    const int64_t t = it / chunks;
-    const int h0 = int(it - t * chunks) * per_warp + grp;
-    float a[NORM_HEADS][4], b[NORM_HEADS][4];
-#pragma unroll
-    for (int j = 0; j < NORM_HEADS; ++j) {
-      const int h = h0 + j * GROUPS;
-      if (h < heads) {
-        const T* x = h < p.n_head ? reinterpret_cast<const T*>(p.q) + t * p.q_st + h * p.q_sh
-                                  : reinterpret_cast<const T*>(p.k) + t * p.k_st + (h - p.n_head) * p.k_sh;
-        load4(x + e0, a[j]);
-        load4(x + e1, b[j]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[j][i] = b[j][i] = 0.f;
-      }
-    }
+    const int64_t t = it < 0x7fffffff ? int64_t(uint32_t(it) / chunks) : it / chunks;
+    const uint32_t ch = uint32_t(it - t * chunks);
     const int64_t pos = position_of(p, t);
-    const bool in_range = pos >= 0 && pos < p.n_pos;
-    float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (rot && in_range) {
-      load4(reinterpret_cast<const T*>(p.cos) + pos * p.cos_st + 4 * l, c);
-      load4(reinterpret_cast<const T*>(p.sin) + pos * p.sin_st + 4 * l, s);
-    }
-    if (!in_range && lane == 0) atomicOr(p.err, DEVERR_ROPE_RANGE);
+    const bool is_q = ch < q_chunks;
+    const int h0 = int(is_q ? ch : ch - q_chunks) * PER_WARP + grp;
+    const int heads = is_q ? p.n_head : p.n_kv_head;
+    const int64_t sh = (is_q ? p.q_sh : p.k_sh), so = (is_q ? p.qo_sh : p.ko_sh);
+    const T* x = (is_q ? reinterpret_cast<const T*>(p.q) + t * p.q_st : reinterpret_cast<const T*>(p.k) + t * p.k_st) +
+                 h0 * sh;
+    T* y = (is_q ? reinterpret_cast<T*>(p.q_out) + t * p.qo_st : reinterpret_cast<T*>(p.k_out) + t * p.ko_st) + h0 * so;
+    Raw a[NORM_HEADS], b[NORM_HEADS];
 #pragma unroll
     for (int j = 0; j < NORM_HEADS; ++j) {
-      const int h = h0 + j * GROUPS;
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ss = fmaf(a[j][i], a[j][i], fmaf(b[j][i], b[j][i], ss));
-#pragma unroll
-      for (int o = LANES / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(FULL_MASK, ss, o);
-      // 1 / sqrt rather than the approximate rsqrt: fp32 rows then keep fp32's accuracy
-      const float inv = in_range ? 1.f / sqrtf(ss * (1.f / D) + p.eps) : 0.f;
-      if (h >= heads) continue;
-      const bool is_q = h < p.n_head;
+      a[j] = b[j] = Raw{};
+      if (h0 + j * GROUPS < heads) {
+        a[j] = __ldcs(reinterpret_cast<const Raw*>(x + e0));
+        b[j] = __ldcs(reinterpret_cast<const Raw*>(x + e1));
+      }
+      x += GROUPS * sh;
+    }
+    const bool in_range = pos >= 0 && pos < p.n_pos;
+    if (!in_range && lane == 0) atomicOr(p.err, DEVERR_ROPE_RANGE);
+    // out_a = inv (x_a w_a cos - x_b w_b sin), out_b = inv (x_a w_a sin + x_b w_b cos): the four
+    // products of weight and angle are the item's, not the head's
+    float ac[4], as[4], bc[4], bs[4];
+    {
       const T* w = reinterpret_cast<const T*>(is_q ? p.wq : p.wk);
-      float wa[4], wb[4], oa[4], ob[4];
-      load4(w + e0, wa);
-      load4(w + e1, wb);
+      float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f}, wa[4], wb[4];
+      F::unpack(__ldg(reinterpret_cast<const Raw*>(w + e0)), wa);
+      F::unpack(__ldg(reinterpret_cast<const Raw*>(w + e1)), wb);
+      if (rot && in_range) {
+        F::unpack(__ldg(reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(p.cos) + pos * p.cos_st + 4 * l)), c);
+        F::unpack(__ldg(reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(p.sin) + pos * p.sin_st + 4 * l)), s);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float ya = a[j][i] * inv * wa[i], yb = b[j][i] * inv * wb[i];
-        oa[i] = rot ? ya * c[i] - yb * s[i] : ya;
-        ob[i] = rot ? ya * s[i] + yb * c[i] : yb;
+        ac[i] = wa[i] * c[i];
+        as[i] = wa[i] * s[i];
+        bc[i] = wb[i] * c[i];
+        bs[i] = wb[i] * s[i];
       }
-      T* y = is_q ? reinterpret_cast<T*>(p.q_out) + t * p.qo_st + h * p.qo_sh
-                  : reinterpret_cast<T*>(p.k_out) + t * p.ko_st + (h - p.n_head) * p.ko_sh;
-      store4(y + e0, oa);
-      store4(y + e1, ob);
+    }
+#pragma unroll
+    for (int j = 0; j < NORM_HEADS; ++j) {
+      float xa[4], xb[4];
+      F::unpack(a[j], xa);
+      F::unpack(b[j], xb);
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ss = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], ss));
+#pragma unroll
+      for (int o = LANES / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(FULL_MASK, ss, o);
+      const float inv = in_range ? rsqrtf(ss * (1.f / D) + p.eps) : 0.f;  // 2 ulp
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float u = (xa[i] * ac[i] - xb[i] * bs[i]) * inv;
+        xb[i] = (xa[i] * as[i] + xb[i] * bc[i]) * inv;
+        xa[i] = u;
+      }
+      if (h0 + j * GROUPS < heads) {
+        *reinterpret_cast<Raw*>(y + e0) = F::pack(xa);
+        *reinterpret_cast<Raw*>(y + e1) = F::pack(xb);
+      }
+      y += GROUPS * so;
     }
   }
 }
@@ -158,7 +178,7 @@ __global__ void __launch_bounds__(256) pd_norm_rope_any_kernel(const NormRopePar
     const int64_t pos = position_of(p, t);
     const bool in_range = pos >= 0 && pos < p.n_pos;
     if (!in_range && lane == 0) atomicOr(p.err, DEVERR_ROPE_RANGE);
-    const float inv = in_range ? 1.f / sqrtf(ss / float(d) + p.eps) : 0.f;
+    const float inv = in_range ? rsqrtf(ss / float(d) + p.eps) : 0.f;
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
       const int e = lane + 32 * n;
@@ -184,7 +204,7 @@ cudaError_t launch_typed(const NormRopeParams& p, bool vec, int sms, cudaStream_
   int64_t items = p.n_tokens * heads;
   if (vec) {
     const int per_warp = 32 / (p.head_dim / 8) * NORM_HEADS;
-    items = p.n_tokens * ((heads + per_warp - 1) / per_warp);
+    items = p.n_tokens * ((p.n_head + per_warp - 1) / per_warp + (p.n_kv_head + per_warp - 1) / per_warp);
   }
   int64_t blocks = (items + warps - 1) / warps;
   if (blocks > int64_t(sms) * 64) blocks = int64_t(sms) * 64;

@@ -75,7 +75,10 @@ def test_strides_positions_and_in_place(cuda_device, aligned):
     q2, k2 = q.to(cuda_device), k.to(cuda_device)
     r = qk_norm_rope(q2, k2, args[0], args[1], *wide, pd, rotary_dim=rotary, q_out=q2, k_out=k2)
     assert r[0] is q2 or r[0].data_ptr() == q2.data_ptr()
-    assert torch.equal(q2, qo) and torch.equal(k2, ko)
+    _check(q2, q, wq, cos, sin, pos, 1e-6, rotary)
+    _check(k2, k, wk, cos, sin, pos, 1e-6, rotary)
+    apart = qk_norm_rope(q.to(cuda_device), k.to(cuda_device), *args, pd)
+    assert torch.equal(q2, apart[0]) and torch.equal(k2, apart[1]), "in place changes no bit"
     # no positions: token t at position t
     r = qk_norm_rope(q.to(cuda_device), kd, *args)
     _check(r[0], q, wq, cos, sin, torch.arange(tokens), 1e-6, rotary)
