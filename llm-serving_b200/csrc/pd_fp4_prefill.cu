@@ -97,6 +97,26 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Two fp32 operations per instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // 16 columns of 32 bits: thread t of the warp writes lane taddr.lane + t.
 __device__ __forceinline__ void st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -342,7 +362,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
         const uint64_t b0 = v_desc + uint64_t((s * C::KV_BYTES) >> 4);
 #pragma unroll
         for (int kk = 0; kk < KT / 16; ++kk)
-          tc::mma_f16_ts(tmem + uint32_t(C::O_COL + q * D), tmem + uint32_t(sb * KT + kk * 8),
+          tc::mma_f16_ts(tmem + uint32_t(C::O_COL + q * D), tmem + uint32_t(sb * KT + KT / 2 + kk * 8),
                          b0 + uint64_t((kk * 2048) >> 4), IDESC_PV, j > 0 || kk > 0);
         tc::commit(bar(Bars::O_DONE + sb));
         if (q == NQ - 1 || j >= tiles[NQ - 1]) tc::commit(bar(Bars::V_EMPTY + s));
@@ -413,7 +433,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(Bars::Q_FULL));
     }
-    const float mul = fabsf(p.scale_log2) * (p.units != nullptr ? __ldg(p.units + h) : 1.f) * down;
+    // never zero (a scale of 0 gives scores below 2^-80 instead), so that a hidden key's -inf stays one
+    const float mul = fmaxf(fabsf(p.scale_log2) * (p.units != nullptr ? __ldg(p.units + h) : 1.f) * down, 1.2e-38f);
     const int lim = live ? lk - chunk + tok : lk - 1;  // last visible key; padding rows see any
     const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t o_tmem = lane_base + uint32_t(C::O_COL + q * D);
@@ -432,23 +453,36 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       tc::fence_after_sync();
       const uint32_t s_tmem = lane_base + uint32_t(sb * KT);
       const bool open = __all_sync(FULL_MASK, j * KT + KT - 1 <= lim);  // no key of the tile is hidden
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-      for (int c = 0; c < KT; c += 32) {
-        uint32_t x[32];
-        tc::ld_32x32b_x32(s_tmem + uint32_t(c), x);
+      // The row's scores in two halves of KT / 2 columns: both give their maximum, the second stays in
+      // registers and goes first, the first is read again. P is stored over the second half's columns,
+      // which are free by then.
+      constexpr int H = KT / 2;
+      float x[H];
+      auto load_half = [&](int c0) {
+#pragma unroll
+        for (int c = 0; c < H; c += 32)
+          tc::ld_32x32b_x32(s_tmem + uint32_t(c0 + c), *reinterpret_cast<uint32_t(*)[32]>(x + c));
         tc::wait_ld();
-        if (open) {
+        if (!open) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i]));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            top[i & 3] = fmaxf(top[i & 3], j * KT + c + i <= lim ? __uint_as_float(x[i]) : -INFINITY);
+          for (int i = 0; i < H; ++i) x[i] = j * KT + c0 + i <= lim ? x[i] : -INFINITY;
         }
-      }
-      // mul > 0: the maximum of the products is the product of the maximum
-      const float tmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mul;
+      };
+      auto max_half = [&]() -> float {
+        float t[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (int i = 4; i < H; i += 8) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) t[k] = fmaxf(fmaxf(t[k], x[i + k]), i + 4 + k < H ? x[i + 4 + k] : t[k]);
+        }
+        return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+      };
+      load_half(0);
+      float top = max_half();
+      load_half(H);
+      top = fmaxf(top, max_half());
+      // mul >= 0: the maximum of the products is the product of the maximum
+      const float tmax = top * mul;
       const bool move = tmax > m_run + HEADROOM || (m_run < -1.0e38f && tmax > m_run);
       if (__any_sync(FULL_MASK, move)) {
         const float alpha = move ? ex2(m_run - tmax) : 1.f;
@@ -473,28 +507,28 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
           }
         }
       }
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-      for (int c = 0; c < KT; c += 32) {
-        uint32_t x[32], w[16];
-        tc::ld_32x32b_x32(s_tmem + uint32_t(c), x);
-        tc::wait_ld();
+      const float2 mul2 = make_float2(mul, mul), neg_m2 = make_float2(-m_run, -m_run);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      auto exp_half = [&](int c0) {  // P of keys c0 .. c0 + H - 1, two to a column
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float a = fmaf(__uint_as_float(x[i]), mul, -m_run), d = fmaf(__uint_as_float(x[i + 1]), mul, -m_run);
-          if (!open) {
-            a = j * KT + c + i <= lim ? a : -INFINITY;
-            d = j * KT + c + i + 1 <= lim ? d : -INFINITY;
+        for (int c = 0; c < H; c += 32) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float2 e = fma2(make_float2(x[c + i], x[c + i + 1]), mul2, neg_m2);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
+            w[i >> 1] = Elem<__half>::pack2(e.x, e.y);
           }
-          a = ex2(a);
-          d = ex2(d);
-          sum[(i >> 1) & 3] += a + d;
-          w[i >> 1] = Elem<__half>::pack2(a, d);
+          st_32x32b_x16(s_tmem + uint32_t(H + (c0 + c) / 2), w);
         }
-        // 32 keys of P take 16 columns, all of them columns whose scores are already read
-        st_32x32b_x16(s_tmem + uint32_t(c / 2), w);
-      }
-      l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      };
+      exp_half(H);
+      load_half(0);
+      exp_half(0);
+      const float2 total = add2(sum[0], sum[1]);
+      l_run += total.x + total.y;
       tc::wait_st();
       tc::fence_before_sync();
       __syncwarp();
