@@ -47,6 +47,7 @@ struct Cfg {
   static constexpr int NSB = 2;                   // S/P buffers: one per block, or two of the one block
   static constexpr int SOFTMAX_WARPS = 4 * NQ;
   static constexpr int DECODE_WARPS = 4;
+  static constexpr int DECODERS = DECODE_WARPS * 32;
   static constexpr int MMA_WARP = SOFTMAX_WARPS + DECODE_WARPS;
   static constexpr int THREADS = (MMA_WARP + 1) * 32;
   static constexpr int STAGES = 2;  // decoded tiles of K, and of V
@@ -81,14 +82,30 @@ struct Bars {
   static constexpr int ABORT = 168;
 };
 
-__device__ __forceinline__ bool thread_wait(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
-  if (limit_ns < TEST_LIMIT_NS) return false;
-  if (mbar_try_wait(bar, parity)) return true;
+// True in one lane of the (converged) warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
+// Bounded wait of one thread. The first look is all it costs when the phase is complete, as it
+// mostly is: a vote over the warp's lanes after every wait cost the MMA warp, whose MMAs queue only
+// briefly, a tenth of the kernel.
+__device__ __forceinline__ bool slow_wait(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
   const unsigned long long t0 = global_timer_ns();
   for (unsigned it = 1;; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((it & 63u) == 0 && global_timer_ns() - t0 > limit_ns) return false;
   }
+}
+__device__ __forceinline__ bool lane_wait(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
+  if (limit_ns < TEST_LIMIT_NS) return false;
+  return mbar_try_wait(bar, parity) || slow_wait(bar, parity, limit_ns);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -125,6 +142,17 @@ __device__ __forceinline__ void st_32x32b_x16(uint32_t taddr, const uint32_t (&r
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
+  return r;
+}
+
+// 16 bytes into shared memory, or zeros.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
@@ -208,118 +236,126 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
     // no query row
   } else if (warp >= C::SOFTMAX_WARPS && warp < C::MMA_WARP) {
     // ---------------------------------------------------------------- decoding warps
-    const int t = tid - C::SOFTMAX_WARPS * 32;  // 0 .. 127
+    const int t = tid - C::SOFTMAX_WARPS * 32;
     constexpr int N = C::PER_THREAD;
     const int32_t* trow = p.table + int64_t(b) * p.bt_stride;
     const int tpb_mask = (1 << p.log2_tpb) - 1;
     const int records = (lk + FP4_TILE - 1) / FP4_TILE;
     const unsigned char* head = p.pages + (int64_t(h) << p.log2_tpb) * REC;
     const uint32_t block_stride = uint32_t(p.n_kv_head << p.log2_tpb) * REC;
-    // Unit i of this thread is unit (i * 128 + t) of the tile: record first, so a warp reads
-    // consecutive bytes.
-    auto rec_of = [&](int tile, int i) -> int { return tile * (KT / 16) + (i * 128 + t) / C::PER_RECORD; };
+    // Unit i of this thread is unit u of record first_rec + i * REC_STEP of the tile.
+    constexpr int REC_STEP = C::DECODERS / C::PER_RECORD;
+    const int u = t % C::PER_RECORD, first_rec = t / C::PER_RECORD;
     auto block_of = [&](int tile, int i) -> int {
-      const int rec = rec_of(tile, i), page = rec >> p.log2_tpb;
+      const int rec = tile * (KT / 16) + first_rec + i * REC_STEP, page = rec >> p.log2_tpb;
       return tile < most && rec < records && page < p.max_blocks ? __ldg(trow + page) : -1;
     };
-    auto record_at = [&](int blk, int rec) -> const unsigned char* {
-      return blk >= 0 && blk < p.n_blocks ? head + uint64_t(blk) * block_stride + (rec & tpb_mask) * REC : nullptr;
-    };
-    const int u = t % C::PER_RECORD;  // unit inside a record (128 is a multiple of PER_RECORD)
-    // K unit: 16 bytes at 16 u of the record's codes, i.e. 32 elements of one token
+    // K unit: 32 elements of token k_tok, 16 tokens side by side, so that a quarter-warp's stores go
+    // to eight rows and, swizzled, to eight banks.
     constexpr int W = D < 128 ? D : 128, CH = W / 32;  // 16-byte chunks of a token in a block
-    const int k_blk = u / (16 * CH), k_tok = (u / CH) % 16, k_ch = u % CH;
+    const int k_tok = u % 16, k_blk = u / 16 / CH, k_ch = u / 16 % CH;
     const int k_el = k_blk * W + k_ch * 32;  // first element
+    const int k_code_off = k_blk * 8 * W + k_tok * (W / 2) + k_ch * 16;
     const int k_scale_off = 8 * D + k_blk * W + k_tok * (W / 16) + k_ch * 2;
-    // V unit: 16 bytes at 16 u of the V codes: group v_gr of tokens v_tok, v_tok + 1
+    const uint32_t k_row = uint32_t((k_el >> 6) * (KT * 128) + k_tok * 128);  // in the tile, of record 0
+    const uint32_t k_x = uint32_t((((k_el & 63) >> 3) ^ (k_tok & 7)) << 4);   // swizzled unit of word 0
+    // V unit: 16 elements of tokens v_tok, v_tok + 1. Even rows of two groups meet the same four banks,
+    // so lanes of odd groups store their two 8-element units in the other order.
     const int v_half = u / (D / 4), v_gr = (u / 4) % (D / 16), v_tok = v_half * 8 + (u % 4) * 2;
+    const bool v_odd = v_gr & 1;
+    const int v_code_off = 9 * D + 16 * u;
     const int v_scale_off = 17 * D + v_half * (D / 2) + v_gr * 8 + (u % 4) * 2;
+    const uint32_t v_row = uint32_t((v_gr >> 2) * (KT * 128) + v_tok * 128);
+    const uint32_t v_x = uint32_t((((v_gr & 3) * 2 + (v_odd ? 1 : 0)) ^ (v_tok & 7)) << 4);
 
     uint4 kraw[N], vraw[N];
     uint32_t ksc[N], vsc[N];
     int blk[N], blk_next[N];
-    auto load = [&](const int (&ids)[N], int tile, uint4 (&code)[N], uint32_t (&scale)[N], int code_off, int scale_off) {
+    const unsigned char* ptr[N];  // the records being loaded, or nullptr
+    auto aim = [&](int tile) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const unsigned char* r = record_at(ids[i], rec_of(tile, i));
+        const int rec = tile * (KT / 16) + first_rec + i * REC_STEP;
+        ptr[i] = blk[i] >= 0 && blk[i] < p.n_blocks ? head + uint64_t(blk[i]) * block_stride + (rec & tpb_mask) * REC
+                                                    : nullptr;
+      }
+    };
+    auto load = [&](uint4 (&code)[N], uint32_t (&scale)[N], int code_off, int scale_off) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
         code[i] = make_uint4(0u, 0u, 0u, 0u);
         scale[i] = 0u;
-        if (r != nullptr) {
-          code[i] = __ldg(reinterpret_cast<const uint4*>(r + code_off));
-          scale[i] = __ldg(reinterpret_cast<const uint16_t*>(r + scale_off));
+        if (ptr[i] != nullptr) {
+          code[i] = __ldg(reinterpret_cast<const uint4*>(ptr[i] + code_off));
+          scale[i] = __ldg(reinterpret_cast<const uint16_t*>(ptr[i] + scale_off));
         }
       }
     };
-    const int k_code_off = 16 * u, v_code_off = 9 * D + 16 * u;
 #pragma unroll
     for (int i = 0; i < N; ++i) blk[i] = block_of(0, i);
-    load(blk, 0, kraw, ksc, k_code_off, k_scale_off);
-    load(blk, 0, vraw, vsc, v_code_off, v_scale_off);
+    aim(0);
+    load(kraw, ksc, k_code_off, k_scale_off);
+    load(vraw, vsc, v_code_off, v_scale_off);
 #pragma unroll
     for (int i = 0; i < N; ++i) blk[i] = block_of(1, i);
+#pragma unroll
+    for (int i = 0; i < N; ++i) blk_next[i] = block_of(2, i);
     bool ok = true;
     for (int j = 0; ok && j < most; ++j) {
       if (__any_sync(FULL_MASK, *abort_flag != 0)) break;
-      const int s = j & 1;
-#pragma unroll
-      for (int i = 0; i < N; ++i) blk_next[i] = block_of(j + 2, i);
-      if (j >= 2 && !warp_wait_phase(bar(Bars::K_EMPTY + s), uint32_t((j / 2 - 1) & 1), p.wait_ns)) {
+      const int s = j % C::STAGES;
+      const uint32_t freed = uint32_t((j / C::STAGES - 1) & 1);  // phase of the stage's previous use
+      if (j >= C::STAGES && !warp_wait_phase(bar(Bars::K_EMPTY + s), freed, p.wait_ns)) {
         ok = false;
         break;
       }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int row = ((i * 128 + t) / C::PER_RECORD) * 16 + k_tok;
         const uint32_t pair = e4m3x2_to_half2(ksc[i]);
-        const uint32_t s0 = __byte_perm(pair, 0, 0x1010), s1 = __byte_perm(pair, 0, 0x3232);
+        const uint32_t sc[2] = {__byte_perm(pair, 0, 0x1010), __byte_perm(pair, 0, 0x3232)};
         const uint32_t w[4] = {kraw[i].x, kraw[i].y, kraw[i].z, kraw[i].w};
-        const uint32_t piece = k_addr(s) + uint32_t((k_el >> 6) * (KT * 128));
-        const int u0 = (k_el & 63) >> 3;
-        // a quarter-warp's lanes are two tokens x four chunks (or four x two): rotating the order
-        // by the piece and the token makes their eight units different
-        const int turn = ((k_el >> 6) & 1) ^ ((k_tok & 1) << 1);
+        const uint32_t row = k_addr(s) + k_row + uint32_t((first_rec + i * REC_STEP) * 2048);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int e = q ^ turn;
+        for (int e = 0; e < 4; ++e) {
           uint32_t x[4];
-          const uint32_t word = e & 2 ? (e & 1 ? w[3] : w[2]) : (e & 1 ? w[1] : w[0]);
-          e2m1x8_to_half2x4(word, x);
-          const uint32_t sc = e & 2 ? s1 : s0;
-          sts128(piece + sw128(row, u0 + e), hmul2_bits(x[0], sc), hmul2_bits(x[1], sc), hmul2_bits(x[2], sc),
-                 hmul2_bits(x[3], sc));
+          e2m1x8_to_half2x4(w[e], x);
+          sts128(row + (k_x ^ uint32_t(e << 4)), hmul2_bits(x[0], sc[e >> 1]), hmul2_bits(x[1], sc[e >> 1]),
+                 hmul2_bits(x[2], sc[e >> 1]), hmul2_bits(x[3], sc[e >> 1]));
         }
       }
-      load(blk, j + 1, kraw, ksc, k_code_off, k_scale_off);
+      aim(j + 1);
+      load(kraw, ksc, k_code_off, k_scale_off);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        blk[i] = blk_next[i];
+        blk_next[i] = block_of(j + 3, i);
+      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(Bars::K_FULL + s));
-      if (j >= 2 && !warp_wait_phase(bar(Bars::V_EMPTY + s), uint32_t((j / 2 - 1) & 1), p.wait_ns)) {
+      if (j >= C::STAGES && !warp_wait_phase(bar(Bars::V_EMPTY + s), freed, p.wait_ns)) {
         ok = false;
         break;
       }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int row = ((i * 128 + t) / C::PER_RECORD) * 16 + v_tok;
-        const int key = j * KT + row;
-        uint32_t sc = e4m3x2_to_half2(vsc[i]);
-        sc &= (key < lk ? 0x0000ffffu : 0u) | (key + 1 < lk ? 0xffff0000u : 0u);  // zeros past the row
-        const uint32_t w[4] = {vraw[i].x, vraw[i].y, vraw[i].z, vraw[i].w};
-        const uint32_t piece = v_addr(s) + uint32_t((v_gr >> 2) * (KT * 128));
-        const int u0 = (v_gr & 3) * 2;
+        const int key = j * KT + (first_rec + i * REC_STEP) * 16 + v_tok;
+        uint32_t pair = e4m3x2_to_half2(vsc[i]);
+        if (key + 1 >= lk) pair &= key < lk ? 0x0000ffffu : 0u;  // zeros past the row
+        const uint32_t sc[2] = {__byte_perm(pair, 0, 0x1010), __byte_perm(pair, 0, 0x3232)};
+        const uint32_t w[4] = {v_odd ? vraw[i].y : vraw[i].x, v_odd ? vraw[i].x : vraw[i].y,
+                               v_odd ? vraw[i].w : vraw[i].z, v_odd ? vraw[i].z : vraw[i].w};
+        const uint32_t row = v_addr(s) + v_row + uint32_t((first_rec + i * REC_STEP) * 2048);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int e = q ^ (v_gr & 1);  // odd groups write their second unit first: no bank twice
-          const uint32_t word = e & 2 ? (e & 1 ? w[3] : w[2]) : (e & 1 ? w[1] : w[0]);
+        for (int e = 0; e < 4; ++e) {  // token v_tok + e / 2: its row is the next one, its swizzle one bit off
           uint32_t x[4];
-          e2m1x8_to_half2x4(word, x);
-          const uint32_t f = e & 2 ? __byte_perm(sc, 0, 0x3232) : __byte_perm(sc, 0, 0x1010);
-          sts128(piece + sw128(row + (e >> 1), u0 + (e & 1)), hmul2_bits(x[0], f), hmul2_bits(x[1], f),
-                 hmul2_bits(x[2], f), hmul2_bits(x[3], f));
+          e2m1x8_to_half2x4(w[e], x);
+          sts128(row + uint32_t((e >> 1) * 128) + (v_x ^ uint32_t(((e & 1) ^ (e >> 1)) << 4)),
+                 hmul2_bits(x[0], sc[e >> 1]), hmul2_bits(x[1], sc[e >> 1]), hmul2_bits(x[2], sc[e >> 1]),
+                 hmul2_bits(x[3], sc[e >> 1]));
         }
       }
-      load(blk, j + 1, vraw, vsc, v_code_off, v_scale_off);
-#pragma unroll
-      for (int i = 0; i < N; ++i) blk[i] = blk_next[i];
+      load(vraw, vsc, v_code_off, v_scale_off);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(Bars::V_FULL + s));
@@ -327,70 +363,74 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
     if (!ok && lane == 0) fail();
   } else if (warp == C::MMA_WARP) {
     // ---------------------------------------------------------------- MMA issuer
-    if (lane == 0 && most > 0) {
+    // The whole warp runs this loop and one elected lane issues, so descriptors and addresses stay
+    // uniform over the warp and no operand of an MMA is moved on its own.
+    if (most > 0) {
       constexpr uint32_t IDESC_S = tc::instr_desc_f16(false, ROWS, KT, false, false);
       constexpr uint32_t IDESC_PV = tc::instr_desc_f16(false, ROWS, D, false, true);
-      bool ok = thread_wait(bar(Bars::Q_FULL), 0u, p.wait_ns);
+      bool ok = lane_wait(bar(Bars::Q_FULL), 0u, p.wait_ns);
       const uint64_t q_desc = tc::smem_desc(sbase + C::OFF_Q, 16u, 1024u);
       const uint64_t k_desc = tc::smem_desc(k_addr(0), 16u, 1024u);
       const uint64_t v_desc = tc::smem_desc(v_addr(0), uint32_t(KT * 128), 1024u);
-      // S/P buffer of (block q, tile j) and the phase of that use on the buffer's barriers
+      // (block q, tile j) uses S/P buffer q for the j-th time or, with one block, buffer j % 2 for
+      // the j / 2-th.
       auto buf = [&](int q, int j) -> int { return NQ == 2 ? q : j & 1; };
       auto use = [&](int j) -> uint32_t { return NQ == 2 ? uint32_t(j) : uint32_t(j >> 1); };
       // S of (q, j), once P V of the buffer's previous use has read its P
-      auto issue_s = [&](int q, int j) -> bool {
+      auto issue_s = [&](int q, int j) {
         const int s = j & 1, sb = buf(q, j);
-        if (!thread_wait(bar(Bars::K_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns)) return false;
-        if (use(j) > 0 && !thread_wait(bar(Bars::O_DONE + sb), (use(j) - 1) & 1u, p.wait_ns)) return false;
+        ok = ok && lane_wait(bar(Bars::K_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns);
+        if (use(j) > 0) ok = ok && lane_wait(bar(Bars::O_DONE + sb), (use(j) - 1) & 1u, p.wait_ns);
+        __syncwarp();
         tc::fence_after_sync();
         const uint64_t a0 = q_desc + uint64_t((q * C::Q_BYTES) >> 4), b0 = k_desc + uint64_t((s * C::KV_BYTES) >> 4);
+        const bool frees = q == NQ - 1 || j >= tiles[NQ - 1];  // the last block that uses this K tile
+        if (elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-          tc::mma_f16_ss(tmem + uint32_t(sb * KT), a0 + uint64_t(((ks >> 2) * (ROWS * 128) + (ks & 3) * 32) >> 4),
-                         b0 + uint64_t(((ks >> 2) * (KT * 128) + (ks & 3) * 32) >> 4), IDESC_S, ks > 0);
-        tc::commit(bar(Bars::S_FULL + sb));
-        // the last block that uses this K tile frees it
-        if (q == NQ - 1 || j >= tiles[NQ - 1]) tc::commit(bar(Bars::K_EMPTY + s));
-        return true;
+          for (int ks = 0; ks < D / 16; ++ks)
+            tc::mma_f16_ss(tmem + uint32_t(sb * KT), a0 + uint64_t(((ks >> 2) * (ROWS * 128) + (ks & 3) * 32) >> 4),
+                           b0 + uint64_t(((ks >> 2) * (KT * 128) + (ks & 3) * 32) >> 4), IDESC_S, ks > 0);
+          tc::commit(bar(Bars::S_FULL + sb));
+          if (frees) tc::commit(bar(Bars::K_EMPTY + s));
+        }
+        __syncwarp();
       };
-      auto issue_pv = [&](int q, int j) -> bool {
+      auto issue_pv = [&](int q, int j) {
         const int s = j & 1, sb = buf(q, j);
-        if (!thread_wait(bar(Bars::P_FULL + sb), use(j) & 1u, p.wait_ns) ||
-            !thread_wait(bar(Bars::V_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns))
-          return false;
+        ok = ok && lane_wait(bar(Bars::V_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns);
+        ok = ok && lane_wait(bar(Bars::P_FULL + sb), use(j) & 1u, p.wait_ns);
+        __syncwarp();
         tc::fence_after_sync();
         const uint64_t b0 = v_desc + uint64_t((s * C::KV_BYTES) >> 4);
+        const bool frees = q == NQ - 1 || j >= tiles[NQ - 1];
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < KT / 16; ++kk)
-          tc::mma_f16_ts(tmem + uint32_t(C::O_COL + q * D), tmem + uint32_t(sb * KT + KT / 2 + kk * 8),
-                         b0 + uint64_t((kk * 2048) >> 4), IDESC_PV, j > 0 || kk > 0);
-        tc::commit(bar(Bars::O_DONE + sb));
-        if (q == NQ - 1 || j >= tiles[NQ - 1]) tc::commit(bar(Bars::V_EMPTY + s));
-        return true;
+          for (int kk = 0; kk < KT / 16; ++kk)
+            tc::mma_f16_ts(tmem + uint32_t(C::O_COL + q * D), tmem + uint32_t(sb * KT + KT / 2 + kk * 8),
+                           b0 + uint64_t((kk * 2048) >> 4), IDESC_PV, j > 0 || kk > 0);
+          tc::commit(bar(Bars::O_DONE + sb));
+          if (frees) tc::commit(bar(Bars::V_EMPTY + s));
+        }
+        __syncwarp();
       };
-      if (NQ == 2) {
+      if (__all_sync(FULL_MASK, ok)) {
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
-          if (ok && tiles[q] > 0) ok = issue_s(q, 0);
-        for (int j = 0; ok && j < most; ++j) {
-          if (*abort_flag) break;
+          if (tiles[q] > 0) issue_s(q, 0);
+      }
+      for (int j = 0; j < most; ++j) {
+        if (!__all_sync(FULL_MASK, ok && *abort_flag == 0)) break;
+        if (NQ == 1 && j + 1 < most) issue_s(0, j + 1);
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            if (ok && j < tiles[q]) ok = issue_pv(q, j);
-            if (ok && j + 1 < tiles[q]) ok = issue_s(q, j + 1);
-          }
-        }
-      } else {
-        if (ok) ok = issue_s(0, 0);
-        for (int j = 0; ok && j < most; ++j) {
-          if (*abort_flag) break;
-          if (j + 1 < most) ok = issue_s(0, j + 1);
-          if (ok) ok = issue_pv(0, j);
+        for (int q = 0; q < NQ; ++q) {
+          if (j < tiles[q]) issue_pv(q, j);
+          if (NQ == 2 && j + 1 < tiles[q]) issue_s(q, j + 1);
         }
       }
-      if (!ok) fail();
-      tc::commit(bar(Bars::DRAIN));  // never leave with an MMA in flight
-      thread_wait(bar(Bars::DRAIN), 0u, DRAIN_LIMIT_NS);
+      if (!__all_sync(FULL_MASK, ok) && lane == 0) fail();
+      if (elect_one()) tc::commit(bar(Bars::DRAIN));  // never leave with an MMA in flight
+      __syncwarp();
+      warp_wait_phase(bar(Bars::DRAIN), 0u, DRAIN_LIMIT_NS);
     }
   } else {
     // ---------------------------------------------------------------- softmax warps
@@ -402,16 +442,39 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
     const int64_t hq = int64_t(h) * p.group + hg;
     float down;  // 1 / the row's power of two
     {
-      const T* src = reinterpret_cast<const T*>(p.q) + int64_t(q_begin + tok) * p.q_st + hq * p.q_sh;
-      float top = 0.f;
-      if (live) {
+      // Q as it is into its place (16-byte units of 8 elements, all copies in flight at once), then
+      // each thread turns its own row into fp16 where it stands. Loops, not straight-line code: what
+      // runs once per CTA is fetched slower than it runs.
+      constexpr int LANES = D / 8, STEP = 128 / LANES;
+      const uint32_t q_base = sbase + uint32_t(C::OFF_Q + q * C::Q_BYTES);
+      {
+        const int t = tid - q * 128, u = t % LANES;
+        const int m0 = row0 + q * ROWS + t / LANES;
+        int mt = m0 / p.group, mh = m0 - mt * p.group;
+        const int dt = STEP / p.group, dh = STEP - dt * p.group;
+        const T* base = reinterpret_cast<const T*>(p.q) + int64_t(q_begin) * p.q_st + int64_t(h) * p.group * p.q_sh + u * 8;
 #pragma unroll 4
-        for (int u = 0; u < D / 8; ++u) {
-          float x[8];
-          E::unpack(__ldg(reinterpret_cast<const uint4*>(src) + u), x);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+        for (int rr = t / LANES; rr < ROWS; rr += STEP) {
+          const bool in = row0 + q * ROWS + rr < rows;
+          cp_async16(q_base + uint32_t((u >> 3) * (ROWS * 128)) + sw128(rr, u & 7),
+                     base + (in ? int64_t(mt) * p.q_st + int64_t(mh) * p.q_sh : 0), in);
+          mt += dt;
+          mh += dh;
+          if (mh >= p.group) {
+            mh -= p.group;
+            ++mt;
+          }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + q) : "memory");  // the block's rows are in
+      }
+      float top = 0.f;
+#pragma unroll 4
+      for (int u = 0; u < D / 8; ++u) {
+        float x[8];
+        E::unpack(lds128(q_base + uint32_t((u >> 3) * (ROWS * 128)) + sw128(r, u & 7)), x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(x[k]));
       }
       int e = int(__float_as_uint(top) >> 23);
       e = e == 0 || e == 255 ? 140 : e;
@@ -421,13 +484,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       down = __uint_as_float(uint32_t(127 - shift) << 23);
 #pragma unroll 4
       for (int u = 0; u < D / 8; ++u) {
+        const uint32_t a = q_base + uint32_t((u >> 3) * (ROWS * 128)) + sw128(r, u & 7);
         float x[8];
-        E::unpack(live ? __ldg(reinterpret_cast<const uint4*>(src) + u) : make_uint4(0u, 0u, 0u, 0u), x);
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = Elem<__half>::pack2(x[2 * i] * up, x[2 * i + 1] * up);
-        sts128(sbase + C::OFF_Q + uint32_t(q * C::Q_BYTES + (u >> 3) * (ROWS * 128)) + sw128(r, u & 7), w[0], w[1], w[2],
-               w[3]);
+        E::unpack(lds128(a), x);
+        sts128(a, Elem<__half>::pack2(x[0] * up, x[1] * up), Elem<__half>::pack2(x[2] * up, x[3] * up),
+               Elem<__half>::pack2(x[4] * up, x[5] * up), Elem<__half>::pack2(x[6] * up, x[7] * up));
       }
       fence_proxy_async_smem();
       __syncwarp();

@@ -69,7 +69,7 @@ bool use_tiles(int64_t total_q, int32_t max_seqlen_q, int32_t batch, int32_t n_k
                int32_t head_dim, int sms) {
   constexpr double A = 260.0 / 32, B = 2600.0 / 128;
   const double units = double(n_kv_head) * (double(total_q) * group / 8 + 0.5 * batch);
-  const int64_t block = head_dim == 256 ? 128 : 256;
+  const int64_t block = 128;
   const int64_t ctas = int64_t(batch) * n_kv_head * ((int64_t(max_seqlen_q) * group + block - 1) / block);
   return double((ctas + sms - 1) / sms) * B < units / sms * A;
 }
