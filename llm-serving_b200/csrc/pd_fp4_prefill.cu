@@ -379,7 +379,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       // S of (q, j), once P V of the buffer's previous use has read its P
       auto issue_s = [&](int q, int j) {
         const int s = j & 1, sb = buf(q, j);
-        ok = ok && lane_wait(bar(Bars::K_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns);
+        if (q == 0 || j >= tiles[0])  // else the first block has waited for this K tile
+          ok = ok && lane_wait(bar(Bars::K_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns);
         if (use(j) > 0) ok = ok && lane_wait(bar(Bars::O_DONE + sb), (use(j) - 1) & 1u, p.wait_ns);
         __syncwarp();
         tc::fence_after_sync();
@@ -397,7 +398,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       };
       auto issue_pv = [&](int q, int j) {
         const int s = j & 1, sb = buf(q, j);
-        ok = ok && lane_wait(bar(Bars::V_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns);
+        if (q == 0 || j >= tiles[0])
+          ok = ok && lane_wait(bar(Bars::V_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns);
         ok = ok && lane_wait(bar(Bars::P_FULL + sb), use(j) & 1u, p.wait_ns);
         __syncwarp();
         tc::fence_after_sync();
