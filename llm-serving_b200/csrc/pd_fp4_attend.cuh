@@ -422,9 +422,12 @@ struct Worker {
   }
 };
 
-// A partial unit of this CTA: tiles [t0, t1) of unit `unit` (kv head, column block) of row b.
-struct Piece {
+// A partial unit of this CTA: tiles [t0, t1) of the `tiles` of unit `unit` of row `row`, with what a
+// join needs to know of it, so that no join looks lengths up or divides again.
+struct alignas(16) Piece {
   int row, unit, t0, t1;  // row < 0: none
+  int tiles, h, first, cols;
+  int q_begin, pad[3];
 };
 
 // Joins `n` pieces' four elements of column col: ml(i) is piece i's (m, l) block, acc(i) its elements.
@@ -446,11 +449,12 @@ __device__ __forceinline__ void join4(int n, int col, Ml ml, Acc acc, float (&x)
 }
 
 template <typename T>
-__device__ __forceinline__ void store_out4(const Fp4AttendParams& p, const Row& r, int h, int n, int e, float unit,
-                                           const float (&x)[4], float l) {
+__device__ __forceinline__ void store_out4(const Fp4AttendParams& p, const Piece& a, int col, int e, const float (&x)[4],
+                                           float l) {
+  const float unit = p.units != nullptr ? __ldg(p.units + p.n_kv_head + a.h) : 1.f;
   const float inv = l > 0.f ? unit / l : 0.f;
-  const int tok = n / p.group, hg = n - tok * p.group;
-  T* dst = reinterpret_cast<T*>(p.out) + int64_t(r.q_begin + tok) * p.o_st + int64_t(h * p.group + hg) * p.o_sh + e;
+  const int n = a.first + col, tok = n / p.group, hg = n - tok * p.group;
+  T* dst = reinterpret_cast<T*>(p.out) + int64_t(a.q_begin + tok) * p.o_st + int64_t(a.h * p.group + hg) * p.o_sh + e;
   *reinterpret_cast<uint2*>(dst) =
       make_uint2(Elem<T>::pack2(x[0] * inv, x[1] * inv), Elem<T>::pack2(x[2] * inv, x[3] * inv));
 }
@@ -480,13 +484,36 @@ struct Cursor {
   int b, unit, tile, tiles, units;
 };
 
+// a / b for a >= 0, b > 0; the 64-bit division only where it is needed.
+__device__ __forceinline__ long long quotient(long long a, int b) {
+  return (a >> 32) == 0 ? (long long)(uint32_t(a) / uint32_t(b)) : a / b;
+}
+
+// [0, total) cut into n runs whose lengths differ by one at most: where run c begins, and the run of f.
+struct Split {
+  long long q;
+  int r;
+  __device__ __forceinline__ Split(long long total, int n) : q(quotient(total, n)), r(int(total - q * n)) {}
+  __device__ __forceinline__ long long begin(int c) const { return c * q + min(c, r); }
+  __device__ __forceinline__ int run(long long f) const {
+    const long long longer = r * (q + 1);  // runs below r have q + 1
+    return f < longer ? int(quotient(f, int(q + 1))) : r + int(quotient(f - longer, int(q)));
+  }
+};
+
+__device__ __forceinline__ unsigned atom_add_acq_rel(unsigned* p, unsigned v) {
+  unsigned old;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+  return old;
+}
+
 template <typename T, int D, int NW>
 __global__ void __launch_bounds__(NW * 32, 1)
     pd_fp4_attend_kernel(const __grid_constant__ Fp4AttendParams p, int stages, int max_cols, int min_tiles) {
   constexpr int REC = fp4_record_bytes(D);
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ long long warp_sums[2][NW];
-  __shared__ unsigned last_flags[2];
+  __shared__ int arrival[2][3];  // per cut: last to arrive, first CTA, CTAs
   const Smem L = smem_layout(p.batch, NW, max_cols, D, stages);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   long long* pre = reinterpret_cast<long long*>(smem + L.pre_off);
@@ -501,28 +528,60 @@ __global__ void __launch_bounds__(NW * 32, 1)
 
   // ---- tiles of every row, their prefix sums, the unit count and the longest row
   long long total, units_total;
-  int longest;
-  {
-    if (lane < stages) mbar_init(bars + lane * 8u, 1);
-    fence_barrier_init();
+  int longest, row, row_unit;  // row and unit of the CTA's unit, where each CTA has one
+  bool whole;
+  if (lane < stages) mbar_init(bars + lane * 8u, 1);
+  if (lane < 2) pieces[2 * warp + lane].row = -1;
+  fence_barrier_init();
+  auto row_work = [&](int b) -> int2 {
+    const Row r = row_of(p, b);
+    return make_int2(r.lk > TILE ? (r.lk + TILE - 1) / TILE : 1, p.n_kv_head * ((r.sq * p.group + COLS - 1) / COLS));
+  };
+  auto up = [&](long long x, int o) -> long long { return __shfl_up_sync(FULL_MASK, x, o); };
+  if (p.batch <= 32) {
+    // A row to a lane, and every warp for itself: all write the same values, each reads its own, and
+    // no barrier is needed.
+    const int2 w = lane < p.batch ? row_work(lane) : make_int2(0, 0);
+    long long incl = (long long)w.x * w.y;
+    int unit_incl = w.y;
+    longest = w.y > 0 ? w.x : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long f = up(incl, o);
+      const int g = __shfl_up_sync(FULL_MASK, unit_incl, o);
+      if (lane >= o) {
+        incl += f;
+        unit_incl += g;
+      }
+      longest = max(longest, __shfl_xor_sync(FULL_MASK, longest, o));
+    }
+    total = __shfl_sync(FULL_MASK, incl, 31);
+    units_total = __shfl_sync(FULL_MASK, unit_incl, 31);
+    if (lane < p.batch) {
+      pre[lane] = incl - (long long)w.x * w.y;
+      rows[lane] = w;
+    }
+    __syncwarp();
+    whole = units_total <= gridDim.x && longest <= WHOLE_TILES * NW;
+    row = __ffs(__ballot_sync(FULL_MASK, unit_incl > int(blockIdx.x))) - 1;
+    row_unit = int(blockIdx.x) - __shfl_sync(FULL_MASK, unit_incl - w.y, row < 0 ? 0 : row);
+  } else {
     const int per = (p.batch + NW * 32 - 1) / (NW * 32);
     const int b0 = tid * per;
     long long sum = 0, usum = 0;
     int most = 0;
     for (int b = b0; b < b0 + per && b < p.batch; ++b) {
-      const Row r = row_of(p, b);
-      const int tiles = r.lk > TILE ? (r.lk + TILE - 1) / TILE : 1;
-      const int units = p.n_kv_head * ((r.sq * p.group + COLS - 1) / COLS);
-      rows[b] = make_int2(tiles, units);
-      sum += (long long)tiles * units;
-      usum += units;
-      most = units > 0 && tiles > most ? tiles : most;
+      const int2 w = row_work(b);
+      rows[b] = w;
+      sum += (long long)w.x * w.y;
+      usum += w.y;
+      most = w.y > 0 && w.x > most ? w.x : most;
     }
     long long incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(FULL_MASK, incl, o);
-      if (lane >= o) incl += up;
+      const long long f = up(incl, o);
+      if (lane >= o) incl += f;
       usum += __shfl_xor_sync(FULL_MASK, usum, o);
       most = max(most, __shfl_xor_sync(FULL_MASK, most, o));
     }
@@ -530,11 +589,11 @@ __global__ void __launch_bounds__(NW * 32, 1)
       warp_sums[0][warp] = incl;
       warp_sums[1][warp] = (usum << 31) | most;  // both below 2^31
     }
-    if (tid < 2 * NW) pieces[tid].row = -1;
     __syncthreads();
     long long at = incl - sum;
     total = units_total = 0;
     longest = 0;
+#pragma unroll 1
     for (int w = 0; w < NW; ++w) {
       if (w < warp) at += warp_sums[0][w];
       total += warp_sums[0][w];
@@ -545,38 +604,33 @@ __global__ void __launch_bounds__(NW * 32, 1)
       pre[b] = at;
       at += (long long)rows[b].x * rows[b].y;
     }
-    if (tid == 0) pre[p.batch] = total;
     __syncthreads();
+    whole = units_total <= gridDim.x && longest <= WHOLE_TILES * NW;
+    row = 0;
+    row_unit = int(blockIdx.x);
+    if (whole)
+      while (row < p.batch && row_unit >= rows[row].y) row_unit -= rows[row++].y;
   }
   if (total == 0) return;
 
-  // ---- this CTA's run [c0, c1) and this warp's part of it
-  const bool whole = units_total <= gridDim.x && longest <= WHOLE_TILES * NW;
-  long long ctas = whole ? units_total : (total + NW * min_tiles - 1) / (NW * min_tiles);
-  ctas = ctas < gridDim.x ? ctas : gridDim.x;
-  if (blockIdx.x >= ctas) return;
-  auto find_row = [&](long long f) -> int {  // last b with pre[b] <= f: the row of tile f
-    int lo = 0, hi = p.batch - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (pre[mid] <= f) lo = mid; else hi = mid - 1;
-    }
-    return lo;
-  };
+  // ---- this CTA's run of tiles and this warp's part of it
+  const long long wanted = whole ? units_total : quotient(total + NW * min_tiles - 1, NW * min_tiles);
+  const int ctas = int(wanted < gridDim.x ? wanted : gridDim.x);
+  if (int(blockIdx.x) >= ctas) return;
+  const Split split(total, ctas);  // where units are not whole CTAs'
   long long c0, c1;
-  if (whole) {  // the blockIdx-th unit
-    int b = 0, u = int(blockIdx.x);
-    while (u >= rows[b].y) u -= rows[b++].y;
-    c0 = pre[b] + (long long)u * rows[b].x;
-    c1 = c0 + rows[b].x;
+  if (whole) {
+    c0 = pre[row] + (long long)row_unit * rows[row].x;
+    c1 = c0 + rows[row].x;
   } else {
-    c0 = blockIdx.x * total / ctas;
-    c1 = (blockIdx.x + 1) * total / ctas;
+    c0 = split.begin(blockIdx.x);
+    c1 = split.begin(blockIdx.x + 1);
   }
   const int in_cta = int(c1 - c0);
   const int warps = min(NW, (in_cta + min_tiles - 1) / min_tiles);
-  const long long f0 = c0 + (long long)in_cta * min(warp, warps) / warps;
-  const int count = warp < warps ? int(c0 + (long long)in_cta * (warp + 1) / warps - f0) : 0;
+  const int wq = in_cta / warps, wr = in_cta - wq * warps;
+  const long long f0 = c0 + warp * wq + min(warp, wr);
+  const int count = warp < warps ? wq + (warp < wr ? 1 : 0) : 0;
 
   if (count > 0) {
     constexpr uint32_t STAGE = 2 * REC;
@@ -593,23 +647,42 @@ __global__ void __launch_bounds__(NW * 32, 1)
       }
     };
     Cursor at;
-    at.b = find_row(f0);
+    if (p.batch <= 32) {  // the last row that begins at or before the tile
+      at.b = 31 - __clz(__ballot_sync(FULL_MASK, lane < p.batch && pre[lane < p.batch ? lane : 0] <= f0));
+    } else {
+      int lo = 0, hi = p.batch - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (pre[mid] <= f0) lo = mid; else hi = mid - 1;
+      }
+      at.b = lo;
+    }
     {
       const long long r = f0 - pre[at.b];
       at.tiles = rows[at.b].x;
       at.units = rows[at.b].y;
-      at.unit = int(r / at.tiles);
+      at.unit = int(quotient(r, at.tiles));
       at.tile = int(r - (long long)at.unit * at.tiles);
     }
 
-    // ---- prefetch: tile `ahead`, its blocks from a window of 32 block ids held by the lanes, the
-    // next 32 already loading. A window starts at a tile's first page, so a tile's two pages
-    // (block_size 16) are always in one window.
+    // ---- prefetch: tile `ahead`. Lane l holds the address of the unit's page win_page + l (this head's
+    // records of it) and issues that page's copies itself; the block ids of the next 32 pages are
+    // already loading. A window starts at a tile's first page, so a tile's two pages (block_size
+    // 16) are in one window.
     Cursor ahead = at;
-    int win = 0, win_next = 0, win_page = 0, last_page = 0, records = 0;
+    const unsigned char* page_at = nullptr;
+    int id_next = 0, win_page = 0, last_page = 0, records = 0;
+    unsigned dead = 0;  // pages of the window that are outside the pool, or past the row
     const unsigned char* head_pages = nullptr;  // this head's first record of block 0
+    const uint32_t block_stride = uint32_t(p.n_kv_head << p.log2_tpb) * REC;
     auto entry = [&](int page) -> int {
       return page <= last_page ? __ldg(p.table + int64_t(ahead.b) * p.bt_stride + page) : -1;
+    };
+    auto open_window = [&](int id) {  // the window at win_page, whose block ids are `id`
+      const bool live = id >= 0 && id < p.n_blocks;
+      page_at = head_pages + (live ? uint64_t(id) * block_stride : 0);
+      dead = __ballot_sync(FULL_MASK, !live);
+      id_next = entry(win_page + 32 + lane);
     };
     auto open_ahead = [&]() {
       const int h = ahead.unit / (ahead.units / p.n_kv_head);
@@ -617,11 +690,9 @@ __global__ void __launch_bounds__(NW * 32, 1)
       records = (row_of(p, ahead.b).lk + FP4_TILE - 1) / FP4_TILE;
       last_page = min(((records + (1 << p.log2_tpb) - 1) >> p.log2_tpb), p.max_blocks) - 1;
       win_page = (2 * ahead.tile) >> p.log2_tpb;
-      win = entry(win_page + lane);
-      win_next = entry(win_page + 32 + lane);
+      open_window(entry(win_page + lane));
     };
     open_ahead();
-    const uint32_t block_stride = uint32_t(p.n_kv_head << p.log2_tpb) * REC;
     int issued = 0;
     uint32_t fill = 0;  // stage of the next copy
     auto issue = [&]() {
@@ -631,35 +702,32 @@ __global__ void __launch_bounds__(NW * 32, 1)
       if (page >= 32) {
         win_page += 32;
         page -= 32;
-        win = win_next;
-        win_next = entry(win_page + 32 + lane);
+        open_window(id_next);
       }
       const uint32_t dst = ring + fill * STAGE, bar = bars + fill * 8u;
-      const int blk0 = __shfl_sync(FULL_MASK, win, page);
-      const int blk1 = p.log2_tpb == 0 ? __shfl_sync(FULL_MASK, win, (page + 1) & 31) : blk0;
       const bool two = rec + 1 < records;
-      const bool live0 = blk0 >= 0 && blk0 < p.n_blocks, live1 = blk1 >= 0 && blk1 < p.n_blocks;
-      if (live0 && (live1 || !two)) {
-        if (lane == 0) {
-          mbar_arrive_expect_tx(bar, two ? STAGE : REC);
-          const unsigned char* src0 = head_pages + uint64_t(blk0) * block_stride;
-          if (p.log2_tpb == 0) {
-            bulk_load(dst, src0, REC, bar, policy);
-            if (two) bulk_load(dst + REC, head_pages + uint64_t(blk1) * block_stride, REC, bar, policy);
-          } else {  // both records in one page, one after the other
-            bulk_load(dst, src0 + (rec & ((1 << p.log2_tpb) - 1)) * REC, two ? STAGE : REC, bar, policy);
-          }
+      const unsigned needs = two && p.log2_tpb == 0 ? 3u : 1u;
+      if (((dead >> page) & needs) == 0) {
+        // the page's lane announces the bytes and copies; with one record to a page, the next lane copies
+        // the second (its bytes may be counted before they are announced: the phase waits for the
+        // announcing arrival)
+        const int mine = lane - page;
+        if (mine == 0) mbar_arrive_expect_tx(bar, two ? STAGE : REC);
+        if (p.log2_tpb == 0) {
+          if (mine == 0 || (mine == 1 && two)) bulk_load(dst + mine * REC, page_at, REC, bar, policy);
+        } else if (mine == 0) {  // both records in one page, one after the other
+          bulk_load(dst, page_at + (rec & ((1 << p.log2_tpb) - 1)) * REC, two ? STAGE : REC, bar, policy);
         }
       } else {  // a block outside the pool reads zeros
-        const int sub = rec & ((1 << p.log2_tpb) - 1);
+        const int in_page = rec & ((1 << p.log2_tpb) - 1);
 #pragma unroll 1
         for (int r = 0; r < 2; ++r) {
-          const bool live = r == 0 ? live0 : live1;
-          const int in_page = p.log2_tpb == 0 ? 0 : sub + r;
-          const uint4* src = reinterpret_cast<const uint4*>(
-              head_pages + (live ? uint64_t(r == 0 ? blk0 : blk1) * block_stride + in_page * REC : 0));
+          const int holder = p.log2_tpb == 0 ? (page + r) & 31 : page;
+          const uint64_t at64 = __shfl_sync(FULL_MASK, reinterpret_cast<uint64_t>(page_at), holder);
+          const bool live = (r == 0 || two) && !((dead >> holder) & 1u);
+          const uint4* src = reinterpret_cast<const uint4*>(at64) + (p.log2_tpb == 0 ? 0 : (in_page + r) * (REC / 16));
           for (int i = lane; i < REC / 16; i += 32) {
-            const uint4 v = live && (r == 0 || two) ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+            const uint4 v = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
             asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + r * REC + i * 16), "r"(v.x), "r"(v.y),
                          "r"(v.z), "r"(v.w)
                          : "memory");
@@ -684,11 +752,11 @@ __global__ void __launch_bounds__(NW * 32, 1)
     int taken = 0;
     bool ok = true;
     for (int n = 0; n < count;) {
-      const Row row = row_of(p, at.b);
+      const Row r = row_of(p, at.b);
       const int cbs = at.units / p.n_kv_head;
       const int h = at.unit / cbs, first = (at.unit - h * cbs) * COLS;
       const int begin = at.tile, end = min(at.tiles, at.tile + count - n);
-      wk.start(p, row, h, first);
+      wk.start(p, r, h, first);
       for (int tile = begin; tile < end; ++tile) {
         if (ok && !warp_wait_phase(bars + stage * 8u, phase, p.wait_ns)) {
           ok = false;  // the rest of the run is left out; its pieces and arrivals still happen
@@ -697,7 +765,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
         if (!ok) continue;
         __syncwarp();  // every lane is done with the stage that the next copy fills
         issue();
-        wk.tile(ring + stage * STAGE, tile * TILE, row.lk - tile * TILE);
+        wk.tile(ring + stage * STAGE, tile * TILE, r.lk - tile * TILE);
         ++taken;
         if (++stage == uint32_t(stages)) {
           stage = 0;
@@ -706,11 +774,12 @@ __global__ void __launch_bounds__(NW * 32, 1)
       }
       n += end - begin;
       if (begin == 0 && end == at.tiles) {
-        wk.finish(p, row, h, first);
+        wk.finish(p, r, h, first);
       } else {
         const int slot = 2 * warp + (begin == 0 ? 1 : 0);
-        wk.store_piece(piece_ml + slot * 2 * COLS, piece_acc(slot), min(COLS, row.sq * p.group - first));
-        if (lane == 0) pieces[slot] = Piece{at.b, at.unit, begin, end};
+        wk.store_piece(piece_ml + slot * 2 * COLS, piece_acc(slot), min(COLS, r.sq * p.group - first));
+        if (lane == 0)
+          pieces[slot] = Piece{at.b, at.unit, begin, end, at.tiles, h, first, min(COLS, r.sq * p.group - first), r.q_begin, {}};
       }
       if (n < count) step_unit(at);
     }
@@ -728,40 +797,36 @@ __global__ void __launch_bounds__(NW * 32, 1)
   // ---- joins within the CTA
   __syncthreads();
   static_assert(2 * NW <= 32, "one lane per piece");
-  Piece mine{-1, 0, 0, 0};
-  if (lane < 2 * NW) mine = pieces[lane];
-  const unsigned valid = __ballot_sync(FULL_MASK, mine.row >= 0);
+  int2 mine = make_int2(-1, 0);
+  if (lane < 2 * NW) mine = make_int2(pieces[lane].row, pieces[lane].unit);
+  const unsigned valid = __ballot_sync(FULL_MASK, mine.x >= 0);
   if (valid == 0) return;  // uniform over the CTA
   const unsigned below = valid & ((1u << lane) - 1u);
   const int prev = below ? 31 - __clz(below) : lane;
-  const int prev_row = __shfl_sync(FULL_MASK, mine.row, prev), prev_unit = __shfl_sync(FULL_MASK, mine.unit, prev);
-  const bool opens = mine.row >= 0 && (below == 0 || prev_row != mine.row || prev_unit != mine.unit);
-  unsigned heads = __ballot_sync(FULL_MASK, opens);
+  const int prev_row = __shfl_sync(FULL_MASK, mine.x, prev), prev_unit = __shfl_sync(FULL_MASK, mine.y, prev);
+  unsigned heads =
+      __ballot_sync(FULL_MASK, mine.x >= 0 && (below == 0 || prev_row != mine.x || prev_unit != mine.y));
   float* const cta_part = p.partials + size_t(blockIdx.x) * 2 * partial_floats(D);
   int task = 0;
   int cut0 = -1, cut1 = -1;  // first piece of the unit cut at the CTA's front, and at its back
+#pragma unroll 1
   while (heads) {
     const int s0 = __ffs(heads) - 1;
     heads &= heads - 1;
     const unsigned upto = heads ? (1u << (__ffs(heads) - 1)) - 1u : 0xffffffffu;
     const unsigned members = valid & upto & ~((1u << s0) - 1u);
     const Piece a = pieces[s0];
-    const int2 rw = rows[a.row];
-    const bool complete = a.t0 == 0 && pieces[31 - __clz(members)].t1 == rw.x;
-    const Row r = row_of(p, a.row);
-    const int cbs = rw.y / p.n_kv_head;
-    const int h = a.unit / cbs, first = (a.unit - h * cbs) * COLS;
-    const int cols = min(COLS, r.sq * p.group - first);
+    const bool complete = a.t0 == 0 && pieces[31 - __clz(members)].t1 == a.tiles;
     const int slot = a.t0 > 0 ? 0 : 1;
     if (!complete) {
       if (slot == 0) cut0 = s0; else cut1 = s0;
     }
-    const float unit = p.units != nullptr ? __ldg(p.units + p.n_kv_head + h) : 1.f;
-    const int n = __popc(members);
-    for (int ch = 0; ch * 128 < cols * D; ++ch, ++task) {
-      if (task % NW != warp) continue;
+    const int n = __popc(members), chunks = (a.cols * D + 127) / 128;
+    // chunk c of the group is task + c: this warp's are those that leave remainder `warp`
+#pragma unroll 1
+    for (int ch = (warp - task % NW + NW) % NW; ch < chunks; ch += NW) {
       const int e = ch * 128 + lane * 4;
-      if (e >= cols * D) continue;
+      if (e >= a.cols * D) continue;
       const int col = e / D;
       float x[4], m, l;
       // after the first piece, each further one is the next warp's leading piece
@@ -769,7 +834,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
       join4(n, col, [&](int i) { return piece_ml + index(i) * 2 * COLS; },
             [&](int i) { return *reinterpret_cast<const float4*>(piece_acc(index(i)) + e); }, x, m, l);
       if (complete) {
-        store_out4<T>(p, r, h, first + col, e - col * D, unit, x, l);
+        store_out4<T>(p, a, col, e - col * D, x, l);
       } else {
         float* part = cta_part + slot * partial_floats(D);
         if (e % D == 0) {
@@ -779,36 +844,35 @@ __global__ void __launch_bounds__(NW * 32, 1)
         *reinterpret_cast<float4*>(part + 2 * COLS + e) = make_float4(x[0], x[1], x[2], x[3]);
       }
     }
+    task += chunks;
   }
   if (cut0 < 0 && cut1 < 0) return;  // uniform
 
-  // ---- joins between CTAs: the last one to arrive at a unit joins its partials, in CTA order
-  __threadfence();
+  // ---- joins between CTAs: the last one to arrive at a unit joins its partials, in CTA order. One
+  // thread arrives for each cut; the barrier before it puts the CTA's stores ahead of its release.
+  __syncthreads();
+  if (lane == 0 && warp < 2) {
+    const int at = warp == 0 ? cut0 : cut1;
+    int last = 0;
+    if (at >= 0) {
+      const Piece& a = pieces[at];
+      const long long u0 = pre[a.row] + (long long)a.unit * a.tiles;
+      const int cta0 = split.run(u0), n = split.run(u0 + a.tiles - 1) - cta0 + 1;
+      last = atom_add_acq_rel(p.counters + cta0, 1u) == unsigned(n - 1);
+      if (last) p.counters[cta0] = 0u;  // zero again for the next launch
+      arrival[warp][1] = cta0;
+      arrival[warp][2] = n;
+    }
+    arrival[warp][0] = last;
+  }
   __syncthreads();
 #pragma unroll 1
   for (int s = 0; s < 2; ++s) {
-    const int at = s == 0 ? cut0 : cut1;
-    if (at < 0) continue;
-    const Piece a = pieces[at];
-    const int2 rw = rows[a.row];
-    const long long u0 = pre[a.row] + (long long)a.unit * rw.x, u1 = u0 + rw.x - 1;
-    // the CTA of tile f: the largest c with c * total / ctas <= f
-    const int cta0 = int(((u0 + 1) * ctas + total - 1) / total - 1);
-    const int n = int(((u1 + 1) * ctas + total - 1) / total - 1) - cta0 + 1;
-    if (tid == 0) {
-      const unsigned old = atomicAdd(p.counters + cta0, 1u);
-      last_flags[s] = old == unsigned(n - 1);
-      if (last_flags[s]) p.counters[cta0] = 0u;  // zero again for the next launch
-      __threadfence();
-    }
-    __syncthreads();
-    if (!last_flags[s]) continue;
-    const Row r = row_of(p, a.row);
-    const int cbs = rw.y / p.n_kv_head;
-    const int h = a.unit / cbs, first = (a.unit - h * cbs) * COLS;
-    const int cols = min(COLS, r.sq * p.group - first);
-    const float unit = p.units != nullptr ? __ldg(p.units + p.n_kv_head + h) : 1.f;
-    for (int e = tid * 4; e < cols * D; e += NW * 128) {
+    if (!arrival[s][0]) continue;
+    const Piece a = pieces[s == 0 ? cut0 : cut1];
+    const int cta0 = arrival[s][1], n = arrival[s][2];
+    // the cuts' elements side by side: the second's on the threads that the first's leave
+    for (int e = ((tid + (s == 0 ? 0 : NW * 16)) % (NW * 32)) * 4; e < a.cols * D; e += NW * 128) {
       const int col = e / D;
       float x[4], m, l;
       auto part = [&](int i) -> const float* {  // the first CTA's is its unit that goes on, the others' their first
@@ -816,7 +880,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
       };
       join4(n, col, part,
             [&](int i) { return __ldcg(reinterpret_cast<const float4*>(part(i) + 2 * COLS + e)); }, x, m, l);
-      store_out4<T>(p, r, h, first + col, e - col * D, unit, x, l);
+      store_out4<T>(p, a, col, e - col * D, x, l);
     }
   }
 }
