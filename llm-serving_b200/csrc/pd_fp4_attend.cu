@@ -35,7 +35,7 @@ cudaError_t launch_t(const Fp4AttendParams& p, int sms, cudaStream_t stream) {
     if (err != cudaSuccess) return err;
     if (dev < 64) attr_smem[dev] = bytes;
   }
-  fn<<<dim3(unsigned(sms)), NW * 32, bytes, stream>>>(p, stages, cols, 1);
+  fn<<<dim3(unsigned(sms)), NW * 32, bytes, stream>>>(p, stages, cols);
   return cudaGetLastError();
 }
 

@@ -33,8 +33,7 @@
 // acc) pieces that the CTA joins in shared memory; a unit cut between CTAs goes through the
 // workspace and the last CTA to arrive joins it, in piece order whoever arrives last, so results
 // do not depend on timing, and a CTA that is not last leaves. Where there are no more units than
-// CTAs and a CTA can take a unit in a few tiles per warp, each unit gets one CTA: the join
-// between CTAs (some 3 us of fences and arrivals) would cost more than it spreads.
+// CTAs, a unit may get a CTA of its own instead (JOIN_TILES).
 #pragma once
 
 #include "pd_fp4.cuh"
@@ -49,8 +48,13 @@ namespace fp4 {
 constexpr int MAX_ROWS = 1024;  // rows of one launch (their prefix sums are in shared memory)
 constexpr int COLS = 8;         // columns of a unit
 constexpr int TILE = 2 * FP4_TILE;  // keys of a warp's step: two records
-// Tiles per warp up to which a unit is one CTA's (when there are no more units than CTAs).
-constexpr int WHOLE_TILES = 4;
+// What a join between CTAs costs, in tiles of one CTA: where there are no more units than CTAs, units
+// stay whole if the longest is at most this much more than an even share. One row of 700 tokens (22
+// tiles, 8 units) takes 9.6 us whole and 9.9 cut, of 2048 (64 tiles) 14.5 and 10.0; 16 rows of 2048
+// (128 units) 15.4 and 18.3.
+constexpr int JOIN_TILES = 24;
+// Fewest tiles of a CTA where units are cut: one row of 2048 tokens takes 10.0 us with 8, 10.7 with 4.
+constexpr int CTA_TILES = 8;
 // A running maximum below every score: finite, so that exp2(score - maximum) needs no special case
 // for columns that have seen no key (their scores are -inf).
 constexpr float NO_MAX = -3.0e38f;
@@ -509,7 +513,7 @@ __device__ __forceinline__ unsigned atom_add_acq_rel(unsigned* p, unsigned v) {
 
 template <typename T, int D, int NW>
 __global__ void __launch_bounds__(NW * 32, 1)
-    pd_fp4_attend_kernel(const __grid_constant__ Fp4AttendParams p, int stages, int max_cols, int min_tiles) {
+    pd_fp4_attend_kernel(const __grid_constant__ Fp4AttendParams p, int stages, int max_cols) {
   constexpr int REC = fp4_record_bytes(D);
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ long long warp_sums[2][NW];
@@ -562,7 +566,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
       rows[lane] = w;
     }
     __syncwarp();
-    whole = units_total <= gridDim.x && longest <= WHOLE_TILES * NW;
+    whole = units_total <= gridDim.x && longest <= quotient(total, gridDim.x) + JOIN_TILES;
     row = __ffs(__ballot_sync(FULL_MASK, unit_incl > int(blockIdx.x))) - 1;
     row_unit = int(blockIdx.x) - __shfl_sync(FULL_MASK, unit_incl - w.y, row < 0 ? 0 : row);
   } else {
@@ -605,7 +609,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
       at += (long long)rows[b].x * rows[b].y;
     }
     __syncthreads();
-    whole = units_total <= gridDim.x && longest <= WHOLE_TILES * NW;
+    whole = units_total <= gridDim.x && longest <= quotient(total, gridDim.x) + JOIN_TILES;
     row = 0;
     row_unit = int(blockIdx.x);
     if (whole)
@@ -614,7 +618,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
   if (total == 0) return;
 
   // ---- this CTA's run of tiles and this warp's part of it
-  const long long wanted = whole ? units_total : quotient(total + NW * min_tiles - 1, NW * min_tiles);
+  const long long wanted = whole ? units_total : quotient(total + CTA_TILES - 1, CTA_TILES);
   const int ctas = int(wanted < gridDim.x ? wanted : gridDim.x);
   if (int(blockIdx.x) >= ctas) return;
   const Split split(total, ctas);  // where units are not whole CTAs'
@@ -627,7 +631,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
     c1 = split.begin(blockIdx.x + 1);
   }
   const int in_cta = int(c1 - c0);
-  const int warps = min(NW, (in_cta + min_tiles - 1) / min_tiles);
+  const int warps = min(NW, in_cta);
   const int wq = in_cta / warps, wr = in_cta - wq * warps;
   const long long f0 = c0 + warp * wq + min(warp, wr);
   const int count = warp < warps ? wq + (warp < wr ? 1 : 0) : 0;
