@@ -61,17 +61,20 @@ int rows_common(Fp4RowsParams& p, int dtype, bool read, const int64_t* k_strides
 }
 
 // Whether a chunk call runs on tcgen05 tiles. Per visible key, the warp kernel's time goes with the
-// 8-column units of query rows over the SMs (about A clocks for each at 32 keys), the tile
-// kernel's with the waves of its CTAs, one block of 256 (at head_dim 256: 128) query rows each
-// (about B clocks at 128 keys). Lengths stay on the device, but both times are proportional to
-// them, so the comparison needs only the counts the host has.
+// 8-column units of query rows per SM, the tile kernel's with the waves of its CTAs, one block of 256
+// (at head_dim 256: 128) query rows each, whatever part of the block is filled; a wave costs what
+// WAVE_UNITS units per SM cost. Lengths stay on the device, but both times are proportional to them, so the
+// comparison needs only the counts the host has. Measured, warp kernel and tiles, 16 heads on 8 of 128
+// with 2048 keys: 16 rows of 8 tokens (2.2 units per SM, one wave) 28.6 and 42.6 us, of 16 (3.9) 42.8 and
+// 42.7, of 32 (7.4) 72.9 and 43.2, one row of 1024 tokens (13.9) 185 and 60; 8 heads on 2 of 256: 16 rows
+// of 16 tokens (1.8) 43.7 and 57.3, of 32 (3.6) 72.1 and 58.6.
 bool use_tiles(int64_t total_q, int32_t max_seqlen_q, int32_t batch, int32_t n_kv_head, int32_t group,
                int32_t head_dim, int sms) {
-  constexpr double A = 260.0 / 32, B = 2600.0 / 128;
+  const double WAVE_UNITS = head_dim == 256 ? 2.7 : 4.0;
+  const int64_t block = head_dim == 256 ? 128 : 256;
   const double units = double(n_kv_head) * (double(total_q) * group / 8 + 0.5 * batch);
-  const int64_t block = 128;
   const int64_t ctas = int64_t(batch) * n_kv_head * ((int64_t(max_seqlen_q) * group + block - 1) / block);
-  return double((ctas + sms - 1) / sms) * B < units / sms * A;
+  return double((ctas + sms - 1) / sms) * WAVE_UNITS < units / sms;
 }
 
 int attend_common(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, const void* pages, int64_t n_blocks, int32_t block_size,
