@@ -13,13 +13,18 @@ the down projection; then the final norm, the tied lm_head and a greedy argmax.
 
 :meth:`PagedDecoder.step` only reads and writes fixed buffers, so a whole step can be captured
 with :class:`serve.graph.DecodeStepGraph`; the next step's input token is this step's argmax on
-the device. This is not part of the library (``bench.py`` and ``tests/`` import it).
+the device. Over a 4-bit cache (:class:`model.paged_fp4.Fp4KV`) the step normalises and rotates q and k
+in one launch (``model.qk_norm.qk_norm_rope``), and :meth:`PagedDecoder.prefill` runs prompt chunks.
+This is not part of the library (``bench.py``, ``sample_fp4.py`` and ``tests/`` import it).
 """
 
 from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+
+from model.paged_fp4 import Fp4KV
+from model.qk_norm import qk_norm_rope
 
 VOCAB, HIDDEN, INTER = 151936, 1024, 3072
 THETA, EPS = 1e6, 1e-6
@@ -34,11 +39,11 @@ def rope_tables(n_pos: int, rotary: int, device):
 
 
 class PagedDecoder:
-    """Random-init decoder of ``n_layer`` layers over a :class:`PagedKV` of matching heads."""
+    """Random-init decoder of ``n_layer`` layers over a :class:`PagedKV` of matching heads (``None``: none
+    yet, see :meth:`attach`)."""
 
     def __init__(self, kv, *, n_layer: int, n_head: int, n_kv_head: int, head_dim: int, rotary: int,
                  max_pos: int, seed: int = 0, device="cuda"):
-        self.kv = kv
         self.n_layer, self.h, self.hkv, self.d, self.rotary = n_layer, n_head, n_kv_head, head_dim, rotary
         gen = torch.Generator(device=device).manual_seed(seed)
 
@@ -53,10 +58,16 @@ class PagedDecoder:
                        for _ in range(n_layer)]
         self.norm = ones(HIDDEN)
         self.cos, self.sin = rope_tables(max_pos, rotary, device)
-        B = kv.batch
+        if kv is not None:
+            self.attach(kv)
+
+    def attach(self, kv) -> None:
+        """Step over container ``kv`` from now on, with new step buffers."""
+        self.kv = kv
+        B, device = kv.batch, self.embed.device
         self.tok = torch.zeros(B, dtype=torch.long, device=device)   # input token of the step
         self.next = torch.zeros(B, dtype=torch.long, device=device)  # greedy output of the step
-        self.prepare_q = torch.zeros(B, n_head, 1, head_dim, dtype=torch.bfloat16, device=device)
+        self.prepare_q = torch.zeros(B, self.h, 1, self.d, dtype=torch.bfloat16, device=device)
 
     @staticmethod
     def _rms(x, w):
@@ -71,9 +82,57 @@ class PagedDecoder:
         out = qr * cos + rotated * sin
         return out if r == q.shape[-1] else torch.cat([out, q[..., r:]], dim=-1)
 
+    def _qkv(self, h, L, positions):
+        """Normalised and rotated q ``(T, H, D)`` and k, and v, of tokens at ``positions``."""
+        H, HKV, D = self.h, self.hkv, self.d
+        qkv = (h @ L["wqkv"].T).view(-1, H + 2 * HKV, D)
+        q, k, v = qkv.split((H, HKV, HKV), dim=1)
+        q, k = qk_norm_rope(q, k, L["qn"], L["kn"], self.cos, self.sin, positions, eps=EPS, rotary_dim=self.rotary,
+                            q_out=q, k_out=k)
+        return q, k, v
+
+    def _mlp(self, x, L):
+        gu = self._rms(x, L["ln2"]) @ L["wgu"].T
+        return x + (F.silu(gu[:, :INTER]) * gu[:, INTER:]) @ L["wd"].T
+
+    def prefill(self, pool, chunks, tables, starts) -> torch.Tensor:
+        """Run a chunk of prompt tokens per row (lists of ids; row ``b`` starts at position ``starts[b]`` of
+        block table ``tables[b]``) through every layer, its K/V into ``pool`` (an ``Fp4Pool``). Returns
+        the logits ``(B, VOCAB)`` after each row's last token."""
+        device, bs = self.embed.device, pool.block_size
+        ends = [s + len(c) for s, c in zip(starts, chunks)]
+        position = [s + i for s, c in zip(starts, chunks) for i in range(len(c))]
+        slot = [t[p // bs] * bs + p % bs for t, s, e in zip(tables, starts, ends) for p in range(s, e)]
+        offset = torch.tensor([0] + [len(c) for c in chunks]).cumsum(0)
+        ids, positions, slots = torch.tensor([[i for c in chunks for i in c], position, slot]).to(device)
+        width = max(len(t) for t in tables)
+        table = torch.tensor([list(t) + [0] * (width - len(t)) for t in tables], dtype=torch.int32).to(device)
+        cu, seqlen = offset.to(device, torch.int32), torch.tensor(ends, dtype=torch.int32).to(device)
+        longest = max(len(c) for c in chunks)
+        x = self.embed[ids]
+        for li, L in enumerate(self.layers):
+            q, k, v = self._qkv(self._rms(x, L["ln1"]), L, positions)
+            pool.write_slots(li, slots, k, v)
+            a = pool.prefill(li, q, table, cu, seqlen, longest)
+            x = self._mlp(x + a.flatten(1) @ L["wo"].T, L)
+        return self._rms(x[offset[1:].to(device) - 1], self.norm) @ self.embed.T
+
+    def _step_fp4(self) -> None:
+        kv = self.kv
+        x = self.embed[self.tok]  # (B, HIDDEN)
+        for li, L in enumerate(self.layers):
+            q, k, v = self._qkv(self._rms(x, L["ln1"]), L, kv.pos)
+            kv.write(li, k.unsqueeze(2), v.unsqueeze(2))
+            a = kv.attend(li, q.unsqueeze(2))
+            x = self._mlp(x + a.flatten(1) @ L["wo"].T, L)
+        torch.argmax(self._rms(x, self.norm) @ self.embed.T, dim=-1, out=self.next)
+        self.tok.copy_(self.next)
+
     def step(self) -> None:
         """One greedy decode step of every row: reads :attr:`tok`, writes :attr:`next`. Call it
         between ``kv.build_mask(next_token=True)`` and ``kv.advance()``."""
+        if isinstance(self.kv, Fp4KV):
+            return self._step_fp4()
         kv = self.kv
         B, H, HKV, D = kv.batch, self.h, self.hkv, self.d
         pos = kv.pos  # the position this step's token is written at

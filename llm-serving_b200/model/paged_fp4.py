@@ -31,6 +31,7 @@ import torch
 from model import _native
 from model.paged import PagedKV, PagedPool, _positive
 from model.triton_decode import _pow2, _raise_first
+from serve.block_copy import copy_blocks
 
 __all__ = ["Fp4KV", "Fp4Pool", "fp4_pages", "fp4_workspace", "paged_decode_fp4", "paged_prefill_fp4", "read_slots_fp4",
            "write_slots_fp4"]
@@ -223,6 +224,17 @@ class Fp4KV(PagedKV):
             if violated:
                 raise error(message)
         return self._decode(layer, q, out)
+
+    def move_blocks(self, src, dst, remap) -> None:
+        """Carry out a compaction plan (``SharedBlockManager.compact()``) on the pool and on this
+        container's block table, in one launch; a captured step stays valid. Other holders of the
+        pool's blocks renumber theirs by ``remap``."""
+        if len(remap) != self.pool.n_blocks:
+            raise ValueError(f"remap must have one entry per block ({self.pool.n_blocks}), got {len(remap)}")
+        copy_blocks(self.pool, src, dst, block_table=self._block_table_tensor,
+                    remap=torch.tensor(remap, dtype=torch.int32, device=self.device))
+        self.block_tables = [[remap[i] for i in table] for table in self.block_tables]
+        self._slot_cache = None
 
     def _decode(self, layer: int, q: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         layer = self.pool._check_layer(layer)
