@@ -221,10 +221,14 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
     most = max(most, tiles[q]);
   }
 
-  tc::fence_before_sync();
-  __syncthreads();
-  tc::fence_after_sync();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + Bars::TMEM_SLOT);
+  // Every role meets here once, with its first loads already in flight; returns the TMEM address.
+  auto meet = [&]() -> uint32_t {
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    return *reinterpret_cast<volatile uint32_t*>(smem + Bars::TMEM_SLOT);
+  };
+  uint32_t tmem;
   auto k_addr = [&](int s) -> uint32_t { return sbase + uint32_t(C::OFF_K + s * C::KV_BYTES); };
   auto v_addr = [&](int s) -> uint32_t { return sbase + uint32_t(C::OFF_V + s * C::KV_BYTES); };
   auto fail = [&]() {
@@ -232,8 +236,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
     atomicOr(p.err, DEVERR_WAIT_TIMEOUT);
   };
 
-  if (row0 >= rows) {
-    // no query row
+  if (row0 >= rows) {  // no query row
+    tmem = meet();
   } else if (warp >= C::SOFTMAX_WARPS && warp < C::MMA_WARP) {
     // ---------------------------------------------------------------- decoding warps
     const int t = tid - C::SOFTMAX_WARPS * 32;
@@ -268,6 +272,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
     const uint32_t v_row = uint32_t((v_gr >> 2) * (KT * 128) + v_tok * 128);
     const uint32_t v_x = uint32_t((((v_gr & 3) * 2 + (v_odd ? 1 : 0)) ^ (v_tok & 7)) << 4);
 
+    // a negative scale's sign goes into K, so that the score multiplier is never negative
+    const uint32_t k_sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;
     uint4 kraw[N], vraw[N];
     uint32_t ksc[N], vsc[N];
     int blk[N], blk_next[N];
@@ -300,6 +306,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
     for (int i = 0; i < N; ++i) blk[i] = block_of(1, i);
 #pragma unroll
     for (int i = 0; i < N; ++i) blk_next[i] = block_of(2, i);
+    tmem = meet();
     bool ok = true;
     for (int j = 0; ok && j < most; ++j) {
       if (__any_sync(FULL_MASK, *abort_flag != 0)) break;
@@ -311,7 +318,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const uint32_t pair = e4m3x2_to_half2(ksc[i]);
+        const uint32_t pair = e4m3x2_to_half2(ksc[i]) ^ k_sign;
         const uint32_t sc[2] = {__byte_perm(pair, 0, 0x1010), __byte_perm(pair, 0, 0x3232)};
         const uint32_t w[4] = {kraw[i].x, kraw[i].y, kraw[i].z, kraw[i].w};
         const uint32_t row = k_addr(s) + k_row + uint32_t((first_rec + i * REC_STEP) * 2048);
@@ -365,6 +372,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
     // ---------------------------------------------------------------- MMA issuer
     // The whole warp runs this loop and one elected lane issues, so descriptors and addresses stay
     // uniform over the warp and no operand of an MMA is moved on its own.
+    tmem = meet();
     if (most > 0) {
       constexpr uint32_t IDESC_S = tc::instr_desc_f16(false, ROWS, KT, false, false);
       constexpr uint32_t IDESC_PV = tc::instr_desc_f16(false, ROWS, D, false, true);
@@ -440,62 +448,74 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
     const int r = (warp & 3) * 32 + lane;  // row of the block = TMEM lane
     const int n = row0 + q * ROWS + r;
     const bool live = n < rows;
-    const int tok = live ? n / p.group : 0, hg = live ? n - tok * p.group : 0;
-    const int64_t hq = int64_t(h) * p.group + hg;
-    float down;  // 1 / the row's power of two
+    const int tok = live ? n / p.group : 0;
+    float down = 1.f;  // 1 / the row's power of two
+    // Q as it is into its place (16-byte units of 8 elements, all copies in flight at once); bf16 rows are
+    // then turned into fp16 where they stand, a thread its own row.
+    constexpr int LANES = D / 8, STEP = 128 / LANES;
+    const uint32_t q_base = sbase + uint32_t(C::OFF_Q + q * C::Q_BYTES);
     {
-      // Q as it is into its place (16-byte units of 8 elements, all copies in flight at once), then
-      // each thread turns its own row into fp16 where it stands. Loops, not straight-line code: what
-      // runs once per CTA is fetched slower than it runs.
-      constexpr int LANES = D / 8, STEP = 128 / LANES;
-      const uint32_t q_base = sbase + uint32_t(C::OFF_Q + q * C::Q_BYTES);
-      {
-        const int t = tid - q * 128, u = t % LANES;
-        const int m0 = row0 + q * ROWS + t / LANES;
-        int mt = m0 / p.group, mh = m0 - mt * p.group;
-        const int dt = STEP / p.group, dh = STEP - dt * p.group;
-        const T* base = reinterpret_cast<const T*>(p.q) + int64_t(q_begin) * p.q_st + int64_t(h) * p.group * p.q_sh + u * 8;
+      const int t = tid - q * 128, u = t % LANES;
+      const int m0 = row0 + q * ROWS + t / LANES;
+      int mt = m0 / p.group, mh = m0 - mt * p.group;
+      const int dt = STEP / p.group, dh = STEP - dt * p.group;
+      const T* base = reinterpret_cast<const T*>(p.q) + int64_t(q_begin) * p.q_st + int64_t(h) * p.group * p.q_sh + u * 8;
 #pragma unroll 4
-        for (int rr = t / LANES; rr < ROWS; rr += STEP) {
-          const bool in = row0 + q * ROWS + rr < rows;
-          cp_async16(q_base + uint32_t((u >> 3) * (ROWS * 128)) + sw128(rr, u & 7),
-                     base + (in ? int64_t(mt) * p.q_st + int64_t(mh) * p.q_sh : 0), in);
-          mt += dt;
-          mh += dh;
-          if (mh >= p.group) {
-            mh -= p.group;
-            ++mt;
-          }
+      for (int rr = t / LANES; rr < ROWS; rr += STEP) {
+        const bool in = row0 + q * ROWS + rr < rows;
+        cp_async16(q_base + uint32_t((u >> 3) * (ROWS * 128)) + sw128(rr, u & 7),
+                   base + (in ? int64_t(mt) * p.q_st + int64_t(mh) * p.q_sh : 0), in);
+        mt += dt;
+        mh += dh;
+        if (mh >= p.group) {
+          mh -= p.group;
+          ++mt;
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + q) : "memory");  // the block's rows are in
       }
-      float top = 0.f;
-#pragma unroll 4
-      for (int u = 0; u < D / 8; ++u) {
-        float x[8];
-        E::unpack(lds128(q_base + uint32_t((u >> 3) * (ROWS * 128)) + sw128(r, u & 7)), x);
+    }
+    tmem = meet();
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + q) : "memory");  // the block's rows are in
+      constexpr int KEEP = LANES < 16 ? LANES : 16;  // units of a row in registers at a time
+      auto unit = [&](int u) -> uint32_t { return q_base + uint32_t((u >> 3) * (ROWS * 128)) + sw128(r, u & 7); };
+      uint4 w[KEEP];
+      __nv_bfloat162 top2 = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll 1
+      for (int u0 = LANES - KEEP; u0 >= 0; u0 -= KEEP) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(x[k]));
+        for (int i = 0; i < KEEP; ++i) w[i] = lds128(unit(u0 + i));
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i) {
+          const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(&w[i]);
+          const __nv_bfloat162 m = __hmax2(__hmax2(__habs2(v[0]), __habs2(v[1])), __hmax2(__habs2(v[2]), __habs2(v[3])));
+          top2 = __hmax2(top2, m);
+        }
       }
+      const float top = fmaxf(__low2float(top2), __high2float(top2));
       int e = int(__float_as_uint(top) >> 23);
       e = e == 0 || e == 255 ? 140 : e;
       const int shift = max(-100, min(100, 140 - e));
-      // a negative scale's sign goes into q, so that the score multiplier is never negative
-      const float up = copysignf(__uint_as_float(uint32_t(127 + shift) << 23), p.scale_log2);
+      const float up = __uint_as_float(uint32_t(127 + shift) << 23);
       down = __uint_as_float(uint32_t(127 - shift) << 23);
-#pragma unroll 4
-      for (int u = 0; u < D / 8; ++u) {
-        const uint32_t a = q_base + uint32_t((u >> 3) * (ROWS * 128)) + sw128(r, u & 7);
-        float x[8];
-        E::unpack(lds128(a), x);
-        sts128(a, Elem<__half>::pack2(x[0] * up, x[1] * up), Elem<__half>::pack2(x[2] * up, x[3] * up),
-               Elem<__half>::pack2(x[4] * up, x[5] * up), Elem<__half>::pack2(x[6] * up, x[7] * up));
+#pragma unroll 1
+      for (int u0 = 0; u0 < LANES; u0 += KEEP) {
+        if (u0 > 0) {
+#pragma unroll
+          for (int i = 0; i < KEEP; ++i) w[i] = lds128(unit(u0 + i));
+        }
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i) {
+          float x[8];
+          E::unpack(w[i], x);
+          sts128(unit(u0 + i), Elem<__half>::pack2(x[0] * up, x[1] * up), Elem<__half>::pack2(x[2] * up, x[3] * up),
+                 Elem<__half>::pack2(x[4] * up, x[5] * up), Elem<__half>::pack2(x[6] * up, x[7] * up));
+        }
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(Bars::Q_FULL));
     }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(Bars::Q_FULL));
     // never zero (a scale of 0 gives scores below 2^-80 instead), so that a hidden key's -inf stays one
     const float mul = fmaxf(fabsf(p.scale_log2) * (p.units != nullptr ? __ldg(p.units + h) : 1.f) * down, 1.2e-38f);
     const int lim = live ? lk - chunk + tok : lk - 1;  // last visible key; padding rows see any
@@ -608,7 +628,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       tc::fence_after_sync();
       const float unit = p.units != nullptr ? __ldg(p.units + p.n_kv_head + h) : 1.f;
       const float inv = l_run > 0.f ? unit / l_run : 0.f;
-      T* dst = reinterpret_cast<T*>(p.out) + int64_t(q_begin + tok) * p.o_st + hq * p.o_sh;
+      // Through the warp's own 32 rows of the Q tile, which no MMA reads any more: stores of whole rows.
+      // (A thread storing its own row meets 32 lines with every store: 2 us per CTA.)
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
@@ -619,15 +640,31 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
-        if (live) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint32_t w[4];
+        for (int u = 0; u < 4; ++u) {
+          uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = E::pack2(__uint_as_float(o[8 * u + 2 * i]) * inv, __uint_as_float(o[8 * u + 2 * i + 1]) * inv);
-            *reinterpret_cast<uint4*>(dst + c + 8 * u) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          for (int i = 0; i < 4; ++i)
+            w[i] = E::pack2(__uint_as_float(o[8 * u + 2 * i]) * inv, __uint_as_float(o[8 * u + 2 * i + 1]) * inv);
+          const int at = c / 8 + u;
+          sts128(q_base + uint32_t((at >> 3) * (ROWS * 128)) + sw128(r, at & 7), w[0], w[1], w[2], w[3]);
+        }
+      }
+      __syncwarp();
+      constexpr int AT_ONCE = 32 / LANES;  // rows of a store
+      const int u = lane % LANES, r0 = (warp & 3) * 32 + lane / LANES, m0 = row0 + q * ROWS + r0;
+      int mt = m0 / p.group, mh = m0 - mt * p.group;
+      const int dt = AT_ONCE / p.group, dh = AT_ONCE - dt * p.group;
+      T* base = reinterpret_cast<T*>(p.out) + int64_t(q_begin) * p.o_st + int64_t(h) * p.group * p.o_sh + u * 8;
+#pragma unroll 4
+      for (int i = 0; i < 32; i += AT_ONCE) {
+        const uint4 w = lds128(q_base + uint32_t((u >> 3) * (ROWS * 128)) + sw128(r0 + i, u & 7));
+        if (m0 + i < rows) *reinterpret_cast<uint4*>(base + int64_t(mt) * p.o_st + int64_t(mh) * p.o_sh) = w;
+        mt += dt;
+        mh += dh;
+        if (mh >= p.group) {
+          mh -= p.group;
+          ++mt;
         }
       }
     }
