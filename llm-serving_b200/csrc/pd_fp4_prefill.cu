@@ -203,6 +203,21 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
   const int b = int(blockIdx.x) % p.batch;
   const int h = (int(blockIdx.x) / p.batch) % p.n_kv_head;
   const int qblock = blocks - 1 - int(blockIdx.x) / pairs;
+  // Unit i of decoding thread t is unit u of record first_rec + i * REC_STEP of the tile. The first
+  // tile's block ids are loaded beside the lengths; whether a record is the row's is asked later.
+  constexpr int N = C::PER_THREAD;
+  constexpr int REC_STEP = C::DECODERS / C::PER_RECORD;
+  const int t = tid - C::SOFTMAX_WARPS * 32, u = t % C::PER_RECORD, first_rec = t / C::PER_RECORD;
+  const int32_t* trow = p.table + int64_t(b) * p.bt_stride;
+  auto block_of = [&](int tile, int i) -> int {
+    const int page = (tile * (KT / 16) + first_rec + i * REC_STEP) >> p.log2_tpb;
+    return page < p.max_blocks ? __ldg(trow + page) : -1;
+  };
+  int blk[N];
+  if (warp >= C::SOFTMAX_WARPS && warp < C::MMA_WARP) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) blk[i] = block_of(0, i);
+  }
   const int q_begin = min(max(__ldg(p.cu_q + b), 0), p.total_q);
   const int chunk = max(min(max(__ldg(p.cu_q + b + 1), 0), p.total_q) - q_begin, 0);
   const int sq = min(chunk, p.max_seqlen_q);
@@ -240,20 +255,10 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
     tmem = meet();
   } else if (warp >= C::SOFTMAX_WARPS && warp < C::MMA_WARP) {
     // ---------------------------------------------------------------- decoding warps
-    const int t = tid - C::SOFTMAX_WARPS * 32;
-    constexpr int N = C::PER_THREAD;
-    const int32_t* trow = p.table + int64_t(b) * p.bt_stride;
     const int tpb_mask = (1 << p.log2_tpb) - 1;
     const int records = (lk + FP4_TILE - 1) / FP4_TILE;
     const unsigned char* head = p.pages + (int64_t(h) << p.log2_tpb) * REC;
     const uint32_t block_stride = uint32_t(p.n_kv_head << p.log2_tpb) * REC;
-    // Unit i of this thread is unit u of record first_rec + i * REC_STEP of the tile.
-    constexpr int REC_STEP = C::DECODERS / C::PER_RECORD;
-    const int u = t % C::PER_RECORD, first_rec = t / C::PER_RECORD;
-    auto block_of = [&](int tile, int i) -> int {
-      const int rec = tile * (KT / 16) + first_rec + i * REC_STEP, page = rec >> p.log2_tpb;
-      return tile < most && rec < records && page < p.max_blocks ? __ldg(trow + page) : -1;
-    };
     // K unit: 32 elements of token k_tok, 16 tokens side by side, so that a quarter-warp's stores go
     // to eight rows and, swizzled, to eight banks.
     constexpr int W = D < 128 ? D : 128, CH = W / 32;  // 16-byte chunks of a token in a block
@@ -276,13 +281,13 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
     const uint32_t k_sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;
     uint4 kraw[N], vraw[N];
     uint32_t ksc[N], vsc[N];
-    int blk[N], blk_next[N];
+    int blk_next[N];
     const unsigned char* ptr[N];  // the records being loaded, or nullptr
     auto aim = [&](int tile) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int rec = tile * (KT / 16) + first_rec + i * REC_STEP;
-        ptr[i] = blk[i] >= 0 && blk[i] < p.n_blocks ? head + uint64_t(blk[i]) * block_stride + (rec & tpb_mask) * REC
+        ptr[i] = rec < records && blk[i] >= 0 && blk[i] < p.n_blocks ? head + uint64_t(blk[i]) * block_stride + (rec & tpb_mask) * REC
                                                     : nullptr;
       }
     };
@@ -297,8 +302,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
         }
       }
     };
-#pragma unroll
-    for (int i = 0; i < N; ++i) blk[i] = block_of(0, i);
     aim(0);
     load(kraw, ksc, k_code_off, k_scale_off);
     load(vraw, vsc, v_code_off, v_scale_off);
@@ -518,6 +521,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
     if (lane == 0) mbar_arrive(bar(Bars::Q_FULL));
     // never zero (a scale of 0 gives scores below 2^-80 instead), so that a hidden key's -inf stays one
     const float mul = fmaxf(fabsf(p.scale_log2) * (p.units != nullptr ? __ldg(p.units + h) : 1.f) * down, 1.2e-38f);
+    const float v_unit = p.units != nullptr ? __ldg(p.units + p.n_kv_head + h) : 1.f;
     const int lim = live ? lk - chunk + tok : lk - 1;  // last visible key; padding rows see any
     const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t o_tmem = lane_base + uint32_t(C::O_COL + q * D);
@@ -548,7 +552,12 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
         tc::wait_ld();
         if (!open) {
 #pragma unroll
-          for (int i = 0; i < H; ++i) x[i] = j * KT + c0 + i <= lim ? x[i] : -INFINITY;
+          for (int c = 0; c < H; c += 32) {
+            const int seen = lim - (j * KT + c0 + c);  // the last visible of these columns
+            if (__all_sync(FULL_MASK, seen >= 31)) continue;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[c + i] = i <= seen ? x[c + i] : -INFINITY;
+          }
         }
       };
       auto max_half = [&]() -> float {
@@ -626,8 +635,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       if (lane == 0) fail();
     } else {
       tc::fence_after_sync();
-      const float unit = p.units != nullptr ? __ldg(p.units + p.n_kv_head + h) : 1.f;
-      const float inv = l_run > 0.f ? unit / l_run : 0.f;
+      const float inv = l_run > 0.f ? v_unit / l_run : 0.f;
       // Through the warp's own 32 rows of the Q tile, which no MMA reads any more: stores of whole rows.
       // (A thread storing its own row meets 32 lines with every store: 2 us per CTA.)
 #pragma unroll 1
