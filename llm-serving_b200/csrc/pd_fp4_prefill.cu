@@ -49,7 +49,15 @@ struct Cfg {
   static constexpr int DECODE_WARPS = 4;
   static constexpr int DECODERS = DECODE_WARPS * 32;
   static constexpr int MMA_WARP = SOFTMAX_WARPS + DECODE_WARPS;
-  static constexpr int THREADS = (MMA_WARP + 1) * 32;
+  static constexpr int THREADS = (MMA_WARP + 4) * 32;  // the MMA warp's group of four: three are idle
+  // Registers are dealt anew between the groups, so that a softmax thread holds a row's KT scores: with
+  // 128 for everyone it had to read half of them twice, 99 us against 94 on the 1001-token chunks.
+  static constexpr int LAUNCH_REGS = 65536 / THREADS / 8 * 8;
+  static constexpr int SOFTMAX_REGS = NQ == 2 ? 184 : 208;
+  static constexpr int DECODE_REGS = NQ == 2 ? 96 : 112;
+  static constexpr int MMA_REGS = 48;
+  static_assert(SOFTMAX_WARPS * SOFTMAX_REGS + DECODE_WARPS * DECODE_REGS + 4 * MMA_REGS <= THREADS / 32 * LAUNCH_REGS,
+                "a split above the launch's registers would wait for ever");
   static constexpr int STAGES = 2;  // decoded tiles of K, and of V
   static constexpr int Q_BYTES = ROWS * D * 2;
   static constexpr int KV_BYTES = KT * D * 2;
@@ -106,6 +114,16 @@ __device__ __forceinline__ bool slow_wait(uint32_t bar, uint32_t parity, unsigne
 __device__ __forceinline__ bool lane_wait(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
   if (limit_ns < TEST_LIMIT_NS) return false;
   return mbar_try_wait(bar, parity) || slow_wait(bar, parity, limit_ns);
+}
+
+// A warpgroup's registers from here on.
+template <int REGS>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -255,6 +273,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
     tmem = meet();
   } else if (warp >= C::SOFTMAX_WARPS && warp < C::MMA_WARP) {
     // ---------------------------------------------------------------- decoding warps
+    regs_down<C::DECODE_REGS>();
     const int tpb_mask = (1 << p.log2_tpb) - 1;
     const int records = (lk + FP4_TILE - 1) / FP4_TILE;
     const unsigned char* head = p.pages + (int64_t(h) << p.log2_tpb) * REC;
@@ -371,82 +390,88 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       if (lane == 0) mbar_arrive(bar(Bars::V_FULL + s));
     }
     if (!ok && lane == 0) fail();
-  } else if (warp == C::MMA_WARP) {
-    // ---------------------------------------------------------------- MMA issuer
-    // The whole warp runs this loop and one elected lane issues, so descriptors and addresses stay
-    // uniform over the warp and no operand of an MMA is moved on its own.
-    tmem = meet();
-    if (most > 0) {
-      constexpr uint32_t IDESC_S = tc::instr_desc_f16(false, ROWS, KT, false, false);
-      constexpr uint32_t IDESC_PV = tc::instr_desc_f16(false, ROWS, D, false, true);
-      bool ok = lane_wait(bar(Bars::Q_FULL), 0u, p.wait_ns);
-      const uint64_t q_desc = tc::smem_desc(sbase + C::OFF_Q, 16u, 1024u);
-      const uint64_t k_desc = tc::smem_desc(k_addr(0), 16u, 1024u);
-      const uint64_t v_desc = tc::smem_desc(v_addr(0), uint32_t(KT * 128), 1024u);
-      // (block q, tile j) uses S/P buffer q for the j-th time or, with one block, buffer j % 2 for
-      // the j / 2-th.
-      auto buf = [&](int q, int j) -> int { return NQ == 2 ? q : j & 1; };
-      auto use = [&](int j) -> uint32_t { return NQ == 2 ? uint32_t(j) : uint32_t(j >> 1); };
-      // S of (q, j), once P V of the buffer's previous use has read its P
-      auto issue_s = [&](int q, int j) {
-        const int s = j & 1, sb = buf(q, j);
-        if (q == 0 || j >= tiles[0])  // else the first block has waited for this K tile
-          ok = ok && lane_wait(bar(Bars::K_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns);
-        if (use(j) > 0) ok = ok && lane_wait(bar(Bars::O_DONE + sb), (use(j) - 1) & 1u, p.wait_ns);
-        __syncwarp();
-        tc::fence_after_sync();
-        const uint64_t a0 = q_desc + uint64_t((q * C::Q_BYTES) >> 4), b0 = k_desc + uint64_t((s * C::KV_BYTES) >> 4);
-        const bool frees = q == NQ - 1 || j >= tiles[NQ - 1];  // the last block that uses this K tile
-        if (elect_one()) {
+  } else if (warp >= C::MMA_WARP) {
+    regs_down<C::MMA_REGS>();
+    if (warp > C::MMA_WARP) {
+      tmem = meet();
+    } else {  // (one meeting before the branch costs the compiler 150 bytes of spills)
+      // ---------------------------------------------------------------- MMA issuer
+      // The whole warp runs this loop and one elected lane issues, so descriptors and addresses stay
+      // uniform over the warp and no operand of an MMA is moved on its own.
+      tmem = meet();
+      if (most > 0) {
+        constexpr uint32_t IDESC_S = tc::instr_desc_f16(false, ROWS, KT, false, false);
+        constexpr uint32_t IDESC_PV = tc::instr_desc_f16(false, ROWS, D, false, true);
+        bool ok = lane_wait(bar(Bars::Q_FULL), 0u, p.wait_ns);
+        const uint64_t q_desc = tc::smem_desc(sbase + C::OFF_Q, 16u, 1024u);
+        const uint64_t k_desc = tc::smem_desc(k_addr(0), 16u, 1024u);
+        const uint64_t v_desc = tc::smem_desc(v_addr(0), uint32_t(KT * 128), 1024u);
+        // (block q, tile j) uses S/P buffer q for the j-th time or, with one block, buffer j % 2 for
+        // the j / 2-th.
+        auto buf = [&](int q, int j) -> int { return NQ == 2 ? q : j & 1; };
+        auto use = [&](int j) -> uint32_t { return NQ == 2 ? uint32_t(j) : uint32_t(j >> 1); };
+        // S of (q, j), once P V of the buffer's previous use has read its P
+        auto issue_s = [&](int q, int j) {
+          const int s = j & 1, sb = buf(q, j);
+          if (q == 0 || j >= tiles[0])  // else the first block has waited for this K tile
+            ok = ok && lane_wait(bar(Bars::K_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns);
+          if (use(j) > 0) ok = ok && lane_wait(bar(Bars::O_DONE + sb), (use(j) - 1) & 1u, p.wait_ns);
+          __syncwarp();
+          tc::fence_after_sync();
+          const uint64_t a0 = q_desc + uint64_t((q * C::Q_BYTES) >> 4), b0 = k_desc + uint64_t((s * C::KV_BYTES) >> 4);
+          const bool frees = q == NQ - 1 || j >= tiles[NQ - 1];  // the last block that uses this K tile
+          if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks)
-            tc::mma_f16_ss(tmem + uint32_t(sb * KT), a0 + uint64_t(((ks >> 2) * (ROWS * 128) + (ks & 3) * 32) >> 4),
-                           b0 + uint64_t(((ks >> 2) * (KT * 128) + (ks & 3) * 32) >> 4), IDESC_S, ks > 0);
-          tc::commit(bar(Bars::S_FULL + sb));
-          if (frees) tc::commit(bar(Bars::K_EMPTY + s));
+            for (int ks = 0; ks < D / 16; ++ks)
+              tc::mma_f16_ss(tmem + uint32_t(sb * KT), a0 + uint64_t(((ks >> 2) * (ROWS * 128) + (ks & 3) * 32) >> 4),
+                             b0 + uint64_t(((ks >> 2) * (KT * 128) + (ks & 3) * 32) >> 4), IDESC_S, ks > 0);
+            tc::commit(bar(Bars::S_FULL + sb));
+            if (frees) tc::commit(bar(Bars::K_EMPTY + s));
+          }
+          __syncwarp();
+        };
+        auto issue_pv = [&](int q, int j) {
+          const int s = j & 1, sb = buf(q, j);
+          if (q == 0 || j >= tiles[0])
+            ok = ok && lane_wait(bar(Bars::V_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns);
+          ok = ok && lane_wait(bar(Bars::P_FULL + sb), use(j) & 1u, p.wait_ns);
+          __syncwarp();
+          tc::fence_after_sync();
+          const uint64_t b0 = v_desc + uint64_t((s * C::KV_BYTES) >> 4);
+          const bool frees = q == NQ - 1 || j >= tiles[NQ - 1];
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < KT / 16; ++kk)
+              tc::mma_f16_ts(tmem + uint32_t(C::O_COL + q * D), tmem + uint32_t(sb * KT + KT / 2 + kk * 8),
+                             b0 + uint64_t((kk * 2048) >> 4), IDESC_PV, j > 0 || kk > 0);
+            tc::commit(bar(Bars::O_DONE + sb));
+            if (frees) tc::commit(bar(Bars::V_EMPTY + s));
+          }
+          __syncwarp();
+        };
+        if (__all_sync(FULL_MASK, ok)) {
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+            if (tiles[q] > 0) issue_s(q, 0);
         }
-        __syncwarp();
-      };
-      auto issue_pv = [&](int q, int j) {
-        const int s = j & 1, sb = buf(q, j);
-        if (q == 0 || j >= tiles[0])
-          ok = ok && lane_wait(bar(Bars::V_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns);
-        ok = ok && lane_wait(bar(Bars::P_FULL + sb), use(j) & 1u, p.wait_ns);
-        __syncwarp();
-        tc::fence_after_sync();
-        const uint64_t b0 = v_desc + uint64_t((s * C::KV_BYTES) >> 4);
-        const bool frees = q == NQ - 1 || j >= tiles[NQ - 1];
-        if (elect_one()) {
+        for (int j = 0; j < most; ++j) {
+          if (!__all_sync(FULL_MASK, ok && *abort_flag == 0)) break;
+          if (NQ == 1 && j + 1 < most) issue_s(0, j + 1);
 #pragma unroll
-          for (int kk = 0; kk < KT / 16; ++kk)
-            tc::mma_f16_ts(tmem + uint32_t(C::O_COL + q * D), tmem + uint32_t(sb * KT + KT / 2 + kk * 8),
-                           b0 + uint64_t((kk * 2048) >> 4), IDESC_PV, j > 0 || kk > 0);
-          tc::commit(bar(Bars::O_DONE + sb));
-          if (frees) tc::commit(bar(Bars::V_EMPTY + s));
+          for (int q = 0; q < NQ; ++q) {
+            if (j < tiles[q]) issue_pv(q, j);
+            if (NQ == 2 && j + 1 < tiles[q]) issue_s(q, j + 1);
+          }
         }
+        if (!__all_sync(FULL_MASK, ok) && lane == 0) fail();
+        if (elect_one()) tc::commit(bar(Bars::DRAIN));  // never leave with an MMA in flight
         __syncwarp();
-      };
-      if (__all_sync(FULL_MASK, ok)) {
-#pragma unroll
-        for (int q = 0; q < NQ; ++q)
-          if (tiles[q] > 0) issue_s(q, 0);
+        warp_wait_phase(bar(Bars::DRAIN), 0u, DRAIN_LIMIT_NS);
       }
-      for (int j = 0; j < most; ++j) {
-        if (!__all_sync(FULL_MASK, ok && *abort_flag == 0)) break;
-        if (NQ == 1 && j + 1 < most) issue_s(0, j + 1);
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-          if (j < tiles[q]) issue_pv(q, j);
-          if (NQ == 2 && j + 1 < tiles[q]) issue_s(q, j + 1);
-        }
-      }
-      if (!__all_sync(FULL_MASK, ok) && lane == 0) fail();
-      if (elect_one()) tc::commit(bar(Bars::DRAIN));  // never leave with an MMA in flight
-      __syncwarp();
-      warp_wait_phase(bar(Bars::DRAIN), 0u, DRAIN_LIMIT_NS);
     }
   } else {
     // ---------------------------------------------------------------- softmax warps
+    regs_up<C::SOFTMAX_REGS>();
     const int q = warp >> 2;
     const int r = (warp & 3) * 32 + lane;  // row of the block = TMEM lane
     const int n = row0 + q * ROWS + r;
@@ -540,39 +565,29 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       tc::fence_after_sync();
       const uint32_t s_tmem = lane_base + uint32_t(sb * KT);
       const bool open = __all_sync(FULL_MASK, j * KT + KT - 1 <= lim);  // no key of the tile is hidden
-      // The row's scores in two halves of KT / 2 columns: both give their maximum, the second stays in
-      // registers and goes first, the first is read again. P is stored over the second half's columns,
-      // which are free by then.
-      constexpr int H = KT / 2;
-      float x[H];
-      auto load_half = [&](int c0) {
+      // The row's scores stay in registers from the maximum to P, which is stored over the upper half of
+      // their columns.
+      float x[KT];
 #pragma unroll
-        for (int c = 0; c < H; c += 32)
-          tc::ld_32x32b_x32(s_tmem + uint32_t(c0 + c), *reinterpret_cast<uint32_t(*)[32]>(x + c));
-        tc::wait_ld();
-        if (!open) {
+      for (int c = 0; c < KT; c += 32)
+        tc::ld_32x32b_x32(s_tmem + uint32_t(c), *reinterpret_cast<uint32_t(*)[32]>(x + c));
+      tc::wait_ld();
+      if (!open) {
 #pragma unroll
-          for (int c = 0; c < H; c += 32) {
-            const int seen = lim - (j * KT + c0 + c);  // the last visible of these columns
-            if (__all_sync(FULL_MASK, seen >= 31)) continue;
+        for (int c = 0; c < KT; c += 32) {
+          const int seen = lim - (j * KT + c);  // the last visible of these columns
+          if (__all_sync(FULL_MASK, seen >= 31)) continue;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[c + i] = i <= seen ? x[c + i] : -INFINITY;
-          }
+          for (int i = 0; i < 32; ++i) x[c + i] = i <= seen ? x[c + i] : -INFINITY;
         }
-      };
-      auto max_half = [&]() -> float {
-        float t[4] = {x[0], x[1], x[2], x[3]};
+      }
+      float t[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int i = 4; i < H; i += 8) {
+      for (int i = 4; i < KT; i += 8) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) t[k] = fmaxf(fmaxf(t[k], x[i + k]), i + 4 + k < H ? x[i + 4 + k] : t[k]);
-        }
-        return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-      };
-      load_half(0);
-      float top = max_half();
-      load_half(H);
-      top = fmaxf(top, max_half());
+        for (int k = 0; k < 4; ++k) t[k] = fmaxf(fmaxf(t[k], x[i + k]), i + 4 + k < KT ? x[i + 4 + k] : t[k]);
+      }
+      const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
       // mul >= 0: the maximum of the products is the product of the maximum
       const float tmax = top * mul;
       const bool move = tmax > m_run + HEADROOM || (m_run < -1.0e38f && tmax > m_run);
@@ -601,24 +616,19 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       }
       const float2 mul2 = make_float2(mul, mul), neg_m2 = make_float2(-m_run, -m_run);
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      auto exp_half = [&](int c0) {  // P of keys c0 .. c0 + H - 1, two to a column
 #pragma unroll
-        for (int c = 0; c < H; c += 32) {
-          uint32_t w[16];
+      for (int c = 0; c < KT; c += 32) {  // two keys to a column
+        uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float2 e = fma2(make_float2(x[c + i], x[c + i + 1]), mul2, neg_m2);
-            e.x = ex2(e.x);
-            e.y = ex2(e.y);
-            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
-            w[i >> 1] = Elem<__half>::pack2(e.x, e.y);
-          }
-          st_32x32b_x16(s_tmem + uint32_t(H + (c0 + c) / 2), w);
+        for (int i = 0; i < 32; i += 2) {
+          float2 e = fma2(make_float2(x[c + i], x[c + i + 1]), mul2, neg_m2);
+          e.x = ex2(e.x);
+          e.y = ex2(e.y);
+          sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
+          w[i >> 1] = Elem<__half>::pack2(e.x, e.y);
         }
-      };
-      exp_half(H);
-      load_half(0);
-      exp_half(0);
+        st_32x32b_x16(s_tmem + uint32_t(KT / 2 + c / 2), w);
+      }
       const float2 total = add2(sum[0], sum[1]);
       l_run += total.x + total.y;
       tc::wait_st();
