@@ -44,6 +44,7 @@ template <int D>
 struct Cfg {
   static constexpr int NQ = D <= 128 ? 2 : 1;     // blocks of query rows per CTA
   static constexpr int KT = D <= 128 ? 128 : 64;  // keys per tile (the S MMA's N)
+  static constexpr int PART = KT / 2;             // keys of a tile whose P V may start before the others' P
   static constexpr int NSB = 2;                   // S/P buffers: one per block, or two of the one block
   static constexpr int SOFTMAX_WARPS = 4 * NQ;
   static constexpr int DECODE_WARPS = 4;
@@ -86,6 +87,7 @@ struct Bars {
   static constexpr int O_DONE = 12;  // [2] P V that read the buffer completed (commit)
   static constexpr int Q_FULL = 14;  // Q stored: one arrival per softmax warp
   static constexpr int DRAIN = 15;
+  static constexpr int P_PART = 16;  // [2] P of the tile's first PART keys written
   static constexpr int TMEM_SLOT = 160;  // byte offsets
   static constexpr int ABORT = 168;
 };
@@ -204,6 +206,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
         mbar_init(bar(Bars::V_EMPTY + i), 1);
         mbar_init(bar(Bars::S_FULL + i), 1);
         mbar_init(bar(Bars::P_FULL + i), 4);
+        mbar_init(bar(Bars::P_PART + i), 4);
         mbar_init(bar(Bars::O_DONE + i), 1);
       }
       mbar_init(bar(Bars::Q_FULL), C::SOFTMAX_WARPS);
@@ -434,16 +437,25 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
           const int s = j & 1, sb = buf(q, j);
           if (q == 0 || j >= tiles[0])
             ok = ok && lane_wait(bar(Bars::V_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns);
+          const uint64_t b0 = v_desc + uint64_t((s * C::KV_BYTES) >> 4);
+          const bool frees = q == NQ - 1 || j >= tiles[NQ - 1];
+          auto part = [&](int k0, int k1) {
+#pragma unroll
+            for (int kk = k0; kk < k1; ++kk)
+              tc::mma_f16_ts(tmem + uint32_t(C::O_COL + q * D), tmem + uint32_t(sb * KT + KT / 2 + kk * 8),
+                             b0 + uint64_t((kk * 2048) >> 4), IDESC_PV, j > 0 || kk > 0);
+          };
+          // the first PART keys while the softmax is at the others
+          ok = ok && lane_wait(bar(Bars::P_PART + sb), use(j) & 1u, p.wait_ns);
+          __syncwarp();
+          tc::fence_after_sync();
+          if (elect_one()) part(0, C::PART / 16);
+          __syncwarp();
           ok = ok && lane_wait(bar(Bars::P_FULL + sb), use(j) & 1u, p.wait_ns);
           __syncwarp();
           tc::fence_after_sync();
-          const uint64_t b0 = v_desc + uint64_t((s * C::KV_BYTES) >> 4);
-          const bool frees = q == NQ - 1 || j >= tiles[NQ - 1];
           if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < KT / 16; ++kk)
-              tc::mma_f16_ts(tmem + uint32_t(C::O_COL + q * D), tmem + uint32_t(sb * KT + KT / 2 + kk * 8),
-                             b0 + uint64_t((kk * 2048) >> 4), IDESC_PV, j > 0 || kk > 0);
+            part(C::PART / 16, KT / 16);
             tc::commit(bar(Bars::O_DONE + sb));
             if (frees) tc::commit(bar(Bars::V_EMPTY + s));
           }
@@ -628,6 +640,12 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
           w[i >> 1] = Elem<__half>::pack2(e.x, e.y);
         }
         st_32x32b_x16(s_tmem + uint32_t(KT / 2 + c / 2), w);
+        if (c + 32 == C::PART) {
+          tc::wait_st();
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(Bars::P_PART + sb));
+        }
       }
       const float2 total = add2(sum[0], sum[1]);
       l_run += total.x + total.y;
