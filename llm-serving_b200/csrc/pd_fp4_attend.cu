@@ -21,6 +21,7 @@ template <typename T, int D>
 cudaError_t launch_t(const Fp4AttendParams& p, int sms, cudaStream_t stream) {
   constexpr int NW = Warps<D>::NW;
   auto fn = fp4::pd_fp4_attend_kernel<T, D, NW>;
+  static_assert(fp4::smem_layout(fp4::MAX_ROWS, NW, fp4::COLS, D, 2).bytes <= kMaxSmem, "the longest launch fits");
   const int64_t most = int64_t(p.max_seqlen_q) * p.group;
   const int cols = int(most < fp4::COLS ? most : fp4::COLS);
   int stages = 4;  // as many as shared memory holds

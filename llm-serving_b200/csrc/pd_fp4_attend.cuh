@@ -45,7 +45,7 @@ namespace pd {
 
 namespace fp4 {
 
-constexpr int MAX_ROWS = 1024;  // rows of one launch (their prefix sums are in shared memory)
+constexpr int MAX_ROWS = 896;  // rows of one launch (their prefix sums are in shared memory)
 constexpr int COLS = 8;         // columns of a unit
 constexpr int TILE = 2 * FP4_TILE;  // keys of a warp's step: two records
 // What a join between CTAs costs, in tiles of one CTA: where there are no more units than CTAs, units
@@ -471,8 +471,8 @@ struct Smem {
   int pre_off, rows_off, piece_off, ml_off, acc_off, ring_off, bytes;
 };
 
-__host__ __device__ inline Smem smem_layout(int batch, int nw, int cols, int d, int stages) {
-  Smem s;
+__host__ __device__ constexpr Smem smem_layout(int batch, int nw, int cols, int d, int stages) {
+  Smem s{};
   s.pre_off = nw * stages * 8;
   s.rows_off = s.pre_off + (batch + 1) * 8;
   s.piece_off = (s.rows_off + batch * 8 + 15) & ~15;

@@ -65,12 +65,13 @@ int rows_common(Fp4RowsParams& p, int dtype, bool read, const int64_t* k_strides
 // (at head_dim 256: 128) query rows each, whatever part of the block is filled; a wave costs what
 // WAVE_UNITS units per SM cost. Lengths stay on the device, but both times are proportional to them, so the
 // comparison needs only the counts the host has. Measured, warp kernel and tiles, 16 heads on 8 of 128
-// with 2048 keys: 16 rows of 8 tokens (2.2 units per SM, one wave) 28.6 and 42.6 us, of 16 (3.9) 42.8 and
-// 42.7, of 32 (7.4) 72.9 and 43.2, one row of 1024 tokens (13.9) 185 and 60; 8 heads on 2 of 256: 16 rows
-// of 16 tokens (1.8) 43.7 and 57.3, of 32 (3.6) 72.1 and 58.6.
+// with 2048 keys: 16 rows of 8 tokens (2.2 units per SM, one wave) 28.5 and 38.1 us, of 16 (3.9) 42.4 and
+// 38.5, of 32 (7.4) 72.8 and 38.9, one row of 1024 tokens (13.9) 185 and 52; 8 heads on 2 of 256: 16 rows
+// of 16 tokens (1.8) 43.6 and 48.3, of 32 (3.6) 72.3 and 48.6; 4 heads on 4 of 64: one row of 1024 tokens
+// (3.5) 39.2 and 47.1, 16 rows of 128 (7.1) 51.9 and 31.1.
 bool use_tiles(int64_t total_q, int32_t max_seqlen_q, int32_t batch, int32_t n_kv_head, int32_t group,
                int32_t head_dim, int sms) {
-  const double WAVE_UNITS = head_dim == 256 ? 2.7 : 4.0;
+  const double WAVE_UNITS = head_dim == 256 ? 2.1 : head_dim == 128 ? 3.3 : 4.3;
   const int64_t block = head_dim == 256 ? 128 : 256;
   const double units = double(n_kv_head) * (double(total_q) * group / 8 + 0.5 * batch);
   const int64_t ctas = int64_t(batch) * n_kv_head * ((int64_t(max_seqlen_q) * group + block - 1) / block);

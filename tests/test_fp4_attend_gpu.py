@@ -249,6 +249,23 @@ def test_many_rows_in_one_call(cuda_device, kernel):
     _check(chunk[pick], want, mean)
 
 
+@pytest.mark.parametrize("n,heads,d", [(897, 8, 128), (1000, 8, 128), (1024, 8, 64), (1024, 8, 256), (2100, 3, 128)])
+def test_many_rows_of_wide_groups(cuda_device, n, heads, d):
+    """As many rows as a launch takes, or more, at the widest unit (eight columns)."""
+    from model.paged_fp4 import paged_decode_fp4
+
+    g = torch.Generator().manual_seed(1)
+    lengths = torch.randint(0, 60, (n,), generator=g)
+    pages, _ = _pool([16 * 64], 1, d, 16, seed=2)
+    table = torch.randint(0, 64, (n, 4), generator=g, dtype=torch.int32)
+    q = torch.randn(n, heads, d, generator=g).to(torch.bfloat16)
+    got = paged_decode_fp4(*(t.to(cuda_device) for t in (q, pages, table, lengths.to(torch.int32))))
+    pick = [0, 600, 895, 896, n - 1]
+    want, mean = ref.attention(q[pick], pages, table[pick], lengths[pick].tolist(), [1] * len(pick), torch.ones(2, 1),
+                               d ** -0.5)
+    _check(got[pick], want, mean)
+
+
 def test_wait_limit_sets_the_error_word_and_the_next_call_is_right(cuda_device, kernel):
     from model import _native
     from model.paged_fp4 import paged_decode_fp4, paged_prefill_fp4
