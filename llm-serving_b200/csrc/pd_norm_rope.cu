@@ -12,7 +12,8 @@
 // rotary pairs itself (4 elements at i and 4 at i + R/2), so the rotation needs no exchange and the
 // norm one shuffle reduction over the D / 8 lanes of a head. A warp takes NORM_HEADS heads of one
 // token per lane group and issues their loads together: the cos/sin row is read once for
-// them, and a lane has 64 bytes in flight.
+// them, and a lane has 64 bytes in flight. Measured: 6001 tokens of 8 + 2 heads of 256, fp16, 62 MB,
+// 14.4 us (4.3 TB/s, two thirds of the copy rate; some 2 us of it the launch); one token 2.3 us.
 #include "pd_internal.h"
 #include "pd_norm_rope.cuh"
 
