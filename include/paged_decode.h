@@ -340,8 +340,8 @@ int pd_qk_norm_rope(const void* q, int64_t q_st, int64_t q_sh, const void* k, in
  *   V scales    D bytes  [2][D / 16 groups][8 tokens]
  * A code is e2m1 (0 .5 1 1.5 2 3 4 6 and a sign bit); an element stands for code * scale *
  * units[kv][head], units (2, n_kv_head) fp32 powers of two on the device (NULL: all 1). 4.5 bits
- * an element. head_dim 64, 128 or 256, block_size a power of two >= 16 (PD_ERR_UNSUPPORTED
- * otherwise). The reference has no quantised cache.
+ * an element. head_dim 64, 128 or 256, block_size a power of two >= 16, a block below 2 GiB
+ * (PD_ERR_UNSUPPORTED otherwise). The reference has no quantised cache.
  *
  * pd_fp4_write_slots quantises token i of k / v (n_tokens, n_kv_head, D; strides of token and
  * head, unit last) into flat slot slot_ids[i] (pd_kv_append_slots' slots): scale = e4m3(max |x /

@@ -36,6 +36,8 @@ int launched(cudaError_t e, const char* what) {
 int check_pool(const void* pages, int64_t n_blocks, int32_t block_size, int32_t n_kv_head, int32_t head_dim) {
   if (n_blocks < 1 || n_kv_head < 1 || !pow2(block_size)) return PD_ERR_INVALID;
   if (!fp4_head_dim(head_dim) || block_size < FP4_TILE) return PD_ERR_UNSUPPORTED;
+  // the kernels hold a block's bytes and offsets in it in 32 bits
+  if (int64_t(n_kv_head) * (block_size / FP4_TILE) > 0x7fffffff / fp4_record_bytes(head_dim)) return PD_ERR_UNSUPPORTED;
   if (pages == nullptr || !aligned(pages, 16)) return PD_ERR_INVALID;
   return PD_OK;
 }

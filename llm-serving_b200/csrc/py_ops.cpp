@@ -121,6 +121,7 @@ Pages pages_of(const Tensor& pages, const Tensor* units, const char* what) {
   VALUE((rec == 18 * 64 || rec == 18 * 128 || rec == 18 * 256) && tpb >= 1 && (tpb & (tpb - 1)) == 0 &&
             pages.size(1) >= 1 && pages.size(0) >= 1,
         "pages of shape ", pages.sizes(), " are not 4-bit pages of head_dim 64, 128 or 256");
+  VALUE(tpb * pages.size(1) <= 0x7fffffff / rec, "a block of 4-bit pages must be below 2 GiB, got shape ", pages.sizes());
   VALUE(pages.is_contiguous() && aligned16(pages), "pages must be contiguous and 16-byte aligned");
   Pages p;
   p.data = pages.data_ptr();

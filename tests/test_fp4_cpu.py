@@ -74,6 +74,15 @@ def test_decode_arguments(over, status):
     assert _decode(**over) == status
 
 
+@pytest.mark.parametrize("bs,hkv,d,status", [
+    (1 << 23, 1, 128, _native.PD_OK), (1 << 24, 1, 128, _native.PD_ERR_UNSUPPORTED), (1 << 20, 16, 128, _native.PD_ERR_UNSUPPORTED),
+    (1 << 22, 2, 256, _native.PD_ERR_UNSUPPORTED), (1 << 30, 4, 64, _native.PD_ERR_UNSUPPORTED),
+])
+def test_a_block_is_below_two_gib(bs, hkv, d, status):
+    assert _write(bs=bs, hkv=hkv, d=d, n=0) == status
+    assert _decode(bs=bs, hkv=hkv, H=hkv, d=d, maxb=1, B=0) == status
+
+
 def test_prefill_and_copy_arguments():
     args = [PTR, 4, 1024, 128, PTR, 4, 16, None, PTR, 4, 4, None, PTR, PTR, 1024, 128, 2, 2, 4, 2, 128, _native.PD_BF16,
             1.0, PTR, 0, None]
