@@ -13,7 +13,7 @@
 // norm one shuffle reduction over the D / 8 lanes of a head. A warp takes NORM_HEADS heads of one
 // token per lane group and issues their loads together: the cos/sin row is read once for
 // them, and a lane has 64 bytes in flight. Measured: 6001 tokens of 8 + 2 heads of 256, fp16, 62 MB,
-// 14.1 us (4.4 TB/s, two thirds of the copy rate; some 2 us of it the launch); one token 2.3 us.
+// 14.1 us (4.4 TB/s, two thirds of the copy rate; some 2 us of it the launch); one token 2.1 us.
 #include "pd_internal.h"
 #include "pd_norm_rope.cuh"
 
