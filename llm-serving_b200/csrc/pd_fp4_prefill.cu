@@ -23,8 +23,11 @@
 //  P V and next S, and each decoded tile serves 256 rows. At head_dim 256 TMEM holds one block
 //  (O takes 256 of its 512 columns), which alternates between two S buffers instead.
 //  * fp16 q enters as it is, bf16 q as fp16 with a power of two per row that puts its largest element
-//    near 2^13 (exact for every element within 2^-27 of the largest); P as fp16: 2^-12 relative on weights whose
-//    sum is kept unrounded, below half an ulp of the result.
+//    near 2^13 (exact for every element within 2^-27 of the largest).
+//  * P enters as fp16, weights whose sum is kept unrounded in fp32. For bf16 results one fp16 is enough: its
+//    2^-11 relative is an eighth of a bf16 half ulp. fp16 results are no coarser than that, so they get a
+//    second MMA with what the first fp16 left, over the scores' lower columns: 2^-22, as the warp kernel does
+//    (the chunks below in fp16: 117.6 us, 90.5 with one part).
 //  * Tokens past the row have P = 0, and their V is stored as zeros, so whatever bytes a page holds
 //    there never reach O.
 //  * Every wait is bounded; a role whose wait runs out records DEVERR_WAIT_TIMEOUT and raises the
@@ -39,6 +42,8 @@
 #include "paged_decode.h"
 #include "pd_fp4.cuh"
 #include "pd_tcgen05.cuh"
+
+#include <type_traits>
 
 namespace pd {
 
@@ -196,6 +201,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
   using E = Elem<T>;
   constexpr int REC = fp4_record_bytes(D);
   constexpr int NQ = C::NQ, KT = C::KT;
+  constexpr int PARTS = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;  // fp16 operands that P is the sum of
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t raw = smem_addr(smem_raw);
@@ -449,8 +455,10 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
           auto part = [&](int k0, int k1) {
 #pragma unroll
             for (int kk = k0; kk < k1; ++kk)
-              tc::mma_f16_ts(tmem + uint32_t(C::O_COL + q * D), tmem + uint32_t(sb * KT + KT / 2 + kk * 8),
-                             b0 + uint64_t((kk * 2048) >> 4), IDESC_PV, j > 0 || kk > 0);
+#pragma unroll
+              for (int i = 0; i < PARTS; ++i)  // the first part in the upper half of the buffer's columns
+                tc::mma_f16_ts(tmem + uint32_t(C::O_COL + q * D), tmem + uint32_t(sb * KT + (1 - i) * (KT / 2) + kk * 8),
+                               b0 + uint64_t((kk * 2048) >> 4), IDESC_PV, j > 0 || kk > 0 || i > 0);
           };
           // the first PART keys while the softmax is at the others
           ok = ok && lane_wait(bar(Bars::P_PART + sb), use(j) & 1u, p.wait_ns);
@@ -585,7 +593,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       const uint32_t s_tmem = lane_base + uint32_t(sb * KT);
       const bool open = __all_sync(FULL_MASK, j * KT + KT - 1 <= lim);  // no key of the tile is hidden
       // The row's scores stay in registers from the maximum to P, which is stored over the upper half of
-      // their columns.
+      // their columns, its second part over the lower.
       float x[KT];
 #pragma unroll
       for (int c = 0; c < KT; c += 32)
@@ -637,7 +645,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int c = 0; c < KT; c += 32) {  // two keys to a column
-        uint32_t w[16];
+        uint32_t w[16], rest[PARTS == 2 ? 16 : 1];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           float2 e = fma2(make_float2(x[c + i], x[c + i + 1]), mul2, neg_m2);
@@ -645,8 +653,14 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
           e.y = ex2(e.y);
           sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
           w[i >> 1] = Elem<__half>::pack2(e.x, e.y);
+          if constexpr (PARTS == 2) {
+            float f[2];
+            Elem<__half>::unpack2(w[i >> 1], f);
+            rest[i >> 1] = Elem<__half>::pack2(e.x - f[0], e.y - f[1]);
+          }
         }
         st_32x32b_x16(s_tmem + uint32_t(KT / 2 + c / 2), w);
+        if constexpr (PARTS == 2) st_32x32b_x16(s_tmem + uint32_t(c / 2), rest);
         if (c + 32 == C::PART) {
           tc::wait_st();
           tc::fence_before_sync();
