@@ -30,6 +30,13 @@ namespace pd {
 constexpr int FP4_TILE = 16;   // tokens of a record
 constexpr int FP4_GROUP = 16;  // elements that share a scale
 
+// Attention weights are kept as 2^(s - m + SHIFT), m the running maximum, and the sums carry the same factor.
+// The maximum moves only when a score passes it by 2^HEADROOM, so a weight stays below 2^15, inside fp16, and one
+// of 2^-21 of the largest is still a normal fp16 number. (Without the factor that end was 2^-14: rows with
+// one key far above the others lost the others' bits.)
+constexpr float FP4_HEADROOM = 8.f;
+constexpr float FP4_P_SHIFT = 7.f;
+
 __host__ __device__ constexpr int fp4_record_bytes(int d) { return 18 * d; }
 
 // Byte offsets inside a record: of the 8 code bytes of group `gr` (16 elements) of token `t`, and

@@ -20,8 +20,9 @@
 // both, so the products are those of the values the cache stands for.
 //  * q enters as fp16: a column is scaled by a power of two that puts its largest element near
 //    2^13, exact for fp16 and for every bf16 element within 2^-27 of the largest.
-//  * P enters as fp16 (2^-12 relative, on weights whose sum is kept unrounded in fp32): below half
-//    an ulp of the 16-bit result.
+//  * P enters as one fp16 for bf16 results: a result is off by at most 2^-11 of the weighted mean of |v|
+//    (the weights' sum is kept unrounded in fp32), an eighth of a bf16 half ulp of that mean. fp16 results,
+//    no coarser than that, get two fp16 parts (2^-22).
 //  * tokens past the row are masked to P = 0 and their V scales to 0, so whatever bytes a page
 //    holds there (a NaN scale included) never reaches the sums.
 //
@@ -64,9 +65,6 @@ constexpr int CTA_TILES = 8;
 // A running maximum below every score: finite, so that exp2(score - maximum) needs no special case
 // for columns that have seen no key (their scores are -inf).
 constexpr float NO_MAX = -3.0e38f;
-// The running maximum moves only when a score passes it by more than 2^HEADROOM: rescaling the
-// accumulators is then rare, and P stays below 2^8, which fp16 holds as exactly as smaller values.
-constexpr float HEADROOM = 8.f;
 
 // Floats of one CTA-level partial: m and l of 8 columns, then 8 x D accumulators.
 __host__ __device__ constexpr int partial_floats(int d) { return 2 * COLS + COLS * d; }
@@ -151,8 +149,8 @@ struct Worker {
   int lane, g, c;
   uint32_t qb[KS][2];
   float o[MT][4];
-  float m_run[2], l_run[2];
-  float bar[2];  // m_run + HEADROOM: the scores that move the maximum
+  float m_run[2], l_run[2];  // reference (a maximum less FP4_P_SHIFT) and sum of the weights
+  float bar[2];  // the scores above it move the reference: FP4_HEADROOM over the maximum it was set from
   float mul[2];  // score multiplier of columns 2c, 2c + 1
   int lim[2];    // their last visible key
   int open_lim;  // keys up to this one are visible to every live column
@@ -335,10 +333,10 @@ struct Worker {
         float t = top[j];
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) t = fmaxf(t, __shfl_xor_sync(FULL_MASK, t, off));
-        t = fmaxf(t, m_run[j]);
+        t = fmaxf(t - FP4_P_SHIFT, m_run[j]);
         const float alpha = ex2(m_run[j] - t);
         m_run[j] = t;
-        bar[j] = t + HEADROOM;
+        bar[j] = t + (FP4_P_SHIFT + FP4_HEADROOM);  // rescaling the accumulators is then rare
         l_run[j] *= alpha;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -352,7 +350,7 @@ struct Worker {
       sc[i] = ex2(sc[i] - m_run[i & 1]);
       l_run[i & 1] += sc[i];
     }
-    // P is one fp16 operand for bf16 outputs (2^-12 is an eighth of their half ulp) and a hi + lo pair
+    // P is one fp16 operand for bf16 outputs (2^-11 is an eighth of their half ulp) and a hi + lo pair
     // for fp16 outputs, whose rounding is no coarser than fp16 P's
     constexpr int PARTS = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
 #pragma unroll

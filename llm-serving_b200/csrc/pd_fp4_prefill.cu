@@ -17,16 +17,17 @@
 //    from TMEM, where the softmax wrote it over the S it came from, a tile's first half as soon as it is
 //    there (two halves 91.6 us, one whole 94.1 on the chunks below);
 //  * 4 softmax warps per block of query rows, one thread per row (TMEM lane = row): maximum over the
-//    row's scores, P = 2^(s - m) as fp16, and the fp32 sum; no exchange between threads. The maximum
+//    row's scores, P = 2^(s - m + 7) as fp16, and the fp32 sum; no exchange between threads. The maximum
 //    moves only when a tile passes it by 2^8, so rescaling O in TMEM is rare.
 //  With NQ = 2 the blocks alternate: while the softmax of one runs, the tensor cores do the other's
 //  P V and next S, and each decoded tile serves 256 rows. At head_dim 256 TMEM holds one block
 //  (O takes 256 of its 512 columns), which alternates between two S buffers instead.
 //  * fp16 q enters as it is, bf16 q as fp16 with a power of two per row that puts its largest element
 //    near 2^13 (exact for every element within 2^-27 of the largest).
-//  * P enters as fp16, weights whose sum is kept unrounded in fp32. For bf16 results one fp16 is enough: its
-//    2^-11 relative is an eighth of a bf16 half ulp. fp16 results are no coarser than that, so they get a
-//    second MMA with what the first fp16 left, over the scores' lower columns: 2^-22, as the warp kernel does
+//  * P enters as fp16, weights whose sum is kept unrounded in fp32. For bf16 results one fp16 is enough: a
+//    result is off by at most 2^-11 of the weighted mean of |v|, an eighth of a bf16 half ulp of that mean.
+//    fp16 results are no coarser than that, so they get a second MMA with what the first fp16 left, kept
+//    in the scores' lower columns: 2^-22, as the warp kernel does
 //    (the chunks below in fp16: 117.6 us, 90.5 with one part).
 //  * Tokens past the row have P = 0, and their V is stored as zeros, so whatever bytes a page holds
 //    there never reach O.
@@ -49,8 +50,7 @@ namespace pd {
 
 namespace {
 
-constexpr int ROWS = 128;        // query rows of a block (the MMA's M)
-constexpr float HEADROOM = 8.f;  // log2 headroom before the running maximum is moved
+constexpr int ROWS = 128;  // query rows of a block (the MMA's M)
 
 template <int D>
 struct Cfg {
@@ -617,10 +617,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
       // mul >= 0: the maximum of the products is the product of the maximum
       const float tmax = top * mul;
-      const bool move = tmax > m_run + HEADROOM || (m_run < -1.0e38f && tmax > m_run);
+      const bool move = tmax > m_run + (FP4_P_SHIFT + FP4_HEADROOM) || (m_run < -1.0e38f && tmax > m_run);
       if (__any_sync(FULL_MASK, move)) {
-        const float alpha = move ? ex2(m_run - tmax) : 1.f;
-        if (move) m_run = tmax;
+        const float ref = tmax - FP4_P_SHIFT;
+        const float alpha = move ? ex2(m_run - ref) : 1.f;
+        if (move) m_run = ref;
         l_run *= alpha;
         if (j > 0) {  // O *= alpha once P V of tile j - 1 has landed
           const int pb = NQ == 2 ? q : (j - 1) & 1;

@@ -13,6 +13,8 @@ To that comes the output's rounding, half an ulp.
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -38,6 +40,62 @@ def _check(got, want, mean, keys, largest):
     err = (got.cpu().double() - want).abs()
     assert torch.isfinite(got).all()
     assert (err <= bound).all(), f"worst {float((err / bound).max()):.3g} times the bound"
+
+
+def _sink(n, hkv, d, bs=16):
+    """Pages whose key 0 has element 0 at 6 and values 0; every other key is 0 with positive values."""
+    g = torch.Generator().manual_seed(d)
+    blocks = -(-n // bs)
+    codes = torch.randint(1, 8, (blocks * bs, hkv, d), generator=g)
+    kc, ks, vc, vs = ref.places(d)
+    pages = torch.zeros(blocks, hkv, bs // 16, 18 * d, dtype=torch.uint8)
+    for t in range(blocks * bs):
+        rec = pages[t // bs, :, t % bs // 16]
+        rec[:, ks[t % 16]] = rec[:, vs[t % 16]] = 0x38  # a scale of 1
+        if t:
+            rec[:, vc[t % 16]] = (codes[t, :, 0::2] | (codes[t, :, 1::2] << 4)).to(torch.uint8)
+        else:
+            rec[:, kc[0][0]] = 7  # 6 in element 0
+    return pages, torch.arange(blocks, dtype=torch.int32)[None]
+
+
+# The other keys' weight is 37.45 * 2^-24 of the sink's: between two of fp16's numbers, were the sink's 1.
+GAP = 24 - math.log2(37.45)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_small_weights_beside_a_large_one_decode(cuda_device, dtype, d):
+    from model.paged_fp4 import paged_decode_fp4
+
+    n, rows, hkv, heads = 320, 300, 8, 16
+    pages, table = _sink(n, hkv, d)
+    q = torch.zeros(1, heads, d, dtype=dtype)
+    q[..., 0] = 1
+    scale = GAP * math.log(2) / 6
+    want, mean = ref.attention(q, pages, table, [n], [1], torch.ones(2, hkv), scale)
+    got = paged_decode_fp4(q.to(cuda_device).expand(rows, heads, d), pages.to(cuda_device),
+                           table.to(cuda_device).expand(rows, -1),
+                           torch.full((rows,), n, dtype=torch.int32, device=cuda_device), scale=scale)
+    _check(got, want.expand(rows, heads, d), mean.expand(rows, heads, d), n, 6.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_small_weights_beside_a_large_one_chunks(cuda_device, kernel, dtype, d):
+    from model.paged_fp4 import paged_prefill_fp4
+
+    n, rows, hkv, heads, chunk = 320, 4, 8, 16, 300
+    pages, table = _sink(n, hkv, d)
+    q = torch.zeros(chunk, heads, d, dtype=dtype)
+    q[..., 0] = 1
+    scale = GAP * math.log(2) / 6
+    want, mean = ref.attention(q, pages, table, [n], [chunk], torch.ones(2, hkv), scale)
+    got = paged_prefill_fp4(q.to(cuda_device).repeat(rows, 1, 1), pages.to(cuda_device),
+                            table.to(cuda_device).expand(rows, -1),
+                            torch.arange(rows + 1, dtype=torch.int32, device=cuda_device) * chunk,
+                            torch.full((rows,), n, dtype=torch.int32, device=cuda_device), chunk, scale=scale)
+    _check(got, want.repeat(rows, 1, 1), mean.repeat(rows, 1, 1), n, 6.0)
 
 
 def _exact_scores(rows, heads, hkv, d, seed):
