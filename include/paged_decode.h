@@ -365,7 +365,8 @@ int pd_fp4_read_slots(const void* pages, int64_t n_blocks, int32_t block_size, c
 
 /* pd_fp4_decode is pd_decode over 4-bit pages, pd_fp4_prefill is pd_prefill over them (same
  * arguments, masks and conventions): q and out fp16 or bf16, any number of q heads per kv head;
- * total_q is the packed tensors' token count, which offsets in cu_seqlens_q never pass.
+ * total_q is the packed tensors' token count, which offsets in cu_seqlens_q never pass (total_q * n_head
+ * up to 2^30, PD_ERR_UNSUPPORTED above), and max_seqlen_q any bound on the chunks, loose ones at no cost.
  * A block id outside the pool reads zeros. workspace: pd_fp4_workspace_bytes(head_dim) bytes of
  * device memory, 256-byte aligned, ZERO-FILLED before its first launch (every launch leaves its
  * counters at zero again); two launches that may run concurrently must not share one. */

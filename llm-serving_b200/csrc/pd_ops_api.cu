@@ -93,6 +93,11 @@ int attend_common(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, co
   if (max_blocks > 0 && bt_stride < max_blocks) return PD_ERR_INVALID;
   const int64_t capacity = int64_t(max_blocks) * block_size;
   if (capacity > (int64_t(1) << 30)) return PD_ERR_INVALID;
+  // the kernels index query rows (a token's heads side by side) in 32 bits, up to a block of rows past the last
+  if (total_q * n_head > (int64_t(1) << 30)) return PD_ERR_UNSUPPORTED;
+  // no chunk is longer than the packed tensor: a loose bound neither changes the choice of the kernel nor
+  // launches blocks past the last row
+  max_seqlen_q = int32_t(max_seqlen_q < total_q ? max_seqlen_q : total_q);
   if (batch == 0 || max_seqlen_q == 0) return PD_OK;
   if (seqlen == nullptr || (block_table == nullptr && max_blocks > 0)) return PD_ERR_INVALID;
   if (q == nullptr || out == nullptr || !aligned(q, 16) || !aligned(out, 16)) return PD_ERR_INVALID;
