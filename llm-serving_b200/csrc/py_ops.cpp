@@ -12,7 +12,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/zeros.h>
 #include <Python.h>
-#include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -21,6 +21,7 @@
 #include <torch/csrc/utils/python_numbers.h>
 
 #include <cmath>
+#include <iterator>
 #include <map>
 #include <vector>
 
@@ -242,15 +243,23 @@ Tensor new_workspace(const at::Device& device) {
   return at::zeros({int64_t(lib.pd_fp4_workspace_bytes(256))}, at::TensorOptions(at::kByte).device(device));
 }
 
-// The workspace of a (device, stream): zero-filled once and left at zero by every launch.
+// The workspace of a call that was given none: zero-filled once and left at zero by every launch. Eager
+// calls share one per (device, stream). A captured call never takes that one, also where its stream has
+// it already: the graph may be replayed on another stream beside the eager calls, or beside another graph. A
+// capture has its own, per stream, whose zero fill is a node of the graph; it is dropped here with the first
+// call after the capture's end, its memory staying in the graph's pool.
 Tensor stream_workspace(const at::Device& device, void* stream) {
-  static auto* cache = new std::map<std::pair<int, void*>, Tensor>;  // never destroyed: outlives no context
-  const auto key = std::make_pair(int(device.index()), stream);
-  const auto found = cache->find(key);
-  if (found != cache->end()) return found->second;
-  const Tensor ws = new_workspace(device);
-  // under capture the zero fill is a node of the graph, so the buffer belongs to that graph alone
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) (*cache)[key] = ws;
+  using Workspaces = std::map<std::pair<int, void*>, Tensor>;
+  static auto* eager = new Workspaces;  // never destroyed: outlives no context
+  static auto* captures = new std::map<unsigned long long, Workspaces>;  // by capture
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long capture = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &capture));
+  const bool captured = status != cudaStreamCaptureStatusNone;
+  for (auto it = captures->begin(); it != captures->end();)
+    it = captured && it->first == capture ? std::next(it) : captures->erase(it);
+  Tensor& ws = (captured ? (*captures)[capture] : *eager)[std::make_pair(int(device.index()), stream)];
+  if (!ws.defined()) ws = new_workspace(device);
   return ws;
 }
 

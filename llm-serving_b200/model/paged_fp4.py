@@ -85,8 +85,8 @@ def paged_decode_fp4(q, pages, block_table, seqlen, *, units=None, scale: float 
     ``q`` ``(B, H, D)`` fp16 or bf16; ``block_table`` int32 ``(B, max_blocks)``, of whose row ``b`` only
     the first ``ceil(seqlen[b] / block_size)`` entries matter; ``seqlen`` ``(B,)`` int32 (int64 is
     cast). Returns ``(B, H, D)`` in ``q.dtype``. ``workspace`` (optional) is a tensor of
-    :func:`fp4_workspace` that no concurrent launch uses; without it the calls of one stream
-    share one.
+    :func:`fp4_workspace` that no concurrent launch uses; without it the eager calls of one stream
+    share one, and those of a graph's capture another that is the graph's own.
     """
     ops = _native.ops or _native.require_ops()
     return ops.fp4_decode(q, pages, block_table, seqlen, units, scale, out, workspace)
@@ -176,11 +176,12 @@ class Fp4Pool(PagedPool):
         return read_slots_fp4(self.pages[layer], slot_ids, self.dtype if dtype is None else dtype,
                               units=self.units[layer])
 
-    def prefill(self, layer: int, q, block_table, cu_seqlens_q, seqlen_k, max_seqlen_q: int, *, scale=None):
+    def prefill(self, layer: int, q, block_table, cu_seqlens_q, seqlen_k, max_seqlen_q: int, *, scale=None,
+                workspace=None):
         """:func:`paged_prefill_fp4` over one layer's pages."""
         layer = self._check_layer(layer)
         return paged_prefill_fp4(q, self.pages[layer], block_table, cu_seqlens_q, seqlen_k, max_seqlen_q,
-                                 units=self.units[layer], scale=scale)
+                                 units=self.units[layer], scale=scale, workspace=workspace)
 
     def bytes(self) -> int:
         """Physical bytes of the pool: 9/16 of a byte per element of K and V."""
