@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(256) pd_norm_rope_any_kernel(const NormRopePar
     const bool in_range = pos >= 0 && pos < p.n_pos;
     if (!in_range && lane == 0) atomicOr(p.err, DEVERR_ROPE_RANGE);
     const float inv = in_range ? rsqrtf(ss / float(d) + p.eps) : 0.f;
+    __syncwarp();  // every lane has read its partners before a lane stores over them (shuffles order no memory)
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
       const int e = lane + 32 * n;
