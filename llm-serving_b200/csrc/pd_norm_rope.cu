@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(THREADS, 8) pd_norm_rope_kernel(const NormRope
       for (int i = 0; i < 4; ++i) ss = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], ss));
 #pragma unroll
       for (int o = LANES / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(FULL_MASK, ss, o);
-      const float inv = in_range ? rsqrtf(ss * (1.f / D) + p.eps) : 0.f;  // 2 ulp
+      const float inv = rsqrtf(ss * (1.f / D) + p.eps);  // 2 ulp
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float u = (xa[i] * ac[i] - xb[i] * bs[i]) * inv;
@@ -136,8 +136,9 @@ __global__ void __launch_bounds__(THREADS, 8) pd_norm_rope_kernel(const NormRope
         xa[i] = u;
       }
       if (h0 + j * GROUPS < heads) {
-        *reinterpret_cast<Raw*>(y + e0) = F::pack(xa);
-        *reinterpret_cast<Raw*>(y + e1) = F::pack(xb);
+        // zeros by choice, not by a product: 0 times an infinity would be NaN
+        *reinterpret_cast<Raw*>(y + e0) = in_range ? F::pack(xa) : Raw{};
+        *reinterpret_cast<Raw*>(y + e1) = in_range ? F::pack(xb) : Raw{};
       }
       y += GROUPS * so;
     }
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(256) pd_norm_rope_any_kernel(const NormRopePar
     const int64_t pos = position_of(p, t);
     const bool in_range = pos >= 0 && pos < p.n_pos;
     if (!in_range && lane == 0) atomicOr(p.err, DEVERR_ROPE_RANGE);
-    const float inv = in_range ? rsqrtf(ss / float(d) + p.eps) : 0.f;
+    const float inv = rsqrtf(ss / float(d) + p.eps);
     __syncwarp();  // every lane has read its partners before a lane stores over them (shuffles order no memory)
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
@@ -195,7 +196,7 @@ __global__ void __launch_bounds__(256) pd_norm_rope_any_kernel(const NormRopePar
         const float other = u[n] * inv;
         r = e < half ? own * c - other * s : other * s + own * c;
       }
-      y[e] = E::from_float(r);
+      y[e] = E::from_float(in_range ? r : 0.f);
     }
   }
 }

@@ -1,4 +1,5 @@
-"""Head norm with rotation: rows normalised in place by the kernel for any head_dim and alignment."""
+"""Head norm with rotation: rows normalised in place by the kernel for any head_dim and alignment, and rows
+at positions outside the tables."""
 
 from __future__ import annotations
 
@@ -40,3 +41,21 @@ def test_in_place_changes_no_bit_at_any_head_dim_and_alignment(cuda_device, dtyp
         assert torch.equal(qi, want[0]) and torch.equal(ki, want[1])
         rest = (5 + 2) * d + offset
         assert torch.equal(work[:, rest:], qkv[:, rest:]) and torch.equal(work[:, :offset], qkv[:, :offset])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("d,rotary", [(128, 128), (64, 32), (256, 0), (80, 20)])
+def test_a_position_outside_the_tables_gives_zeros_whatever_the_row_holds(cuda_device, dtype, d, rotary):
+    from model import _native
+    from model.qk_norm import qk_norm_rope
+
+    q = torch.ones(4, 3, d, dtype=dtype, device=cuda_device)
+    q[1, 0, 0], q[1, 1, 1], q[1, 2, d - 1] = float("inf"), -float("inf"), float("nan")
+    k = q[:, :1].clone()
+    w = torch.ones(d, dtype=dtype, device=cuda_device)
+    w[0] = float("inf")
+    tables = torch.ones(8, max(rotary // 2, 1), dtype=dtype, device=cuda_device)
+    assert _native.device_error() == 0
+    qo, ko = qk_norm_rope(q, k, w, w, tables, tables, torch.tensor([0, 8, -1, 7], device=cuda_device), rotary_dim=rotary)
+    assert _native.device_error() == _native.DEVERR_ROPE_RANGE
+    assert (qo[1:3] == 0).all() and (ko[1:3] == 0).all()
