@@ -3,9 +3,9 @@
 //
 // For each pool tensor and each pair i, block dst[i] takes the bytes of block src[i]; then every
 // table entry e in [0, n_blocks) becomes remap[e]. What a fork (its last, partly filled page), a
-// copy on write and a compaction need. No destination is also a source and destinations are
-// distinct (the block manager's plans guarantee both), so the copies are independent and one
-// launch does them all.
+// copy on write and a compaction need. No destination is also a source of another copy and destinations
+// are distinct (the caller's contract: one plan of the block manager, or plans of which none starts from a
+// block that another has yet to fill), so the copies are independent and one launch does them all.
 //
 // Bound by memory: every byte is read and written once. A block is cut into 8 KB pieces, one CTA
 // of 256 threads with two 16-byte loads in flight per thread for each; the pieces of all pairs and

@@ -14,10 +14,8 @@ from model import _native
 __all__ = ["copy_blocks"]
 
 
-def _ids(name: str, ids, pool: torch.Tensor) -> torch.Tensor:
-    """A device vector of block ids from Python ints (a tensor passes as it is)."""
-    if isinstance(ids, torch.Tensor):
-        return ids
+def _checked(name: str, ids, pool: torch.Tensor) -> list[int]:
+    """Block ids given as Python ints."""
     ids = list(ids)
     for i in ids:
         if isinstance(i, bool) or not isinstance(i, int):
@@ -26,7 +24,7 @@ def _ids(name: str, ids, pool: torch.Tensor) -> torch.Tensor:
             raise IndexError(f"{name}: block id {i} outside the pool's {pool.shape[0]} blocks")
     if name == "dst" and len(set(ids)) != len(ids):
         raise ValueError("dst holds a block id twice")
-    return torch.tensor(ids, dtype=torch.int64, device=pool.device)
+    return ids
 
 
 def copy_blocks(pools, src, dst, *, block_table=None, remap=None) -> None:
@@ -35,9 +33,11 @@ def copy_blocks(pools, src, dst, *, block_table=None, remap=None) -> None:
     ``pools`` is a ``PagedPool`` / ``Fp4Pool``, or tensors whose first dimension is the blocks, all
     with one shape and type, contiguous, on one CUDA device. ``src`` and ``dst`` are device vectors
     (int32 or int64; ids outside the pool are skipped and set ``_native.DEVERR_COPY_RANGE`` in the
-    device error word) or Python ints (checked here). Destinations must be distinct and none may
-    also be a source, as the block manager's plans guarantee; nothing on the host can check device
-    vectors without waiting for them. With ``block_table`` (int32 ``(B, max_blocks)``) and
+    device error word) or Python ints (checked here: ValueError). Destinations must be distinct and none
+    may be the source of another copy: the copies run side by side. One plan of the block manager
+    keeps to that; plans joined into one call do only if none was made from a block that another has
+    yet to fill (a fork of a fork: copy before the second). Nothing on the host can check device vectors
+    without waiting for them. With ``block_table`` (int32 ``(B, max_blocks)``) and
     ``remap`` (int32 ``(n_blocks,)``), every table entry ``e`` inside the pool becomes ``remap[e]``
     in the same launch. Runs on the current stream.
     """
@@ -49,5 +49,13 @@ def copy_blocks(pools, src, dst, *, block_table=None, remap=None) -> None:
     if not isinstance(src, torch.Tensor) or not isinstance(dst, torch.Tensor):
         if not pools or not isinstance(pools[0], torch.Tensor) or pools[0].dim() == 0:
             raise ValueError("copy_blocks needs at least one pool of (n_blocks, ...) elements")
-        src, dst = _ids("src", src, pools[0]), _ids("dst", dst, pools[0])
+        src, dst = (ids if isinstance(ids, torch.Tensor) else _checked(name, ids, pools[0])
+                    for name, ids in (("src", src), ("dst", dst)))
+        if isinstance(src, list) and isinstance(dst, list):
+            sources = set(src)
+            for a, b in zip(src, dst):
+                if b in sources and a != b:
+                    raise ValueError(f"block {b} is the destination of one copy and the source of another")
+        src, dst = (ids if isinstance(ids, torch.Tensor) else torch.tensor(ids, dtype=torch.int64, device=pools[0].device)
+                    for ids in (src, dst))
     ops.block_copy(pools, src, dst, block_table, remap)

@@ -66,9 +66,10 @@ class SharedBlockManager(BlockManager):
 
     def fork(self, table: Sequence[int], length: int) -> tuple[list[int], list[tuple[int, int]]] | None:
         """A continuation of the first ``length`` tokens of ``table``: its own block table of the
-        same width and the ``(from, to)`` copies it needs before either writes on. Blocks that the
-        ``length`` tokens fill are shared; the rest are reserved, and a partly filled last one is
-        copied. ``None`` (nothing changed) when the free blocks do not suffice."""
+        same width and the ``(from, to)`` copies it needs before either writes on, and before the new
+        table is forked, copied or compacted itself. Blocks that the ``length`` tokens fill are
+        shared; the rest are reserved, and a partly filled last one is copied. ``None`` (nothing
+        changed) when the free blocks do not suffice."""
         table = self._check_held(table)
         length = _count("length", length, allow_zero=True)
         if length > len(table) * self.block_size:
@@ -84,7 +85,8 @@ class SharedBlockManager(BlockManager):
     def make_writable(self, table: list[int], index: int) -> list[tuple[int, int]] | None:
         """Before a write into block ``table[index]``: when others hold it too, puts a block of its
         own in its place in ``table`` and returns the copy that fills it (``[]`` when it is already
-        its own, ``None`` when no block is free)."""
+        its own, ``None`` when no block is free). Carry the copy out before the block is forked or
+        copied again."""
         if not 0 <= index < len(table):
             raise IndexError(f"index {index} outside a table of {len(table)} blocks")
         self._check_held([table[index]])
