@@ -23,6 +23,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "pd_common.cuh"
 
 namespace pd {
@@ -152,6 +154,20 @@ struct Fp4AttendParams {
   unsigned* err;
   unsigned long long wait_ns;
 };
+
+// Raises a kernel's dynamic shared memory limit on the current device, once. The limit is the kernel's, not
+// the call's, so that first calls of two host threads set the same value whatever they need themselves.
+constexpr int FP4_MAX_DEVICES = 64;
+using SmemRaised = std::atomic<bool>[FP4_MAX_DEVICES];
+template <typename Kernel>
+cudaError_t raise_smem_limit(Kernel fn, int bytes, SmemRaised& raised) {
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess || (dev < FP4_MAX_DEVICES && raised[dev].load(std::memory_order_acquire))) return err;
+  err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess && dev < FP4_MAX_DEVICES) raised[dev].store(true, std::memory_order_release);
+  return err;
+}
 
 // Launchers. sms: multiprocessors of the current device.
 cudaError_t launch_fp4_rows(const Fp4RowsParams& p, int dtype, bool read, bool vec, int sms, cudaStream_t stream);

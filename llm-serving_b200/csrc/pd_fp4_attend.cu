@@ -28,15 +28,9 @@ cudaError_t launch_t(const Fp4AttendParams& p, int sms, cudaStream_t stream) {
   int stages = 4;  // as many as shared memory holds
   while (stages > 2 && fp4::smem_layout(p.batch, NW, cols, D, stages).bytes > kMaxSmem) --stages;
   const int bytes = fp4::smem_layout(p.batch, NW, cols, D, stages).bytes;
-  static int attr_smem[64] = {0};
-  int dev = 0;
-  cudaError_t err = cudaGetDevice(&dev);
+  static SmemRaised raised{};
+  const cudaError_t err = raise_smem_limit(fn, kMaxSmem, raised);
   if (err != cudaSuccess) return err;
-  if (dev >= 64 || attr_smem[dev] < bytes) {
-    err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (err != cudaSuccess) return err;
-    if (dev < 64) attr_smem[dev] = bytes;
-  }
   fn<<<dim3(unsigned(sms)), NW * 32, bytes, stream>>>(p, stages, cols);
   return cudaGetLastError();
 }

@@ -741,15 +741,9 @@ template <typename T, int D>
 cudaError_t launch_t(const Fp4AttendParams& p, cudaStream_t stream) {
   using C = Cfg<D>;
   auto fn = pd_fp4_prefill_kernel<T, D>;
-  static bool attr_set[64] = {false};
-  int dev = 0;
-  cudaError_t err = cudaGetDevice(&dev);
+  static SmemRaised raised{};
+  const cudaError_t err = raise_smem_limit(fn, C::SMEM, raised);
   if (err != cudaSuccess) return err;
-  if (dev >= 64 || !attr_set[dev]) {
-    err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    if (err != cudaSuccess) return err;
-    if (dev < 64) attr_set[dev] = true;
-  }
   const int64_t rows = int64_t(p.max_seqlen_q) * p.group;
   const int64_t blocks = (rows + C::NQ * ROWS - 1) / (C::NQ * ROWS);
   const int64_t ctas = blocks * p.batch * p.n_kv_head;
