@@ -184,11 +184,12 @@ struct Worker {
     for (int i = 0; i < KS * 4; ++i) top = fmaxf(top, fabsf(x[i]));
     top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, 1));
     top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, 2));
-    // 2^(13 - floor(log2 top)), within 2^+-100; 1 for zero and for non-finite columns
+    // 2^(13 - floor(log2 top)), at most 2^126 (its inverse is a normal number); 1 for zero and for
+    // non-finite columns
     int e = int(__float_as_uint(top) >> 23);
     e = e == 0 || e == 255 ? 140 : e;
     int shift = 140 - e;
-    shift = shift > 100 ? 100 : (shift < -100 ? -100 : shift);
+    shift = shift > 126 ? 126 : shift;  // at least -114
     const float up = __uint_as_float(uint32_t(127 + shift) << 23);
     const float down = __uint_as_float(uint32_t(127 - shift) << 23);
 #pragma unroll

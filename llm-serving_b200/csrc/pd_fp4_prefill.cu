@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       const float top = fmaxf(__low2float(top2), __high2float(top2));
       int e = int(__float_as_uint(top) >> 23);
       e = e == 0 || e == 255 ? 140 : e;
-      const int shift = max(-100, min(100, 140 - e));
+      const int shift = min(126, 140 - e);  // at least -114; its inverse is a normal number
       const float up = __uint_as_float(uint32_t(127 + shift) << 23);
       down = __uint_as_float(uint32_t(127 - shift) << 23);
 #pragma unroll 1

@@ -146,3 +146,20 @@ def test_values_that_cancel_decode(cuda_device, dtype, d):
     got = paged_decode_fp4(*(t.to(cuda_device) for t in (q.to(dtype), pages, table, torch.tensor(lengths, dtype=torch.int32))),
                            scale=scale)
     _check(got, want, mean, max(lengths), 6.0)
+
+
+@pytest.mark.parametrize("exponent", [-122, -101, 100, 118])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_queries_over_the_range_of_bf16(cuda_device, kernel, d, exponent):
+    """Queries as large and as small as bf16 holds them, with a scale that brings the scores back."""
+    from model.paged_fp4 import paged_decode_fp4, paged_prefill_fp4
+
+    q, pages, table, chunks, lengths = _exact_scores([(40, 70), (5, 5)], 4, 2, d, seed=d + 2)
+    q = (q * 2.0 ** exponent).to(torch.bfloat16)
+    scale = 0.7 / d ** 0.5 * 2.0 ** -exponent
+    want, mean = ref.attention(q, pages, table, lengths, chunks, torch.ones(2, 2), scale)
+    cu = torch.tensor([0, 40, 45], dtype=torch.int32)
+    dev = [t.to(cuda_device) for t in (q, pages, table, cu, torch.tensor(lengths, dtype=torch.int32))]
+    _check(paged_prefill_fp4(*dev, 40, scale=scale), want, mean, 70, 6.0)
+    want, mean = ref.attention(q[:2], pages, table, lengths, [1, 1], torch.ones(2, 2), scale)
+    _check(paged_decode_fp4(dev[0][:2], *dev[1:3], dev[4], scale=scale), want, mean, 70, 6.0)
