@@ -7,7 +7,8 @@ CUDA runtime, so the .so only needs the driver (``libcuda.so.1``) at run time an
 loaded (not used) on a host without a GPU.
 
 The Python binding of the newer operators, ``pd_ops.so``, is compiled beside it with g++ against
-torch's headers; it calls the library through addresses it is handed and links to nothing of it.
+torch's headers; it calls the library through addresses it is handed and links to nothing of it. Where
+torch or g++ is missing, the library is built without it.
 
 Usage: ``python llm-serving_b200/build.py [--force] [--verbose]``. The output lands next to
 this file and is rebuilt only when a source is newer than it.
@@ -16,10 +17,14 @@ this file and is rebuilt only when a source is newer than it.
 from __future__ import annotations
 
 import argparse
+import importlib.metadata
+import importlib.util
 import os
 import re
+import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -31,6 +36,8 @@ LIB = HERE / "libpaged_decode.so"
 #: The Python binding of the newer operators (csrc/py_ops.cpp): a CPython extension over torch's
 #: C++ API that calls the library's C ABI. Compiled by the host compiler, no device code.
 OPS = HERE / "pd_ops.so"
+#: The torch and interpreter it was compiled for: another of either rebuilds it.
+OPS_STAMP = BUILD / "pd_ops.stamp"
 
 SOURCES = [
     "pd_api.cu",
@@ -89,12 +96,42 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(dep.stat().st_mtime > mtime for dep in deps)
 
 
-def _ops_command() -> list[str]:
-    import sysconfig
+def _torch_root() -> Path | None:
+    """Where torch is installed, without importing it; None where it is not."""
+    spec = importlib.util.find_spec("torch")
+    return Path(spec.origin).resolve().parent if spec is not None and spec.origin else None
 
+
+def _ops_missing() -> str | None:
+    """What the binding's build lacks on this host, or None."""
+    root = _torch_root()
+    if root is None:
+        return "torch is not installed"
+    if not (root / "include" / "ATen").is_dir():
+        return f"torch's headers are not in {root / 'include'}"
+    return None if shutil.which("g++") else "g++ is not on PATH"
+
+
+def _ops_stamp() -> str:
+    """What the binding was compiled against besides its sources: torch and the interpreter."""
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:  # a source tree: its location has to do
+        version = "?"
+    return f"torch {version} in {_torch_root()}, {sysconfig.get_config_var('SOABI')}"
+
+
+def _ops_stale() -> bool:
+    source = CSRC / "py_ops.cpp"
+    if _stale(OPS, [source, *_headers(source)]):
+        return True
+    return not OPS_STAMP.exists() or OPS_STAMP.read_text() != _ops_stamp()
+
+
+def _ops_command() -> list[str]:
     import torch
 
-    root = Path(torch.__file__).resolve().parent
+    root = _torch_root()
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     includes = [INCLUDE, CSRC, root / "include", root / "include/torch/csrc/api/include",
                 sysconfig.get_paths()["include"], Path(cuda) / "include"]
@@ -105,7 +142,10 @@ def _ops_command() -> list[str]:
 
 
 def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False) -> Path:
-    """Compile and link the library; returns its path. Raises on a compiler error."""
+    """Compile and link the library, and the Python binding beside it; returns the library's path.
+
+    Raises on a compiler error. The library needs nvcc alone: on a host without what the binding needs
+    (torch with its headers, g++) it is built all the same, and a line on stderr says what is missing."""
     BUILD.mkdir(exist_ok=True)
     nvcc = _nvcc()
     objects = []
@@ -119,32 +159,35 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
             if ptxas_verbose:
                 cmd[1:1] = ["-Xptxas", "-v"]
             jobs.append(cmd)
-    ops_source = CSRC / "py_ops.cpp"
     compile_jobs = len(jobs)
-    if force or _stale(OPS, [ops_source, *_headers(ops_source)]):
+    missing = _ops_missing()
+    if missing is not None:
+        OPS.unlink(missing_ok=True)  # what is there may be for another torch
+        sys.stderr.write(f"{OPS.name} is not built: {missing}\n")
+    elif force or _ops_stale():
+        OPS_STAMP.unlink(missing_ok=True)
         jobs.append(_ops_command())
 
     def run(cmd):
         if verbose:
             print(" ".join(cmd), flush=True)
-        proc = subprocess.run(cmd, capture_output=True, text=True)
-        return cmd, proc
+        return cmd, subprocess.run(cmd, capture_output=True, text=True)
+
+    def checked(cmd, proc):
+        if proc.returncode != 0 or verbose or ptxas_verbose:
+            sys.stderr.write(proc.stdout + proc.stderr)
+        if proc.returncode != 0:
+            raise RuntimeError(f"{Path(cmd[0]).name} failed ({proc.returncode}): {' '.join(cmd)}")
 
     with ThreadPoolExecutor(max_workers=max(1, min(len(jobs), os.cpu_count() or 1))) as pool:
-        for cmd, proc in pool.map(run, jobs):
-            if proc.returncode != 0 or verbose or ptxas_verbose:
-                sys.stderr.write(proc.stdout + proc.stderr)
-            if proc.returncode != 0:
-                raise RuntimeError(f"{Path(cmd[0]).name} failed ({proc.returncode}): {' '.join(cmd)}")
-
+        done = list(pool.map(run, jobs))
+    for cmd, proc in done[:compile_jobs]:
+        checked(cmd, proc)
     if force or compile_jobs or _stale(LIB, objects):
-        cmd = [nvcc, *ARCH, "-shared", "-cudart", "static", "-o", str(LIB), *map(str, objects)]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        proc = subprocess.run(cmd, capture_output=True, text=True)
-        if proc.returncode != 0:
-            sys.stderr.write(proc.stdout + proc.stderr)
-            raise RuntimeError(f"link failed ({proc.returncode})")
+        checked(*run([nvcc, *ARCH, "-shared", "-cudart", "static", "-o", str(LIB), *map(str, objects)]))
+    for cmd, proc in done[compile_jobs:]:  # the binding, after the library stands
+        checked(cmd, proc)
+        OPS_STAMP.write_text(_ops_stamp())
     return LIB
 
 
