@@ -563,6 +563,13 @@ class PagedKV:
         self._refresh_slots()
 
     # ---------------------------------------------------------------- helpers
+    def move_blocks(self, src, dst, remap) -> None:
+        """Refused: the block table is fixed for the container's life (its decode plan keeps parts of it
+        between launches). Compact the pool between containers; an ``Fp4KV`` moves live."""
+        raise RuntimeError(
+            "a PagedKV's block table is fixed: move the pool's blocks with serve.block_copy.copy_blocks and build a new "
+            "container over the renumbered tables (captured steps included)")
+
     def past_len(self) -> int:
         return max(self._host_valid) if self._host_valid else 0
 

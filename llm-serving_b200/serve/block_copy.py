@@ -39,7 +39,9 @@ def copy_blocks(pools, src, dst, *, block_table=None, remap=None) -> None:
     yet to fill (a fork of a fork: copy before the second). Nothing on the host can check device vectors
     without waiting for them. With ``block_table`` (int32 ``(B, max_blocks)``) and
     ``remap`` (int32 ``(n_blocks,)``), every table entry ``e`` inside the pool becomes ``remap[e]``
-    in the same launch. Runs on the current stream.
+    in the same launch; that is for tables of the caller's own and for ``Fp4KV.move_blocks``, not for the
+    table of a live ``PagedKV``, which is fixed: after moving a ``PagedPool``'s blocks, build its
+    containers and captured steps anew over renumbered tables. Runs on the current stream.
     """
     ops = _native.ops or _native.require_ops()
     if hasattr(pools, "block_tensors"):
