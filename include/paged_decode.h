@@ -346,7 +346,7 @@ int pd_qk_norm_rope(const void* q, int64_t q_st, int64_t q_sh, const void* k, in
  * pd_fp4_write_slots quantises token i of k / v (n_tokens, n_kv_head, D; strides of token and
  * head, unit last) into flat slot slot_ids[i] (pd_kv_append_slots' slots): scale = e4m3(max |x /
  * unit| / 6), code = e2m1(x / unit / scale), both to nearest with ties to even, saturating; NaN
- * counts as zero. pd_fp4_write_table takes row b's slot from its block table and position, as
+ * counts as zero; the sign of a zero code is not defined. pd_fp4_write_table takes row b's slot from its block table and position, as
  * pd_kv_append_table does. pd_fp4_read_slots writes the values back as dst_dtype (exact for units
  * of 1 in 16 bits; rounded to nearest where the type's range ends). Slots outside the pool are
  * skipped (read: zeros) and flagged with PD_DEVERR_APPEND_RANGE. */

@@ -38,8 +38,9 @@
 //
 // Measured, bf16, 16 heads on 8 of 128: 32 rows of 8192 tokens, 302 MB, 66.9 us (4.5 TB/s, 0.69 of the
 // copy rate; the loads alone reach 0.95), 32 of 2048 25.2 us, one of 700 9.7 us; 61 rows of skewed lengths,
-// 8 heads on 2 of 256, fp16, 59 MB, 28.6 us. What is left over the bytes: 339 warp instructions per record
-// (64 conversions, 64 multiplies and 16 MMAs of them at least; schedulers issue in 0.62 of their
+// 8 heads on 2 of 256, fp16, 59 MB, 28.6 us; in fp16 (P in two parts) the first two take 74.3 and 27.3. What is
+// left over the bytes: 339 warp instructions per record, 312 in the loop and the rest what a warp spends
+// outside it (64 conversions, 64 multiplies and 16 MMAs at least; schedulers issue in 0.62 of their
 // cycles, with 4 warps each to choose from), and some 6 us of start, joins and launch.
 #pragma once
 

@@ -7,18 +7,22 @@
 // which is exact in fp32 and, for u = 1, in fp16 and bf16.
 //
 // Bound by memory in bytes (a token's rows are read once and 9/16 of a byte per element written),
-// in practice by instructions: 16 elements are 41 bytes of traffic, so at the copy rate an SM has some
-// 180 issue slots a warp's 512 elements. One thread handles one group of 16: its maximum and its
+// in practice by instructions and latency: 16 elements are 41 bytes of traffic, so at the copy rate an SM has
+// some 180 issue slots a warp's 512 elements; the write takes 193 and issues in 57 % of its active cycles
+// (half of the warps fit: 45 registers, and most wait on their source), the read 155 in 41 %, held up by its
+// loads of 8 bytes and of one. One thread handles one group of 16: its maximum and its
 // eight code bytes are its own, so there is no exchange between threads; consecutive threads
 // take consecutive groups of a row, so a warp reads 1 KB of 16-bit source in one run.
 //
 // Measured: 7001 bf16 tokens of 8 heads of 128 written into scattered slots and read back, two
-// launches, 74 MB, 21.8 us (3.4 TB/s); 32 tokens 4.3 us for the two. A token is 8 or 64 bytes at a time of a
-// record, so scattered writes meet each 32-byte sector of V several times in L2; tokens of one
+// launches, 74 MB, 21.9 us (3.4 TB/s), apart 9.2 and 11.2; into slots in order 9.1 and 10.4. fp32 rows, whose
+// codes come from comparisons, 22.8 and 19.3. 32 tokens 4.2 us for the two (fp32 6.1). A token is 8 or 64 bytes at a
+// time of a record, so scattered writes meet each 32-byte sector of V several times in L2; tokens of one
 // record written together do not.
 //
-// The rounding is exact, not approximately so, which is what lets a reader compare pages bit for bit.
-// A 16-bit x has at most 11 significant bits and scale * tie at most 7, so x / scale is either a tie
+// The rounding is exact, not approximately so, which is what lets a reader compare bit for bit what pages
+// stand for. (Their bytes may differ in the sign of a zero code: a negative element below 2^-17 of a code
+// step becomes +0 from 16 bits and -0 from fp32.) A 16-bit x has at most 11 significant bits and scale * tie at most 7, so x / scale is either a tie
 // exactly or at least 2^-11 (relative) away from it: fma(x, 1 / scale, 192) - 192 rounds the quotient
 // (which the reciprocal's 2 ulp leave within 2^-20) to a multiple of 2^-16, which restores exact ties and moves nothing across one, and the
 // hardware conversion then rounds it to a code. fp32 sources have no such gap: their codes come

@@ -13,7 +13,9 @@
 // norm one shuffle reduction over the D / 8 lanes of a head. A warp takes NORM_HEADS heads of one
 // token per lane group and issues their loads together: the cos/sin row is read once for
 // them, and a lane has 64 bytes in flight. Measured: 6001 tokens of 8 + 2 heads of 256, fp16, 62 MB,
-// 14.1 us (4.4 TB/s, two thirds of the copy rate; some 2 us of it the launch); one token 2.1 us.
+// 14.0 us (4.4 TB/s, two thirds of the copy rate; some 2 us of it the launch); one token 2.2 us. Rows at
+// any other head_dim or alignment take the second kernel, one element of 2 or 4 bytes at a time: 6001 tokens of
+// 16 + 8 heads of 128, bf16, 14.5 us aligned and 89 us one element off; of 96, 84 us; one token 3.0 us.
 #include "pd_internal.h"
 #include "pd_norm_rope.cuh"
 
@@ -22,7 +24,7 @@ namespace pd {
 namespace {
 
 constexpr int NORM_HEADS = 4;  // heads in flight per lane group
-constexpr int THREADS = 128;    // of a CTA: small, so that the last ones spread evenly (14.1 us against 14.4 with 256)
+constexpr int THREADS = 128;    // of a CTA: small, so that the last ones spread evenly (14.1 us, 14.4 with 256)
 
 // 4 consecutive elements as they are in memory: 8 bytes of 16-bit types, 16 of fp32.
 template <typename T>

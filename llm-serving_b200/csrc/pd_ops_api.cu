@@ -70,7 +70,11 @@ int rows_common(Fp4RowsParams& p, int dtype, bool read, const int64_t* k_strides
 // with 2048 keys: 16 rows of 8 tokens (2.2 units per SM, one wave) 28.5 and 38.1 us, of 16 (3.9) 42.4 and
 // 38.5, of 32 (7.4) 72.8 and 38.9, one row of 1024 tokens (13.9) 185 and 52; 8 heads on 2 of 256: 16 rows
 // of 16 tokens (1.8) 43.6 and 48.3, of 32 (3.6) 72.3 and 48.6; 4 heads on 4 of 64: one row of 1024 tokens
-// (3.5) 39.2 and 47.1, 16 rows of 128 (7.1) 51.9 and 31.1.
+// (3.5) 39.2 and 47.1, 16 rows of 128 (7.1) 51.9 and 31.1. In fp16 P's second part slows both: 16 rows of
+// 8 tokens 30.9 and 48.0, of 16 47.5 and 48.2, of 32 80.3 and 48.3; with the same constants the choice is within
+// 12 % of the better kernel (the worst, 32 rows of 16 tokens with 1024 keys, 49.4 and 55.0), but for few rows
+// whose keys are far fewer than their fellows' counts suggest (4 rows of 64 tokens with 512 keys at
+// head_dim 256 25.2 and 21.0).
 bool use_tiles(int64_t total_q, int32_t max_seqlen_q, int32_t batch, int32_t n_kv_head, int32_t group,
                int32_t head_dim, int sms) {
   const double WAVE_UNITS = head_dim == 256 ? 2.1 : head_dim == 128 ? 3.3 : 4.3;

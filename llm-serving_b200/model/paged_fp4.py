@@ -39,6 +39,7 @@ __all__ = ["Fp4KV", "Fp4Pool", "fp4_pages", "fp4_workspace", "paged_decode_fp4",
 _HEAD_DIMS = (64, 128, 256)
 _QUERY_DTYPES = (torch.float16, torch.bfloat16)
 
+
 def _pool_rules(block_size, head_dim):
     yield not _pow2(block_size) or block_size < 16, lambda: (
         f"block_size must be a power of two of at least 16, got {block_size}")
@@ -80,7 +81,7 @@ def read_slots_fp4(pages, slot_ids, dtype=torch.bfloat16, *, units=None):
 
 def paged_decode_fp4(q, pages, block_table, seqlen, *, units=None, scale: float | None = None, out=None,
                      workspace=None):
-    """Decode one query token per row against 4-bit pages (one kernel launch).
+    """Decode one query token per row against 4-bit pages (one kernel launch for every 896 rows).
 
     ``q`` ``(B, H, D)`` fp16 or bf16; ``block_table`` int32 ``(B, max_blocks)``, of whose row ``b`` only
     the first ``ceil(seqlen[b] / block_size)`` entries matter; ``seqlen`` ``(B,)`` int32 (int64 is
@@ -94,13 +95,14 @@ def paged_decode_fp4(q, pages, block_table, seqlen, *, units=None, scale: float 
 
 def paged_prefill_fp4(q, pages, block_table, cu_seqlens_q, seqlen_k, max_seqlen_q: int, *, units=None,
                       scale: float | None = None, out=None, workspace=None):
-    """Causal attention of a chunk of query tokens per row over 4-bit pages (one kernel launch).
+    """Causal attention of a chunk of query tokens per row over 4-bit pages (one kernel launch for every
+    896 rows).
 
     ``paged_prefill``'s contract: ``q`` is the packed ``(total_q, H, D)``, row ``b`` owning
     ``q[cu_seqlens_q[b]:cu_seqlens_q[b + 1]]``; the chunk's K/V are already in the pages, and its token
     ``i`` of ``Sq`` sees keys ``0 .. seqlen_k[b] - Sq + i``. ``max_seqlen_q`` must be at least the longest
-    chunk; tokens of a longer one past it are left unwritten. ``workspace`` as in
-    :func:`paged_decode_fp4`.
+    chunk (a loose bound costs nothing); tokens of a longer one past it are left unwritten. ``workspace``
+    as in :func:`paged_decode_fp4`.
     """
     ops = _native.ops or _native.require_ops()
     return ops.fp4_prefill(q, pages, block_table, cu_seqlens_q, seqlen_k, max_seqlen_q, units, scale, out, workspace)
@@ -190,7 +192,7 @@ class Fp4Pool(PagedPool):
 
 class Fp4KV(PagedKV):
     """Decode-time container over an :class:`Fp4Pool`: ``PagedKV``'s step protocol, with the step's
-    token quantised by ``write`` (one launch) and read by ``attend`` (one launch).
+    token quantised by ``write`` (one launch) and read by ``attend`` (one launch for every 896 rows).
 
     K comes rotated (``qk_norm_rope`` rotates q and k together); ``write(rope=...)`` is refused.
     """
