@@ -687,7 +687,9 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) pd_fp4_prefill_kernel(cons
       tc::fence_after_sync();
       const float inv = l_run > 0.f ? v_unit / l_run : 0.f;
       // Through the warp's own 32 rows of the Q tile, which no MMA reads any more, so that a store
-      // instruction writes whole rows instead of 16 bytes of 32 of them.
+      // instruction writes whole rows instead of 16 bytes of 32 of them. The block's other warps copied Q
+      // there: the first S says that their copies have landed, and without one a barrier has to.
+      if (mine == 0) asm volatile("bar.sync %0, 128;" ::"r"(1 + q) : "memory");
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
