@@ -72,9 +72,9 @@ int rows_common(Fp4RowsParams& p, int dtype, bool read, const int64_t* k_strides
 // of 16 tokens (1.8) 43.6 and 48.3, of 32 (3.6) 72.3 and 48.6; 4 heads on 4 of 64: one row of 1024 tokens
 // (3.5) 39.2 and 47.1, 16 rows of 128 (7.1) 51.9 and 31.1. In fp16 P's second part slows both: 16 rows of
 // 8 tokens 30.9 and 48.0, of 16 47.5 and 48.2, of 32 80.3 and 48.3; with the same constants the choice is within
-// 12 % of the better kernel (the worst, 32 rows of 16 tokens with 1024 keys, 49.4 and 55.0), but for few rows
-// whose keys are far fewer than their fellows' counts suggest (4 rows of 64 tokens with 512 keys at
-// head_dim 256 25.2 and 21.0).
+// 12 % of the better kernel over 64 such shapes (the worst, 32 rows of 16 tokens with 1024 keys, 49.4 and
+// 55.0), but for one with few keys, where the warp kernel's start counts more (in both types: 4 rows of 64
+// tokens with 512 keys at head_dim 256, 25.2 and 21.0).
 bool use_tiles(int64_t total_q, int32_t max_seqlen_q, int32_t batch, int32_t n_kv_head, int32_t group,
                int32_t head_dim, int sms) {
   const double WAVE_UNITS = head_dim == 256 ? 2.1 : head_dim == 128 ? 3.3 : 4.3;
