@@ -146,6 +146,12 @@ int geometry(int n_head, int n_kv_head, int head_dim, int block_size, int dtype,
   const int row_bytes = head_dim * elem_size(dtype);
   g->tile = 4096 / row_bytes;
   g->box_tokens = block_size < g->tile ? block_size : g->tile;
+  // A tile takes its boxes side by side, and a TMA copy into shared memory starts on 128 bytes.
+  if (g->box_tokens * row_bytes % 128 != 0) {
+    snprintf(g_last_error, sizeof(g_last_error), "a block of one head has %d bytes, the kernel needs a multiple of 128",
+             block_size * row_bytes);
+    return PD_ERR_UNSUPPORTED;
+  }
   int mode;
   {
     std::lock_guard<std::mutex> lock(g_mutex);

@@ -21,7 +21,8 @@ no fallback: without the library or CUDA every entry point raises ``RuntimeError
 What runs underneath is the C ABI of ``include/paged_decode.h`` (``pd_decode`` and
 ``pd_plan_*``): a TMA-fed, warp-pipelined sm_100a kernel that balances KV pages over every SM
 and merges split rows in the same launch. Differences from the reference that a caller can
-observe: ``head_dim`` must be in 8..256 (a power of two, as before); pool strides must be
+observe: ``head_dim`` must be in 8..256 (a power of two, as before); a block of one head holds at least
+128 bytes; pool strides must be
 16-byte multiples with a unit ``head_dim`` stride -- ``paged_decode`` copies a pool that is
 not, ``paged_decode_plan`` refuses it; and a table entry outside the pool reads zeros
 instead of faulting.
@@ -108,6 +109,9 @@ def _contract(q, k_cache, v_cache, block_table, seqlen):
     yield not _pow2(head_dim), lambda: f"head_dim must be a power of two for the kernel, got {head_dim}"
     yield not _MIN_HEAD_DIM <= head_dim <= _MAX_HEAD_DIM, lambda: (
         f"head_dim {head_dim} is outside the sm_100a kernel's range {_MIN_HEAD_DIM}..{_MAX_HEAD_DIM}")
+    block_bytes = block_size * head_dim * q.element_size()
+    yield min(block_bytes, 4096) % 128 != 0, lambda: (
+        f"a block of one head needs a multiple of 128 bytes for the sm_100a kernel, got {block_bytes}")
 
     batch = q.shape[0]
     yield block_table.dim() != 2, lambda: (
