@@ -382,6 +382,65 @@ int pd_fp4_prefill(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, c
                    int32_t batch, int32_t max_seqlen_q, int32_t n_head, int32_t n_kv_head, int32_t head_dim,
                    int32_t dtype, float scale_log2, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------- a cache of bounded length
+ * No reference counterpart. The pools, tables and lengths are pd_decode's.
+ *
+ * Window: the query at position i sees key j iff j <= i and (i - j < window or j < sinks), window >= 1,
+ * sinks >= 0. Only pages that hold a visible token are looked up. Any number of q heads per kv head. */
+
+/* Bytes of the workspace of pd_decode_window and pd_decode_weights, and of each half of
+ * pd_plan_create_window's; any contents, one workspace per stream, never shared with other entry points. */
+size_t pd_decode_window_workspace_bytes(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim,
+                                        int32_t dtype);
+
+/* pd_decode where row b's query sits at position seqlen[b] - 1 and sees its window. */
+int pd_decode_window(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache, const void* v_cache,
+                     int64_t n_blocks, int32_t block_size, const int64_t* k_strides, const int64_t* v_strides,
+                     const int32_t* block_table, int64_t bt_stride, int32_t max_blocks, const int32_t* seqlen,
+                     int32_t window, int32_t sinks, void* out, int64_t o_sb, int64_t o_sh, int32_t batch,
+                     int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype, float scale_log2,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* pd_plan_create for windowed rows: every run of the plan is pd_decode_window's. */
+int pd_plan_create_window(pd_plan** plan, int32_t n_layer, const void* const* k_caches,
+                          const void* const* v_caches, int64_t n_blocks, int32_t block_size,
+                          const int64_t* k_strides, const int64_t* v_strides, const int32_t* block_table,
+                          int64_t bt_stride, int32_t max_blocks, const int32_t* seqlen, int32_t window, int32_t sinks,
+                          int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype,
+                          float scale_log2, void* workspace, size_t workspace_bytes);
+
+/* Scratch of pd_decode_weights (16-byte aligned, any contents). */
+size_t pd_decode_weights_scratch_bytes(int32_t batch, int32_t n_head, int32_t max_blocks, int32_t block_size);
+
+/* pd_decode that also adds, for j < seqlen[b], the sum over the q heads of kv head g of their weight of token j
+ * to weights[b * w_sb + g * w_sh + j] (fp32; w_len >= max_blocks * block_size). */
+int pd_decode_weights(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache, const void* v_cache,
+                      int64_t n_blocks, int32_t block_size, const int64_t* k_strides, const int64_t* v_strides,
+                      const int32_t* block_table, int64_t bt_stride, int32_t max_blocks, const int32_t* seqlen,
+                      float* weights, int64_t w_sb, int64_t w_sh, int64_t w_len, void* out, int64_t o_sb, int64_t o_sh,
+                      int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype,
+                      float scale_log2, void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes,
+                      void* stream);
+
+/* Scratch of pd_evict (16-byte aligned, any contents). */
+size_t pd_evict_scratch_bytes(int32_t n_layer, int32_t batch, int32_t n_kv_head, int32_t keep);
+
+/* Per (layer, row, kv head) of n = seqlen[b] > keep tokens: the first `sinks` and the last `recent` stay
+ * (sinks + recent <= keep), and of the others those with the keep - sinks - recent largest weights (a tie keeps
+ * the lower index; NaN is the smallest). The kept tokens' K and V take, in order, positions 0 .. keep - 1 of
+ * new_table's pages, or of block_table's (new_table NULL: in place); shorter rows stay as they are (they are
+ * copied to new_table's). weights (n_layer, B, H_kv, w_len) by strides of the first three; weights_out takes the kept
+ * ones, zeros behind them (it may be weights), seqlen_out min(n, keep) (it may be seqlen). A block written for one
+ * row is read or written for no other. A block id outside the pool is skipped and sets PD_DEVERR_COPY_RANGE.
+ * Rows of 16-byte multiples; every layer's pools have one layout. */
+int pd_evict(void* const* k_caches, void* const* v_caches, int32_t n_layer, int64_t n_blocks, int32_t block_size,
+             int32_t n_kv_head, int32_t head_dim, int32_t dtype, const int64_t* k_strides, const int64_t* v_strides,
+             const int32_t* block_table, int64_t bt_stride, int32_t max_blocks, const int32_t* new_table,
+             int64_t nbt_stride, int32_t new_max_blocks, const int32_t* seqlen, int32_t* seqlen_out,
+             const float* weights, const int64_t* w_strides, float* weights_out, const int64_t* wo_strides,
+             int64_t w_len, int32_t batch, int32_t keep, int32_t recent, int32_t sinks, void* scratch,
+             size_t scratch_bytes, void* stream);
+
 /* ---------------------------------------------------------------- page copies
  *
  * pd_block_copy -- block dst[i] takes the bytes of block src[i] in each of n_pools pools

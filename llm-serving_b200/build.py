@@ -48,6 +48,12 @@ SOURCES = [
     "pd_decode_f32.cu",
     "pd_decode_mma_bf16.cu",
     "pd_decode_mma_f16.cu",
+    "pd_decode_var_bf16.cu",
+    "pd_decode_var_f16.cu",
+    "pd_decode_var_f32.cu",
+    "pd_decode_var_mma_bf16.cu",
+    "pd_decode_var_mma_f16.cu",
+    "pd_weights.cu",
     "pd_prefill.cu",
     "pd_prefill_tc.cu",
     "pd_ops_api.cu",
@@ -56,6 +62,7 @@ SOURCES = [
     "pd_fp4_attend.cu",
     "pd_fp4_prefill.cu",
     "pd_block_copy.cu",
+    "pd_evict.cu",
 ]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [

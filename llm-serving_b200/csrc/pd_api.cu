@@ -129,19 +129,28 @@ struct Geometry {
   bool mma;        // per-warp kernel with tensor-core tile math (swizzled 5-D pool maps)
   int box_heads;   // kv heads per TMA box: all of them in the shared-stage kernel, else 1
   int stage_bytes; // K + V bytes of one stage (of one warp, or of the CTA when shared)
+  int variant;     // Variant
 };
 
-int geometry(int n_head, int n_kv_head, int head_dim, int block_size, int dtype, Geometry* g) {
+// The variants of the decode kernel (VAR in pd_decode_kernel.cuh) that a call asks for.
+enum Variant { PLAIN = 0, WINDOW = 1, SCORES = 2 };
+
+int geometry(int n_head, int n_kv_head, int head_dim, int block_size, int dtype, Variant variant, Geometry* g) {
   if (!valid_dtype(dtype)) return PD_ERR_INVALID;
   if (n_kv_head < 1 || n_head < 1 || n_head % n_kv_head != 0) return PD_ERR_INVALID;
   if (!pow2(head_dim) || !pow2(block_size)) return PD_ERR_INVALID;
   if (head_dim < 8 || head_dim > 256) return PD_ERR_UNSUPPORTED;
   const int group = n_head / n_kv_head;
   int gt = 8;
-  while (group % gt != 0) gt >>= 1;
+  if (variant == PLAIN) {
+    while (group % gt != 0) gt >>= 1;
+  } else {  // chunks may be partly filled, so that K/V are read by as few items as can be
+    while (gt / 2 >= group) gt >>= 1;
+  }
   g->gt = gt;
   g->gt_index = ilog2_host(gt);
-  g->n_gchunks = group / gt;
+  g->n_gchunks = (group + gt - 1) / gt;
+  g->variant = variant;
   g->d_index = ilog2_host(head_dim) - 3;
   const int row_bytes = head_dim * elem_size(dtype);
   g->tile = 4096 / row_bytes;
@@ -157,7 +166,7 @@ int geometry(int n_head, int n_kv_head, int head_dim, int block_size, int dtype,
     std::lock_guard<std::mutex> lock(g_mutex);
     mode = g_decode_mode;
   }
-  g->cta = mode == 1 && n_kv_head * g->n_gchunks == kCtaConsumerWarps && gt <= 4 &&
+  g->cta = variant == PLAIN && mode == 1 && n_kv_head * g->n_gchunks == kCtaConsumerWarps && gt <= 4 &&
            (dtype == PD_BF16 || dtype == PD_F16) && head_dim >= 64;
   g->mma = !g->cta && mode != 2 && (dtype == PD_BF16 || dtype == PD_F16) && head_dim >= 64 &&
            g->box_tokens >= 8;
@@ -169,8 +178,19 @@ int geometry(int n_head, int n_kv_head, int head_dim, int block_size, int dtype,
 DecodeLaunchFn launcher_for(int dtype, const Geometry& g) {
   if (g.cta) return dtype == PD_BF16 ? decode_launcher_cta_bf16(g.d_index, g.gt_index)
                                      : decode_launcher_cta_f16(g.d_index, g.gt_index);
+  if (g.mma && g.variant != PLAIN)
+    return dtype == PD_BF16 ? decode_launcher_var_mma_bf16(g.variant, g.d_index, g.gt_index)
+                            : decode_launcher_var_mma_f16(g.variant, g.d_index, g.gt_index);
   if (g.mma) return dtype == PD_BF16 ? decode_launcher_mma_bf16(g.d_index, g.gt_index)
                                      : decode_launcher_mma_f16(g.d_index, g.gt_index);
+  if (g.variant != PLAIN) {
+    switch (dtype) {
+      case PD_F32: return decode_launcher_var_f32(g.d_index, g.gt_index);
+      case PD_F16: return decode_launcher_var_f16(g.d_index, g.gt_index);
+      case PD_BF16: return decode_launcher_var_bf16(g.d_index, g.gt_index);
+    }
+    return nullptr;
+  }
   switch (dtype) {
     case PD_F32: return decode_launcher_f32(g.d_index, g.gt_index);
     case PD_F16: return decode_launcher_f16(g.d_index, g.gt_index);
@@ -360,9 +380,11 @@ struct Prepared {
 int prepare(Prepared* P, int64_t n_blocks, int32_t block_size, const int32_t* block_table,
             int64_t bt_stride, int32_t max_blocks, const int32_t* seqlen, int32_t batch,
             int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype, float scale_log2,
-            void* workspace, size_t workspace_bytes) {
+            void* workspace, size_t workspace_bytes, Variant variant = PLAIN, int32_t window = 0,
+            int32_t sinks = 0) {
   if (batch < 0 || max_blocks < 0 || n_blocks < 1) return PD_ERR_INVALID;
-  int st = geometry(n_head, n_kv_head, head_dim, block_size, dtype, &P->g);
+  if (variant == WINDOW && (window < 1 || sinks < 0)) return PD_ERR_INVALID;
+  int st = geometry(n_head, n_kv_head, head_dim, block_size, dtype, variant, &P->g);
   if (st != PD_OK) return st;
   P->fn = launcher_for(dtype, P->g);
   if (P->fn == nullptr) return PD_ERR_UNSUPPORTED;
@@ -430,11 +452,14 @@ int prepare(Prepared* P, int64_t n_blocks, int32_t block_size, const int32_t* bl
   p.smem_arrays_off = P->L.arrays_off;
   p.smem_stage_off = P->L.stage_off;
   p.scale_log2 = scale_log2;
+  // No row is longer than 2^30 tokens: larger windows and more sinks see the same.
+  p.window = variant == WINDOW ? std::min(window, 1 << 30) : 1 << 30;
+  p.sinks = variant == WINDOW ? std::min(sinks, 1 << 30) : 0;
   {  // everything besides the lengths that the work split depends on
     uint64_t x = 0x243F6A8885A308D3ull;
     const int64_t shape[] = {batch, n_head, n_kv_head, head_dim, dtype, block_size, max_blocks,
                              P->L.grid, P->L.warps, P->L.stages, P->L.min_tiles, P->L.rows_per_launch,
-                             P->g.gt, P->g.mma, P->g.cta, p.row_cost};
+                             P->g.gt, P->g.mma, P->g.cta, p.row_cost, variant, p.window, p.sinks};
     for (int64_t v : shape) {
       x = (x ^ uint64_t(v)) * 0x100000001B3ull;
       x ^= x >> 29;
@@ -481,7 +506,8 @@ struct AppendArgs {
 int run_prepared(const Prepared& P, const CUtensorMap& kmap, const CUtensorMap& vmap, const void* q,
                  int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh, float* pm,
                  float* pl, float* pacc, int mode, int dtype, cudaStream_t stream,
-                 const AppendArgs* app = nullptr, bool overlap = false, uint32_t* seq = nullptr) {
+                 const AppendArgs* app = nullptr, bool overlap = false, uint32_t* seq = nullptr,
+                 float* scores = nullptr) {
   const int batch = P.base.batch;
   const int es = elem_size(dtype);
   for (int b0 = 0; b0 < batch; b0 += P.L.rows_per_launch) {
@@ -512,6 +538,11 @@ int run_prepared(const Prepared& P, const CUtensorMap& kmap, const CUtensorMap& 
       p.part_m = pm + int64_t(b0) * p.n_head;
       p.part_l = pl + int64_t(b0) * p.n_head;
       p.part_acc = pacc + int64_t(b0) * p.n_head * head_dim;
+    }
+    if (scores != nullptr) {
+      p.scores = scores + int64_t(b0) * p.n_head * p.capacity;
+      p.part_m = pm + int64_t(b0) * p.n_head;
+      p.part_l = pl + int64_t(b0) * p.n_head;
     }
     if (P.base.table) p.table = P.base.table + int64_t(b0) * P.base.bt_stride;
     p.seqlen = P.base.seqlen + b0;
@@ -555,11 +586,12 @@ int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache
                   int32_t max_blocks, const int32_t* seqlen, void* out, int64_t o_sb, int64_t o_sh,
                   float* pm, float* pl, float* pacc, int mode, int32_t batch, int32_t n_head,
                   int32_t n_kv_head, int32_t head_dim, int32_t dtype, float scale_log2,
-                  void* workspace, size_t workspace_bytes, void* stream) {
+                  void* workspace, size_t workspace_bytes, void* stream, Variant variant = PLAIN, int32_t window = 0,
+                  int32_t sinks = 0, float* scores = nullptr) {
   if (k_strides == nullptr || v_strides == nullptr) return PD_ERR_INVALID;
   Prepared P;
   int st = prepare(&P, n_blocks, block_size, block_table, bt_stride, max_blocks, seqlen, batch,
-                   n_head, n_kv_head, head_dim, dtype, scale_log2, workspace, workspace_bytes);
+                   n_head, n_kv_head, head_dim, dtype, scale_log2, workspace, workspace_bytes, variant, window, sinks);
   if (st != PD_OK) return st;
   if (batch == 0) return PD_OK;
   if (check_rows(q, q_sb, q_sh, dtype) != PD_OK) return PD_ERR_INVALID;
@@ -574,7 +606,18 @@ int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache
                    P.g.box_tokens, P.g.box_heads, P.g.mma);
   if (st != PD_OK) return st;
   return run_prepared(P, kmap, vmap, q, q_sb, q_sh, out, o_sb, o_sh, pm, pl, pacc, mode, dtype,
-                      static_cast<cudaStream_t>(stream));
+                      static_cast<cudaStream_t>(stream), nullptr, false, nullptr, scores);
+}
+
+size_t workspace_bytes(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype,
+                       Variant variant) {
+  Geometry g;
+  if (geometry(n_head, n_kv_head, head_dim, 16, dtype, variant, &g) != PD_OK) return 0;
+  int dev = 0;
+  if (current_device(&dev) != PD_OK) return 0;
+  Launch L;
+  if (launch_shape(dev, batch, g, &L) != PD_OK) return 0;
+  return workspace_layout(batch, n_kv_head, g, head_dim, L).total;
 }
 
 }  // namespace
@@ -618,6 +661,57 @@ struct pd_plan {
   mutable uint32_t seq = 0;  // launches made: selects the workspace half of the next one
 };
 
+static int plan_create(pd_plan** plan, int32_t n_layer, const void* const* k_caches, const void* const* v_caches,
+                       int64_t n_blocks, int32_t block_size, const int64_t* k_strides, const int64_t* v_strides,
+                       const int32_t* block_table, int64_t bt_stride, int32_t max_blocks, const int32_t* seqlen,
+                       int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype,
+                       float scale_log2, void* workspace, size_t workspace_bytes, Variant variant, int32_t window,
+                       int32_t sinks) {
+  if (plan == nullptr) return PD_ERR_INVALID;
+  *plan = nullptr;
+  if (n_layer < 1 || k_caches == nullptr || v_caches == nullptr || batch < 1) return PD_ERR_INVALID;
+  if (k_strides == nullptr || v_strides == nullptr) return PD_ERR_INVALID;
+  pd_plan* h = new (std::nothrow) pd_plan;
+  if (h == nullptr) return PD_ERR_INVALID;
+  int st = prepare(&h->P, n_blocks, block_size, block_table, bt_stride, max_blocks, seqlen, batch,
+                   n_head, n_kv_head, head_dim, dtype, scale_log2, workspace, workspace_bytes, variant, window, sinks);
+  if (st != PD_OK) {
+    delete h;
+    return st;
+  }
+  h->n_layer = n_layer;
+  h->dtype = dtype;
+  // Step cache of the work split: one batch chunk per launch and the per-warp kernel.
+  if (batch <= h->P.L.rows_per_launch && !h->P.g.cta)
+    h->P.base.step_rec = static_cast<unsigned char*>(workspace) + h->P.ws.step_off;
+  h->q_sh = head_dim;
+  h->q_sb = int64_t(n_head) * head_dim;
+  h->n_blocks = n_blocks;
+  for (int i = 0; i < 3; ++i) {
+    h->k_strides[i] = k_strides[i];
+    h->v_strides[i] = v_strides[i];
+  }
+  h->kmaps.resize(n_layer);
+  h->vmaps.resize(n_layer);
+  h->k_pools.resize(n_layer);
+  h->v_pools.resize(n_layer);
+  for (int layer = 0; layer < n_layer; ++layer) {
+    h->k_pools[layer] = const_cast<void*>(k_caches[layer]);
+    h->v_pools[layer] = const_cast<void*>(v_caches[layer]);
+    st = encode_pool(&h->kmaps[layer], k_caches[layer], n_blocks, block_size, n_kv_head, head_dim,
+                     k_strides, dtype, h->P.g.box_tokens, h->P.g.box_heads, h->P.g.mma);
+    if (st == PD_OK)
+      st = encode_pool(&h->vmaps[layer], v_caches[layer], n_blocks, block_size, n_kv_head, head_dim,
+                       v_strides, dtype, h->P.g.box_tokens, h->P.g.box_heads, h->P.g.mma);
+    if (st != PD_OK) {
+      delete h;
+      return st;
+    }
+  }
+  *plan = h;
+  return PD_OK;
+}
+
 extern "C" {
 
 const char* pd_status_string(int status) {
@@ -656,13 +750,12 @@ int pd_device_error(unsigned int* bits, int clear) {
 
 size_t pd_decode_workspace_bytes(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim,
                                  int32_t dtype) {
-  Geometry g;
-  if (geometry(n_head, n_kv_head, head_dim, 16, dtype, &g) != PD_OK) return 0;
-  int dev = 0;
-  if (current_device(&dev) != PD_OK) return 0;
-  Launch L;
-  if (launch_shape(dev, batch, g, &L) != PD_OK) return 0;
-  return workspace_layout(batch, n_kv_head, g, head_dim, L).total;
+  return workspace_bytes(batch, n_head, n_kv_head, head_dim, dtype, PLAIN);
+}
+
+size_t pd_decode_window_workspace_bytes(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim,
+                                        int32_t dtype) {
+  return workspace_bytes(batch, n_head, n_kv_head, head_dim, dtype, WINDOW);
 }
 
 int pd_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache, const void* v_cache,
@@ -675,6 +768,69 @@ int pd_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache, co
                        block_table, bt_stride, max_blocks, seqlen, out, o_sb, o_sh, nullptr, nullptr,
                        nullptr, 0, batch, n_head, n_kv_head, head_dim, dtype, scale_log2, workspace,
                        workspace_bytes, stream);
+}
+
+int pd_decode_window(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache, const void* v_cache,
+                     int64_t n_blocks, int32_t block_size, const int64_t* k_strides, const int64_t* v_strides,
+                     const int32_t* block_table, int64_t bt_stride, int32_t max_blocks, const int32_t* seqlen,
+                     int32_t window, int32_t sinks, void* out, int64_t o_sb, int64_t o_sh, int32_t batch,
+                     int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype, float scale_log2,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  return decode_common(q, q_sb, q_sh, k_cache, v_cache, n_blocks, block_size, k_strides, v_strides, block_table,
+                       bt_stride, max_blocks, seqlen, out, o_sb, o_sh, nullptr, nullptr, nullptr, 0, batch, n_head,
+                       n_kv_head, head_dim, dtype, scale_log2, workspace, workspace_bytes, stream, WINDOW, window,
+                       sinks);
+}
+
+size_t pd_decode_weights_scratch_bytes(int32_t batch, int32_t n_head, int32_t max_blocks, int32_t block_size) {
+  if (batch < 0 || n_head < 1 || max_blocks < 0 || block_size < 1) return 0;
+  // (m, l) of every row and head, then the scores of every head and token
+  return round_up(size_t(batch) * n_head * 8, 256) + size_t(batch) * n_head * size_t(max_blocks) * block_size * 4;
+}
+
+int pd_decode_weights(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache, const void* v_cache,
+                      int64_t n_blocks, int32_t block_size, const int64_t* k_strides, const int64_t* v_strides,
+                      const int32_t* block_table, int64_t bt_stride, int32_t max_blocks, const int32_t* seqlen,
+                      float* weights, int64_t w_sb, int64_t w_sh, int64_t w_len, void* out, int64_t o_sb, int64_t o_sh,
+                      int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype,
+                      float scale_log2, void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes,
+                      void* stream) {
+  if (w_len < int64_t(max_blocks) * block_size) return PD_ERR_INVALID;
+  if (n_kv_head > 65535) return PD_ERR_UNSUPPORTED;  // a grid's second dimension
+  if (batch > 0 && max_blocks > 0) {
+    if (weights == nullptr) return PD_ERR_INVALID;
+    if (scratch == nullptr || !aligned16(scratch) ||
+        scratch_bytes < pd_decode_weights_scratch_bytes(batch, n_head, max_blocks, block_size))
+      return api_message(PD_ERR_WORKSPACE, "scratch is smaller than pd_decode_weights_scratch_bytes");
+  }
+  float* m = static_cast<float*>(scratch);
+  float* l = m == nullptr ? nullptr : m + int64_t(batch) * n_head;
+  float* scores =
+      m == nullptr ? nullptr : reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + round_up(size_t(batch) * n_head * 8, 256));
+  const int st = decode_common(q, q_sb, q_sh, k_cache, v_cache, n_blocks, block_size, k_strides, v_strides, block_table,
+                               bt_stride, max_blocks, seqlen, out, o_sb, o_sh, m, l, nullptr, 0, batch, n_head,
+                               n_kv_head, head_dim, dtype, scale_log2, workspace, workspace_bytes, stream, SCORES, 0, 0,
+                               scores);
+  if (st != PD_OK || batch == 0 || max_blocks == 0) return st;
+  int dev = 0;
+  if (current_device(&dev) != PD_OK) return PD_ERR_CUDA;
+  WeightsParams p{};
+  p.scores = scores;
+  p.m = m;
+  p.l = l;
+  p.seqlen = seqlen;
+  p.weights = weights;
+  p.w_sb = w_sb;
+  p.w_sh = w_sh;
+  p.batch = batch;
+  p.n_kv_head = n_kv_head;
+  p.group = n_head / n_kv_head;
+  p.capacity = max_blocks * block_size;
+  p.sms = sm_count(dev);
+  const cudaError_t e = launch_weights(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "weights launch");
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return PD_OK;
 }
 
 int pd_prefill(const void* q, int64_t q_st, int64_t q_sh, const void* k_cache, const void* v_cache,
@@ -769,49 +925,20 @@ int pd_plan_create(pd_plan** plan, int32_t n_layer, const void* const* k_caches,
                    int64_t bt_stride, int32_t max_blocks, const int32_t* seqlen, int32_t batch,
                    int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype,
                    float scale_log2, void* workspace, size_t workspace_bytes) {
-  if (plan == nullptr) return PD_ERR_INVALID;
-  *plan = nullptr;
-  if (n_layer < 1 || k_caches == nullptr || v_caches == nullptr || batch < 1) return PD_ERR_INVALID;
-  if (k_strides == nullptr || v_strides == nullptr) return PD_ERR_INVALID;
-  pd_plan* h = new (std::nothrow) pd_plan;
-  if (h == nullptr) return PD_ERR_INVALID;
-  int st = prepare(&h->P, n_blocks, block_size, block_table, bt_stride, max_blocks, seqlen, batch,
-                   n_head, n_kv_head, head_dim, dtype, scale_log2, workspace, workspace_bytes);
-  if (st != PD_OK) {
-    delete h;
-    return st;
-  }
-  h->n_layer = n_layer;
-  h->dtype = dtype;
-  // Step cache of the work split: one batch chunk per launch and the per-warp kernel.
-  if (batch <= h->P.L.rows_per_launch && !h->P.g.cta)
-    h->P.base.step_rec = static_cast<unsigned char*>(workspace) + h->P.ws.step_off;
-  h->q_sh = head_dim;
-  h->q_sb = int64_t(n_head) * head_dim;
-  h->n_blocks = n_blocks;
-  for (int i = 0; i < 3; ++i) {
-    h->k_strides[i] = k_strides[i];
-    h->v_strides[i] = v_strides[i];
-  }
-  h->kmaps.resize(n_layer);
-  h->vmaps.resize(n_layer);
-  h->k_pools.resize(n_layer);
-  h->v_pools.resize(n_layer);
-  for (int layer = 0; layer < n_layer; ++layer) {
-    h->k_pools[layer] = const_cast<void*>(k_caches[layer]);
-    h->v_pools[layer] = const_cast<void*>(v_caches[layer]);
-    st = encode_pool(&h->kmaps[layer], k_caches[layer], n_blocks, block_size, n_kv_head, head_dim,
-                     k_strides, dtype, h->P.g.box_tokens, h->P.g.box_heads, h->P.g.mma);
-    if (st == PD_OK)
-      st = encode_pool(&h->vmaps[layer], v_caches[layer], n_blocks, block_size, n_kv_head, head_dim,
-                       v_strides, dtype, h->P.g.box_tokens, h->P.g.box_heads, h->P.g.mma);
-    if (st != PD_OK) {
-      delete h;
-      return st;
-    }
-  }
-  *plan = h;
-  return PD_OK;
+  return plan_create(plan, n_layer, k_caches, v_caches, n_blocks, block_size, k_strides, v_strides, block_table,
+                     bt_stride, max_blocks, seqlen, batch, n_head, n_kv_head, head_dim, dtype, scale_log2, workspace,
+                     workspace_bytes, PLAIN, 0, 0);
+}
+
+int pd_plan_create_window(pd_plan** plan, int32_t n_layer, const void* const* k_caches,
+                          const void* const* v_caches, int64_t n_blocks, int32_t block_size,
+                          const int64_t* k_strides, const int64_t* v_strides, const int32_t* block_table,
+                          int64_t bt_stride, int32_t max_blocks, const int32_t* seqlen, int32_t window, int32_t sinks,
+                          int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype,
+                          float scale_log2, void* workspace, size_t workspace_bytes) {
+  return plan_create(plan, n_layer, k_caches, v_caches, n_blocks, block_size, k_strides, v_strides, block_table,
+                     bt_stride, max_blocks, seqlen, batch, n_head, n_kv_head, head_dim, dtype, scale_log2, workspace,
+                     workspace_bytes, WINDOW, window, sinks);
 }
 
 int pd_plan_run(const pd_plan* plan, int32_t layer, const void* q, void* out, void* stream) {

@@ -465,6 +465,21 @@ struct DecodeParams {
   const void* rope_sin;
   int64_t rope_stride;
   int32_t rope_dim;
+  // Window variant: the query sees the last `window` tokens and the first `sinks`.
+  int32_t window;
+  int32_t sinks;
+  // Weights variant: scores (B, H_kv, capacity, group) in log2 units; with them part_m / part_l
+  // (B, H) take the rows' maximum and normaliser although mode is 0.
+  float* scores;
+};
+
+struct WeightsParams {
+  const float* scores;    // (B, H_kv, capacity, group) in log2 units
+  const float *m, *l;     // (B, H)
+  const int32_t* seqlen;  // (B,)
+  float* weights;         // row b, kv head h, token j at b * w_sb + h * w_sh + j
+  int64_t w_sb, w_sh;
+  int32_t batch, n_kv_head, group, capacity, sms;
 };
 
 struct AppendParams {

@@ -38,9 +38,17 @@
 //    next 32 prefetched), so a TMA issue never waits on a dependent global load inside a
 //    row. Table entries past ceil(seqlen / bs) are never read; an entry outside the pool
 //    makes TMA fill zeros instead of faulting.
+//  * VAR adds, in kernels of their own: bit 0, a window (pd_decode_window): a row's tiles are those
+//    that hold a visible token -- the first `sinks` and the last `window` -- numbered without the gap
+//    between them, so the split, its cache and the merge work on them as on a shorter row, and no
+//    hidden page is looked up or read but for the tokens that share a tile with a visible one; bit 1,
+//    every score and the rows' (m, l) are stored for the attention weights (pd_decode_weights).
 //  * Every mbarrier wait is bounded (1 s of %globaltimer). On expiry the warp records
 //    DEVERR_WAIT_TIMEOUT, drains its in-flight copies (bounded again) and returns.
 #pragma once
+
+#include <atomic>
+#include <type_traits>
 
 #include "pd_common.cuh"
 #include "pd_decode_mma.cuh"
@@ -87,6 +95,36 @@ template <typename T, int D, int GT>
 struct ConsumerSel<true, T, D, GT> {
   using W = MmaWorker<T, D, GT>;
   static constexpr int R = MmaCfg<T, D, GT>::R;
+};
+
+// The visible tiles of a row under a window: those of the first `sinks` tokens (tiles 0 .. st - 1) and
+// those of the last `window` (tiles st + skip ..), tile t of them being tile t + (t >= st ? skip : 0) of
+// the row. Without a window: every tile.
+template <int LOG_TILE>
+struct VisibleTiles {
+  int window, sinks, st;
+  __device__ __forceinline__ VisibleTiles(int window_, int sinks_)
+      : window(window_), sinks(sinks_), st((sinks_ + (1 << LOG_TILE) - 1) >> LOG_TILE) {}
+  __device__ __forceinline__ int first(int len) const { return len > window ? len - window : 0; }  // of the window
+  __device__ __forceinline__ int skip(int len) const {
+    const int gap = (first(len) >> LOG_TILE) - st;
+    return gap > 0 ? gap : 0;
+  }
+  __device__ __forceinline__ int count(int len) const { return ((len + (1 << LOG_TILE) - 1) >> LOG_TILE) - skip(len); }
+  __device__ __forceinline__ int row_tile(int t, int len) const { return t >= st ? t + skip(len) : t; }
+};
+
+// Which tokens of a tile count: those below `rows` (LiveRows), under a window only those at or past
+// `lo` or below `sk` (LiveWindow; `all`: every token of the tile).
+struct LiveRows {
+  int rows;
+  bool full;
+  __device__ __forceinline__ bool operator()(int t) const { return t < rows; }
+};
+struct LiveWindow {
+  int rows, lo, sk;
+  bool full;
+  __device__ __forceinline__ bool operator()(int t) const { return full || (t < rows && (t >= lo || t < sk)); }
 };
 
 // Position of a worker inside the unit sequence.
@@ -245,11 +283,37 @@ __device__ __forceinline__ int worker_of(int64_t u, int64_t units, int workers) 
 // kv heads (one TMA copy each per block part) into a shared stage, and the consumer warps --
 // warp j streams item j -- read their head's rows from it and release the stage on an
 // "empty" barrier. Contiguous block-sized copies keep the DRAM stream dense.
-template <typename T, int D, int GT, bool CTA, bool MMA>
+template <typename T, int D, int GT, bool CTA, bool MMA, int VAR>
 __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUtensorMap& kmap,
                                                 const CUtensorMap& vmap, unsigned char* smem) {
   using C = DecodeCfg<T, D, GT>;
   using E = Elem<T>;
+  constexpr bool WIN = (VAR & 1) != 0, LOG = (VAR & 2) != 0;
+  static_assert(!(CTA && VAR), "the shared-stage kernel has no variants");
+  using Live = std::conditional_t<WIN, LiveWindow, LiveRows>;
+  const VisibleTiles<C::LOG_TILE> vis(WIN ? p.window : 0, WIN ? p.sinks : 0);
+  auto tiles_of = [&](int len) -> int {
+    if constexpr (WIN) return vis.count(len);
+    return (len + C::TILE - 1) >> C::LOG_TILE;
+  };
+  // Query heads of chunk gc: the variants' last chunk may hold fewer than GT (its other columns are
+  // computed with q = 0 and dropped).
+  auto heads_of = [&](int gc) -> int { return VAR ? min(GT, p.group - gc * GT) : GT; };
+  // Tile of the row that a cursor's tile is.
+  auto row_tile = [&](const Cursor& c) -> int {
+    if constexpr (WIN) return vis.row_tile(c.tile, c.len);
+    return c.tile;
+  };
+  auto live_of = [&](const Cursor& c) -> Live {
+    const int tok0 = row_tile(c) << C::LOG_TILE;
+    const int rows = c.len - tok0;
+    if constexpr (WIN) {
+      const int lo = vis.first(c.len) - tok0, sk = vis.sinks - tok0;
+      return LiveWindow{rows, lo, sk, rows >= C::TILE && (lo <= 0 || sk >= C::TILE)};
+    } else {
+      return LiveRows{rows, rows >= C::TILE};
+    }
+  };
   const int tid = threadIdx.x;
   const int lane = tid & 31;
   const int warp = tid >> 5;
@@ -383,7 +447,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
       // Fused append: the tile holding the appended token takes it from the source when the
       // row reads that position (a position inside [0, len) is inside the table).
       if (p.append) apos[b] = pos >= 0 && pos < len ? int(pos) : -1;
-      local += (len + C::TILE - 1) >> C::LOG_TILE;
+      local += tiles_of(len);
     }
     int incl = local;
 #pragma unroll
@@ -416,7 +480,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
     int run = warp_sums[warp] + incl - local;
     for (int b = b0; b < b1; ++b) {
       pre[b] = run;
-      run += (lens[b] + C::TILE - 1) >> C::LOG_TILE;
+      run += tiles_of(lens[b]);
     }
     __syncthreads();
     if (use_step) {
@@ -668,7 +732,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
   const uint64_t kv_policy = l2_policy_evict_first();
   auto issue = [&](const Cursor& c, int s) {
     const int h = c.h;
-    const int tok0 = c.tile << C::LOG_TILE;
+    const int tok0 = row_tile(c) << C::LOG_TILE;
     const int remain = c.len - tok0;  // >= 1
     const int nvalid = min(nbox, (remain + box_tokens - 1) >> log2_box);
     const int npages = (c.len + bs - 1) >> p.log2_bs;
@@ -699,7 +763,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
   // tiles later, does not wait on DRAM.
   auto prefetch_q = [&](const Cursor& c) {
     constexpr int LINES = (C::ROW_BYTES + 127) / 128;  // 128-byte lines per q row
-    if (lane < GT * LINES) {
+    if (lane < heads_of(c.gc) * LINES) {
       const int hq = c.h * p.group + c.gc * GT + lane / LINES;
       prefetch_l2(reinterpret_cast<const unsigned char*>(p.q) +
                   (int64_t(c.b) * p.q_sb + int64_t(hq) * p.q_sh) * C::ES + (lane % LINES) * 128);
@@ -789,10 +853,10 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
   unsigned long long early_old = 0;   // add returned early_old)
 
   // Phase A of a tile: q.K for every (row, q head) of the stage, reduce-scattered so this
-  // lane ends with its R held scores, scaled to log2 units and masked past valid_rows.
-  auto tile_scores = [&](int stage, int valid_rows, float (&sc)[RR]) {
+  // lane ends with its R held scores, scaled to log2 units, -inf for tokens that do not count.
+  auto tile_scores = [&](int stage, const Live& live, float (&sc)[RR]) {
     if constexpr (MMA) {
-      mw.scores(stages_addr + uint32_t(stage) * uint32_t(stage_stride), valid_rows, p.scale_log2, sc);
+      mw.scores(stages_addr + uint32_t(stage) * uint32_t(stage_stride), live, p.scale_log2, sc);
     } else {
       const unsigned char* ks = my_stages + size_t(stage) * stage_stride + head_off;
       float sv[C::NV];
@@ -830,7 +894,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
 #pragma unroll
       for (int j = 0; j < C::R; ++j) {
         const float x = sv[j] * p.scale_log2;
-        sc[j] = hold_row[j] < valid_rows ? x : -INFINITY;
+        sc[j] = live(hold_row[j]) ? x : -INFINITY;
       }
     }
   };
@@ -879,11 +943,11 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
   };
 
   // Phase B, part 2: probabilities, their shuffle to the lanes that own each row's V chunk,
-  // and P.V into the fp32 accumulators. Rows at or past valid_rows contribute exact zeros
+  // and P.V into the fp32 accumulators. Tokens that do not count contribute exact zeros
   // (their V is zeroed too, so stale bytes -- even NaN patterns -- never reach acc).
-  auto tile_pv = [&](int stage, const float (&sc)[RR], int valid_rows, bool full) {
+  auto tile_pv = [&](int stage, const float (&sc)[RR], const Live& live, bool full) {
     if constexpr (MMA) {
-      mw.pv(stages_addr + uint32_t(stage) * uint32_t(stage_stride) + uint32_t(kv_stage_bytes), sc, valid_rows, full);
+      mw.pv(stages_addr + uint32_t(stage) * uint32_t(stage_stride) + uint32_t(kv_stage_bytes), sc, live, full);
     } else {
       float pj[C::R];
 #pragma unroll
@@ -910,9 +974,9 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
           E::unpack_pairs(raw, &vf[c * (C::EPC / 2)]);
         }
         if (!full) {
-          const bool live = row < valid_rows;
+          const bool counts = live(row);
 #pragma unroll
-          for (int e = 0; e < C::PPL; ++e) vf[e] = live ? vf[e] : make_float2(0.f, 0.f);
+          for (int e = 0; e < C::PPL; ++e) vf[e] = counts ? vf[e] : make_float2(0.f, 0.f);
         }
 #pragma unroll
         for (int g = 0; g < GT; ++g) {
@@ -927,18 +991,39 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
     }
   };
 
+  // The tile's scores to p.scores[b][h][token][q head of the group], for the weights' kernel.
+  auto store_scores = [&](const Cursor& c, const Live& live, const float (&sc)[RR]) {
+    if constexpr (LOG) {
+      if constexpr (VAR == 3) {
+        if (p.scores == nullptr) return;
+      }
+      const int tok0 = row_tile(c) << C::LOG_TILE;
+      float* dst = p.scores + ((int64_t(c.b) * p.n_kv_head + c.h) * p.capacity + tok0) * p.group + c.gc * GT;
+      if constexpr (MMA) {
+        mw.store_scores(dst, p.group, heads_of(c.gc), live, sc);
+      } else if (primary) {
+#pragma unroll
+        for (int j = 0; j < C::R; ++j)
+          if (live(hold_row[j]) && hold_g[j] < heads_of(c.gc)) dst[int64_t(hold_row[j]) * p.group + hold_g[j]] = sc[j];
+      }
+    }
+  };
+
   auto start_segment = [&](const Cursor& c) {
     if constexpr (MMA) {
-      mw.start(reinterpret_cast<const T*>(p.q) + int64_t(c.b) * p.q_sb, p.q_sh, c.h * p.group + c.gc * GT);
+      mw.start(reinterpret_cast<const T*>(p.q) + int64_t(c.b) * p.q_sb, p.q_sh, c.h * p.group + c.gc * GT,
+               heads_of(c.gc));
     } else {
       const int hq = c.h * p.group + c.gc * GT;
       const T* qrow = reinterpret_cast<const T*>(p.q) + int64_t(c.b) * p.q_sb;
+      const int heads = heads_of(c.gc);
 #pragma unroll
       for (int g = 0; g < GT; ++g) {
 #pragma unroll
         for (int cc = 0; cc < C::CPL; ++cc) {
-          const uint4 raw = __ldg(reinterpret_cast<const uint4*>(qrow + int64_t(hq + g) * p.q_sh +
-                                                                   (cc * C::LPR + pl) * C::EPC));
+          uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+          if (!VAR || g < heads)
+            raw = __ldg(reinterpret_cast<const uint4*>(qrow + int64_t(hq + g) * p.q_sh + (cc * C::LPR + pl) * C::EPC));
           E::unpack_pairs(raw, &qf[g][cc * (C::EPC / 2)]);
         }
         m_run[g] = -INFINITY;
@@ -956,7 +1041,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
   auto patch = [&](const Cursor& c, int stage) {
     if (!p.append) return;
     const int ap = apos[c.b];
-    if (ap < 0 || (ap >> C::LOG_TILE) != c.tile) return;
+    if (ap < 0 || (ap >> C::LOG_TILE) != row_tile(c)) return;
     const int t = ap & (C::TILE - 1);
     unsigned char* ktile = my_stages + size_t(stage) * stage_stride;
     unsigned char* krow = ktile + t * row_stride + head_off;
@@ -1052,6 +1137,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
     const bool from_global = src.kind != 2;
     const int mh = mitem / p.n_gchunks;
     const int mhq0 = mh * p.group + (mitem - mh * p.n_gchunks) * GT;
+    const int mheads = heads_of(mitem - mh * p.n_gchunks);
     // The item's output is GROUPS float4 groups, head-major; lane l owns groups t * 32 + l,
     // so each load instruction of the warp reads 512 contiguous bytes of a partial. Every lane
     // keeps the running maximum and normaliser of all GT heads (from broadcast loads).
@@ -1156,6 +1242,8 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
             dst_ml[g] = pick(M, g);
             dst_ml[GT + g] = pick(L, g);
           }
+        } else if (VAR && g >= mheads) {
+          continue;
         } else if (p.mode == 0) {
           const float inv = 1.f / fmaxf(pick(L, g), 1.f);
           T* o = reinterpret_cast<T*>(p.out) + int64_t(mb) * p.o_sb + int64_t(mhq0 + g) * p.o_sh + col;
@@ -1163,6 +1251,12 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
           o[1] = E::from_float(a[t].y * inv);
           o[2] = E::from_float(a[t].z * inv);
           o[3] = E::from_float(a[t].w * inv);
+          if constexpr (LOG) {
+            if (col == 0 && p.part_m != nullptr) {
+              p.part_m[hrow0 + g] = pick(M, g);
+              p.part_l[hrow0 + g] = pick(L, g);
+            }
+          }
         } else {
           *reinterpret_cast<float4*>(p.part_acc + (hrow0 + g) * D + col) = a[t];
           if (col == 0) {  // the lane that owns the head's first column
@@ -1223,7 +1317,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
   patch(cur, 0);
   start_segment(cur);
   seg_first_tile = cur.tile;
-  tile_scores(0, cur.len - (cur.tile << C::LOG_TILE), sc_cur);
+  tile_scores(0, live_of(cur), sc_cur);
 
   for (int64_t k = 0; k < nunits; ++k) {
     const bool has_next = k + 1 < nunits;
@@ -1238,9 +1332,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
       }
       patch(nxt, s_n);
     }
-    const int tok0 = cur.tile << C::LOG_TILE;
-    const int valid_rows = cur.len - tok0;  // rows [0, valid_rows) of tile k are live
-    const bool full_tile = valid_rows >= C::TILE;
+    const Live live = live_of(cur);
     const int hq0 = cur.h * p.group + cur.gc * GT;  // first q head of this item
 
     tile_max_update(sc_cur);
@@ -1248,11 +1340,12 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
     // otherwise) and phase B of tile k are independent chains, run side by side. Shared
     // stages: a warp holds one stage at a time, so that more of them are in flight; the
     // CTA's other warps cover the latency instead.
-    if (!CTA) tile_scores(s_n, nxt.len - (nxt.tile << C::LOG_TILE), sc_nxt);
-    if (__builtin_expect(full_tile, 1)) {
-      tile_pv(s, sc_cur, valid_rows, true);
+    if (!CTA) tile_scores(s_n, live_of(nxt), sc_nxt);
+    store_scores(cur, live, sc_cur);
+    if (__builtin_expect(live.full, 1)) {
+      tile_pv(s, sc_cur, live, true);
     } else {
-      tile_pv(s, sc_cur, valid_rows, false);
+      tile_pv(s, sc_cur, live, false);
     }
     __syncwarp();
 
@@ -1265,7 +1358,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
           return epoch;
         }
         patch(nxt, s_n);
-        tile_scores(s_n, nxt.len - (nxt.tile << C::LOG_TILE), sc_nxt);
+        tile_scores(s_n, live_of(nxt), sc_nxt);
       }
     } else if (issued < nunits) {
       // Refill the stage just consumed with the tile `stages` ahead.
@@ -1299,7 +1392,11 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
         mw.total_l(lt);
         if (whole) {
           if (p.mode == 0) {
-            mw.store_out(reinterpret_cast<T*>(p.out) + int64_t(cur.b) * p.o_sb + int64_t(hq0) * p.o_sh, p.o_sh, lt);
+            mw.store_out(reinterpret_cast<T*>(p.out) + int64_t(cur.b) * p.o_sb + int64_t(hq0) * p.o_sh, p.o_sh, lt, heads_of(cur.gc));
+            if constexpr (LOG) {
+              const int64_t hrow = int64_t(cur.b) * p.n_head + hq0;
+              if (p.part_m != nullptr) mw.store_ml(p.part_m + hrow, p.part_l + hrow, lt, heads_of(cur.gc));
+            }
           } else {
             const int64_t hrow = int64_t(cur.b) * p.n_head + hq0;
             mw.store_ml(p.part_m + hrow, p.part_l + hrow, lt);
@@ -1331,10 +1428,22 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
         }
         if (whole) {
           if (p.mode == 0) {
+            if constexpr (LOG) {
+              if (lane == 0 && p.part_m != nullptr) {
+                const int64_t hrow = int64_t(cur.b) * p.n_head + hq0;
+#pragma unroll
+                for (int g = 0; g < GT; ++g) {
+                  if (g >= heads_of(cur.gc)) break;
+                  p.part_m[hrow + g] = m_run[g];
+                  p.part_l[hrow + g] = l_tot[g];
+                }
+              }
+            }
             if (rg == 0) {
               T* orow = reinterpret_cast<T*>(p.out) + int64_t(cur.b) * p.o_sb;
 #pragma unroll
               for (int g = 0; g < GT; ++g) {
+                if (VAR && g >= heads_of(cur.gc)) break;
                 const float inv = 1.f / fmaxf(l_tot[g], 1.f);
 #pragma unroll
                 for (int c = 0; c < C::CPL; ++c) {
@@ -1424,7 +1533,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
       // Tile k+1 opens a new item: its scores above used the old q. Reload and redo.
       start_segment(nxt);
       seg_first_tile = 0;
-      tile_scores(s_n, nxt.len, sc_nxt);
+      tile_scores(s_n, live_of(nxt), sc_nxt);
     }
 #pragma unroll
     for (int j = 0; j < RR; ++j) sc_cur[j] = sc_nxt[j];
@@ -1505,29 +1614,34 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
   return epoch;
 }
 
-template <typename T, int D, int GT, bool CTA, bool MMA>
+template <typename T, int D, int GT, bool CTA, bool MMA, int VAR>
 __global__ void __launch_bounds__(CTA ? 288 : 256, 1)
     pd_decode_kernel(const __grid_constant__ DecodeParams p, const __grid_constant__ CUtensorMap kmap,
                      const __grid_constant__ CUtensorMap vmap) {
   extern __shared__ __align__(1024) unsigned char smem[];
-  const uint32_t epoch = decode_body<T, D, GT, CTA, MMA>(p, kmap, vmap, smem);
+  const uint32_t epoch = decode_body<T, D, GT, CTA, MMA, VAR>(p, kmap, vmap, smem);
   __syncwarp();
   if ((threadIdx.x & 31) == 0)
     leave_launch(p.exit_counter, p.epoch_word, epoch, p.tag_salt, gridDim.x * (blockDim.x >> 5), p.err);
 }
 
-template <typename T, int D, int GT, bool CTA = false, bool MMA = false>
+constexpr int MAX_DYNAMIC_SMEM = 232448;  // 227 KB: the opt-in limit of a block on sm_100
+
+template <typename T, int D, int GT, bool CTA = false, bool MMA = false, int VAR = 0>
 cudaError_t launch_decode(const DecodeParams& p, const CUtensorMap& kmap, const CUtensorMap& vmap,
                           dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool pdl) {
-  auto fn = pd_decode_kernel<T, D, GT, CTA, MMA>;
-  static int attr_smem[64] = {0};  // per-device dynamic-smem opt-in already granted
+  auto fn = pd_decode_kernel<T, D, GT, CTA, MMA, VAR>;
+  // Per-device dynamic shared memory, opted into once for the most a block can have, so that the first
+  // calls of two host threads cannot lower each other's limit.
+  static std::atomic<bool> opted[64];
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
-  if (dev < 64 && attr_smem[dev] < int(smem)) {
-    err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!opted[dev].load(std::memory_order_acquire)) {
+    err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_DYNAMIC_SMEM);
     if (err != cudaSuccess) return err;
-    attr_smem[dev] = int(smem);
+    opted[dev].store(true, std::memory_order_release);
   }
   if (!pdl) {
     fn<<<grid, block, smem, stream>>>(p, kmap, vmap);

@@ -98,9 +98,9 @@ struct MmaWorker {
     }
   }
 
-  // Opens an item: q rows hq0 .. hq0 + GT - 1 of qrow (head stride q_sh) as B fragments.
-  __device__ __forceinline__ void start(const T* qrow, int64_t q_sh, int hq0) {
-    const bool live = g < GT;
+  // Opens an item: q rows hq0 .. hq0 + heads - 1 (heads <= GT) of qrow (head stride q_sh) as B fragments.
+  __device__ __forceinline__ void start(const T* qrow, int64_t q_sh, int hq0, int heads) {
+    const bool live = g < heads;
     const T* qh = qrow + int64_t(hq0 + (live ? g : 0)) * q_sh + 2 * c;
 #pragma unroll
     for (int ks = 0; ks < M::KS; ++ks) {
@@ -116,9 +116,10 @@ struct MmaWorker {
     for (int dm = 0; dm < M::DM; ++dm) o[dm][0] = o[dm][1] = o[dm][2] = o[dm][3] = 0.f;
   }
 
-  // Scores of the K tile at shared address kbase, scaled to log2 units; tokens at or past
-  // valid_rows get -inf.
-  __device__ __forceinline__ void scores(uint32_t kbase, int valid_rows, float scale_log2,
+  // Scores of the K tile at shared address kbase, scaled to log2 units; tokens that do not count (live(token)
+  // is false) get -inf.
+  template <typename Live>
+  __device__ __forceinline__ void scores(uint32_t kbase, const Live& live, float scale_log2,
                                          float (&sc)[M::R]) const {
     float acc[M::MT][M::CH][4];
 #pragma unroll
@@ -151,7 +152,7 @@ struct MmaWorker {
 #pragma unroll
       for (int ch = 1; ch < M::CH; ++ch) s += acc[mt][ch][i];
       const int tok = mt * 16 + ((j >> 1) & 1) * 8 + g;
-      sc[j] = tok < valid_rows ? s * scale_log2 : -INFINITY;
+      sc[j] = live(tok) ? s * scale_log2 : -INFINITY;
     }
   }
 
@@ -197,15 +198,36 @@ struct MmaWorker {
     bl = movmatrix_trans(lo);
   }
 
-  // Keeps the 16-bit halves of V pairs whose token (t, t + 1) is below valid_rows.
-  __device__ __forceinline__ static uint32_t pair_mask(int t, int valid_rows) {
-    return (t < valid_rows ? 0x0000ffffu : 0u) | (t + 1 < valid_rows ? 0xffff0000u : 0u);
+  // Keeps the 16-bit halves of V pairs whose token (t, t + 1) counts.
+  template <typename Live>
+  __device__ __forceinline__ static uint32_t pair_mask(int t, const Live& live) {
+    return (live(t) ? 0x0000ffffu : 0u) | (live(t + 1) ? 0xffff0000u : 0u);
+  }
+
+  // The tile's scores, token t's of the item's q heads at dst + t * group.
+  template <typename Live>
+  __device__ __forceinline__ void store_scores(float* dst, int group, int heads, const Live& live,
+                                               const float (&sc)[M::R]) const {
+#pragma unroll
+    for (int j = 0; j < M::R; j += 2) {
+      const int tok = (j >> 2) * 16 + ((j >> 1) & 1) * 8 + g;
+      if (2 * c < heads && live(tok)) {
+        float* d = dst + int64_t(tok) * group + 2 * c;
+        if ((group & 1) == 0) {  // 8-byte aligned
+          *reinterpret_cast<float2*>(d) = make_float2(sc[j], sc[j + 1]);
+        } else {
+          d[0] = sc[j];
+          if (2 * c + 1 < heads) d[1] = sc[j + 1];
+        }
+      }
+    }
   }
 
   // Probabilities of the tile and O^T += V^T P^T from the V tile at shared address vbase.
-  // Tokens at or past valid_rows have P = 0 and their V is masked to zero (stale bytes, even
+  // Tokens that do not count have P = 0 and their V is masked to zero (stale bytes, even
   // NaN patterns, never reach the accumulators).
-  __device__ __forceinline__ void pv(uint32_t vbase, const float (&sc)[M::R], int valid_rows, bool full) {
+  template <typename Live>
+  __device__ __forceinline__ void pv(uint32_t vbase, const float (&sc)[M::R], const Live& live, bool full) {
     float pr[M::R];
 #pragma unroll
     for (int j = 0; j < M::R; ++j) {
@@ -215,7 +237,7 @@ struct MmaWorker {
     if constexpr (M::HALF) {
       uint32_t bh, bl;
       p_operand(pr[0], pr[1], bh, bl);
-      const uint32_t mk = full ? 0xffffffffu : pair_mask(2 * c, valid_rows);
+      const uint32_t mk = full ? 0xffffffffu : pair_mask(2 * c, live);
 #pragma unroll
       for (int dm = 0; dm < M::DM; dm += 2) {
         uint32_t a[4];
@@ -233,8 +255,8 @@ struct MmaWorker {
         uint32_t bh0, bl0, bh1, bl1;
         p_operand(pr[kp * 4 + 0], pr[kp * 4 + 1], bh0, bl0);
         p_operand(pr[kp * 4 + 2], pr[kp * 4 + 3], bh1, bl1);
-        const uint32_t mk0 = full ? 0xffffffffu : pair_mask(kp * 16 + 2 * c, valid_rows);
-        const uint32_t mk1 = full ? 0xffffffffu : pair_mask(kp * 16 + 8 + 2 * c, valid_rows);
+        const uint32_t mk0 = full ? 0xffffffffu : pair_mask(kp * 16 + 2 * c, live);
+        const uint32_t mk1 = full ? 0xffffffffu : pair_mask(kp * 16 + 8 + 2 * c, live);
 #pragma unroll
         for (int dm = 0; dm < M::DM; ++dm) {
           uint32_t a[4];
@@ -264,15 +286,15 @@ struct MmaWorker {
   // Normalised output of the item's GT heads: out_h0 points at head hq0, head stride o_sh.
   // Each (d, head) pair is transposed to (head, d) pairs so that a lane stores 4 bytes of one
   // head row.
-  __device__ __forceinline__ void store_out(T* out_h0, int64_t o_sh, const float (&l_tot)[2]) const {
+  __device__ __forceinline__ void store_out(T* out_h0, int64_t o_sh, const float (&l_tot)[2], int heads) const {
     const float inv0 = 1.f / fmaxf(l_tot[0], 1.f);
     const float inv1 = 1.f / fmaxf(l_tot[1], 1.f);
-    T* dst = out_h0 + int64_t(g < GT ? g : 0) * o_sh + 2 * c;
+    T* dst = out_h0 + int64_t(g < heads ? g : 0) * o_sh + 2 * c;
 #pragma unroll
     for (int dm = 0; dm < M::DM; ++dm) {
       const uint32_t y0 = movmatrix_trans(E::pack2(o[dm][0] * inv0, o[dm][1] * inv1));
       const uint32_t y1 = movmatrix_trans(E::pack2(o[dm][2] * inv0, o[dm][3] * inv1));
-      if (g < GT) {
+      if (g < heads) {
         *reinterpret_cast<unsigned int*>(dst + dm * 16) = y0;
         *reinterpret_cast<unsigned int*>(dst + dm * 16 + 8) = y1;
       }
@@ -292,11 +314,11 @@ struct MmaWorker {
   }
 
   // (m, l) of the item's heads into m_dst[h], l_dst[h] (lanes 0..3 hold columns 2c, 2c + 1).
-  __device__ __forceinline__ void store_ml(float* m_dst, float* l_dst, const float (&l_tot)[2]) const {
+  __device__ __forceinline__ void store_ml(float* m_dst, float* l_dst, const float (&l_tot)[2], int heads = GT) const {
     if (g == 0) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        if (2 * c + e < GT) {
+        if (2 * c + e < heads) {
           m_dst[2 * c + e] = m_run[e];
           l_dst[2 * c + e] = l_tot[e];
         }

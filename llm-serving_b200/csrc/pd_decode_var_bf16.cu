@@ -1,0 +1,20 @@
+// pd_decode_var_bf16.cu -- CUDA-core decode kernels for __nv_bfloat16 K/V that take a window and store scores
+// (variant 3: each by its arguments): head dims 8..256, q-head chunks of 1, 2, 4 or 8.
+#include "pd_decode_kernel.cuh"
+
+namespace pd {
+
+#define PD_VAR_ROW(D)                                                                                  \
+  {launch_decode<__nv_bfloat16, D, 1, false, false, 3>, launch_decode<__nv_bfloat16, D, 2, false, false, 3>, \
+   launch_decode<__nv_bfloat16, D, 4, false, false, 3>, launch_decode<__nv_bfloat16, D, 8, false, false, 3>}
+
+static const DecodeLaunchFn kVarTable[6][4] = {PD_VAR_ROW(8),  PD_VAR_ROW(16),  PD_VAR_ROW(32),
+                                              PD_VAR_ROW(64), PD_VAR_ROW(128), PD_VAR_ROW(256)};
+#undef PD_VAR_ROW
+
+DecodeLaunchFn decode_launcher_var_bf16(int d_index, int gt_index) {
+  if (d_index < 0 || d_index >= 6 || gt_index < 0 || gt_index >= 4) return nullptr;
+  return kVarTable[d_index][gt_index];
+}
+
+}  // namespace pd

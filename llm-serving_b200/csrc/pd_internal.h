@@ -15,6 +15,16 @@ DecodeLaunchFn decode_launcher_cta_bf16(int d_index, int gt_index);
 // (d_index 3..5), bf16 / fp16.
 DecodeLaunchFn decode_launcher_mma_f16(int d_index, int gt_index);
 DecodeLaunchFn decode_launcher_mma_bf16(int d_index, int gt_index);
+// Decode kernels with a window and / or stored scores (VAR of pd_decode_kernel.cuh). Tensor-core: one
+// variant each (1 window, 2 scores); CUDA-core: both by their arguments.
+DecodeLaunchFn decode_launcher_var_mma_f16(int variant, int d_index, int gt_index);
+DecodeLaunchFn decode_launcher_var_mma_bf16(int variant, int d_index, int gt_index);
+DecodeLaunchFn decode_launcher_var_f32(int d_index, int gt_index);
+DecodeLaunchFn decode_launcher_var_f16(int d_index, int gt_index);
+DecodeLaunchFn decode_launcher_var_bf16(int d_index, int gt_index);
+
+// weights[b][h][j] += the sum over the group of exp2(score - m) / l (pd_weights.cu).
+cudaError_t launch_weights(const WeightsParams& p, cudaStream_t stream);
 
 // Append: copies K and V rows into their pool slots. src/dst dtype codes as PD_F32/F16/BF16.
 cudaError_t launch_append(const AppendParams& p, int src_dtype, int dst_dtype, bool vec16,

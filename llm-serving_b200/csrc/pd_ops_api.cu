@@ -1,10 +1,11 @@
-// pd_ops_api.cu -- the extern "C" boundary of the head norm with rotation, the 4-bit pages and the
-// page copies (declared in include/paged_decode.h): argument checks on the host, then the launch.
+// pd_ops_api.cu -- the extern "C" boundary of the head norm with rotation, the 4-bit pages, the
+// page copies and the eviction (declared in include/paged_decode.h): argument checks on the host, then the launch.
 #include <atomic>
 
 #include "paged_decode.h"
 #include "pd_api_internal.h"
 #include "pd_block_copy.cuh"
+#include "pd_evict.cuh"
 #include "pd_fp4.cuh"
 #include "pd_norm_rope.cuh"
 
@@ -315,6 +316,101 @@ int pd_set_fp4_prefill_mode(int32_t mode) {
 }
 
 int pd_get_fp4_prefill_mode(void) { return g_fp4_prefill_mode.load(std::memory_order_relaxed); }
+
+size_t pd_evict_scratch_bytes(int32_t n_layer, int32_t batch, int32_t n_kv_head, int32_t keep) {
+  if (n_layer < 0 || batch < 0 || n_kv_head < 1 || keep < 1) return 0;
+  const size_t items = size_t(n_layer) * batch * n_kv_head;
+  return items * 8 + items * size_t(keep) * 4;
+}
+
+int pd_evict(void* const* k_caches, void* const* v_caches, int32_t n_layer, int64_t n_blocks, int32_t block_size,
+             int32_t n_kv_head, int32_t head_dim, int32_t dtype, const int64_t* k_strides, const int64_t* v_strides,
+             const int32_t* block_table, int64_t bt_stride, int32_t max_blocks, const int32_t* new_table,
+             int64_t nbt_stride, int32_t new_max_blocks, const int32_t* seqlen, int32_t* seqlen_out,
+             const float* weights, const int64_t* w_strides, float* weights_out, const int64_t* wo_strides,
+             int64_t w_len, int32_t batch, int32_t keep, int32_t recent, int32_t sinks, void* scratch,
+             size_t scratch_bytes, void* stream) {
+  if (!valid_dtype(dtype) || n_layer < 0 || n_blocks < 1 || n_kv_head < 1 || head_dim < 1 || !pow2(block_size))
+    return PD_ERR_INVALID;
+  if (batch < 0 || max_blocks < 0 || new_max_blocks < 0 || keep < 1 || recent < 0 || sinks < 0) return PD_ERR_INVALID;
+  if (int64_t(recent) + sinks > keep) return PD_ERR_INVALID;
+  const int64_t capacity = int64_t(max_blocks) * block_size;
+  if (capacity > (int64_t(1) << 30) || int64_t(new_max_blocks) * block_size > (int64_t(1) << 30)) return PD_ERR_INVALID;
+  if (w_len < capacity || bt_stride < max_blocks) return PD_ERR_INVALID;
+  const int es = elem_size(dtype);
+  if (head_dim * es % 16 != 0) return PD_ERR_UNSUPPORTED;
+  if (n_layer == 0 || batch == 0) return PD_OK;
+  if (k_caches == nullptr || v_caches == nullptr || k_strides == nullptr || v_strides == nullptr ||
+      w_strides == nullptr || wo_strides == nullptr || seqlen == nullptr || seqlen_out == nullptr ||
+      (max_blocks > 0 && (block_table == nullptr || weights == nullptr)) || (w_len > 0 && weights_out == nullptr))
+    return PD_ERR_INVALID;
+  // What the kept tokens need of the new pages.
+  if (new_table != nullptr &&
+      (nbt_stride < new_max_blocks || int64_t(new_max_blocks) * block_size < (keep < capacity ? keep : capacity)))
+    return PD_ERR_INVALID;
+  for (int i = 0; i < 3; ++i)
+    if (k_strides[i] * es % 16 != 0 || v_strides[i] * es % 16 != 0) return PD_ERR_INVALID;
+  for (int i = 0; i < n_layer; ++i)
+    if (k_caches[i] == nullptr || v_caches[i] == nullptr || !aligned(k_caches[i], 16) || !aligned(v_caches[i], 16))
+      return PD_ERR_INVALID;
+  // no row holds more than its table: a larger budget evicts nothing either
+  keep = int32_t(keep < capacity + 1 ? keep : capacity + 1);
+  if (recent + sinks > keep) recent = sinks = 0;
+  const int64_t items = int64_t(batch) * n_kv_head;
+  if (items > 0x7fffffff / (2 * EVICT_LAYERS * 128)) return PD_ERR_UNSUPPORTED;  // CTAs of a launch
+  if (scratch == nullptr || !aligned(scratch, 16) || scratch_bytes < pd_evict_scratch_bytes(n_layer, batch, n_kv_head, keep))
+    return api_message(PD_ERR_WORKSPACE, "scratch is smaller than pd_evict_scratch_bytes");
+  EvictParams p{};
+  if (api_device(&p.sms, &p.err) != PD_OK) return PD_ERR_CUDA;
+  p.k_sb = k_strides[0] * es / 16;
+  p.k_sn = k_strides[1] * es / 16;
+  p.k_sh = k_strides[2] * es / 16;
+  p.v_sb = v_strides[0] * es / 16;
+  p.v_sn = v_strides[1] * es / 16;
+  p.v_sh = v_strides[2] * es / 16;
+  p.n_blocks = n_blocks;
+  p.table = block_table;
+  p.bt_stride = bt_stride;
+  p.fresh = new_table != nullptr;
+  p.new_table = p.fresh ? new_table : block_table;
+  p.nbt_stride = p.fresh ? nbt_stride : bt_stride;
+  p.seqlen = seqlen;
+  p.w_sl = w_strides[0];
+  p.w_sb = w_strides[1];
+  p.w_sh = w_strides[2];
+  p.wo_sl = wo_strides[0];
+  p.wo_sb = wo_strides[1];
+  p.wo_sh = wo_strides[2];
+  p.w_len = w_len;
+  p.batch = batch;
+  p.n_kv_head = n_kv_head;
+  p.chunks = head_dim * es / 16;
+  p.log2_bs = ilog2_host(block_size);
+  p.max_blocks = max_blocks;
+  p.new_max_blocks = p.fresh ? new_max_blocks : max_blocks;
+  p.capacity = int32_t(capacity);
+  p.keep = keep;
+  p.recent = recent;
+  p.sinks = sinks;
+  int2* info = static_cast<int2*>(scratch);
+  int32_t* order = reinterpret_cast<int32_t*>(info + n_layer * items);
+  for (int l0 = 0; l0 < n_layer; l0 += EVICT_LAYERS) {
+    p.layers = n_layer - l0 < EVICT_LAYERS ? n_layer - l0 : EVICT_LAYERS;
+    for (int i = 0; i < p.layers; ++i) {
+      p.k[i] = k_caches[l0 + i];
+      p.v[i] = v_caches[l0 + i];
+    }
+    p.weights = weights + l0 * p.w_sl;
+    p.weights_out = weights_out + l0 * p.wo_sl;
+    p.info = info + l0 * items;
+    p.order = order + l0 * items * keep;
+    p.seqlen_out = l0 + p.layers == n_layer ? seqlen_out : nullptr;  // every launch reads the old lengths
+    const int st = launched(launch_evict(p, static_cast<cudaStream_t>(stream)), "eviction launch");
+    if (st != PD_OK) return st;
+    api_count_launch();  // two kernels
+  }
+  return PD_OK;
+}
 
 int pd_block_copy(void* const* pools, int32_t n_pools, int64_t n_blocks, int64_t block_bytes, const void* src,
                   const void* dst, int32_t id_dtype, int64_t n_pairs, int32_t* block_table, int64_t table_rows,

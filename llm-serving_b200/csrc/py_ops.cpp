@@ -1,4 +1,5 @@
-// py_ops.cpp -- Python binding of the head norm with rotation, the 4-bit pages and the page copies.
+// py_ops.cpp -- Python binding of the head norm with rotation, the 4-bit pages, the page copies and the
+// cache of bounded length.
 //
 // These calls sit on the path of every decode step, where a launch's host time is the operator's
 // time: through ctypes and Python-level checks a call took 17 to 37 us for 2 to 4 us of kernel.
@@ -20,6 +21,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/python_numbers.h>
 
+#include <algorithm>
 #include <cmath>
 #include <iterator>
 #include <map>
@@ -33,7 +35,8 @@ using at::Tensor;
 
 #define PD_ENTRIES(X) \
   X(pd_qk_norm_rope) X(pd_fp4_write_slots) X(pd_fp4_write_table) X(pd_fp4_read_slots) X(pd_fp4_workspace_bytes) \
-  X(pd_fp4_decode) X(pd_fp4_prefill) X(pd_block_copy)
+  X(pd_fp4_decode) X(pd_fp4_prefill) X(pd_block_copy) X(pd_decode_window_workspace_bytes) X(pd_decode_window) \
+  X(pd_decode_weights_scratch_bytes) X(pd_decode_weights) X(pd_evict_scratch_bytes) X(pd_evict)
 #define PD_FIELD(name) decltype(&::name) name = nullptr;
 struct Entries {
   PD_ENTRIES(PD_FIELD)
@@ -243,15 +246,20 @@ Tensor new_workspace(const at::Device& device) {
   return at::zeros({int64_t(lib.pd_fp4_workspace_bytes(256))}, at::TensorOptions(at::kByte).device(device));
 }
 
-// The workspace of a call that was given none: zero-filled once and left at zero by every launch. Eager
+// The workspace of a call that was given none, of at least what `fresh` makes for it. Eager
 // calls share one per (device, stream). A captured call never takes that one, also where its stream has
 // it already: the graph may be replayed on another stream beside the eager calls, or beside another graph. A
-// capture has its own, per stream, whose zero fill is a node of the graph; it is dropped here with the first
+// capture has its own, per stream (a zero fill is a node of the graph); it is dropped here with the first
 // call after the capture's end, its memory staying in the graph's pool.
-Tensor stream_workspace(const at::Device& device, void* stream) {
-  using Workspaces = std::map<std::pair<int, void*>, Tensor>;
-  static auto* eager = new Workspaces;  // never destroyed: outlives no context
-  static auto* captures = new std::map<unsigned long long, Workspaces>;  // by capture
+using Workspaces = std::map<std::pair<int, void*>, Tensor>;
+struct StreamWorkspaces {
+  Workspaces eager;
+  std::map<unsigned long long, Workspaces> captures;  // by capture
+};
+template <typename Fresh>
+Tensor stream_workspace(StreamWorkspaces& all, const at::Device& device, void* stream, int64_t bytes, const Fresh& fresh) {
+  Workspaces *eager = &all.eager;
+  auto* captures = &all.captures;
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   unsigned long long capture = 0;
   C10_CUDA_CHECK(cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &capture));
@@ -259,8 +267,21 @@ Tensor stream_workspace(const at::Device& device, void* stream) {
   for (auto it = captures->begin(); it != captures->end();)
     it = captured && it->first == capture ? std::next(it) : captures->erase(it);
   Tensor& ws = (captured ? (*captures)[capture] : *eager)[std::make_pair(int(device.index()), stream)];
-  if (!ws.defined()) ws = new_workspace(device);
+  if (!ws.defined() || ws.numel() < bytes) ws = fresh();
   return ws;
+}
+
+// The 4-bit attention's: zero-filled once and left at zero by every launch.
+Tensor fp4_workspace(const at::Device& device, void* stream) {
+  static auto* all = new StreamWorkspaces;  // never destroyed: outlives no context
+  return stream_workspace(*all, device, stream, 1, [&] { return new_workspace(device); });
+}
+
+// The decode kernel's variants': any contents.
+Tensor decode_workspace(const at::Device& device, void* stream, int64_t bytes) {
+  static auto* all = new StreamWorkspaces;
+  return stream_workspace(*all, device, stream, bytes,
+                          [&] { return at::detail::empty_cuda({bytes}, at::kByte, device, std::nullopt); });
 }
 
 // Rows the kernels read: unit last stride, 16-byte aligned rows; a copy where they are not so already.
@@ -322,7 +343,7 @@ PyObject* attend(PyObject* const* a, bool chunk) {
           "workspace must be a contiguous uint8 tensor on ", q0.device());
     ws = *w;
   } else {
-    ws = stream_workspace(q0.device(), stream);
+    ws = fp4_workspace(q0.device(), stream);
   }
   const Tensor q = kernel_rows(q0), lens = int32(seqlen);
   const Tensor table = (table0.size(1) > 1 && table0.stride(1) != 1) || (rows > 1 && table0.stride(0) < table0.size(1))
@@ -499,6 +520,300 @@ PyObject* block_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------ a cache of bounded length
+
+struct Pools {
+  int64_t n_blocks, hkv;
+  int block_size, d, dtype;
+  int64_t ks[3], vs[3];
+};
+
+// One layer's K and V pools as the kernels take them.
+Pools pools_of(const Tensor& k, const Tensor& v, const char* what) {
+  cuda(k, "k_cache", what);
+  cuda(v, "v_cache", what);
+  VALUE(k.dim() == 4 && v.dim() == 4, "k_cache/v_cache must be (n_blocks, block_size, H_kv, D), got ", k.sizes(), " / ",
+        v.sizes());
+  VALUE(k.sizes() == v.sizes(), "k_cache/v_cache shapes differ: ", k.sizes(), " vs ", v.sizes());
+  Pools p;
+  p.dtype = dtype_code(k.scalar_type());
+  VALUE(p.dtype >= 0 && v.scalar_type() == k.scalar_type(), "k_cache/v_cache must share one dtype of fp32, fp16 or bf16, got ",
+        k.scalar_type(), " / ", v.scalar_type());
+  same_device(v, "v_cache", k, "k_cache");
+  p.n_blocks = k.size(0);
+  p.hkv = k.size(2);
+  const int64_t bs = k.size(1), d = k.size(3);
+  VALUE(p.n_blocks >= 1 && p.hkv >= 1 && p.hkv <= 65535, "k_cache needs blocks and 1 to 65535 heads, got ", k.sizes());
+  VALUE(bs >= 1 && (bs & (bs - 1)) == 0 && bs <= (1 << 30), "block_size must be a power of two, got ", bs);
+  VALUE(d >= 8 && d <= 256 && (d & (d - 1)) == 0, "head_dim must be a power of two in 8..256, got ", d);
+  p.block_size = int(bs);
+  p.d = int(d);
+  const int64_t es = k.element_size();
+  VALUE(std::min(bs * d * es, int64_t(4096)) % 128 == 0, "a block of one head needs a multiple of 128 bytes, got ", bs * d * es);
+  for (const bool first : {true, false}) {  // (k and v may be one tensor)
+    const Tensor* t = first ? &k : &v;
+    VALUE(t->stride(3) == 1 && aligned16(*t), "a pool needs a unit head_dim stride and a 16-byte aligned base");
+    for (int i = 0; i < 3; ++i) {
+      VALUE(t->stride(i) > 0 && t->stride(i) * es % 16 == 0, "a pool's strides must be positive multiples of 16 bytes, got ",
+            t->strides());
+      (first ? p.ks : p.vs)[i] = t->stride(i);
+    }
+  }
+  return p;
+}
+
+// An int32 block table of `rows` rows with unit columns (a copy where it has other strides).
+Tensor table_of(const Tensor& t, const char* name, int64_t rows, const Tensor& as, const char* as_name) {
+  VALUE(t.dim() == 2 && t.size(0) == rows, name, " must be (", rows, ", max_blocks), got shape ", t.sizes());
+  VALUE(t.scalar_type() == at::kInt, name, " must be int32, got ", t.scalar_type());
+  VALUE(t.size(1) <= 0x7fffffff, name, " is too wide");
+  same_device(t, name, as, as_name);
+  return (t.size(1) > 1 && t.stride(1) != 1) || (rows > 1 && t.stride(0) < t.size(1)) ? t.contiguous() : t;
+}
+
+// Whether no two rows (runs of the last, unit-stride dimension) of t share memory, as nested strides tell.
+bool disjoint_rows(const Tensor& t) {
+  if (t.numel() == 0) return true;
+  std::vector<std::pair<int64_t, int64_t>> dims;  // (stride, size)
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
+  std::sort(dims.begin(), dims.end());
+  int64_t extent = t.size(t.dim() - 1);
+  for (const auto& [stride, size] : dims) {
+    if (stride < extent) return false;
+    extent += stride * (size - 1);
+  }
+  return true;
+}
+
+// decode_window(q, k, v, table, seqlen, window, sinks, scale, out, workspace) and
+// decode_weights(q, k, v, table, seqlen, weights, scale, out, workspace).
+PyObject* decode_variant(PyObject* const* a, bool windowed) {
+  const char* what = windowed ? "paged_decode_window" : "paged_decode_weights";
+  const Tensor &q0 = tensor(a[0], "q"), &k = tensor(a[1], "k_cache"), &v = tensor(a[2], "v_cache");
+  const Tensor &table0 = tensor(a[3], "block_table"), &seqlen = tensor(a[4], "seqlen");
+  cuda(q0, "q", what);
+  const Pools p = pools_of(k, v, what);
+  VALUE(q0.dim() == 3, "q must be (B, H, D), got shape ", q0.sizes());
+  VALUE(q0.scalar_type() == k.scalar_type(), "q/k_cache/v_cache must share one dtype, got ", q0.scalar_type(), ", ",
+        k.scalar_type());
+  VALUE(q0.size(2) == p.d, "q head_dim ", q0.size(2), " != cache head_dim ", p.d);
+  VALUE(q0.size(1) >= 1 && q0.size(1) % p.hkv == 0, "n_head (", q0.size(1), ") must be a multiple of n_kv_head (", p.hkv,
+        ")");
+  same_device(k, "k_cache", q0, "q");
+  const int64_t rows = q0.size(0), heads = q0.size(1);
+  VALUE(rows <= 0x7fffffff / heads, "too many query rows");
+  VALUE(seqlen.dim() == 1 && seqlen.size(0) == rows, "seqlen must be (", rows, ",), got shape ", seqlen.sizes());
+  VALUE(index_type(seqlen), "seqlen must be int32 or int64, got ", seqlen.scalar_type());
+  same_device(seqlen, "seqlen", q0, "q");
+  const c10::cuda::CUDAGuard guard(q0.device());
+  const Tensor table = table_of(table0, "block_table", rows, q0, "q");
+  const int64_t capacity = table.size(1) * p.block_size;
+  VALUE(capacity <= (int64_t(1) << 30), "a row's table holds at most 2^30 tokens, got ", capacity);
+  int64_t window = 0, sinks = 0;
+  const Tensor* weights = nullptr;
+  if (windowed) {
+    window = THPUtils_unpackLong(a[5]);
+    sinks = THPUtils_unpackLong(a[6]);
+    VALUE(window >= 1, "window must be at least 1, got ", window);
+    VALUE(sinks >= 0, "sinks must be at least 0, got ", sinks);
+    window = std::min<int64_t>(window, 1 << 30);  // no row is longer
+    sinks = std::min<int64_t>(sinks, 1 << 30);
+  } else {
+    weights = &tensor(a[5], "weights");
+    VALUE(weights->scalar_type() == at::kFloat && weights->dim() == 3 && weights->size(0) == rows &&
+              weights->size(1) == p.hkv && weights->size(2) >= capacity,
+          "weights must be float32 (", rows, ", ", p.hkv, ", at least ", capacity, "), got ", weights->sizes(), " ",
+          weights->scalar_type());
+    same_device(*weights, "weights", q0, "q");
+    VALUE(weights->size(2) <= 1 || weights->stride(2) == 1, "weights needs a unit last stride (it is updated in place)");
+    VALUE(disjoint_rows(*weights), "weights rows must not overlap (it is updated in place), got strides ",
+          weights->strides());
+  }
+  const int at = windowed ? 7 : 6;  // scale, out, workspace
+  const double scale = a[at] == Py_None ? 1.0 / std::sqrt(double(p.d)) : PyFloat_AsDouble(a[at]);
+  if (PyErr_Occurred()) return nullptr;
+  Tensor out;
+  if (const Tensor* o = optional(a[at + 1], "out")) {
+    VALUE(o->sizes() == q0.sizes() && o->scalar_type() == q0.scalar_type() && o->device() == q0.device() &&
+              o->is_contiguous() && aligned16(*o),
+          "out must be a contiguous, 16-byte aligned ", q0.sizes(), " ", q0.scalar_type(), " tensor on ", q0.device());
+    out = *o;
+  } else {
+    out = new_like(q0);
+  }
+  if (rows == 0) return THPVariable_Wrap(out);
+  void* stream = stream_of(q0);
+  const int64_t need =
+      int64_t(lib.pd_decode_window_workspace_bytes(int(rows), int(heads), int(p.hkv), p.d, p.dtype));
+  Tensor ws;
+  if (const Tensor* w = optional(a[at + 2], "workspace")) {
+    VALUE(w->scalar_type() == at::kByte && w->is_contiguous() && w->device() == q0.device() && w->numel() >= need,
+          "workspace must be a contiguous uint8 tensor of at least ", need, " bytes on ", q0.device());
+    ws = *w;
+  } else {
+    ws = decode_workspace(q0.device(), stream, need);
+  }
+  const int64_t es = q0.element_size();
+  Tensor q = q0;
+  if (q.stride(2) != 1 || q.stride(0) * es % 16 != 0 || q.stride(1) * es % 16 != 0 || !aligned16(q)) {
+    q = q0.contiguous();
+    if (!aligned16(q) || q.data_ptr() == q0.data_ptr()) q = q0.clone(at::MemoryFormat::Contiguous);
+  }
+  const Tensor lens = int32(seqlen);
+  const int64_t bt_stride = std::max(table.stride(0), table.size(1));  // one row may have any stride
+  const float scale_log2 = float(scale * 1.4426950408889634);
+  int status;
+  if (windowed) {
+    status = lib.pd_decode_window(q.const_data_ptr(), q.stride(0), q.stride(1), k.const_data_ptr(), v.const_data_ptr(),
+                                  p.n_blocks, p.block_size, p.ks, p.vs, table.const_data_ptr<int32_t>(), bt_stride,
+                                  int(table.size(1)), lens.const_data_ptr<int32_t>(), int(window), int(sinks),
+                                  out.data_ptr(), out.stride(0), out.stride(1), int(rows), int(heads), int(p.hkv), p.d,
+                                  p.dtype, scale_log2, ws.data_ptr(), size_t(ws.numel()), stream);
+  } else {
+    const int64_t bytes =
+        int64_t(lib.pd_decode_weights_scratch_bytes(int(rows), int(heads), int(table.size(1)), p.block_size));
+    const Tensor scratch = at::detail::empty_cuda({bytes}, at::kByte, q0.device(), std::nullopt);
+    status = lib.pd_decode_weights(q.const_data_ptr(), q.stride(0), q.stride(1), k.const_data_ptr(), v.const_data_ptr(),
+                                   p.n_blocks, p.block_size, p.ks, p.vs, table.const_data_ptr<int32_t>(), bt_stride,
+                                   int(table.size(1)), lens.const_data_ptr<int32_t>(), weights->data_ptr<float>(),
+                                   weights->stride(0), weights->stride(1), weights->size(2), out.data_ptr(),
+                                   out.stride(0), out.stride(1), int(rows), int(heads), int(p.hkv), p.d, p.dtype,
+                                   scale_log2, ws.data_ptr(), size_t(ws.numel()), scratch.data_ptr(),
+                                   size_t(scratch.numel()), stream);
+  }
+  if (failed(status, windowed ? "pd_decode_window" : "pd_decode_weights")) return nullptr;
+  return THPVariable_Wrap(out);
+}
+
+PyObject* decode_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 10, "decode_window");
+  return decode_variant(a, true);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* decode_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 9, "decode_weights");
+  return decode_variant(a, false);
+  END_HANDLE_TH_ERRORS
+}
+
+// decode_window_workspace(rows, heads, kv_heads, head_dim, like): a workspace for calls of that shape.
+PyObject* decode_window_workspace(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 5, "decode_window_workspace");
+  const Tensor& like = tensor(a[4], "like");
+  cuda(like, "like", "decode_workspace");
+  int64_t x[4];
+  for (int i = 0; i < 4; ++i) {
+    x[i] = THPUtils_unpackLong(a[i]);
+    VALUE(x[i] >= 0 && x[i] <= 0x7fffffff, "sizes must be 31-bit");
+  }
+  const c10::cuda::CUDAGuard guard(like.device());
+  const size_t bytes = lib.pd_decode_window_workspace_bytes(int(x[0]), int(x[1]), int(x[2]), int(x[3]),
+                                                            dtype_code(like.scalar_type()));
+  VALUE(bytes > 0, "no decode of ", x[0], " rows of ", x[1], " heads on ", x[2], " of ", x[3], " in ", like.scalar_type());
+  return THPVariable_Wrap(at::detail::empty_cuda({int64_t(bytes)}, at::kByte, like.device(), std::nullopt));
+  END_HANDLE_TH_ERRORS
+}
+
+// evict(ks, vs, table, seqlen, weights, keep, recent, sinks, new_table, seqlen_out, weights_out)
+PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 11, "evict");
+  TORCH_CHECK_TYPE(PyList_Check(a[0]) && PyList_Check(a[1]), "k_caches and v_caches must be lists");
+  const Py_ssize_t layers = PyList_GET_SIZE(a[0]);
+  VALUE(layers >= 1 && PyList_GET_SIZE(a[1]) == layers, "evict_tokens needs one k_cache and v_cache per layer, got ", layers,
+        " / ", PyList_GET_SIZE(a[1]));
+  VALUE(layers <= 65535, "too many layers");
+  const Tensor &k0 = tensor(PyList_GET_ITEM(a[0], 0), "k_cache"), &v0 = tensor(PyList_GET_ITEM(a[1], 0), "v_cache");
+  const Pools p = pools_of(k0, v0, "evict_tokens");
+  std::vector<void*> ks(layers), vs(layers);
+  for (Py_ssize_t i = 0; i < layers; ++i) {
+    const Tensor &k = tensor(PyList_GET_ITEM(a[0], i), "k_cache"), &v = tensor(PyList_GET_ITEM(a[1], i), "v_cache");
+    for (const auto& [t, first] : {std::make_pair(&k, &k0), std::make_pair(&v, &v0)})
+      VALUE(t->sizes() == first->sizes() && t->strides() == first->strides() && t->scalar_type() == first->scalar_type() &&
+                t->device() == first->device() && aligned16(*t),
+            "every layer's pools must have one shape, layout, dtype and device, 16-byte aligned; layer ", i, " has ",
+            t->sizes(), " ", t->strides(), " ", t->scalar_type(), " on ", t->device());
+    ks[i] = k.data_ptr();
+    vs[i] = v.data_ptr();
+  }
+  const Tensor &seqlen0 = tensor(a[3], "seqlen"), &weights = tensor(a[4], "weights");
+  VALUE(seqlen0.dim() == 1, "seqlen must be (B,), got shape ", seqlen0.sizes());
+  VALUE(index_type(seqlen0), "seqlen must be int32 or int64, got ", seqlen0.scalar_type());
+  same_device(seqlen0, "seqlen", k0, "the pools");
+  const int64_t rows = seqlen0.size(0);
+  const c10::cuda::CUDAGuard guard(k0.device());
+  const Tensor table = table_of(tensor(a[2], "block_table"), "block_table", rows, k0, "the pools");
+  const int64_t capacity = table.size(1) * p.block_size;
+  VALUE(capacity <= (int64_t(1) << 30), "a row's table holds at most 2^30 tokens, got ", capacity);
+  auto sums = [&](const Tensor& t, const char* name) {
+    VALUE(t.scalar_type() == at::kFloat && t.dim() == 4 && t.size(0) == layers && t.size(1) == rows && t.size(2) == p.hkv &&
+              t.size(3) >= capacity,
+          name, " must be float32 (", layers, ", ", rows, ", ", p.hkv, ", at least ", capacity, "), got ", t.sizes(), " ",
+          t.scalar_type());
+    same_device(t, name, k0, "the pools");
+    VALUE(t.size(3) <= 1 || t.stride(3) == 1, name, " needs a unit last stride");
+  };
+  sums(weights, "weights");
+  const int64_t keep0 = THPUtils_unpackLong(a[5]), recent = THPUtils_unpackLong(a[6]), sinks = THPUtils_unpackLong(a[7]);
+  VALUE(keep0 >= 1, "keep must be at least 1, got ", keep0);
+  VALUE(recent >= 0 && sinks >= 0 && recent <= keep0 && sinks <= keep0 - recent,
+        "recent and sinks must be at least 0 and fit into keep (", keep0, "), got ", recent, " and ", sinks);
+  // a budget that no row exceeds evicts nothing, whatever it is
+  const bool all_fit = keep0 > capacity;
+  const int keep = all_fit ? int(capacity) + 1 : int(keep0);
+  Tensor fresh;
+  if (const Tensor* t = optional(a[8], "new_table")) {
+    fresh = table_of(*t, "new_table", rows, k0, "the pools");
+    VALUE(fresh.size(1) * p.block_size >= std::min<int64_t>(keep, capacity), "new_table holds ", fresh.size(1) * p.block_size,
+          " tokens, but rows may keep ", std::min<int64_t>(keep, capacity));
+    VALUE(fresh.size(1) * p.block_size <= (int64_t(1) << 30), "a row's table holds at most 2^30 tokens");
+  }
+  Tensor lens_out, sums_out;
+  if (const Tensor* t = optional(a[9], "seqlen_out")) {
+    VALUE(t->dim() == 1 && t->size(0) == rows && t->scalar_type() == at::kInt && t->is_contiguous(),
+          "seqlen_out must be a contiguous int32 (", rows, ",) tensor, got ", t->sizes(), " ", t->scalar_type());
+    same_device(*t, "seqlen_out", k0, "the pools");
+    lens_out = *t;
+  } else {
+    lens_out = at::detail::empty_cuda({rows}, at::kInt, k0.device(), std::nullopt);
+  }
+  if (const Tensor* t = optional(a[10], "weights_out")) {
+    sums(*t, "weights_out");
+    VALUE(t->size(3) == weights.size(3), "weights_out must be as long as weights, got ", t->size(3), " and ", weights.size(3));
+    VALUE(t->is_contiguous() || (t->data_ptr() == weights.data_ptr() && t->strides() == weights.strides()),
+          "weights_out must be contiguous, or weights itself");
+    VALUE(t->data_ptr() != weights.data_ptr() || t->strides() == weights.strides(),
+          "weights_out shares weights' memory with other strides");
+    VALUE(disjoint_rows(*t), "weights_out rows must not overlap, got strides ", t->strides());
+    sums_out = *t;
+  } else {
+    sums_out = at::detail::empty_cuda(weights.sizes(), at::kFloat, k0.device(), std::nullopt);
+  }
+  if (rows == 0) return pair(lens_out, sums_out);
+  const Tensor lens = int32(seqlen0);
+  const int64_t bytes = int64_t(lib.pd_evict_scratch_bytes(int(layers), int(rows), int(p.hkv), keep));
+  const Tensor scratch = at::detail::empty_cuda({bytes}, at::kByte, k0.device(), std::nullopt);
+  const int64_t w_st[3] = {weights.stride(0), weights.stride(1), weights.stride(2)};
+  const int64_t wo_st[3] = {sums_out.stride(0), sums_out.stride(1), sums_out.stride(2)};
+  if (failed(lib.pd_evict(ks.data(), vs.data(), int(layers), p.n_blocks, p.block_size, int(p.hkv), p.d, p.dtype, p.ks, p.vs,
+                          table.const_data_ptr<int32_t>(), std::max(table.stride(0), table.size(1)), int(table.size(1)),
+                          fresh.defined() ? fresh.const_data_ptr<int32_t>() : nullptr,
+                          fresh.defined() ? std::max(fresh.stride(0), fresh.size(1)) : 0,
+                          fresh.defined() ? int(fresh.size(1)) : 0, lens.const_data_ptr<int32_t>(),
+                          lens_out.data_ptr<int32_t>(), weights.const_data_ptr<float>(), w_st, sums_out.data_ptr<float>(),
+                          wo_st, weights.size(3), int(rows), keep, all_fit ? 0 : int(recent), all_fit ? 0 : int(sinks),
+                          scratch.data_ptr(), size_t(bytes), stream_of(k0)),
+             "pd_evict"))
+    return nullptr;
+  return pair(lens_out, sums_out);
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(addresses, check): {"pd_...": int} of the loaded library, and _native.check.
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -529,6 +844,10 @@ PyMethodDef methods[] = {
     PD_METHOD("fp4_prefill", prefill),
     PD_METHOD("fp4_workspace", workspace),
     PD_METHOD("block_copy", block_copy),
+    PD_METHOD("decode_window", decode_window),
+    PD_METHOD("decode_weights", decode_weights),
+    PD_METHOD("decode_window_workspace", decode_window_workspace),
+    PD_METHOD("evict", evict),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "pd_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -151,6 +151,33 @@ _SIGNATURES = {
         [ctypes.POINTER(_c_ptr), _c_i32, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i32, _c_i64, _c_ptr, _c_i64,
          _c_i64, _c_i64, _c_ptr, _c_ptr],
     ),
+    "pd_decode_window_workspace_bytes": (_c_size, [_c_i32] * 5),
+    "pd_decode_window": (
+        ctypes.c_int,
+        [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i32, _c_i64p, _c_i64p, _c_ptr, _c_i64,
+         _c_i32, _c_ptr, _c_i32, _c_i32, _c_ptr, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_float,
+         _c_ptr, _c_size, _c_ptr],
+    ),
+    "pd_plan_create_window": (
+        ctypes.c_int,
+        [ctypes.POINTER(_c_ptr), _c_i32, ctypes.POINTER(_c_ptr), ctypes.POINTER(_c_ptr), _c_i64, _c_i32, _c_i64p,
+         _c_i64p, _c_ptr, _c_i64, _c_i32, _c_ptr, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_float,
+         _c_ptr, _c_size],
+    ),
+    "pd_decode_weights_scratch_bytes": (_c_size, [_c_i32] * 4),
+    "pd_decode_weights": (
+        ctypes.c_int,
+        [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i32, _c_i64p, _c_i64p, _c_ptr, _c_i64,
+         _c_i32, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
+         _c_i32, _c_float, _c_ptr, _c_size, _c_ptr, _c_size, _c_ptr],
+    ),
+    "pd_evict_scratch_bytes": (_c_size, [_c_i32] * 4),
+    "pd_evict": (
+        ctypes.c_int,
+        [ctypes.POINTER(_c_ptr), ctypes.POINTER(_c_ptr), _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i64p,
+         _c_i64p, _c_ptr, _c_i64, _c_i32, _c_ptr, _c_i64, _c_i32, _c_ptr, _c_ptr, _c_ptr, _c_i64p, _c_ptr, _c_i64p,
+         _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_ptr, _c_size, _c_ptr],
+    ),
     "pd_set_decode_tuning": (ctypes.c_int, [_c_i32, _c_i32, _c_i32, _c_i32]),
     "pd_get_decode_tuning": (ctypes.c_int, [ctypes.POINTER(_c_i32)] * 4),
     "pd_set_decode_mode": (ctypes.c_int, [_c_i32, _c_i32, _c_i32]),
