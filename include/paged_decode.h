@@ -401,6 +401,16 @@ int pd_decode_window(const void* q, int64_t q_sb, int64_t q_sh, const void* k_ca
                      int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype, float scale_log2,
                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* pd_prefill where each query sees its window: token t of row b's S = cu[b + 1] - cu[b] packed ones sits at
+ * position seqlen_k[b] - S + t. total_q bounds the packed tensor; a loose max_seqlen_q costs nothing. A block id
+ * outside the pool reads zeros. fp16 / bf16, head_dim 64, 128 or 256, block_size >= 8. */
+int pd_prefill_window(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, const void* k_cache,
+                      const void* v_cache, int64_t n_blocks, int32_t block_size, const int64_t* k_strides,
+                      const int64_t* v_strides, const int32_t* block_table, int64_t bt_stride, int32_t max_blocks,
+                      const int32_t* cu_seqlens_q, const int32_t* seqlen_k, int32_t window, int32_t sinks, void* out,
+                      int64_t o_st, int64_t o_sh, int32_t batch, int32_t max_seqlen_q, int32_t n_head,
+                      int32_t n_kv_head, int32_t head_dim, int32_t dtype, float scale_log2, void* stream);
+
 /* pd_plan_create for windowed rows: every run of the plan is pd_decode_window's. */
 int pd_plan_create_window(pd_plan** plan, int32_t n_layer, const void* const* k_caches,
                           const void* const* v_caches, int64_t n_blocks, int32_t block_size,

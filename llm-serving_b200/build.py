@@ -63,6 +63,7 @@ SOURCES = [
     "pd_fp4_prefill.cu",
     "pd_block_copy.cu",
     "pd_evict.cu",
+    "pd_window_prefill.cu",
 ]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [

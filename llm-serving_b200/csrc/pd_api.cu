@@ -12,6 +12,7 @@
 #include "paged_decode.h"
 #include "pd_api_internal.h"
 #include "pd_internal.h"
+#include "pd_window.cuh"
 
 namespace pd {
 
@@ -901,6 +902,77 @@ int pd_prefill(const void* q, int64_t q_st, int64_t q_sh, const void* k_cache, c
                            : launch_prefill(p, kmap, vmap, dtype, head_dim, group, max_seqlen_q, batch,
                                             n_kv_head, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "prefill launch");
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return PD_OK;
+}
+
+int pd_prefill_window(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, const void* k_cache,
+                      const void* v_cache, int64_t n_blocks, int32_t block_size, const int64_t* k_strides,
+                      const int64_t* v_strides, const int32_t* block_table, int64_t bt_stride, int32_t max_blocks,
+                      const int32_t* cu_seqlens_q, const int32_t* seqlen_k, int32_t window, int32_t sinks, void* out,
+                      int64_t o_st, int64_t o_sh, int32_t batch, int32_t max_seqlen_q, int32_t n_head,
+                      int32_t n_kv_head, int32_t head_dim, int32_t dtype, float scale_log2, void* stream) {
+  if (!valid_dtype(dtype) || n_head < 1 || n_kv_head < 1 || n_head % n_kv_head != 0) return PD_ERR_INVALID;
+  if (batch < 0 || max_seqlen_q < 0 || max_blocks < 0 || n_blocks < 1 || total_q < 0 || total_q > 0x7fffffff)
+    return PD_ERR_INVALID;
+  if (!pow2(block_size) || window < 1 || sinks < 0) return PD_ERR_INVALID;
+  if (dtype == PD_F32 || (head_dim != 64 && head_dim != 128 && head_dim != 256) || block_size < 8)
+    return PD_ERR_UNSUPPORTED;
+  if (k_strides == nullptr || v_strides == nullptr) return PD_ERR_INVALID;
+  if (max_blocks > 0 && bt_stride < max_blocks) return PD_ERR_INVALID;
+  const int64_t capacity = int64_t(max_blocks) * block_size;
+  if (capacity > (int64_t(1) << 30)) return PD_ERR_INVALID;
+  // the kernel indexes query rows (a token's heads side by side) in 32 bits, up to a block of rows past the last,
+  // and a pool's blocks
+  if (total_q * n_head > (int64_t(1) << 30) || n_blocks >= 0x7fffffff) return PD_ERR_UNSUPPORTED;
+  max_seqlen_q = int32_t(max_seqlen_q < total_q ? max_seqlen_q : total_q);
+  if (batch == 0 || max_seqlen_q == 0) return PD_OK;
+  if (cu_seqlens_q == nullptr || seqlen_k == nullptr || (block_table == nullptr && max_blocks > 0))
+    return PD_ERR_INVALID;
+  if (check_rows(q, q_st, q_sh, dtype) != PD_OK || check_rows(out, o_st, o_sh, dtype) != PD_OK) return PD_ERR_INVALID;
+  int dev = 0;
+  if (current_device(&dev) != PD_OK) return PD_ERR_CUDA;
+  WindowPrefillParams p{};
+  p.err = error_word(dev);
+  if (p.err == nullptr) return PD_ERR_CUDA;
+  const int box_tokens = block_size < WINDOW_BOX ? block_size : WINDOW_BOX;
+  // Copies of 8-token groups of all pieces where the pools' blocks are evenly spaced (any contiguous pool), of
+  // one piece otherwise.
+  p.grouped = k_strides[0] == int64_t(block_size) * k_strides[1] && v_strides[0] == int64_t(block_size) * v_strides[1] &&
+              (n_blocks + 1) * (block_size / 8) <= 0x7fffffff;
+  CUtensorMap kmap, vmap;
+  for (int i = 0; i < 2; ++i) {
+    const int st = encode_pool(i ? &vmap : &kmap, i ? v_cache : k_cache, n_blocks, block_size, n_kv_head, head_dim,
+                               i ? v_strides : k_strides, dtype, box_tokens, 1, true,
+                               p.grouped ? SW_GROUPED : SW_ONE_PIECE);
+    if (st != PD_OK) return st;
+  }
+  p.q = q;
+  p.q_st = q_st;
+  p.q_sh = q_sh;
+  p.out = out;
+  p.o_st = o_st;
+  p.o_sh = o_sh;
+  p.cu_q = cu_seqlens_q;
+  p.seqlen = seqlen_k;
+  p.table = block_table;
+  p.bt_stride = bt_stride;
+  p.n_blocks = n_blocks;
+  p.total_q = int32_t(total_q);
+  p.max_seqlen_q = max_seqlen_q;
+  p.batch = batch;
+  p.n_kv_head = n_kv_head;
+  p.group = n_head / n_kv_head;
+  p.max_blocks = max_blocks;
+  p.capacity = int32_t(capacity);
+  p.log2_bs = ilog2_host(block_size);
+  p.log2_box = ilog2_host(box_tokens);
+  p.window = std::min(window, 1 << 30);  // no row is longer
+  p.sinks = std::min(sinks, 1 << 30);
+  p.scale_log2 = scale_log2;
+  p.wait_ns = g_wait_limit_ns.load(std::memory_order_relaxed);
+  const cudaError_t e = launch_window_prefill(p, kmap, vmap, dtype, head_dim, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "window prefill launch");
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return PD_OK;
 }

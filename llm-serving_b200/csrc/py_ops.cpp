@@ -36,6 +36,7 @@ using at::Tensor;
 #define PD_ENTRIES(X) \
   X(pd_qk_norm_rope) X(pd_fp4_write_slots) X(pd_fp4_write_table) X(pd_fp4_read_slots) X(pd_fp4_workspace_bytes) \
   X(pd_fp4_decode) X(pd_fp4_prefill) X(pd_block_copy) X(pd_decode_window_workspace_bytes) X(pd_decode_window) \
+  X(pd_prefill_window) \
   X(pd_decode_weights_scratch_bytes) X(pd_decode_weights) X(pd_evict_scratch_bytes) X(pd_evict)
 #define PD_FIELD(name) decltype(&::name) name = nullptr;
 struct Entries {
@@ -586,6 +587,87 @@ bool disjoint_rows(const Tensor& t) {
   return true;
 }
 
+Tensor aligned_rows(const Tensor& q0) {
+  const int64_t es = q0.element_size();
+  if (q0.stride(2) == 1 && q0.stride(0) * es % 16 == 0 && q0.stride(1) * es % 16 == 0 && aligned16(q0)) return q0;
+  const Tensor q = q0.contiguous();
+  return aligned16(q) && q.data_ptr() != q0.data_ptr() ? q : q0.clone(at::MemoryFormat::Contiguous);
+}
+
+// window and sinks, cut to what no row exceeds.
+void window_of(PyObject* w, PyObject* s, int64_t& window, int64_t& sinks) {
+  window = THPUtils_unpackLong(w);
+  sinks = THPUtils_unpackLong(s);
+  VALUE(window >= 1, "window must be at least 1, got ", window);
+  VALUE(sinks >= 0, "sinks must be at least 0, got ", sinks);
+  window = std::min<int64_t>(window, 1 << 30);
+  sinks = std::min<int64_t>(sinks, 1 << 30);
+}
+
+// What every attention call over pools asks of q.
+void queries_of(const Tensor& q, const Tensor& k, const Pools& p, const char* shape) {
+  VALUE(q.dim() == 3, "q must be ", shape, ", got shape ", q.sizes());
+  VALUE(q.scalar_type() == k.scalar_type(), "q/k_cache/v_cache must share one dtype, got ", q.scalar_type(), ", ",
+        k.scalar_type());
+  VALUE(q.size(2) == p.d, "q head_dim ", q.size(2), " != cache head_dim ", p.d);
+  VALUE(q.size(1) >= 1 && q.size(1) % p.hkv == 0, "n_head (", q.size(1), ") must be a multiple of n_kv_head (", p.hkv, ")");
+  same_device(k, "k_cache", q, "q");
+}
+
+// The result of a call: `given` (contiguous, like q) or a new tensor.
+Tensor result_of(PyObject* given, const Tensor& q) {
+  const Tensor* o = optional(given, "out");
+  if (o == nullptr) return new_like(q);
+  VALUE(o->sizes() == q.sizes() && o->scalar_type() == q.scalar_type() && o->device() == q.device() &&
+            o->is_contiguous() && aligned16(*o),
+        "out must be a contiguous, 16-byte aligned ", q.sizes(), " ", q.scalar_type(), " tensor on ", q.device());
+  return *o;
+}
+
+// prefill_window(q, k, v, table, cu, seqlen, longest, window, sinks, scale, out)
+PyObject* prefill_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 11, "prefill_window");
+  const Tensor &q0 = tensor(a[0], "q"), &k = tensor(a[1], "k_cache"), &v = tensor(a[2], "v_cache");
+  const Tensor &cu = tensor(a[4], "cu_seqlens_q"), &seqlen = tensor(a[5], "seqlen_k");
+  cuda(q0, "q", "paged_prefill_window");
+  const Pools p = pools_of(k, v, "paged_prefill_window");
+  queries_of(q0, k, p, "(total_q, H, D)");
+  VALUE(p.dtype != PD_F32, "paged_prefill_window needs fp16 or bf16, got fp32");
+  VALUE(p.d >= 64, "head_dim must be 64, 128 or 256, got ", p.d);
+  VALUE(p.block_size >= 8, "block_size must be at least 8, got ", p.block_size);
+  VALUE(seqlen.dim() == 1, "seqlen_k must be 1-D, got shape ", seqlen.sizes());
+  const int64_t rows = seqlen.size(0), heads = q0.size(1), total = q0.size(0);
+  VALUE(rows <= 0x7fffffff && total <= (1 << 30) / heads, "too many query rows");
+  VALUE(index_type(seqlen), "seqlen_k must be int32 or int64, got ", seqlen.scalar_type());
+  same_device(seqlen, "seqlen_k", q0, "q");
+  VALUE(cu.dim() == 1 && cu.size(0) == rows + 1, "cu_seqlens_q must be (", rows + 1, ",), got ", cu.sizes());
+  VALUE(index_type(cu), "cu_seqlens_q must be int32 or int64, got ", cu.scalar_type());
+  same_device(cu, "cu_seqlens_q", q0, "q");
+  const c10::cuda::CUDAGuard guard(q0.device());
+  const Tensor table = table_of(tensor(a[3], "block_table"), "block_table", rows, q0, "q");
+  VALUE(table.size(1) * p.block_size <= (int64_t(1) << 30), "a row's table holds at most 2^30 tokens");
+  const int64_t longest = std::min<int64_t>(THPUtils_unpackLong(a[6]), total);
+  int64_t window, sinks;
+  window_of(a[7], a[8], window, sinks);
+  const double scale = a[9] == Py_None ? 1.0 / std::sqrt(double(p.d)) : PyFloat_AsDouble(a[9]);
+  if (PyErr_Occurred()) return nullptr;
+  const Tensor out = result_of(a[10], q0);
+  if (rows == 0 || longest <= 0) return THPVariable_Wrap(out);
+  const Tensor q = aligned_rows(q0), offsets = int32(cu), lens = int32(seqlen);
+  if (failed(lib.pd_prefill_window(q.const_data_ptr(), total, q.stride(0), q.stride(1), k.const_data_ptr(),
+                                   v.const_data_ptr(), p.n_blocks, p.block_size, p.ks, p.vs,
+                                   table.const_data_ptr<int32_t>(), std::max(table.stride(0), table.size(1)),
+                                   int(table.size(1)), offsets.const_data_ptr<int32_t>(), lens.const_data_ptr<int32_t>(),
+                                   int(window), int(sinks), out.data_ptr(), out.stride(0), out.stride(1), int(rows),
+                                   int(longest), int(heads), int(p.hkv), p.d, p.dtype,
+                                   float(scale * 1.4426950408889634), stream_of(q0)),
+             "pd_prefill_window"))
+    return nullptr;
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 // decode_window(q, k, v, table, seqlen, window, sinks, scale, out, workspace) and
 // decode_weights(q, k, v, table, seqlen, weights, scale, out, workspace).
 PyObject* decode_variant(PyObject* const* a, bool windowed) {
@@ -594,13 +676,7 @@ PyObject* decode_variant(PyObject* const* a, bool windowed) {
   const Tensor &table0 = tensor(a[3], "block_table"), &seqlen = tensor(a[4], "seqlen");
   cuda(q0, "q", what);
   const Pools p = pools_of(k, v, what);
-  VALUE(q0.dim() == 3, "q must be (B, H, D), got shape ", q0.sizes());
-  VALUE(q0.scalar_type() == k.scalar_type(), "q/k_cache/v_cache must share one dtype, got ", q0.scalar_type(), ", ",
-        k.scalar_type());
-  VALUE(q0.size(2) == p.d, "q head_dim ", q0.size(2), " != cache head_dim ", p.d);
-  VALUE(q0.size(1) >= 1 && q0.size(1) % p.hkv == 0, "n_head (", q0.size(1), ") must be a multiple of n_kv_head (", p.hkv,
-        ")");
-  same_device(k, "k_cache", q0, "q");
+  queries_of(q0, k, p, "(B, H, D)");
   const int64_t rows = q0.size(0), heads = q0.size(1);
   VALUE(rows <= 0x7fffffff / heads, "too many query rows");
   VALUE(seqlen.dim() == 1 && seqlen.size(0) == rows, "seqlen must be (", rows, ",), got shape ", seqlen.sizes());
@@ -613,12 +689,7 @@ PyObject* decode_variant(PyObject* const* a, bool windowed) {
   int64_t window = 0, sinks = 0;
   const Tensor* weights = nullptr;
   if (windowed) {
-    window = THPUtils_unpackLong(a[5]);
-    sinks = THPUtils_unpackLong(a[6]);
-    VALUE(window >= 1, "window must be at least 1, got ", window);
-    VALUE(sinks >= 0, "sinks must be at least 0, got ", sinks);
-    window = std::min<int64_t>(window, 1 << 30);  // no row is longer
-    sinks = std::min<int64_t>(sinks, 1 << 30);
+    window_of(a[5], a[6], window, sinks);
   } else {
     weights = &tensor(a[5], "weights");
     VALUE(weights->scalar_type() == at::kFloat && weights->dim() == 3 && weights->size(0) == rows &&
@@ -633,15 +704,7 @@ PyObject* decode_variant(PyObject* const* a, bool windowed) {
   const int at = windowed ? 7 : 6;  // scale, out, workspace
   const double scale = a[at] == Py_None ? 1.0 / std::sqrt(double(p.d)) : PyFloat_AsDouble(a[at]);
   if (PyErr_Occurred()) return nullptr;
-  Tensor out;
-  if (const Tensor* o = optional(a[at + 1], "out")) {
-    VALUE(o->sizes() == q0.sizes() && o->scalar_type() == q0.scalar_type() && o->device() == q0.device() &&
-              o->is_contiguous() && aligned16(*o),
-          "out must be a contiguous, 16-byte aligned ", q0.sizes(), " ", q0.scalar_type(), " tensor on ", q0.device());
-    out = *o;
-  } else {
-    out = new_like(q0);
-  }
+  const Tensor out = result_of(a[at + 1], q0);
   if (rows == 0) return THPVariable_Wrap(out);
   void* stream = stream_of(q0);
   const int64_t need =
@@ -654,12 +717,7 @@ PyObject* decode_variant(PyObject* const* a, bool windowed) {
   } else {
     ws = decode_workspace(q0.device(), stream, need);
   }
-  const int64_t es = q0.element_size();
-  Tensor q = q0;
-  if (q.stride(2) != 1 || q.stride(0) * es % 16 != 0 || q.stride(1) * es % 16 != 0 || !aligned16(q)) {
-    q = q0.contiguous();
-    if (!aligned16(q) || q.data_ptr() == q0.data_ptr()) q = q0.clone(at::MemoryFormat::Contiguous);
-  }
+  const Tensor q = aligned_rows(q0);
   const Tensor lens = int32(seqlen);
   const int64_t bt_stride = std::max(table.stride(0), table.size(1));  // one row may have any stride
   const float scale_log2 = float(scale * 1.4426950408889634);
@@ -846,6 +904,7 @@ PyMethodDef methods[] = {
     PD_METHOD("block_copy", block_copy),
     PD_METHOD("decode_window", decode_window),
     PD_METHOD("decode_weights", decode_weights),
+    PD_METHOD("prefill_window", prefill_window),
     PD_METHOD("decode_window_workspace", decode_window_workspace),
     PD_METHOD("evict", evict),
     {nullptr, nullptr, 0, nullptr},

@@ -158,6 +158,12 @@ _SIGNATURES = {
          _c_i32, _c_ptr, _c_i32, _c_i32, _c_ptr, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_float,
          _c_ptr, _c_size, _c_ptr],
     ),
+    "pd_prefill_window": (
+        ctypes.c_int,
+        [_c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i32, _c_i64p, _c_i64p, _c_ptr, _c_i64, _c_i32,
+         _c_ptr, _c_ptr, _c_i32, _c_i32, _c_ptr, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
+         _c_float, _c_ptr],
+    ),
     "pd_plan_create_window": (
         ctypes.c_int,
         [ctypes.POINTER(_c_ptr), _c_i32, ctypes.POINTER(_c_ptr), ctypes.POINTER(_c_ptr), _c_i64, _c_i32, _c_i64p,

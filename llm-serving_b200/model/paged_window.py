@@ -20,7 +20,7 @@ import torch
 
 from model import _native
 
-__all__ = ["decode_workspace", "paged_decode_window"]
+__all__ = ["decode_workspace", "paged_decode_window", "paged_prefill_window"]
 
 
 def decode_workspace(rows: int, n_head: int, n_kv_head: int, head_dim: int, like: torch.Tensor) -> torch.Tensor:
@@ -42,3 +42,21 @@ def paged_decode_window(q, k_cache, v_cache, block_table, seqlen, window: int, *
     """
     ops = _native.ops or _native.require_ops()
     return ops.decode_window(q, k_cache, v_cache, block_table, seqlen, window, sinks, scale, out, workspace)
+
+
+def paged_prefill_window(q, k_cache, v_cache, block_table, cu_seqlens_q, seqlen_k, max_seqlen_q: int, window: int, *,
+                         sinks: int = 0, scale: float | None = None, out=None):
+    """Attention of a chunk of query tokens per row, each against its window of a paged pool (one kernel launch).
+
+    ``paged_prefill``'s contract: ``q`` is the packed ``(total_q, H, D)``, row ``b`` owning
+    ``q[cu_seqlens_q[b]:cu_seqlens_q[b + 1]]``; the chunk's K/V are already in the pools, and its token ``i`` of
+    ``Sq`` sits at position ``seqlen_k[b] - Sq + i``. ``max_seqlen_q`` must be at least the longest chunk (a loose
+    bound costs nothing); tokens of a longer one past it, and those of no row, are left unwritten. A token that
+    sees no key gives zeros.
+
+    fp16 or bf16, head_dim 64, 128 or 256, block_size at least 8, any number of query heads per kv head. Scores
+    and sums are fp32; the weights enter the second product in two 16-bit parts.
+    """
+    ops = _native.ops or _native.require_ops()
+    return ops.prefill_window(q, k_cache, v_cache, block_table, cu_seqlens_q, seqlen_k, max_seqlen_q, window, sinks, scale,
+                              out)
