@@ -4,23 +4,25 @@
 // the ones between the keep - sinks - recent with the largest sums (a tie keeps the lower index; NaN counts as
 // the smallest). The kept tokens' K and V rows close ranks, in their order, and their sums with them.
 //
-// Two launches. (1) select: one CTA per (layer, row, kv head) finds the threshold -- the largest 32-bit pattern
-// that at least as many of the order-preserving keys reach as there are places -- bit by bit, by counting: no
-// histogram, so equal sums cost nothing extra. The keys stay in registers. Then the tokens are ranked in order
-// (ballots and one scan per CTA-wide stretch), which gives the list of kept tokens, and the sums move.
-// (2) move: a CTA takes a column slice of the K or V rows of one (layer, row, kv head) and walks its list in
-// order. In place a token only moves down, so a stretch's rows are all in registers before any of them is
-// stored, and no later source has been overwritten; slices never meet.
+// Two launches. (1) select: one CTA per (layer, row, kv head) finds the threshold -- the largest key that at least as
+// many of the order-preserving 32-bit keys reach as there are places -- by histograms of 256 bins over the range that
+// is left, at first that of the row's own keys, so that two or three rounds mostly do, over a copy in shared memory.
+// Then the tokens are ranked in order (every warp a stretch, after one scan of the stretches' counts), which gives
+// the list of kept tokens, and the sums move.
+// (2) move: a CTA takes the K or V rows (a column slice of them) of one (layer, row, kv head) and walks its list in
+// order, the next stretch's loads under way while it stores. In place a token only moves down, so that a stretch's
+// rows need only be read before one of them is written; slices never meet.
 #include "pd_evict.cuh"
 
+#include <algorithm>
+
 #include "pd_block_copy.cuh"
+#include "pd_smem_limit.cuh"
 
 namespace pd {
 
 namespace {
 
-constexpr int SELECT_THREADS = 512;
-constexpr int SELECT_WARPS = SELECT_THREADS / 32;
 
 // Keys in the order of the sums: NaN below everything, -0 equal to +0.
 __device__ __forceinline__ uint32_t key_of(float w) {
@@ -29,11 +31,20 @@ __device__ __forceinline__ uint32_t key_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// P: keys of a thread in registers, or 0: read again for every count.
-template <int P>
-__global__ void __launch_bounds__(SELECT_THREADS) pd_evict_select_kernel(const __grid_constant__ EvictParams p) {
-  __shared__ int s_count[2][SELECT_WARPS];
-  __shared__ int2 s_scan[2][SELECT_WARPS];
+constexpr int BINS = 256;
+
+// WARPS of a CTA; COPY: the row's sums are copied into shared memory, else read again from global for every pass.
+// (In registers the passes would be unrolled, and a CTA that runs 60 KB of code once waits for its instructions:
+// 2048 rows of 1040 took 68 us.)
+template <int WARPS, bool COPY>
+__global__ void __launch_bounds__(WARPS * 32) pd_evict_select_kernel(const __grid_constant__ EvictParams p) {
+  constexpr int THREADS = WARPS * 32;
+  extern __shared__ float s_sums[];
+  griddep_launch_dependents();
+  __shared__ uint2 s_range[WARPS];
+  __shared__ int s_bins[BINS];
+  __shared__ int4 s_found;  // bin of the threshold, keys above it, keys in it
+  __shared__ int2 s_scan[2][WARPS];
   __shared__ int s_first;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int item = blockIdx.x;  // (layer, row, kv head)
@@ -44,120 +55,179 @@ __global__ void __launch_bounds__(SELECT_THREADS) pd_evict_select_kernel(const _
   float* wo = p.weights_out + layer * p.wo_sl + b * p.wo_sb + h * p.wo_sh;
   const int m = n < p.keep ? n : p.keep;
   if (n <= p.keep) {
-    for (int64_t j = tid; j < p.w_len; j += SELECT_THREADS) wo[j] = j < n ? w[j] : 0.f;
+    for (int64_t j = tid; j < p.w_len; j += THREADS) wo[j] = j < n ? w[j] : 0.f;
     if (tid == 0) p.info[item] = make_int2(n, n);
     return;
   }
   const int lo = p.sinks, hi = n - p.recent, places = p.keep - p.sinks - p.recent;
   if (tid == 0) s_first = n;
-
-  uint32_t key[P ? P : 1];
-  if constexpr (P != 0) {
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const int j = i * SELECT_THREADS + tid;
-      key[i] = j >= lo && j < hi ? key_of(w[j]) : 0u;
+  uint32_t* s_keys = reinterpret_cast<uint32_t*>(s_sums + (COPY ? n : 0));
+  uint32_t low = 0xffffffffu, high = 0u;  // of the middle tokens' keys
+  if constexpr (COPY) {
+#pragma unroll 4
+    for (int j = tid; j < n; j += THREADS) {
+      const float value = w[j];
+      const uint32_t k = key_of(value);
+      s_sums[j] = value;
+      s_keys[j] = k;
+      if (j >= lo && j < hi) {
+        low = min(low, k);
+        high = max(high, k);
+      }
+    }
+  } else {
+    for (int j = lo + tid; j < hi; j += THREADS) {
+      const uint32_t k = key_of(w[j]);
+      low = min(low, k);
+      high = max(high, k);
     }
   }
-  // CTA-wide count of the middle tokens whose key reaches x (x > 0, so that the zeros elsewhere do not).
-  int turn = 0;
-  auto reach = [&](uint32_t x) -> int {
-    int c = 0;
-    if constexpr (P != 0) {
-#pragma unroll
-      for (int i = 0; i < P; ++i) c += key[i] >= x;
-    } else {
-      for (int j = lo + tid; j < hi; j += SELECT_THREADS) c += key_of(w[j]) >= x;
-    }
-    c = __reduce_add_sync(FULL_MASK, c);
-    if (lane == 0) s_count[turn][warp] = c;
-    __syncthreads();
-    c = __reduce_add_sync(FULL_MASK, lane < SELECT_WARPS ? s_count[turn][lane] : 0);
-    turn ^= 1;  // the next count's writes do not meet this one's reads
-    return c;
-  };
-  // The largest x that at least `places` keys reach (0: every key does).
-  uint32_t x = 0u;
-  int got = hi - lo;  // keys that reach x
+  auto key = [&](int j) -> uint32_t { return COPY ? s_keys[j] : key_of(w[j]); };
+  // The threshold x, and how many of the tokens at it stay (the first ones; `exact`: all that reach x stay).
+  uint32_t x = 0xffffffffu;  // no token has this key: it is a NaN's pattern
+  int at = 0;
   if (places > 0) {
-    for (int bit = 31; bit >= 0 && got != places; --bit) {
-      const int c = reach(x | 1u << bit);
-      if (c >= places) {
-        x |= 1u << bit;
-        got = c;
+    low = __reduce_min_sync(FULL_MASK, low);
+    high = __reduce_max_sync(FULL_MASK, high);
+    if constexpr (WARPS > 1) {
+      if (lane == 0) s_range[warp] = make_uint2(low, high);
+      __syncthreads();
+      const uint2 r = s_range[lane < WARPS ? lane : 0];
+      low = __reduce_min_sync(FULL_MASK, r.x);
+      high = __reduce_max_sync(FULL_MASK, r.y);
+    }
+    // Keys low .. low + 2^width - 1 hold the threshold; `need` of them stay.
+    int width = 32 - __clz(high - low), need = places;
+    for (;;) {
+      const int shift = max(width - 8, 0);
+      for (int i = tid; i < BINS; i += THREADS) s_bins[i] = 0;
+      __syncthreads();
+#pragma unroll 4
+      for (int j = lo + tid; j < hi; j += THREADS) {
+        const uint32_t k = key(j), d = k - low;  // (wraps to far above the range for a lower key)
+        if (width == 32 ? k >= low : d >> width == 0) atomicAdd(&s_bins[d >> shift], 1);
+      }
+      __syncthreads();
+      if (warp == 0) {  // lane l: bins 8 l .. 8 l + 7; the first from above with which `need` are reached
+        int c[8], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += c[i] = s_bins[lane * 8 + i];
+        int from = sum;  // keys in this lane's bins and above
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_down_sync(FULL_MASK, from, o);
+          if (lane + o < 32) from += y;
+        }
+        int above = from - sum;
+        if (above < need && from >= need) {
+#pragma unroll
+          for (int i = 7; i >= 0; --i) {
+            if (above + c[i] >= need) {
+              s_found = make_int4(lane * 8 + i, above, c[i], 0);
+              break;
+            }
+            above += c[i];
+          }
+        }
+      }
+      __syncthreads();
+      const int4 f = s_found;
+      low += uint32_t(f.x) << shift;
+      need -= f.y;
+      width = shift;
+      x = low;
+      if (need == f.z) break;  // all of the bin stay
+      if (shift == 0) {        // its keys are one
+        at = need;
+        break;
       }
     }
   }
-  // Above the threshold all stay; of those at it, the first. got == places: all that reach it stay.
-  int above = got, at = 0;
-  if (places == 0) {
-    x = 0xffffffffu;  // no key is that large (it would be a NaN's pattern)
-    above = 0;
-  } else if (got != places) {
-    above = x == 0xffffffffu ? 0 : reach(x + 1u);
-    at = places - above;
-  }
-  const bool exact = at == 0;  // keys >= x are the ones (places == 0: none)
+  const bool exact = at == 0;
+  if (places == 0) __syncthreads();  // the copy (the rounds above have waited for it)
 
   int32_t* order = p.order + int64_t(item) * p.keep;
-  int base = 0, ties = 0;  // kept tokens, and tokens at the threshold, before this stretch
-  int side = 0;
-  __syncthreads();  // s_first
-  for (int j0 = 0; j0 < n; j0 += SELECT_THREADS, side ^= 1) {
-    const int j = j0 + tid;
-    const float value = j < n ? w[j] : 0.f;
-    const bool middle = j >= lo && j < hi;
-    const uint32_t k = key_of(value);
-    const bool tie = middle && !exact && k == x;
-    bool stays = j < n && (!middle || (exact ? k >= x : k > x));
-    const unsigned tie_mask = __ballot_sync(FULL_MASK, tie), stay_mask = __ballot_sync(FULL_MASK, stays);
-    if (lane == 0) s_scan[side][warp] = make_int2(__popc(stay_mask), __popc(tie_mask));
-    __syncthreads();  // also: every value of the stretch is read before one is written
-    int2 before = make_int2(0, 0), all = make_int2(0, 0);
-#pragma unroll
-    for (int i = 0; i < SELECT_WARPS; ++i) {
-      const int2 c = s_scan[side][i];
-      if (i < warp) {
-        before.x += c.x;
-        before.y += c.y;
-      }
-      all.x += c.x;
-      all.y += c.y;
-    }
-    const unsigned lower = (1u << lane) - 1u;
-    const int tie_rank = ties + before.y + __popc(tie_mask & lower);
-    if (tie && tie_rank < at) stays = true;
-    // kept before j: those above or outside, and the ties that still had a place
-    const int rank = base + before.x + __popc(stay_mask & lower) + min(tie_rank, at) - min(ties, at);
-    base += all.x + min(ties + all.y, at) - min(ties, at);
-    ties += all.y;
+  const unsigned lower = (1u << lane) - 1u;
+  auto kept = [&](int j, uint32_t k) -> bool { return j < lo || j >= hi || (exact ? k >= x : k > x); };  // but for a tie
+  auto is_tie = [&](int j, uint32_t k) -> bool { return !exact && k == x && j >= lo && j < hi; };
+  // Token j goes to `rank`, if it stays: `before` kept tokens and `ties` at the threshold lie before its 32.
+  auto place = [&](int j, float value, int before, int ties, unsigned stay_mask, unsigned tie_mask) {
+    const int tie_rank = ties + __popc(tie_mask & lower);
+    const bool stays = (stay_mask >> lane & 1u) || ((tie_mask >> lane & 1u) && tie_rank < at);
+    const int rank = before + min(ties, at) + __popc(stay_mask & lower) + min(tie_rank, at) - min(ties, at);
     if (stays) {
       wo[rank] = value;
       order[rank] = j;
     }
     const unsigned gone = __ballot_sync(FULL_MASK, j < n && !stays);
-    if (gone && lane == 0) atomicMin(&s_first, j0 + warp * 32 + __ffs(gone) - 1);
+    if (gone && lane == 0) atomicMin(&s_first, j + __ffs(gone) - 1);
+  };
+  if constexpr (COPY) {
+    // A warp's stretch of 32-token steps: whether they stay, a bit a step, one scan of the counts, then every
+    // warp ranks its own.
+    const int per = (n + THREADS - 1) / THREADS, start = warp * per * 32 + lane;
+    unsigned long long stay_bits = 0ull, tie_bits = 0ull;
+    for (int i = 0; i < per; ++i) {
+      const int j = start + i * 32;
+      if (j >= n) break;
+      const uint32_t k = s_keys[j];
+      stay_bits |= (unsigned long long)kept(j, k) << i;
+      tie_bits |= (unsigned long long)is_tie(j, k) << i;
+    }
+    const int stay = __reduce_add_sync(FULL_MASK, __popcll(stay_bits));
+    const int tie = __reduce_add_sync(FULL_MASK, __popcll(tie_bits));
+    if (lane == 0) s_scan[0][warp] = make_int2(stay, tie);
+    __syncthreads();
+    const int2 c = lane < warp ? s_scan[0][lane] : make_int2(0, 0);
+    int before = __reduce_add_sync(FULL_MASK, c.x), ties = __reduce_add_sync(FULL_MASK, c.y);
+    for (int i = 0; i < per; ++i) {
+      const int j = start + i * 32;
+      const unsigned stay_mask = __ballot_sync(FULL_MASK, stay_bits >> i & 1ull);
+      const unsigned tie_mask = __ballot_sync(FULL_MASK, tie_bits >> i & 1ull);
+      place(j, j < n ? s_sums[j] : 0.f, before, ties, stay_mask, tie_mask);
+      before += __popc(stay_mask);
+      ties += __popc(tie_mask);
+    }
+  } else {
+    // A CTA-wide stretch at a time: in place, what is written never lies past the stretch at hand.
+    int before = 0, ties = 0, side = 0;
+    __syncthreads();  // s_first
+    for (int j0 = 0; j0 < n; j0 += THREADS, side ^= 1) {
+      const int j = j0 + tid;
+      const float value = j < n ? w[j] : 0.f;
+      const unsigned stay_mask = __ballot_sync(FULL_MASK, j < n && kept(j, key_of(value)));
+      const unsigned tie_mask = __ballot_sync(FULL_MASK, j < n && is_tie(j, key_of(value)));
+      if (lane == 0) s_scan[side][warp] = make_int2(__popc(stay_mask), __popc(tie_mask));
+      __syncthreads();  // also: every sum of the stretch is read before one is written
+      const int2 c = lane < WARPS ? s_scan[side][lane] : make_int2(0, 0);
+      const int2 mine_before = make_int2(__reduce_add_sync(FULL_MASK, lane < warp ? c.x : 0),
+                                         __reduce_add_sync(FULL_MASK, lane < warp ? c.y : 0));
+      place(j, value, before + mine_before.x, ties + mine_before.y, stay_mask, tie_mask);
+      before += __reduce_add_sync(FULL_MASK, c.x);
+      ties += __reduce_add_sync(FULL_MASK, c.y);
+    }
   }
   __syncthreads();  // s_first
-  for (int64_t j = m + tid; j < p.w_len; j += SELECT_THREADS) wo[j] = 0.f;
+  for (int64_t j = m + tid; j < p.w_len; j += THREADS) wo[j] = 0.f;
   if (tid == 0) p.info[item] = make_int2(s_first, m);
 }
 
 constexpr int MOVE_THREADS = 256;
-constexpr int AHEAD = 4;  // rows of a thread in flight
+constexpr int AHEAD = 4;             // rows of a thread in a stretch
+constexpr int CHUNK = MOVE_THREADS;  // rows whose places are looked up at a time
 
-__global__ void __launch_bounds__(MOVE_THREADS) pd_evict_move_kernel(const __grid_constant__ EvictParams p, int log2_slice) {
+// `parts` CTAs share the list of one (layer, row, kv head)'s K or V (new pages only: nothing that is written is
+// read), each of them in slices of 2^log2_slice 16-byte units, at least 4, so that a stretch is at most a chunk.
+__global__ void __launch_bounds__(MOVE_THREADS) pd_evict_move_kernel(const __grid_constant__ EvictParams p, int log2_slice,
+                                                                     int parts) {
+  __shared__ int64_t s_src[2][CHUNK], s_dst[2][CHUNK];
   const int tid = threadIdx.x;
-  const int per = 1 << log2_slice;                  // 16-byte units of a slice
+  const int per = 1 << log2_slice;
   const int slices = (p.chunks + per - 1) >> log2_slice;
-  const int slice = blockIdx.x % slices;
-  const int rest = blockIdx.x / slices;
+  const int slice = blockIdx.x % slices, part = blockIdx.x / slices % parts;
+  const int rest = blockIdx.x / slices / parts;
   const int is_v = rest & 1, item = rest >> 1;
   const int h = item % p.n_kv_head, b = item / p.n_kv_head % p.batch, layer = item / p.n_kv_head / p.batch;
-  griddep_wait();
-  const int2 info = p.info[item];
-  if (p.seqlen_out != nullptr && layer == 0 && h == 0 && is_v == 0 && slice == 0 && tid == 0) p.seqlen_out[b] = info.y;
-  const int32_t* order = p.order + int64_t(item) * p.keep;
   const int32_t* from = p.table + int64_t(b) * p.bt_stride;
   const int32_t* to = p.new_table + int64_t(b) * p.nbt_stride;
   const int64_t sb = is_v ? p.v_sb : p.k_sb, sn = is_v ? p.v_sn : p.k_sn, sh = is_v ? p.v_sh : p.k_sh;
@@ -165,35 +235,89 @@ __global__ void __launch_bounds__(MOVE_THREADS) pd_evict_move_kernel(const __gri
   uint4* pool = static_cast<uint4*>(is_v ? p.v[layer] : p.k[layer]) + h * sh + unit;
   const bool mine = unit < p.chunks;
   const int mask = (1 << p.log2_bs) - 1;
-  const int step = MOVE_THREADS >> log2_slice;
-  // The row of token t by a table of `width` blocks, or nullptr (reported).
-  auto row = [&](const int32_t* table, int width, int t) -> uint4* {
+  const int step = MOVE_THREADS >> log2_slice, my_row = tid >> log2_slice;
+  griddep_wait();
+  const int2 info = p.info[item];
+  if (p.seqlen_out != nullptr && layer == 0 && h == 0 && is_v == 0 && slice == 0 && part == 0 && tid == 0)
+    p.seqlen_out[b] = info.y;
+  const int32_t* order = p.order + int64_t(item) * p.keep;
+  const int all0 = p.fresh ? 0 : info.x, share = ((info.y - all0 + parts - 1) / parts + CHUNK - 1) / CHUNK * CHUNK;
+  const int first = all0 + part * share, count = min(share, info.y - first);
+  // Offset of token t's row by a table of `width` blocks, or -1 (reported).
+  auto row = [&](const int32_t* table, int width, int t) -> int64_t {
     const int page = t >> p.log2_bs;
     const int blk = page < width ? __ldg(table + page) : -1;
     if (blk < 0 || blk >= p.n_blocks) {
       atomicOr(p.err, DEVERR_COPY_RANGE);
-      return nullptr;
+      return -1;
     }
-    return pool + int64_t(blk) * sb + int64_t(t & mask) * sn;
+    return int64_t(blk) * sb + int64_t(t & mask) * sn;
   };
-  for (int r0 = p.fresh ? 0 : info.x; r0 < info.y; r0 += step * AHEAD) {
-    uint4 x[AHEAD];
-    uint4* dst[AHEAD];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int r = r0 + i * step + (tid >> log2_slice);
-      dst[i] = nullptr;
-      if (!mine || r >= info.y) continue;
-      const uint4* src = row(from, p.max_blocks, r < info.x ? r : order[r]);
-      if (src == nullptr) continue;
-      x[i] = *src;
-      dst[i] = row(to, p.new_max_blocks, r);
+  auto look_up = [&](int chunk) {  // a thread a row
+    const int i = chunk * CHUNK + tid, r = first + i;
+    int64_t src = -1, dst = -1;
+    if (i < count) {
+      dst = row(to, p.new_max_blocks, r);
+      src = row(from, p.max_blocks, r < info.x ? r : order[r]);
+      if (src < 0) dst = -1;
     }
-    __syncthreads();  // a stretch's rows are read before one is written
+    s_src[chunk & 1][tid] = src;
+    s_dst[chunk & 1][tid] = dst;
+  };
+  auto load = [&](int i0, uint4 (&x)[AHEAD]) {
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-      if (dst[i] != nullptr) *dst[i] = x[i];
+    for (int k = 0; k < AHEAD; ++k) {
+      const int i = i0 + k * step + my_row;
+      if (i >= count) continue;
+      const int64_t src = s_src[(i / CHUNK) & 1][i % CHUNK];
+      if (mine && src >= 0) x[k] = pool[src];
+    }
+  };
+  if (count <= 0) return;
+  uint4 x[AHEAD], y[AHEAD];
+  look_up(0);
+  __syncthreads();
+  load(0, x);
+  for (int i0 = 0; i0 < count; i0 += step * AHEAD) {
+    __syncthreads();  // this stretch's rows are read before one is written; the last chunk's places are done with
+    if (i0 % CHUNK == 0 && i0 + CHUNK < count) {
+      look_up(i0 / CHUNK + 1);
+      __syncthreads();
+    }
+    load(i0 + step * AHEAD, y);  // in place, what is written now lies before every later source
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int i = i0 + k * step + my_row;
+      if (i >= count) continue;
+      const int64_t dst = s_dst[(i / CHUNK) & 1][i % CHUNK];
+      if (mine && dst >= 0) pool[dst] = x[k];
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) x[k] = y[k];
   }
+}
+
+// Rows of up to so many tokens are copied into shared memory.
+constexpr int COPY_TOKENS = 24576;
+
+template <int WARPS, bool COPY>
+cudaError_t select(const EvictParams& p, int64_t items, cudaStream_t stream) {
+  auto fn = pd_evict_select_kernel<WARPS, COPY>;
+  static SmemRaised raised{};
+  const cudaError_t err = raise_smem_limit(fn, COPY ? COPY_TOKENS * 8 : 0, raised);
+  if (err != cudaSuccess) return err;
+  fn<<<unsigned(items), WARPS * 32, COPY ? size_t(p.capacity) * 8 : 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+// Warps by the row's length: eight or so tokens a thread, 32 warps at most.
+cudaError_t launch_select(const EvictParams& p, int64_t items, cudaStream_t stream) {
+  if (p.capacity <= 512) return select<2, true>(p, items, stream);
+  if (p.capacity <= 2048) return select<4, true>(p, items, stream);
+  if (p.capacity <= 4096) return select<8, true>(p, items, stream);
+  if (p.capacity <= 8192) return select<16, true>(p, items, stream);
+  if (p.capacity <= COPY_TOKENS) return select<32, true>(p, items, stream);
+  return select<32, false>(p, items, stream);
 }
 
 }  // namespace
@@ -201,18 +325,23 @@ __global__ void __launch_bounds__(MOVE_THREADS) pd_evict_move_kernel(const __gri
 cudaError_t launch_evict(const EvictParams& p, cudaStream_t stream) {
   const int64_t items = int64_t(p.layers) * p.batch * p.n_kv_head;
   if (items == 0) return cudaSuccess;
-  void (*select)(EvictParams) = pd_evict_select_kernel<0>;
-  if (p.capacity <= SELECT_THREADS * 4) select = pd_evict_select_kernel<4>;
-  else if (p.capacity <= SELECT_THREADS * 16) select = pd_evict_select_kernel<16>;
-  else if (p.capacity <= SELECT_THREADS * 64) select = pd_evict_select_kernel<64>;
-  select<<<unsigned(items), SELECT_THREADS, 0, stream>>>(p);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = launch_select(p, items, stream);
   if (e != cudaSuccess) return e;
-  // Slices of at least 32 bytes, until there are eight CTAs for every SM.
-  int log2_slice = 0;
+  // Whole rows where there are eight CTAs for every SM; else new pages' lists are shared by CTAs, down to a
+  // chunk each, and rows moved in place are cut into slices, down to 64 bytes.
+  int log2_slice = 2, parts = 1;
   while ((1 << log2_slice) < p.chunks) ++log2_slice;
-  while (log2_slice > 1 && 2 * items * ((p.chunks + (1 << log2_slice) - 1) >> log2_slice) < 8 * int64_t(p.sms)) --log2_slice;
-  const int64_t ctas = 2 * items * ((p.chunks + (1 << log2_slice) - 1) >> log2_slice);
+  int64_t ctas = 2 * items;
+  const int64_t enough = 8 * int64_t(p.sms);
+  if (p.fresh) {
+    parts = int(std::min((enough + ctas - 1) / ctas, int64_t(p.keep + CHUNK - 1) / CHUNK));
+    ctas *= parts;
+  } else {
+    while (log2_slice > 2 && ctas < enough) {
+      --log2_slice;
+      ctas = 2 * items * ((p.chunks + (1 << log2_slice) - 1) >> log2_slice);
+    }
+  }
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -222,7 +351,7 @@ cudaError_t launch_evict(const EvictParams& p, cudaStream_t stream) {
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, pd_evict_move_kernel, p, log2_slice);
+  return cudaLaunchKernelEx(&cfg, pd_evict_move_kernel, p, log2_slice, parts);
 }
 
 }  // namespace pd
