@@ -11,16 +11,14 @@
 //    numbered without the gap between them and cut into tiles of KT keys, so a few sinks cost a copy, not a tile.
 //  * One warp streams K and V tiles by TMA into two rings of stages, a lane a copy, block ids one tile ahead. No block
 //    without a visible token is looked up; where the last tile ends early, V is filled with zeros from outside the pool.
-//  * One warp issues the MMAs: S = Q K^T (M 128, N KT, K head_dim) into TMEM, and O += P V with P read from TMEM,
-//    where the softmax wrote it over the S it came from, a tile's first half as soon as it is there. Before the
-//    P V of a tile whose copies hold tokens that no row of the CTA sees, it zeroes their V, so that whatever bytes they
-//    hold never reach O.
+//  * One warp issues S = Q K^T (M 128, N 64 keys, K head_dim) into one of a block's two S buffers in TMEM, another O += P V
+//    with P read from TMEM, where the softmax wrote it over the S it came from; so a block's next S is there when its
+//    softmax is done with one. A third warp zeroes the V of tokens that a tile's copies hold but no row of the CTA sees,
+//    so that whatever bytes they hold never reach O.
 //  * 4 softmax warps per block of query rows, one thread per row (TMEM lane = row): maximum over the row's
 //    scores, P = 2^(s - m + 7), and the fp32 sum; no exchange between threads. The maximum moves only when a tile
 //    passes it by 2^8, so rescaling O in TMEM is rare.
-//  With NQ = 2 the blocks alternate: while the softmax of one runs, the tensor cores do the other's P V and next S, and
-//  each tile serves 256 rows. At head_dim 256 TMEM holds one block (O takes 256 of its 512 columns), which
-//  alternates between two S buffers instead.
+//  With NQ = 2 a tile serves 256 rows; at head_dim 256 TMEM holds one block (O takes 256 of its 512 columns).
 //  * P enters as two 16-bit operands, P = hi + lo: 2^-17 of the weighted mean of |v| in bf16 and 2^-22 in fp16, as
 //    the causal chunk kernel (pd_prefill_tc.cu) has it; one bf16 part alone would be off by as much as the result's
 //    own rounding. The factor 2^7, which the sums carry too, keeps fp16 weights down to 2^-21 normal numbers.
@@ -39,18 +37,20 @@ namespace pd {
 namespace {
 
 constexpr int ROWS = 128;  // query rows of a block (the MMA's M)
+constexpr int KEYS = 64;   // keys of a softmax step (the S MMA's N)
 constexpr float P_SHIFT = 7.f, HEADROOM = 8.f;
 
 template <int D>
 struct Cfg {
   static constexpr int NQ = D <= 128 ? 2 : 1;     // blocks of query rows per CTA
-  static constexpr int KT = D <= 128 ? 128 : 64;  // keys per tile (the S MMA's N)
-  static constexpr int PART = KT / 2;             // keys of a tile whose P V may start before the others' P
+  static constexpr int KT = D <= 128 ? 128 : 64;  // keys of a tile of K or V in shared memory
+  static constexpr int STEPS = KT / KEYS;         // softmax steps of a tile
   static constexpr int PIECES = D / 64;
   static constexpr int SOFTMAX_WARPS = 4 * NQ;
   static constexpr int TMA_WARP = SOFTMAX_WARPS;
-  static constexpr int MMA_WARP = SOFTMAX_WARPS + 1;
-  static constexpr int THREADS = (SOFTMAX_WARPS + 4) * 32;  // the TMA and MMA warps' group of four: two are idle
+  static constexpr int CLEAR_WARP = SOFTMAX_WARPS + 1;
+  static constexpr int S_WARP = SOFTMAX_WARPS + 2;
+  static constexpr int THREADS = (SOFTMAX_WARPS + 4) * 32;  // and a warp for P V
   // With two blocks, registers are dealt anew between the groups, so that a softmax thread holds a row's KT
   // scores and P; with one, every thread has enough.
   static constexpr bool SPLIT = NQ == 2;
@@ -62,7 +62,7 @@ struct Cfg {
   static constexpr int STAGES = 2;  // tiles of K, and of V
   static constexpr int Q_BYTES = ROWS * D * 2;
   static constexpr int KV_BYTES = KT * D * 2;
-  static constexpr int O_COL = 2 * KT;  // behind two S/P buffers
+  static constexpr int O_COL = NQ * 2 * KEYS;  // behind two S/P buffers a block
   static constexpr int TMEM_COLS = 512;
   static_assert(O_COL + NQ * D <= TMEM_COLS, "TMEM columns");
   static constexpr int OFF_Q = 1024;  // barriers and flags before it
@@ -74,18 +74,18 @@ struct Cfg {
 
 // Barrier slots (8 bytes each) at the front of shared memory.
 struct Bars {
-  static constexpr int K_FULL = 0;   // [2] K tile landed (transaction bytes)
-  static constexpr int V_FULL = 2;   // [2]
-  static constexpr int K_EMPTY = 4;  // [2] every S of the tile completed (commit)
-  static constexpr int V_EMPTY = 6;  // [2] every P V of the tile completed (commit)
-  static constexpr int S_FULL = 8;   // [2] S buffer written (commit)
-  static constexpr int P_FULL = 10;  // [2] P written over it, O rescaled: one arrival per softmax warp
-  static constexpr int O_DONE = 12;  // [2] P V that read the buffer completed (commit)
-  static constexpr int Q_FULL = 14;  // Q stored: one arrival per softmax warp
-  static constexpr int DRAIN = 15;
-  static constexpr int P_PART = 16;      // [2] P of the tile's first PART keys written
-  static constexpr int TMEM_SLOT = 160;  // byte offsets
-  static constexpr int ABORT = 168;
+  static constexpr int K_FULL = 0;    // [2] K tile landed (transaction bytes)
+  static constexpr int V_FULL = 2;    // [2]
+  static constexpr int K_EMPTY = 4;   // [2] every S of the tile completed (commit)
+  static constexpr int V_EMPTY = 6;   // [2] every P V of the tile completed (commit)
+  static constexpr int V_READY = 8;   // [2] V tile's unseen tokens are zeros
+  static constexpr int Q_FULL = 10;   // Q stored: one arrival per softmax warp
+  static constexpr int DRAIN = 11;    // [2]
+  static constexpr int S_FULL = 13;   // [4] S buffer written (commit)
+  static constexpr int P_FULL = 17;   // [4] P written over it, O rescaled: one arrival per softmax warp
+  static constexpr int O_DONE = 21;   // [4] P V that read the buffer completed (commit)
+  static constexpr int TMEM_SLOT = 200;  // byte offsets
+  static constexpr int ABORT = 208;
 };
 
 // The keys that a CTA's query rows see, numbered without the gap between sinks and window: key u of the
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
   auto bar = [&](int slot) -> uint32_t { return sbase + uint32_t(slot) * 8u; };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Bars::ABORT);
 
-  if (warp == C::MMA_WARP) {
+  if (warp == C::S_WARP) {
     if (lane == 0) {
       tma_prefetch_desc(&kmap);
       tma_prefetch_desc(&vmap);
@@ -130,13 +130,15 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
         mbar_init(bar(Bars::V_FULL + i), 1);
         mbar_init(bar(Bars::K_EMPTY + i), 1);
         mbar_init(bar(Bars::V_EMPTY + i), 1);
+        mbar_init(bar(Bars::V_READY + i), 1);
+        mbar_init(bar(Bars::DRAIN + i), 1);
+      }
+      for (int i = 0; i < 2 * NQ; ++i) {
         mbar_init(bar(Bars::S_FULL + i), 1);
         mbar_init(bar(Bars::P_FULL + i), 4);
-        mbar_init(bar(Bars::P_PART + i), 4);
         mbar_init(bar(Bars::O_DONE + i), 1);
       }
       mbar_init(bar(Bars::Q_FULL), C::SOFTMAX_WARPS);
-      mbar_init(bar(Bars::DRAIN), 1);
       *abort_flag = 0;
       fence_barrier_init();
     }
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
   const int box = 1 << p.log2_box;
   // What the CTA's rows see: up to its last token, from its first token's window on, and the sinks.
   Keys keys;
-  int tiles[NQ], most = 0;
+  int steps[NQ], most = 0;  // softmax steps of a block, tiles of the CTA
   {
     const int last = min(row0 + NQ * ROWS, rows) - 1;
     const int end = row0 < rows ? max(ctx + last / p.group + 1, 0) : 0;  // <= lk
@@ -174,8 +176,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
     for (int q = 0; q < NQ; ++q) {
       const int r0 = row0 + q * ROWS;
       const int kend = r0 < rows ? max(ctx + (min(r0 + ROWS, rows) - 1) / p.group + 1, 0) - keys.gap : 0;
-      tiles[q] = max((kend + KT - 1) / KT, 0);
-      most = max(most, tiles[q]);
+      steps[q] = max((kend + KEYS - 1) / KEYS, 0);
+      most = max(most, (steps[q] + C::STEPS - 1) / C::STEPS);
     }
   }
   // Keys that no row of the CTA sees: [blind0, blind1), and from keys.count on.
@@ -199,6 +201,9 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
     *abort_flag = 1;
     atomicOr(p.err, DEVERR_WAIT_TIMEOUT);
   };
+
+  // Step u of block q uses S/P buffer 2 q + u % 2 for the u / 2-th time.
+  const int all_steps = NQ == 2 ? max(steps[0], steps[NQ - 1]) : steps[0];
 
   if (row0 >= rows) {  // no query row
     tmem = meet();
@@ -270,106 +275,71 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
         warp_wait_phase(bar(Bars::K_FULL + j % C::STAGES), uint32_t((j / C::STAGES) & 1), DRAIN_LIMIT_NS);
       for (int j = max(v_done - C::STAGES, 0); j < v_done; ++j)
         warp_wait_phase(bar(Bars::V_FULL + j % C::STAGES), uint32_t((j / C::STAGES) & 1), DRAIN_LIMIT_NS);
-    } else if (warp == C::MMA_WARP) {
-      // ---------------------------------------------------------------- MMA issuer
+    } else if (warp == C::CLEAR_WARP) {
+      // ---------------------------------------------------------------- V of tokens that no row sees
+      tmem = meet();
+      bool ok = true;
+      for (int j = 0; j < most; ++j) {
+        const int s = j & 1;
+        if (__any_sync(FULL_MASK, *abort_flag != 0)) break;
+        if (!warp_wait_phase(bar(Bars::V_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns)) {
+          ok = false;
+          break;
+        }
+        const int u0 = j * KT;
+        auto clear = [&](int lo, int hi) {  // fewer than two copies' tokens
+          lo = max(lo, u0) - u0;
+          hi = min(hi, u0 + KT) - u0;
+          if (lo >= hi) return;
+          for (int i = lane; i < (hi - lo) * (D / 8); i += 32) {
+            const int r = lo + i / (D / 8), u = i % (D / 8);
+            sts128(v_addr(s) + uint32_t(r >> 3) * gstride + uint32_t((r & 7) * 128) + uint32_t(u >> 3) * pstride +
+                       uint32_t((u & 7) << 4),
+                   0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+        };
+        clear(blind0, blind1);
+        clear(keys.count, (keys.count + box - 1) >> p.log2_box << p.log2_box);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(Bars::V_READY + s));
+      }
+      if (!ok && lane == 0) fail();
+    } else if (warp == C::S_WARP) {
+      // ---------------------------------------------------------------- S = Q K^T
       // The whole warp runs this loop and one elected lane issues, so descriptors and addresses stay
       // uniform over the warp and no operand of an MMA is moved on its own.
       tmem = meet();
       if (most > 0) {
-        constexpr uint32_t IDESC_S = tc::instr_desc_f16(BF16, ROWS, KT, false, false);
-        constexpr uint32_t IDESC_PV = tc::instr_desc_f16(BF16, ROWS, D, false, true);
+        constexpr uint32_t IDESC_S = tc::instr_desc_f16(BF16, ROWS, KEYS, false, false);
         bool ok = lane_wait(bar(Bars::Q_FULL), 0u, p.wait_ns);
         const uint64_t q_desc = tc::smem_desc(sbase + C::OFF_Q, 16u, 1024u);
         const uint64_t k_desc = tc::smem_desc(k_addr(0), 16u, gstride);
-        const uint64_t v_desc = tc::smem_desc(v_addr(0), pstride, gstride);
-        // (block q, tile j) uses S/P buffer q for the j-th time or, with one block, buffer j % 2 for
-        // the j / 2-th.
-        auto buf = [&](int q, int j) -> int { return NQ == 2 ? q : j & 1; };
-        auto use = [&](int j) -> uint32_t { return NQ == 2 ? uint32_t(j) : uint32_t(j >> 1); };
-        // S of (q, j), once P V of the buffer's previous use has read its P
-        auto issue_s = [&](int q, int j) {
-          const int s = j & 1, sb = buf(q, j);
-          if (q == 0 || j >= tiles[0])  // else the first block has waited for this K tile
-            ok = ok && lane_wait(bar(Bars::K_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns);
-          if (use(j) > 0) ok = ok && lane_wait(bar(Bars::O_DONE + sb), (use(j) - 1) & 1u, p.wait_ns);
-          __syncwarp();
-          tc::fence_after_sync();
-          const uint64_t a0 = q_desc + uint64_t((q * C::Q_BYTES) >> 4), b0 = k_desc + uint64_t((s * C::KV_BYTES) >> 4);
-          const bool frees = q == NQ - 1 || j >= tiles[NQ - 1];  // the last block that uses this K tile
-          if (elect_one()) {
-#pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks)
-              tc::mma_f16_ss(tmem + uint32_t(sb * KT), a0 + uint64_t(((ks >> 2) * (ROWS * 128) + (ks & 3) * 32) >> 4),
-                             b0 + uint64_t((uint32_t(ks >> 2) * pstride + uint32_t((ks & 3) * 32)) >> 4), IDESC_S, ks > 0);
-            tc::commit(bar(Bars::S_FULL + sb));
-            if (frees) tc::commit(bar(Bars::K_EMPTY + s));
-          }
-          __syncwarp();
-        };
-        // Zeros in the V of tile j's copied keys that no row of the CTA sees.
-        auto clear_v = [&](int j, int s) {
-          const int u0 = j * KT;
-          auto clear = [&](int lo, int hi) {  // fewer than two copies' tokens
-            lo = max(lo, u0) - u0;
-            hi = min(hi, u0 + KT) - u0;
-            if (lo >= hi) return;
-            for (int i = lane; i < (hi - lo) * (D / 8); i += 32) {
-              const int r = lo + i / (D / 8), u = i % (D / 8);
-              sts128(v_addr(s) + uint32_t(r >> 3) * gstride + uint32_t((r & 7) * 128) + uint32_t(u >> 3) * pstride +
-                         uint32_t((u & 7) << 4),
-                     0u, 0u, 0u, 0u);
-            }
-            fence_proxy_async_smem();
-          };
-          clear(blind0, blind1);
-          clear(keys.count, (keys.count + box - 1) >> p.log2_box << p.log2_box);
-          __syncwarp();
-        };
-        auto issue_pv = [&](int q, int j) {
-          const int s = j & 1, sb = buf(q, j);
-          if (q == 0 || j >= tiles[0]) {
-            ok = ok && lane_wait(bar(Bars::V_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns);
-            __syncwarp();
-            if (__all_sync(FULL_MASK, ok)) clear_v(j, s);
-          }
-          const uint64_t b0 = v_desc + uint64_t((s * C::KV_BYTES) >> 4);
-          const bool frees = q == NQ - 1 || j >= tiles[NQ - 1];
-          auto part = [&](int k0, int k1) {
-#pragma unroll
-            for (int kk = k0; kk < k1; ++kk)
-#pragma unroll
-              for (int i = 0; i < 2; ++i)  // hi in the upper half of the buffer's columns, lo in the lower
-                tc::mma_f16_ts(tmem + uint32_t(C::O_COL + q * D), tmem + uint32_t(sb * KT + (1 - i) * (KT / 2) + kk * 8),
-                               b0 + uint64_t((uint32_t(kk) * 2u * gstride) >> 4), IDESC_PV, j > 0 || kk > 0 || i > 0);
-          };
-          // the first PART keys while the softmax is at the others
-          ok = ok && lane_wait(bar(Bars::P_PART + sb), use(j) & 1u, p.wait_ns);
-          __syncwarp();
-          tc::fence_after_sync();
-          if (elect_one()) part(0, C::PART / 16);
-          __syncwarp();
-          ok = ok && lane_wait(bar(Bars::P_FULL + sb), use(j) & 1u, p.wait_ns);
-          __syncwarp();
-          tc::fence_after_sync();
-          if (elect_one()) {
-            part(C::PART / 16, KT / 16);
-            tc::commit(bar(Bars::O_DONE + sb));
-            if (frees) tc::commit(bar(Bars::V_EMPTY + s));
-          }
-          __syncwarp();
-        };
-        if (__all_sync(FULL_MASK, ok)) {
-#pragma unroll
-          for (int q = 0; q < NQ; ++q)
-            if (tiles[q] > 0) issue_s(q, 0);
-        }
-        for (int j = 0; j < most; ++j) {
+        for (int u = 0; u < all_steps; ++u) {
           if (!__all_sync(FULL_MASK, ok && *abort_flag == 0)) break;
-          if (NQ == 1 && j + 1 < most) issue_s(0, j + 1);
+          const int j = u / C::STEPS, s = j & 1, part = u % C::STEPS;
+          if (part == 0) ok = ok && lane_wait(bar(Bars::K_FULL + s), uint32_t((j >> 1) & 1), p.wait_ns);
+          const uint64_t b0 = k_desc + uint64_t((s * C::KV_BYTES) >> 4) + uint64_t((uint32_t(part * (KEYS / 8)) * gstride) >> 4);
+          const bool last = part == C::STEPS - 1 || u == all_steps - 1;  // of the tile
 #pragma unroll
           for (int q = 0; q < NQ; ++q) {
-            if (j < tiles[q]) issue_pv(q, j);
-            if (NQ == 2 && j + 1 < tiles[q]) issue_s(q, j + 1);
+            if (u >= steps[q]) continue;
+            const int sb = 2 * q + (u & 1);
+            // once P V of the buffer's previous use has read its P
+            if (u > 1) ok = ok && lane_wait(bar(Bars::O_DONE + sb), uint32_t(((u >> 1) - 1) & 1), p.wait_ns);
+            __syncwarp();
+            tc::fence_after_sync();
+            const bool frees = last && (q == NQ - 1 || u >= steps[NQ - 1]);  // the last S of this K tile
+            if (elect_one()) {
+#pragma unroll
+              for (int ks = 0; ks < D / 16; ++ks)
+                tc::mma_f16_ss(tmem + uint32_t(sb * KEYS),
+                               q_desc + uint64_t((q * C::Q_BYTES + (ks >> 2) * (ROWS * 128) + (ks & 3) * 32) >> 4),
+                               b0 + uint64_t((uint32_t(ks >> 2) * pstride + uint32_t((ks & 3) * 32)) >> 4), IDESC_S, ks > 0);
+              tc::commit(bar(Bars::S_FULL + sb));
+              if (frees) tc::commit(bar(Bars::K_EMPTY + s));
+            }
+            __syncwarp();
           }
         }
         if (!__all_sync(FULL_MASK, ok) && lane == 0) fail();
@@ -378,7 +348,47 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
         warp_wait_phase(bar(Bars::DRAIN), 0u, DRAIN_LIMIT_NS);
       }
     } else {
+      // ---------------------------------------------------------------- O += P V
       tmem = meet();
+      if (most > 0) {
+        constexpr uint32_t IDESC_PV = tc::instr_desc_f16(BF16, ROWS, D, false, true);
+        const uint64_t v_desc = tc::smem_desc(v_addr(0), pstride, gstride);
+        bool ok = true;
+        for (int u = 0; u < all_steps; ++u) {
+          if (!__all_sync(FULL_MASK, ok && *abort_flag == 0)) break;
+          const int j = u / C::STEPS, s = j & 1, part = u % C::STEPS;
+          const uint32_t landed = uint32_t((j >> 1) & 1);
+          if (part == 0)
+            ok = ok && lane_wait(bar(Bars::V_FULL + s), landed, p.wait_ns) &&
+                 lane_wait(bar(Bars::V_READY + s), landed, p.wait_ns);
+          const uint64_t b0 = v_desc + uint64_t((s * C::KV_BYTES) >> 4) + uint64_t((uint32_t(part * (KEYS / 8)) * gstride) >> 4);
+          const bool last = part == C::STEPS - 1 || u == all_steps - 1;
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            if (u >= steps[q]) continue;
+            const int sb = 2 * q + (u & 1);
+            const bool frees = last && (q == NQ - 1 || u >= steps[NQ - 1]);
+            ok = ok && lane_wait(bar(Bars::P_FULL + sb), uint32_t((u >> 1) & 1), p.wait_ns);
+            __syncwarp();
+            tc::fence_after_sync();
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < KEYS / 16; ++kk)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)  // hi in the upper half of the buffer's columns, lo in the lower
+                  tc::mma_f16_ts(tmem + uint32_t(C::O_COL + q * D), tmem + uint32_t(sb * KEYS + (1 - i) * (KEYS / 2) + kk * 8),
+                                 b0 + uint64_t((uint32_t(kk) * 2u * gstride) >> 4), IDESC_PV, u > 0 || kk > 0 || i > 0);
+              tc::commit(bar(Bars::O_DONE + sb));
+              if (frees) tc::commit(bar(Bars::V_EMPTY + s));
+            }
+            __syncwarp();
+          }
+        }
+        if (!__all_sync(FULL_MASK, ok) && lane == 0) fail();
+        if (elect_one()) tc::commit(bar(Bars::DRAIN + 1));
+        __syncwarp();
+        warp_wait_phase(bar(Bars::DRAIN + 1), 0u, DRAIN_LIMIT_NS);
+      }
     }
   } else {
     // ---------------------------------------------------------------- softmax warps
@@ -434,31 +444,29 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
     const uint32_t o_tmem = lane_base + uint32_t(C::O_COL + q * D);
     float m_run = -3.0e38f, l_run = 0.f;
     bool ok = true;
-    int mine = tiles[0];
-#pragma unroll
-    for (int i = 1; i < NQ; ++i) mine = q == i ? tiles[i] : mine;
+    const int mine = q == 0 ? steps[0] : steps[NQ - 1];
     for (int j = 0; j < mine; ++j) {
-      const int sb = NQ == 2 ? q : j & 1;
-      const uint32_t ph = (NQ == 2 ? uint32_t(j) : uint32_t(j >> 1)) & 1u;
+      const int sb = 2 * q + (j & 1);
+      const uint32_t ph = uint32_t(j >> 1) & 1u;
       if (__any_sync(FULL_MASK, *abort_flag != 0) || !warp_wait_phase(bar(Bars::S_FULL + sb), ph, p.wait_ns)) {
         ok = false;
         break;
       }
       tc::fence_after_sync();
-      const uint32_t s_tmem = lane_base + uint32_t(sb * KT);
-      // no key of the tile is hidden from a row of the warp
-      const int u0 = j * KT;
-      const bool open = __all_sync(FULL_MASK, u0 + KT - 1 <= last_key && (u0 >= first_key || u0 + KT <= own_sinks));
+      const uint32_t s_tmem = lane_base + uint32_t(sb * KEYS);
+      // no key of the step is hidden from a row of the warp
+      const int u0 = j * KEYS;
+      const bool open = __all_sync(FULL_MASK, u0 + KEYS - 1 <= last_key && (u0 >= first_key || u0 + KEYS <= own_sinks));
       // The row's scores stay in registers from the maximum to P, which is stored over the upper half of
       // their columns, its second part over the lower.
-      float x[KT];
+      float x[KEYS];
 #pragma unroll
-      for (int c = 0; c < KT; c += 32)
+      for (int c = 0; c < KEYS; c += 32)
         tc::ld_32x32b_x32(s_tmem + uint32_t(c), *reinterpret_cast<uint32_t(*)[32]>(x + c));
       tc::wait_ld();
       if (!open) {
 #pragma unroll
-        for (int c = 0; c < KT; c += 32) {
+        for (int c = 0; c < KEYS; c += 32) {
           const int v0 = u0 + c;
           const uint32_t mask = bits(first_key - v0, last_key + 1 - v0) | bits(0, own_sinks - v0);
           if (__all_sync(FULL_MASK, mask == 0xffffffffu)) continue;
@@ -468,9 +476,9 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
       }
       float t[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-      for (int i = 4; i < KT; i += 8) {
+      for (int i = 4; i < KEYS; i += 8) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) t[k] = fmaxf(fmaxf(t[k], x[i + k]), i + 4 + k < KT ? x[i + 4 + k] : t[k]);
+        for (int k = 0; k < 4; ++k) t[k] = fmaxf(fmaxf(t[k], x[i + k]), i + 4 + k < KEYS ? x[i + 4 + k] : t[k]);
       }
       const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
       // mul >= 0: the maximum of the products is the product of the maximum
@@ -481,10 +489,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
         const float alpha = move ? ex2(m_run - ref) : 1.f;
         if (move) m_run = ref;
         l_run *= alpha;
-        if (j > 0) {  // O *= alpha once P V of tile j - 1 has landed
-          const int pb = NQ == 2 ? q : (j - 1) & 1;
-          const uint32_t pp = (NQ == 2 ? uint32_t(j - 1) : uint32_t((j - 1) >> 1)) & 1u;
-          if (!warp_wait_phase(bar(Bars::O_DONE + pb), pp, p.wait_ns)) {
+        if (j > 0) {  // O *= alpha once P V of step j - 1 has landed
+          if (!warp_wait_phase(bar(Bars::O_DONE + 2 * q + ((j - 1) & 1)), uint32_t((j - 1) >> 1) & 1u, p.wait_ns)) {
             ok = false;
             break;
           }
@@ -503,7 +509,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
       const float2 mul2 = make_float2(mul, mul), neg_m2 = make_float2(-m_run, -m_run);
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < KT; c += 32) {  // two keys to a column
+      for (int c = 0; c < KEYS; c += 32) {  // two keys to a column
         uint32_t w[16], rest[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
@@ -516,14 +522,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
           E::unpack2(w[i >> 1], f);
           rest[i >> 1] = E::pack2(e.x - f[0], e.y - f[1]);
         }
-        st_32x32b_x16(s_tmem + uint32_t(KT / 2 + c / 2), w);
+        st_32x32b_x16(s_tmem + uint32_t(KEYS / 2 + c / 2), w);
         st_32x32b_x16(s_tmem + uint32_t(c / 2), rest);
-        if (c + 32 == C::PART) {
-          tc::wait_st();
-          tc::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(Bars::P_PART + sb));
-        }
       }
       const float2 total = add2(sum[0], sum[1]);
       l_run += total.x + total.y;
@@ -533,9 +533,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
       if (lane == 0) mbar_arrive(bar(Bars::P_FULL + sb));
     }
     if (ok && mine > 0) {
-      const int lb = NQ == 2 ? q : (mine - 1) & 1;
-      const uint32_t lp = (NQ == 2 ? uint32_t(mine - 1) : uint32_t((mine - 1) >> 1)) & 1u;
-      ok = warp_wait_phase(bar(Bars::O_DONE + lb), lp, p.wait_ns);
+      ok = warp_wait_phase(bar(Bars::O_DONE + 2 * q + ((mine - 1) & 1)), uint32_t((mine - 1) >> 1) & 1u, p.wait_ns);
     }
     if (!ok) {
       if (lane == 0) fail();
@@ -591,7 +589,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
 
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == C::MMA_WARP) {
+  if (warp == C::S_WARP) {
     __syncwarp();
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, C::TMEM_COLS);
