@@ -969,6 +969,7 @@ int pd_prefill_window(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh
   p.log2_box = ilog2_host(box_tokens);
   p.window = std::min(window, 1 << 30);  // no row is longer
   p.sinks = std::min(sinks, 1 << 30);
+  p.sms = sm_count(dev);
   p.scale_log2 = scale_log2;
   p.wait_ns = g_wait_limit_ns.load(std::memory_order_relaxed);
   const cudaError_t e = launch_window_prefill(p, kmap, vmap, dtype, head_dim, static_cast<cudaStream_t>(stream));

@@ -21,6 +21,7 @@ struct WindowPrefillParams {
   int32_t log2_bs, log2_box;  // tokens of a block, and of a copy (window_box_tokens)
   int32_t window, sinks;
   int32_t grouped;  // pool maps: a copy is 8-token groups of all pieces, or one piece
+  int32_t sms;
   float scale_log2;
   unsigned* err;
   unsigned long long wait_ns;
