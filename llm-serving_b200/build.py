@@ -54,6 +54,8 @@ SOURCES = [
     "pd_decode_var_mma_bf16.cu",
     "pd_decode_var_mma_f16.cu",
     "pd_weights.cu",
+    "pd_decode_cluster_bf16.cu",
+    "pd_decode_cluster_f16.cu",
     "pd_prefill.cu",
     "pd_prefill_tc.cu",
     "pd_ops_api.cu",

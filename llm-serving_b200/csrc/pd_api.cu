@@ -581,6 +581,34 @@ int run_prepared(const Prepared& P, const CUtensorMap& kmap, const CUtensorMap& 
   return PD_OK;
 }
 
+// Whether a windowed or weights call takes the kernel of few rows, and how: every item's CTAs have to be on the GPU
+// at once (one to an SM), and a warp's run of tiles has to be short, as only the items' clusters stream. Measured in
+// DESIGN's table; `max_tiles` bounds a row's visible tiles (the lengths are on the device).
+bool use_cluster(const Prepared& P, int batch, int sms, float* weights, ClusterDecode* c, int* stages) {
+  const Geometry& g = P.g;
+  if (!g.mma || g.variant == PLAIN || batch > P.L.rows_per_launch) return false;
+  if (weights != nullptr && g.n_gchunks != 1) return false;
+  const int64_t items = int64_t(batch) * P.base.n_kv_head * g.n_gchunks;
+  if (items > sms) return false;
+  int64_t keys = P.base.capacity;
+  if (g.variant == WINDOW) keys = std::min(keys, int64_t(P.base.window) + P.base.sinks + 2 * g.tile);
+  const int64_t max_tiles = (keys + g.tile - 1) / g.tile;
+  int log2_split = 0;
+  while (log2_split < 3 && (items << (log2_split + 1)) <= sms && max_tiles > (int64_t(8) << log2_split)) ++log2_split;
+  const int64_t run = (max_tiles + (int64_t(8) << log2_split) - 1) / (int64_t(8) << log2_split);  // tiles of a warp
+  if (run > 32) return false;
+  c->log2_split = log2_split;
+  c->scores_bytes = 0;
+  *stages = 3;
+  if (weights != nullptr) {
+    const int64_t bytes = 8 * run * g.tile * g.gt * 4;
+    if (bytes > 65536) return false;
+    c->scores_bytes = int32_t(bytes);
+    *stages = 2;
+  }
+  return true;
+}
+
 int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache, const void* v_cache,
                   int64_t n_blocks, int32_t block_size, const int64_t* k_strides,
                   const int64_t* v_strides, const int32_t* block_table, int64_t bt_stride,
@@ -588,7 +616,7 @@ int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache
                   float* pm, float* pl, float* pacc, int mode, int32_t batch, int32_t n_head,
                   int32_t n_kv_head, int32_t head_dim, int32_t dtype, float scale_log2,
                   void* workspace, size_t workspace_bytes, void* stream, Variant variant = PLAIN, int32_t window = 0,
-                  int32_t sinks = 0, float* scores = nullptr) {
+                  int32_t sinks = 0, float* scores = nullptr, ClusterDecode* cluster = nullptr, bool* done = nullptr) {
   if (k_strides == nullptr || v_strides == nullptr) return PD_ERR_INVALID;
   Prepared P;
   int st = prepare(&P, n_blocks, block_size, block_table, bt_stride, max_blocks, seqlen, batch,
@@ -606,6 +634,28 @@ int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache
   st = encode_pool(&vmap, v_cache, n_blocks, block_size, n_kv_head, head_dim, v_strides, dtype,
                    P.g.box_tokens, P.g.box_heads, P.g.mma);
   if (st != PD_OK) return st;
+  int dev = 0, stages = 0;
+  if (current_device(&dev) != PD_OK) return PD_ERR_CUDA;
+  ClusterDecode c = cluster != nullptr ? *cluster : ClusterDecode{};
+  if (variant != PLAIN && use_cluster(P, batch, sm_count(dev), c.weights, &c, &stages)) {
+    DecodeParams p = P.base;
+    p.q = q;
+    p.q_sb = q_sb;
+    p.q_sh = q_sh;
+    p.out = out;
+    p.o_sb = o_sb;
+    p.o_sh = o_sh;
+    p.stages = stages;
+    p.wait_ns = g_wait_limit_ns.load(std::memory_order_relaxed);
+    const ClusterLaunchFn fn = dtype == PD_BF16 ? cluster_launcher_bf16(c.weights != nullptr, P.g.d_index, P.g.gt_index)
+                                                : cluster_launcher_f16(c.weights != nullptr, P.g.d_index, P.g.gt_index);
+    const cudaError_t e =
+        fn(p, c, kmap, vmap, batch * n_kv_head * P.g.n_gchunks, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "decode launch");
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    if (done != nullptr) *done = true;
+    return PD_OK;
+  }
   return run_prepared(P, kmap, vmap, q, q_sb, q_sh, out, o_sb, o_sh, pm, pl, pacc, mode, dtype,
                       static_cast<cudaStream_t>(stream), nullptr, false, nullptr, scores);
 }
@@ -808,11 +858,16 @@ int pd_decode_weights(const void* q, int64_t q_sb, int64_t q_sh, const void* k_c
   float* l = m == nullptr ? nullptr : m + int64_t(batch) * n_head;
   float* scores =
       m == nullptr ? nullptr : reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + round_up(size_t(batch) * n_head * 8, 256));
+  ClusterDecode c{};
+  c.weights = weights;
+  c.w_sb = w_sb;
+  c.w_sh = w_sh;
+  bool done = false;  // by the kernel of few rows, weights and all
   const int st = decode_common(q, q_sb, q_sh, k_cache, v_cache, n_blocks, block_size, k_strides, v_strides, block_table,
                                bt_stride, max_blocks, seqlen, out, o_sb, o_sh, m, l, nullptr, 0, batch, n_head,
                                n_kv_head, head_dim, dtype, scale_log2, workspace, workspace_bytes, stream, SCORES, 0, 0,
-                               scores);
-  if (st != PD_OK || batch == 0 || max_blocks == 0) return st;
+                               scores, &c, &done);
+  if (st != PD_OK || done || batch == 0 || max_blocks == 0) return st;
   int dev = 0;
   if (current_device(&dev) != PD_OK) return PD_ERR_CUDA;
   WeightsParams p{};

@@ -257,6 +257,33 @@ __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
+// ------------------------------------------------------------------ clusters
+// Every thread of the cluster's CTAs meets; shared memory written before is visible to all after.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of another CTA of the cluster's shared memory.
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_v2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 // ------------------------------------------------------------------ element conversion
 // A "chunk" is 16 bytes of one row: 8 bf16/fp16 or 4 fp32 elements.
 
@@ -473,6 +500,14 @@ struct DecodeParams {
   float* scores;
 };
 
+// What the decode of few rows (pd_decode_cluster.cuh) takes beside DecodeParams.
+struct ClusterDecode {
+  int32_t log2_split;    // CTAs of an item's cluster
+  int32_t scores_bytes;  // shared memory for the scores of a CTA's warps (weights)
+  float* weights;        // row b, kv head h, token j at b * w_sb + h * w_sh + j
+  int64_t w_sb, w_sh;
+};
+
 struct WeightsParams {
   const float* scores;    // (B, H_kv, capacity, group) in log2 units
   const float *m, *l;     // (B, H)
@@ -554,6 +589,8 @@ struct MergeParams {
 
 // Host-side launcher signatures (one instantiation per dtype / head_dim / group tile).
 // pdl: launch with programmatic stream serialisation (may overlap the previous kernel).
+typedef cudaError_t (*ClusterLaunchFn)(const DecodeParams&, const ClusterDecode&, const CUtensorMap&, const CUtensorMap&,
+                                       int items, cudaStream_t);
 typedef cudaError_t (*DecodeLaunchFn)(const DecodeParams&, const CUtensorMap&, const CUtensorMap&,
                                       dim3, dim3, size_t, cudaStream_t, bool pdl);
 

@@ -52,6 +52,7 @@
 
 #include "pd_common.cuh"
 #include "pd_decode_mma.cuh"
+#include "pd_smem_limit.cuh"
 
 namespace pd {
 
@@ -555,8 +556,14 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
   const int rc = colmode ? p.row_cost : 0;
   auto vpre = [&](int b) -> int64_t { return int64_t(pre[b]) + int64_t(rc) * b; };
   const int64_t vcols = colmode ? vpre(B) : 0;
-  // Ranges in use: never more than virtual columns, so that no range is empty.
-  const int col_parts = int(vcols < int64_t(gridDim.x) ? vcols : int64_t(gridDim.x));
+  // Ranges in use: never more than virtual columns, so that no range is empty. The variants also weigh a range's
+  // columns against the merge of a row's pieces, eight to a round trip: columns / parts + parts / rows / 5 is least
+  // at parts = sqrt(5 columns rows) (one row of 4096 tokens: 148 parts 36.0 us).
+  int col_parts = int(vcols < int64_t(gridDim.x) ? vcols : int64_t(gridDim.x));
+  if constexpr (VAR != 0) {
+    const int best = int(sqrtf(5.f * float(ncols) * float(B))) + 1;
+    if (best < col_parts) col_parts = best;
+  }
   // Real column at virtual column v (0 <= v <= vcols); a row's extra columns map to its first tile.
   auto real_col = [&](int64_t v) -> int64_t {
     if (v >= vcols) return ncols;

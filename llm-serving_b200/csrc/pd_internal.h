@@ -23,6 +23,10 @@ DecodeLaunchFn decode_launcher_var_f32(int d_index, int gt_index);
 DecodeLaunchFn decode_launcher_var_f16(int d_index, int gt_index);
 DecodeLaunchFn decode_launcher_var_bf16(int d_index, int gt_index);
 
+// The same for few rows, all of whose CTAs run at once (pd_decode_cluster.cuh).
+ClusterLaunchFn cluster_launcher_f16(bool weights, int d_index, int gt_index);
+ClusterLaunchFn cluster_launcher_bf16(bool weights, int d_index, int gt_index);
+
 // weights[b][h][j] += the sum over the group of exp2(score - m) / l (pd_weights.cu).
 cudaError_t launch_weights(const WeightsParams& p, cudaStream_t stream);
 
