@@ -393,6 +393,11 @@ int pd_fp4_prefill(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, c
 size_t pd_decode_window_workspace_bytes(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim,
                                         int32_t dtype);
 
+/* 1 if a call of these sizes needs neither workspace nor scratch (both may then be NULL): few rows, one launch.
+ * window 0 asks for pd_decode_weights. */
+int32_t pd_decode_window_small(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype,
+                               int32_t block_size, int32_t max_blocks, int32_t window, int32_t sinks);
+
 /* pd_decode where row b's query sits at position seqlen[b] - 1 and sees its window. */
 int pd_decode_window(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache, const void* v_cache,
                      int64_t n_blocks, int32_t block_size, const int64_t* k_strides, const int64_t* v_strides,

@@ -382,7 +382,7 @@ int prepare(Prepared* P, int64_t n_blocks, int32_t block_size, const int32_t* bl
             int64_t bt_stride, int32_t max_blocks, const int32_t* seqlen, int32_t batch,
             int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype, float scale_log2,
             void* workspace, size_t workspace_bytes, Variant variant = PLAIN, int32_t window = 0,
-            int32_t sinks = 0) {
+            int32_t sinks = 0, bool needs_workspace = true) {
   if (batch < 0 || max_blocks < 0 || n_blocks < 1) return PD_ERR_INVALID;
   if (variant == WINDOW && (window < 1 || sinks < 0)) return PD_ERR_INVALID;
   int st = geometry(n_head, n_kv_head, head_dim, block_size, dtype, variant, &P->g);
@@ -395,7 +395,7 @@ int prepare(Prepared* P, int64_t n_blocks, int32_t block_size, const int32_t* bl
   if (st != PD_OK) return st;
   P->ws = workspace_layout(batch, n_kv_head, P->g, head_dim, P->L);
   if (batch > 0) {
-    if (workspace == nullptr || workspace_bytes < P->ws.total) {
+    if (needs_workspace && (workspace == nullptr || workspace_bytes < P->ws.total)) {
       g_last_ws_need = P->ws.total;
       snprintf(g_last_error, sizeof(g_last_error),
                "workspace of %zu bytes is smaller than the %zu bytes this shape needs", workspace_bytes,
@@ -404,7 +404,7 @@ int prepare(Prepared* P, int64_t n_blocks, int32_t block_size, const int32_t* bl
     }
     P->half_bytes = round_up(P->ws.total, 256);
     P->halves = workspace_bytes >= 2 * P->half_bytes ? 2 : 1;
-    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) {
+    if (needs_workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) {
       snprintf(g_last_error, sizeof(g_last_error), "workspace is not 256-byte aligned");
       return PD_ERR_WORKSPACE;
     }
@@ -574,39 +574,64 @@ int run_prepared(const Prepared& P, const CUtensorMap& kmap, const CUtensorMap& 
     }
     const size_t smem = smem_for(P.g.cta, P.L.warps, P.L.stages, rows, P.g.stage_bytes, &p.smem_arrays_off,
                                  &p.smem_stage_off);
-    cudaError_t e = P.fn(p, kmap, vmap, dim3(P.L.grid), dim3(P.L.warps * 32), smem, stream, overlap);
+    // A variant's call on its own waits for the kernel before it inside (wait_first), so it may be launched early.
+    p.wait_first = P.g.variant != PLAIN && seq == nullptr;
+    cudaError_t e =
+        P.fn(p, kmap, vmap, dim3(P.L.grid), dim3(P.L.warps * 32), smem, stream, overlap || p.wait_first != 0);
     if (e != cudaSuccess) return cuda_fail(e, "decode launch");
     g_launches.fetch_add(1, std::memory_order_relaxed);
   }
   return PD_OK;
 }
 
+// cluster_room of a device, asked once.
+int cluster_rooms(int dev, int log2_split) {
+  static std::atomic<int> known[kMaxDevices][4];  // + 1
+  std::atomic<int>& room = known[dev][log2_split];
+  int n = room.load(std::memory_order_relaxed);
+  if (n == 0) {
+    n = cluster_room(log2_split) + 1;
+    room.store(n, std::memory_order_relaxed);
+  }
+  return n - 1;
+}
+
 // Whether a windowed or weights call takes the kernel of few rows, and how: every item's CTAs have to be on the GPU
 // at once (one to an SM), and a warp's run of tiles has to be short, as only the items' clusters stream. Measured in
 // DESIGN's table; `max_tiles` bounds a row's visible tiles (the lengths are on the device).
-bool use_cluster(const Prepared& P, int batch, int sms, float* weights, ClusterDecode* c, int* stages) {
-  const Geometry& g = P.g;
-  if (!g.mma || g.variant == PLAIN || batch > P.L.rows_per_launch) return false;
-  if (weights != nullptr && g.n_gchunks != 1) return false;
-  const int64_t items = int64_t(batch) * P.base.n_kv_head * g.n_gchunks;
-  if (items > sms) return false;
-  int64_t keys = P.base.capacity;
-  if (g.variant == WINDOW) keys = std::min(keys, int64_t(P.base.window) + P.base.sinks + 2 * g.tile);
+bool use_cluster(const Geometry& g, int64_t batch, int n_kv_head, int64_t capacity, int window, int sinks, int dev,
+                 ClusterDecode* c, int* stages) {
+  const bool weights = g.variant == SCORES;
+  if (!g.mma || g.variant == PLAIN || (weights && g.n_gchunks != 1)) return false;
+  const int64_t items = batch * n_kv_head * g.n_gchunks;
+  if (items < 1 || items > sm_count(dev)) return false;
+  int64_t keys = capacity;
+  if (g.variant == WINDOW) keys = std::min(keys, int64_t(window) + sinks + 2 * g.tile);
   const int64_t max_tiles = (keys + g.tile - 1) / g.tile;
   int log2_split = 0;
-  while (log2_split < 3 && (items << (log2_split + 1)) <= sms && max_tiles > (int64_t(8) << log2_split)) ++log2_split;
+  while (log2_split < 3 && items <= cluster_rooms(dev, log2_split + 1) && max_tiles > (int64_t(8) << log2_split)) ++log2_split;
   const int64_t run = (max_tiles + (int64_t(8) << log2_split) - 1) / (int64_t(8) << log2_split);  // tiles of a warp
   if (run > 32) return false;
   c->log2_split = log2_split;
   c->scores_bytes = 0;
   *stages = 3;
-  if (weights != nullptr) {
+  if (weights) {
     const int64_t bytes = 8 * run * g.tile * g.gt * 4;
     if (bytes > 65536) return false;
     c->scores_bytes = int32_t(bytes);
     *stages = 2;
   }
   return true;
+}
+
+bool is_small(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype, int32_t block_size,
+              int32_t max_blocks, Variant variant, int32_t window, int32_t sinks, ClusterDecode* c, int* stages) {
+  Geometry g;
+  int dev = 0;
+  if (batch < 1 || max_blocks < 1 || window < (variant == WINDOW ? 1 : 0) || sinks < 0) return false;
+  if (geometry(n_head, n_kv_head, head_dim, block_size, dtype, variant, &g) != PD_OK || current_device(&dev) != PD_OK)
+    return false;
+  return use_cluster(g, batch, n_kv_head, int64_t(max_blocks) * block_size, window, sinks, dev, c, stages);
 }
 
 int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache, const void* v_cache,
@@ -619,8 +644,14 @@ int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache
                   int32_t sinks = 0, float* scores = nullptr, ClusterDecode* cluster = nullptr, bool* done = nullptr) {
   if (k_strides == nullptr || v_strides == nullptr) return PD_ERR_INVALID;
   Prepared P;
-  int st = prepare(&P, n_blocks, block_size, block_table, bt_stride, max_blocks, seqlen, batch,
-                   n_head, n_kv_head, head_dim, dtype, scale_log2, workspace, workspace_bytes, variant, window, sinks);
+  ClusterDecode c = cluster != nullptr ? *cluster : ClusterDecode{};
+  int stages = 0;
+  bool small = false;
+  if (variant != PLAIN && is_small(batch, n_head, n_kv_head, head_dim, dtype, block_size, max_blocks, variant, window, sinks,
+                                   &c, &stages))
+    small = true;
+  int st = prepare(&P, n_blocks, block_size, block_table, bt_stride, max_blocks, seqlen, batch, n_head, n_kv_head, head_dim,
+                   dtype, scale_log2, workspace, workspace_bytes, variant, window, sinks, !small);
   if (st != PD_OK) return st;
   if (batch == 0) return PD_OK;
   if (check_rows(q, q_sb, q_sh, dtype) != PD_OK) return PD_ERR_INVALID;
@@ -634,10 +665,7 @@ int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache
   st = encode_pool(&vmap, v_cache, n_blocks, block_size, n_kv_head, head_dim, v_strides, dtype,
                    P.g.box_tokens, P.g.box_heads, P.g.mma);
   if (st != PD_OK) return st;
-  int dev = 0, stages = 0;
-  if (current_device(&dev) != PD_OK) return PD_ERR_CUDA;
-  ClusterDecode c = cluster != nullptr ? *cluster : ClusterDecode{};
-  if (variant != PLAIN && use_cluster(P, batch, sm_count(dev), c.weights, &c, &stages)) {
+  if (small) {
     DecodeParams p = P.base;
     p.q = q;
     p.q_sb = q_sb;
@@ -647,8 +675,9 @@ int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache
     p.o_sh = o_sh;
     p.stages = stages;
     p.wait_ns = g_wait_limit_ns.load(std::memory_order_relaxed);
-    const ClusterLaunchFn fn = dtype == PD_BF16 ? cluster_launcher_bf16(c.weights != nullptr, P.g.d_index, P.g.gt_index)
-                                                : cluster_launcher_f16(c.weights != nullptr, P.g.d_index, P.g.gt_index);
+    const bool weights = variant == SCORES;
+    const ClusterLaunchFn fn = dtype == PD_BF16 ? cluster_launcher_bf16(weights, P.g.d_index, P.g.gt_index)
+                                                : cluster_launcher_f16(weights, P.g.d_index, P.g.gt_index);
     const cudaError_t e =
         fn(p, c, kmap, vmap, batch * n_kv_head * P.g.n_gchunks, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(e, "decode launch");
@@ -804,6 +833,14 @@ size_t pd_decode_workspace_bytes(int32_t batch, int32_t n_head, int32_t n_kv_hea
   return workspace_bytes(batch, n_head, n_kv_head, head_dim, dtype, PLAIN);
 }
 
+int32_t pd_decode_window_small(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype,
+                               int32_t block_size, int32_t max_blocks, int32_t window, int32_t sinks) {
+  ClusterDecode c;
+  int stages;
+  return is_small(batch, n_head, n_kv_head, head_dim, dtype, block_size, max_blocks, window > 0 ? WINDOW : SCORES, window,
+                  sinks, &c, &stages);
+}
+
 size_t pd_decode_window_workspace_bytes(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim,
                                         int32_t dtype) {
   return workspace_bytes(batch, n_head, n_kv_head, head_dim, dtype, WINDOW);
@@ -850,8 +887,9 @@ int pd_decode_weights(const void* q, int64_t q_sb, int64_t q_sh, const void* k_c
   if (n_kv_head > 65535) return PD_ERR_UNSUPPORTED;  // a grid's second dimension
   if (batch > 0 && max_blocks > 0) {
     if (weights == nullptr) return PD_ERR_INVALID;
-    if (scratch == nullptr || !aligned16(scratch) ||
-        scratch_bytes < pd_decode_weights_scratch_bytes(batch, n_head, max_blocks, block_size))
+    if ((scratch == nullptr || !aligned16(scratch) ||
+         scratch_bytes < pd_decode_weights_scratch_bytes(batch, n_head, max_blocks, block_size)) &&
+        !pd_decode_window_small(batch, n_head, n_kv_head, head_dim, dtype, block_size, max_blocks, 0, 0))
       return api_message(PD_ERR_WORKSPACE, "scratch is smaller than pd_decode_weights_scratch_bytes");
   }
   float* m = static_cast<float*>(scratch);

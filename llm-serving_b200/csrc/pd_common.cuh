@@ -498,6 +498,7 @@ struct DecodeParams {
   // Weights variant: scores (B, H_kv, capacity, group) in log2 units; with them part_m / part_l
   // (B, H) take the rows' maximum and normaliser although mode is 0.
   float* scores;
+  int32_t wait_first;  // variants: wait for the preceding kernel before anything is read (programmatic launch)
 };
 
 // What the decode of few rows (pd_decode_cluster.cuh) takes beside DecodeParams.

@@ -272,4 +272,27 @@ cudaError_t launch_cluster(const DecodeParams& p, const ClusterDecode& c, const 
   return cudaLaunchKernelEx(&cfg, fn, p, c, kmap, vmap);
 }
 
+// Clusters of 2^log2_split CTAs of this kernel that the current device runs at once (a cluster stays in one of its
+// groups of multiprocessors: of eight CTAs, 15 clusters on 148), 0 where it cannot be asked.
+template <typename T>
+int cluster_room_of(int log2_split) {
+  auto fn = pd_decode_cluster_kernel<T, 128, 2, false>;
+  constexpr int SMEM = MAX_DYNAMIC_SMEM - 16384;
+  static SmemRaised raised{};
+  if (raise_smem_limit(fn, SMEM, raised) != cudaSuccess) return 0;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1u << log2_split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(1u << log2_split);
+  cfg.blockDim = dim3(CLUSTER_WARPS * 32);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  return cudaOccupancyMaxActiveClusters(&n, fn, &cfg) == cudaSuccess ? n : 0;
+}
+
 }  // namespace pd

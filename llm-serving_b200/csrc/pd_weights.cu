@@ -21,7 +21,7 @@ constexpr int AHEAD = 4;  // tokens of a thread in flight
 template <int G>
 __global__ void __launch_bounds__(THREADS) pd_weights_kernel(const WeightsParams p) {
   const int h = blockIdx.y, b = blockIdx.z;
-  griddep_wait();
+  griddep_wait();  // (the next decode is not let in before this kernel is through: its CTAs would take the SMs)
   int len = __ldg(p.seqlen + b);
   len = len < 0 ? 0 : (len > p.capacity ? p.capacity : len);
   const int group = G ? G : p.group;

@@ -35,7 +35,7 @@ using at::Tensor;
 
 #define PD_ENTRIES(X) \
   X(pd_qk_norm_rope) X(pd_fp4_write_slots) X(pd_fp4_write_table) X(pd_fp4_read_slots) X(pd_fp4_workspace_bytes) \
-  X(pd_fp4_decode) X(pd_fp4_prefill) X(pd_block_copy) X(pd_decode_window_workspace_bytes) X(pd_decode_window) \
+  X(pd_fp4_decode) X(pd_fp4_prefill) X(pd_block_copy) X(pd_decode_window_workspace_bytes) X(pd_decode_window_small) X(pd_decode_window) \
   X(pd_prefill_window) \
   X(pd_decode_weights_scratch_bytes) X(pd_decode_weights) X(pd_evict_scratch_bytes) X(pd_evict)
 #define PD_FIELD(name) decltype(&::name) name = nullptr;
@@ -707,16 +707,22 @@ PyObject* decode_variant(PyObject* const* a, bool windowed) {
   const Tensor out = result_of(a[at + 1], q0);
   if (rows == 0) return THPVariable_Wrap(out);
   void* stream = stream_of(q0);
-  const int64_t need =
-      int64_t(lib.pd_decode_window_workspace_bytes(int(rows), int(heads), int(p.hkv), p.d, p.dtype));
+  const bool small = lib.pd_decode_window_small(int(rows), int(heads), int(p.hkv), p.d, p.dtype, p.block_size,
+                                                int(table.size(1)), int(window), int(sinks)) != 0;
+  const Tensor* w = optional(a[at + 2], "workspace");
+  const int64_t need = small && w == nullptr ? 0
+                                             : int64_t(lib.pd_decode_window_workspace_bytes(int(rows), int(heads),
+                                                                                            int(p.hkv), p.d, p.dtype));
   Tensor ws;
-  if (const Tensor* w = optional(a[at + 2], "workspace")) {
+  if (w != nullptr) {
     VALUE(w->scalar_type() == at::kByte && w->is_contiguous() && w->device() == q0.device() && w->numel() >= need,
           "workspace must be a contiguous uint8 tensor of at least ", need, " bytes on ", q0.device());
     ws = *w;
-  } else {
+  } else if (!small) {
     ws = decode_workspace(q0.device(), stream, need);
   }
+  void* const ws_ptr = ws.defined() ? ws.data_ptr() : nullptr;
+  const size_t ws_bytes = ws.defined() ? size_t(ws.numel()) : 0;
   const Tensor q = aligned_rows(q0);
   const Tensor lens = int32(seqlen);
   const int64_t bt_stride = std::max(table.stride(0), table.size(1));  // one row may have any stride
@@ -727,18 +733,20 @@ PyObject* decode_variant(PyObject* const* a, bool windowed) {
                                   p.n_blocks, p.block_size, p.ks, p.vs, table.const_data_ptr<int32_t>(), bt_stride,
                                   int(table.size(1)), lens.const_data_ptr<int32_t>(), int(window), int(sinks),
                                   out.data_ptr(), out.stride(0), out.stride(1), int(rows), int(heads), int(p.hkv), p.d,
-                                  p.dtype, scale_log2, ws.data_ptr(), size_t(ws.numel()), stream);
+                                  p.dtype, scale_log2, ws_ptr, ws_bytes, stream);
   } else {
-    const int64_t bytes =
-        int64_t(lib.pd_decode_weights_scratch_bytes(int(rows), int(heads), int(table.size(1)), p.block_size));
-    const Tensor scratch = at::detail::empty_cuda({bytes}, at::kByte, q0.device(), std::nullopt);
+    Tensor scratch;
+    if (!small)
+      scratch = at::detail::empty_cuda(
+          {int64_t(lib.pd_decode_weights_scratch_bytes(int(rows), int(heads), int(table.size(1)), p.block_size))}, at::kByte,
+          q0.device(), std::nullopt);
     status = lib.pd_decode_weights(q.const_data_ptr(), q.stride(0), q.stride(1), k.const_data_ptr(), v.const_data_ptr(),
                                    p.n_blocks, p.block_size, p.ks, p.vs, table.const_data_ptr<int32_t>(), bt_stride,
                                    int(table.size(1)), lens.const_data_ptr<int32_t>(), weights->data_ptr<float>(),
                                    weights->stride(0), weights->stride(1), weights->size(2), out.data_ptr(),
                                    out.stride(0), out.stride(1), int(rows), int(heads), int(p.hkv), p.d, p.dtype,
-                                   scale_log2, ws.data_ptr(), size_t(ws.numel()), scratch.data_ptr(),
-                                   size_t(scratch.numel()), stream);
+                                   scale_log2, ws_ptr, ws_bytes, small ? nullptr : scratch.data_ptr(),
+                                   small ? 0 : size_t(scratch.numel()), stream);
   }
   if (failed(status, windowed ? "pd_decode_window" : "pd_decode_weights")) return nullptr;
   return THPVariable_Wrap(out);

@@ -151,6 +151,7 @@ _SIGNATURES = {
         [ctypes.POINTER(_c_ptr), _c_i32, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i32, _c_i64, _c_ptr, _c_i64,
          _c_i64, _c_i64, _c_ptr, _c_ptr],
     ),
+    "pd_decode_window_small": (_c_i32, [_c_i32] * 9),
     "pd_decode_window_workspace_bytes": (_c_size, [_c_i32] * 5),
     "pd_decode_window": (
         ctypes.c_int,
