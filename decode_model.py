@@ -135,7 +135,7 @@ class PagedDecoder:
             return self._step_fp4()
         kv = self.kv
         B, H, HKV, D = kv.batch, self.h, self.hkv, self.d
-        pos = kv.pos  # the position this step's token is written at
+        pos = kv.position  # of this step's token in its sequence
         cos, sin = self.cos[pos], self.sin[pos]  # (B, R)
         half = self.rotary // 2
         rope_rows = (cos[:, :half].contiguous(), sin[:, :half].contiguous())

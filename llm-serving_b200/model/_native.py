@@ -292,8 +292,10 @@ def log2e_scale(scale: float) -> float:
     return float(scale) * 1.4426950408889634
 
 
-def workspace_bytes(batch: int, n_head: int, n_kv_head: int, head_dim: int, dtype: torch.dtype) -> int:
-    return int(require().pd_decode_workspace_bytes(batch, n_head, n_kv_head, head_dim, dtype_code(dtype)))
+def workspace_bytes(batch: int, n_head: int, n_kv_head: int, head_dim: int, dtype: torch.dtype, *,
+                    window: bool = False) -> int:
+    need = require().pd_decode_window_workspace_bytes if window else require().pd_decode_workspace_bytes
+    return int(need(batch, n_head, n_kv_head, head_dim, dtype_code(dtype)))
 
 
 def device_error(clear: bool = True) -> int:
@@ -474,7 +476,7 @@ class NativePlan:
     __slots__ = ("_handle", "_lib", "_overlap", "__weakref__")
 
     def __init__(self, k_caches, v_caches, block_table, seqlen, batch, n_head, scale_log2,
-                 workspace) -> None:
+                 workspace, window=None, sinks=0) -> None:
         lib_ = require()
         k0 = k_caches[0]
         n_blocks, bs, hkv, D = k0.shape
@@ -482,13 +484,13 @@ class NativePlan:
         kptrs = (_c_ptr * n)(*[t.data_ptr() for t in k_caches])
         vptrs = (_c_ptr * n)(*[t.data_ptr() for t in v_caches])
         handle = _c_ptr(0)
-        status = lib_.pd_plan_create(
-            ctypes.byref(handle), n, kptrs, vptrs, n_blocks, bs, strides3(k0), strides3(v_caches[0]),
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seqlen.data_ptr(),
-            batch, n_head, hkv, D, dtype_code(k0.dtype), float(scale_log2),
-            workspace.data_ptr(), workspace.numel(),
-        )
-        check(status, "pd_plan_create")
+        layout = (ctypes.byref(handle), n, kptrs, vptrs, n_blocks, bs, strides3(k0), strides3(v_caches[0]),
+                  block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seqlen.data_ptr())
+        rest = (batch, n_head, hkv, D, dtype_code(k0.dtype), float(scale_log2), workspace.data_ptr(), workspace.numel())
+        if window is None:
+            check(lib_.pd_plan_create(*layout, *rest), "pd_plan_create")
+        else:
+            check(lib_.pd_plan_create_window(*layout, int(window), int(sinks), *rest), "pd_plan_create_window")
         self._handle = handle
         self._lib = lib_
         self._overlap = False

@@ -37,7 +37,9 @@ from __future__ import annotations
 import torch
 
 from model import _native
-from model.triton_decode import TRITON_AVAILABLE
+from model.paged_evict import evict_tokens, paged_decode_weights
+from model.paged_window import decode_workspace
+from model.triton_decode import TRITON_AVAILABLE, _raise_first, window_rules
 
 __all__ = ["PagedPool", "PagedKV"]
 
@@ -291,6 +293,11 @@ class PagedKV:
     run's position bound (the RoPE table length). The padded int32 block table is built once
     per container and never mutated; the int32 ``seqlen`` is refreshed in place by
     :meth:`build_mask` and read by the decode plan by reference.
+
+    Two ways to bound a row, which the reference does not have: with ``window`` (and ``sinks``) every step sees the
+    last ``window`` tokens and the first ``sinks`` only, :meth:`hidden_blocks` names the blocks that are out of
+    sight for good; with ``track_weights`` the steps add up each cached token's attention weight in
+    :attr:`weights`, by which :meth:`evict` cuts rows down to a budget.
     """
 
     decode_container = True
@@ -298,7 +305,11 @@ class PagedKV:
 
     def __init__(self, pool: PagedPool, block_tables, lengths, *, rope_len: int, seats=None,
                  n_head: int | None = None, check_bounds: bool = True, fuse_append: bool = True,
-                 overlap_layers: bool = True) -> None:
+                 overlap_layers: bool = True, window: int | None = None, sinks: int = 0,
+                 track_weights: bool = False) -> None:
+        _raise_first(window_rules(window, sinks))
+        if track_weights and window is not None:
+            raise ValueError("a container keeps attention weights (track_weights) or a window, not both")
         lengths = [int(n) for n in lengths]
         rope_len = int(rope_len)
         seats = list(range(len(block_tables))) if seats is None else list(seats)
@@ -347,7 +358,8 @@ class PagedKV:
         # The fused append + decode launch needs rows that never share a block (a row must not
         # read a slot another row appends); tables from BlockManager never do.
         owned = [b for table in self.block_tables for b in table]
-        self.fuse_append = bool(fuse_append) and len(owned) == len(set(owned))
+        self._rows_disjoint = len(owned) == len(set(owned))
+        self.fuse_append = bool(fuse_append) and self._rows_disjoint and not track_weights
         # A fused write + attend right after this container's previous fused attend may start
         # while that launch finishes (programmatic dependent launch): nothing it reads before
         # waiting (seqlen, positions, block table, pools) is written in between. Any other
@@ -355,12 +367,23 @@ class PagedKV:
         # the flag, so the next attend waits for it as usual.
         self.overlap_layers = bool(overlap_layers)
         self._after_attend = False
+        self.window, self.sinks = window, int(sinks)
+        # Tokens of each row that were evicted: its next token sits that much further on in its sequence than in
+        # the cache.
+        self.evicted = torch.zeros(n_rows, dtype=torch.long, device=self.device)
+        self._host_evicted = [0] * n_rows
+        #: (n_layer, rows, n_kv_head, table capacity) float32 with ``track_weights``: every cached token's attention
+        #: weights so far, summed over the steps and over the query heads of a kv head.
+        self.weights: torch.Tensor | None = None
+        if track_weights:
+            self.weights = torch.zeros(self.n_layer, n_rows, self.n_kv_head, width * pool.block_size, device=self.device)
+            self._weights_workspace = decode_workspace(n_rows, n_head, self.n_kv_head, self.head_dim, pool._keys[0])
 
     # ---------------------------------------------------------------- step hooks
     def build_mask(self, *, next_token: bool = False) -> None:
         """Step boundary: ``seqlen := pos + next_token`` as int32, in place (no mask/bias)."""
         self.pool.flush()
-        longest = max(n + int(next_token) for n in self._host_valid)
+        longest = max(n + e + int(next_token) for n, e in zip(self._host_valid, self._host_evicted))
         if self.check_bounds and longest > self.max_len:
             raise IndexError(f"PagedKV overflow: needs {longest} positions, run position bound is {self.max_len}")
         self._seqlen.copy_((self.pos + int(next_token)).to(torch.int32))
@@ -427,8 +450,8 @@ class PagedKV:
         if tuple(k.shape) != expected or tuple(v.shape) != expected:
             raise ValueError(f"write needs {expected}, got {tuple(k.shape)} / {tuple(v.shape)}")
         layer = self.pool._check_layer(layer)
-        if self.check_bounds and max(self._host_pos) >= self.max_len:
-            raise IndexError(f"PagedKV overflow: write position {max(self._host_pos)} >= max_len {self.max_len}")
+        if self.check_bounds and self._last_position() >= self.max_len:
+            raise IndexError(f"PagedKV overflow: write position {self._last_position()} >= max_len {self.max_len}")
         if self._slot_error is not None:
             row, position, block_index, have = self._slot_error
             raise IndexError(
@@ -467,7 +490,7 @@ class PagedKV:
         if self._decode_plan is None:
             self._decode_plan = paged_decode_plan(
                 q3, self.pool._keys, self.pool._values, self._block_table_tensor, self._seqlen,
-                scale=1.0 / (self.head_dim ** 0.5),
+                scale=1.0 / (self.head_dim ** 0.5), window=self.window, sinks=self.sinks,
             )
             # The container's padded table is built once and never edited, so the plan's step
             # cache may keep the table windows of each step's first copies too.
@@ -488,8 +511,12 @@ class PagedKV:
             if violated:
                 raise error(message)
         q3 = q[:, :, 0, :].contiguous()
-        plan = self._plan_for(q3)
         out3 = None if out is None else out[:, :, 0, :]
+        if self.weights is not None:
+            self.pool.flush()
+            self._after_attend = False
+            return self._attend_weights(self.pool._check_layer(layer), q3, self.weights[layer], out3).unsqueeze(2)
+        plan = self._plan_for(q3)
         pending = self.pool._pending
         if (pending is not None and pending.owner is self and pending.layer == int(layer)
                 and pending.stream == torch.cuda.current_stream(self.device)
@@ -503,6 +530,56 @@ class PagedKV:
         self._after_attend = False
         return plan.run(layer, q3, out=out3).unsqueeze(2)
 
+    def _attend_weights(self, layer: int, q3: torch.Tensor, weights: torch.Tensor, out3=None) -> torch.Tensor:
+        return paged_decode_weights(q3, self.pool._keys[layer], self.pool._values[layer], self._block_table_tensor,
+                                    self._seqlen, weights, scale=1.0 / (self.head_dim ** 0.5), out=out3,
+                                    workspace=self._weights_workspace)
+
+    def evict(self, keep: int, *, recent: int = 0, sinks: int = 0) -> None:
+        """Cut every row above ``keep`` cached tokens down to ``keep``, in every layer and in place, by the attention
+        weights so far (``track_weights``): :func:`model.paged_evict.evict_tokens`. Between steps (after
+        :meth:`advance`). The rows' cache positions fall, their sequence positions (:attr:`position`) go on; captured
+        steps stay valid. Rows must not share blocks."""
+        if self.weights is None:
+            raise RuntimeError("PagedKV.evict() needs a container that keeps attention weights (track_weights=True)")
+        if not self._rows_disjoint:
+            raise ValueError("PagedKV.evict() moves tokens in place, but rows of this container share blocks")
+        if self._step_written or self._seqlen_ready:
+            raise RuntimeError("PagedKV.evict() inside a step: call it after advance()")
+        if any(isinstance(x, bool) or not isinstance(x, int) for x in (keep, recent, sinks)):
+            raise ValueError(f"keep, recent and sinks must be ints, got {keep!r}, {recent!r}, {sinks!r}")
+        if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
+            raise ValueError(f"recent ({recent}) and sinks ({sinks}) must be at least 0 and fit into keep ({keep})")
+        self.pool.flush()
+        if max(self._host_pos) <= keep:
+            return
+        left, _ = evict_tokens(self.pool._keys, self.pool._values, self._block_table_tensor, self.pos, self.weights, keep,
+                               recent=recent, sinks=sinks, weights_out=self.weights)
+        self.evicted.add_(self.pos - left)
+        self.pos.copy_(left)
+        self.valid.copy_(left)
+        for row, n in enumerate(self._host_pos):
+            self._host_evicted[row] += max(n - keep, 0)
+            self._host_pos[row] = self._host_valid[row] = min(n, keep)
+        self._refresh_slots()
+
+    @property
+    def position(self) -> torch.Tensor:
+        """Device tensor (rows,) int64: the next token's position in its sequence (its rotary position)."""
+        return self.pos if self.weights is None else self.pos + self.evicted
+
+    def _last_position(self) -> int:
+        return max(n + e for n, e in zip(self._host_pos, self._host_evicted))
+
+    def hidden_blocks(self) -> list[list[int]]:
+        """Per row, the blocks of its table whose tokens no later step sees: those between the sinks and the window
+        of the next token. Their owner may free them; the container goes on with its table as it is."""
+        if self.window is None:
+            return [[] for _ in self.block_tables]
+        bs = self.pool.block_size
+        return [table[-(-self.sinks // bs):max(0, n + 1 - self.window) // bs]
+                for table, n in zip(self.block_tables, self._host_pos)]
+
     def advance(self) -> None:
         """Move every active row's cursor one token (device in place, then host mirrors)."""
         self.pool.flush()
@@ -515,7 +592,7 @@ class PagedKV:
                 self._host_valid[row] = max(self._host_valid[row], self._host_pos[row])
         self._step_written = False
         self._seqlen_ready = False
-        if self.check_bounds and max(self._host_pos) > self.max_len:
+        if self.check_bounds and self._last_position() > self.max_len:
             raise IndexError(f"PagedKV overflow: max_len={self.max_len}; a request decoded past its budget")
         self._refresh_slots()
 
@@ -528,6 +605,9 @@ class PagedKV:
         if tuple(q.shape) != expected:
             raise ValueError(f"prepare needs q {expected}, got {tuple(q.shape)}")
         q3 = q[:, :, 0, :].contiguous()
+        if self.weights is not None:
+            self._attend_weights(0, q3, torch.zeros_like(self.weights[0]))
+            return
         self._plan_for(q3).run(0, q3)
 
     def _host_snapshot(self):
@@ -542,11 +622,11 @@ class PagedKV:
     def _replayed_step(self, next_token: bool) -> None:
         """Host side of one step whose device work was replayed from a graph: the checks that
         build_mask and write make, then the position mirrors advance makes."""
-        longest = max(n + int(next_token) for n in self._host_valid)
+        longest = max(n + e + int(next_token) for n, e in zip(self._host_valid, self._host_evicted))
         if self.check_bounds and longest > self.max_len:
             raise IndexError(f"PagedKV overflow: needs {longest} positions, run position bound is {self.max_len}")
-        if self.check_bounds and max(self._host_pos) >= self.max_len:
-            raise IndexError(f"PagedKV overflow: write position {max(self._host_pos)} >= max_len {self.max_len}")
+        if self.check_bounds and self._last_position() >= self.max_len:
+            raise IndexError(f"PagedKV overflow: write position {self._last_position()} >= max_len {self.max_len}")
         if self._slot_error is not None:
             row, position, block_index, have = self._slot_error
             raise IndexError(

@@ -195,6 +195,16 @@ def _plan_contract(q, block_table, seqlen, k_caches, v_caches):
         f"paged_decode_plan needs one k_cache/v_cache per layer, got {len(k_caches)} / {len(v_caches)}")
 
 
+def window_rules(window, sinks):
+    """A window's contract as (violated, message) rules; ``None`` is no window."""
+    for name, value in (("window", window), ("sinks", sinks)):
+        yield value is not None and (isinstance(value, bool) or not isinstance(value, int)), lambda name=name, value=value: (
+            f"{name} must be an int, got {value!r}")
+    yield window is not None and window < 1, lambda: f"window must be at least 1, got {window}"
+    yield sinks is None or sinks < 0, lambda: f"sinks must be at least 0, got {sinks}"
+    yield window is None and sinks != 0, lambda: f"sinks ({sinks}) need a window"
+
+
 def _plan_layer_contract(k_cache, v_cache, k_first, v_first):
     """Every layer's pools share the first layer's shapes and strides (the plan encodes one
     launch geometry), and TMA can describe them as they are."""
@@ -318,14 +328,19 @@ class PagedDecodePlan:
     int64 seqlen is refused rather than snapshotted), and :meth:`run` checks only the query
     layout. On top of that the plan encodes each layer's two TMA descriptors once (in the
     native ``pd_plan``) and owns the decode workspace.
+
+    With ``window`` every query sees the last ``window`` tokens of its row and the first ``sinks`` only
+    (:mod:`model.paged_window`).
     """
 
     __slots__ = ("n_layer", "grid", "q_shape", "q_dtype", "q_device", "q_strides", "_k", "_v",
                  "_block_table", "_seqlen", "_native_plan", "_workspace", "_stream_cache")
 
-    def __init__(self, q, k_caches, v_caches, block_table, seqlen, *, scale: float | None = None):
+    def __init__(self, q, k_caches, v_caches, block_table, seqlen, *, scale: float | None = None,
+                 window: int | None = None, sinks: int = 0):
         _require_backend()
         _require_cuda_tensors((("q", q), ("block_table", block_table), ("seqlen", seqlen)))
+        _raise_first(window_rules(window, sinks))
         k_caches, v_caches = list(k_caches), list(v_caches)
         _raise_first(_plan_contract(q, block_table, seqlen, k_caches, v_caches))
         b, h, d = q.shape
@@ -347,12 +362,13 @@ class PagedDecodePlan:
         if scale is None:
             scale = 1.0 / math.sqrt(d)
         with torch.cuda.device(q.device):
-            need = _native.workspace_bytes(b, h, k_caches[0].shape[2], d, q.dtype)
+            need = _native.workspace_bytes(b, h, k_caches[0].shape[2], d, q.dtype, window=window is not None)
             # two halves: consecutive launches alternate, which overlapped launches need
             half = -(-max(need, 256) // 256) * 256
             self._workspace = torch.empty(2 * half, dtype=torch.uint8, device=q.device)
             self._native_plan = _native.NativePlan(
-                k_caches, v_caches, block_table, seqlen, b, h, float(scale) * _LOG2E, self._workspace
+                k_caches, v_caches, block_table, seqlen, b, h, float(scale) * _LOG2E, self._workspace,
+                window=None if window is None else min(int(window), 1 << 30), sinks=min(int(sinks), 1 << 30)
             )
         self._stream_cache = None
 
@@ -441,6 +457,7 @@ class PagedDecodePlan:
         return out
 
 
-def paged_decode_plan(q, k_caches, v_caches, block_table, seqlen, *, scale: float | None = None):
+def paged_decode_plan(q, k_caches, v_caches, block_table, seqlen, *, scale: float | None = None,
+                      window: int | None = None, sinks: int = 0):
     """Validate one container's paged-decode tensors and cache their launch state."""
-    return PagedDecodePlan(q, k_caches, v_caches, block_table, seqlen, scale=scale)
+    return PagedDecodePlan(q, k_caches, v_caches, block_table, seqlen, scale=scale, window=window, sinks=sinks)
