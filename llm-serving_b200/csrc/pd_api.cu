@@ -1051,6 +1051,14 @@ int pd_prefill_window(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh
   p.table = block_table;
   p.bt_stride = bt_stride;
   p.n_blocks = n_blocks;
+  p.k = k_cache;
+  p.v = v_cache;
+  p.k_sb = k_strides[0];
+  p.k_sn = k_strides[1];
+  p.k_sh = k_strides[2];
+  p.v_sb = v_strides[0];
+  p.v_sn = v_strides[1];
+  p.v_sh = v_strides[2];
   p.total_q = int32_t(total_q);
   p.max_seqlen_q = max_seqlen_q;
   p.batch = batch;

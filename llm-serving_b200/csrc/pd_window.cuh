@@ -15,6 +15,8 @@ struct WindowPrefillParams {
   const int32_t* table;
   int64_t bt_stride;
   int64_t n_blocks;
+  const void *k, *v;  // the pools, for rows that are computed again (pd_window_prefill.cu)
+  int64_t k_sb, k_sn, k_sh, v_sb, v_sn, v_sh;  // block, token, head
   int32_t total_q, max_seqlen_q;
   int32_t batch, n_kv_head, group;
   int32_t max_blocks, capacity;

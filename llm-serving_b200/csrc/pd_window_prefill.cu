@@ -67,6 +67,7 @@ struct Cfg {
   static constexpr int TMEM_COLS = CTAS == 2 ? 256 : 512;
   static_assert(O_COL + D <= TMEM_COLS && CTAS * TMEM_COLS <= 512, "TMEM columns");
   static constexpr int OFF_ML = 512;  // (m, l) of a row for the cluster's merge; barriers and flags before it
+  static constexpr int OFF_AGAIN = 1536;  // rows that the merge found not finite
   static constexpr int OFF_Q = 2048;
   static constexpr int OFF_K = OFF_Q + Q_BYTES;
   static constexpr int OFF_V = OFF_K + STAGES * KV_BYTES;
@@ -106,6 +107,66 @@ __device__ __forceinline__ uint32_t bits(int lo, int hi) {
   const uint32_t below_hi = hi <= 0 ? 0u : hi >= 32 ? 0xffffffffu : (1u << hi) - 1u;
   const uint32_t below_lo = lo <= 0 ? 0u : lo >= 32 ? 0xffffffffu : (1u << lo) - 1u;
   return below_hi & ~below_lo;
+}
+
+// One query row by one warp, over the keys it sees and no others. The tiles multiply every V of a step with some weight,
+// 0 for a key that a row does not see, and 0 times an infinity or a NaN is a NaN: a row whose result is not finite is
+// computed again here. (A row that sees such a value is not finite again.)
+template <typename T, int D>
+__device__ __noinline__ void row_again(const WindowPrefillParams& p, int b, int h, int lk, int token, int head, int at) {
+  using E = Elem<T>;
+  constexpr int PER = D / 32;
+  const int lane = threadIdx.x & 31;
+  const T* q = reinterpret_cast<const T*>(p.q) + int64_t(token) * p.q_st + int64_t(head) * p.q_sh;
+  const int32_t* trow = p.table + int64_t(b) * p.bt_stride;
+  const int first = max(at - p.window + 1, 0), sinks = min(p.sinks, first), count = sinks + max(at + 1 - first, 0);
+  float m = -INFINITY, l = 0.f, acc[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+  for (int i0 = 0; i0 < count; i0 += 32) {
+    // a lane a key
+    const int i = i0 + lane, j = i < sinks ? i : first + i - sinks, page = j >> p.log2_bs;
+    const int blk = i < count && j < lk && page < p.max_blocks ? __ldg(trow + page) : -1;
+    const bool known = blk >= 0 && blk < p.n_blocks;  // a block outside the pool reads zeros
+    const int in_block = j & ((1 << p.log2_bs) - 1);
+    float s = 0.f;
+    if (known) {
+      const T* k = reinterpret_cast<const T*>(p.k) + int64_t(blk) * p.k_sb + int64_t(in_block) * p.k_sn + int64_t(h) * p.k_sh;
+#pragma unroll 1
+      for (int d = 0; d < D; d += 8) {
+        float x[8], y[8];
+        E::unpack(__ldg(reinterpret_cast<const uint4*>(q + d)), x);
+        E::unpack(__ldg(reinterpret_cast<const uint4*>(k + d)), y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+      }
+    }
+    s = i < count ? s * p.scale_log2 : -INFINITY;
+    float top = s;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
+    const float m_new = fmaxf(m, top), alpha = m == m_new ? 1.f : exp2f(m - m_new);
+    const float w = i < count ? exp2f(s - m_new) : 0.f;
+    m = m_new;
+    l = fmaf(l, alpha, w);  // a lane's own sum
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] *= alpha;
+    const int64_t v_at = int64_t(blk) * p.v_sb + int64_t(in_block) * p.v_sn + int64_t(h) * p.v_sh;
+    for (int t = 0; t < min(32, count - i0); ++t) {  // every lane PER elements of each key
+      const float wt = __shfl_sync(FULL_MASK, w, t);
+      const int64_t row = __shfl_sync(FULL_MASK, (long long)v_at, t);
+      if (!__shfl_sync(FULL_MASK, known, t)) continue;
+      const T* v = reinterpret_cast<const T*>(p.v) + row + lane * PER;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) acc[e] = fmaf(wt, E::to_float(v[e]), acc[e]);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(FULL_MASK, l, o);
+  T* out = reinterpret_cast<T*>(p.out) + int64_t(token) * p.o_st + int64_t(head) * p.o_sh + lane * PER;
+  const float inv = count > 0 ? 1.f / l : 0.f;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) out[e] = E::from_float(acc[e] * inv);
 }
 
 template <typename T, int D>
@@ -501,6 +562,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
       // For the merge: m and l, and O over K and V, which no copy or MMA uses any more; 16-byte units of a row
       // permuted by the row, so that a quarter-warp's stores meet different banks.
       *reinterpret_cast<float2*>(smem + C::OFF_ML + r * 8) = make_float2(m_run, l_run);
+      reinterpret_cast<float*>(smem + C::OFF_AGAIN)[r] = 0.f;
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
@@ -522,6 +584,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
     } else {
       // a row that sees no key gives zeros
       const bool blind = last_key < 0 || !live;
+      float whole = 0.f;  // stays 0 while the row's results are finite
       const float inv = blind ? 0.f : 1.f / l_run;
       // Through the warp's own 32 rows of the Q tile, which no MMA reads any more, so that a store
       // instruction writes whole rows instead of 16 bytes of 32 of them. The block's other warps copied Q
@@ -538,6 +601,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
 #pragma unroll
           for (int k = 0; k < 32; ++k) o[k] = 0u;
         }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) whole = fmaf(__uint_as_float(o[k]), 0.f, whole);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           uint32_t w[4];
@@ -565,19 +630,28 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
           ++mt;
         }
       }
+      unsigned again = __ballot_sync(FULL_MASK, whole != 0.f);  // (a NaN is not 0)
+      while (again != 0u) {
+        const int m = row0 + warp * 32 + __ffs(again) - 1, t = m / p.group;
+        again &= again - 1u;
+        __syncwarp();  // this warp has stored the row
+        row_again<T, D>(p, b, h, lk, q_begin + t, h * p.group + m - t * p.group, ctx + t);
+      }
     }
   }
 
   if (split > 1) {
     __syncwarp();
     cluster_sync();
-    if (merge) {
+    const int live_rows = min(ROWS, rows - row0), mine = merge ? (live_rows - rank + split - 1) >> log2_split : 0;
+    if (warp < C::SOFTMAX_WARPS && row0 < rows) {  // (a warp whose waits ran out has no rows, but meets the others)
       // Row by row, the CTAs' rows dealt in turn: a row's 16-byte units over the lanes.
       constexpr int UNITS = D / 4;
-      const int live_rows = min(ROWS, rows - row0);
-      const int mine = (live_rows - rank + split - 1) >> log2_split;
-      for (int e = tid; e < mine * UNITS; e += 128) {
-        const int r = (e / UNITS << log2_split) + rank, u = e % UNITS;
+      // (all threads of a row's warp take every turn, so that they can vote on it)
+      for (int e0 = 0; e0 < mine * UNITS; e0 += 128) {
+        const int e = e0 + tid;
+        const bool in = e < mine * UNITS;
+        const int r = in ? (e / UNITS << log2_split) + rank : rank, u = e % UNITS;
         const uint32_t ml = sbase + uint32_t(C::OFF_ML + r * 8);
         const uint32_t o = sbase + uint32_t(C::OFF_O + r * (D * 4)) + uint32_t((u ^ (r & 7)) << 4);
         float2 part[8];
@@ -611,8 +685,18 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
         uint2 w;
         w.x = E::pack2(sum.x * inv, sum.y * inv);
         w.y = E::pack2(sum.z * inv, sum.w * inv);
-        *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + int64_t(q_begin + t) * p.o_st +
-                                  int64_t(h * p.group + n - t * p.group) * p.o_sh + u * 4) = w;
+        if (in)
+          *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + int64_t(q_begin + t) * p.o_st +
+                                    int64_t(h * p.group + n - t * p.group) * p.o_sh + u * 4) = w;
+        // A row that is not finite is noted, and computed again once every thread has stored its part.
+        const float whole = sum.x * 0.f + sum.y * 0.f + (sum.z * 0.f + sum.w * 0.f) + inv * 0.f;
+        if (in && whole != 0.f) reinterpret_cast<float*>(smem + C::OFF_AGAIN)[r] = 1.f;
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int i = warp; i < mine; i += C::SOFTMAX_WARPS) {
+        const int r = (i << log2_split) + rank, m = row0 + r, t = m / p.group;
+        if (reinterpret_cast<const float*>(smem + C::OFF_AGAIN)[r] != 0.f)
+          row_again<T, D>(p, b, h, lk, q_begin + t, h * p.group + m - t * p.group, ctx + t);
       }
     }
     __syncwarp();

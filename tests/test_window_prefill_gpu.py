@@ -233,3 +233,36 @@ def test_refusals():
     refused(match="seqlen_k is on", seqlen_k=lens_t.cpu())
     refused(RuntimeError, "requires CUDA", q=q.cpu())
     refused(TypeError, max_seqlen_q="10")
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("rows,hkv,group,d,dtype", [([(300, 400), (5, 90)], 2, 2, 128, BF16), ([(260, 260)], 3, 5, 64, F16),
+                                                    ([(70, 200)], 2, 4, 256, BF16), ([(9, 300)], 8, 2, 128, F16),
+                                                    ([(700, 1700)] * 5, 4, 2, 128, BF16)])
+def test_a_value_that_is_not_finite_reaches_its_viewers_only(value, rows, hkv, group, d, dtype):
+    """V of a few tokens is not finite: queries that see one of them are not either, the others as if it were 0."""
+    window, sinks = 40, 3
+    case = _case(rows, hkv, group, d, 16, dtype)
+    q, k, v, table, cu, lens = case
+    bad = [(b, j) for b, n in enumerate(lens) for j in (10, n // 2, n - 44)]  # the last is in sight of the first queries only
+    clean = v.clone()
+    for b, j in bad:
+        clean[table[b, j // 16], j % 16] = 0
+        v[table[b, j // 16], j % 16] = value
+    want, bound = chunk_reference(q, k, clean, table, cu, lens, window, sinks)
+    got = _run(case, window, sinks)
+    sees = torch.zeros(q.shape[0], dtype=torch.bool)
+    for b, j in bad:
+        for t in range(cu[b], cu[b + 1]):
+            i = lens[b] - (cu[b + 1] - t)
+            sees[t] |= j <= i and (i - j < window or j < sinks)
+    sees = sees.cuda()
+    assert 0 < int(sees.sum())
+    assert not bool(got[sees].isfinite().any())
+    check(got[~sees], want[~sees], bound[~sees])
+
+
+def test_only_blind_rows_beside_a_value_that_is_not_finite():
+    case = _case([(40, 10)], 2, 2, 128, 16, BF16)
+    case[2][:] = float("nan")
+    assert _run(case, 20, 2)[:30].abs().max() == 0
