@@ -207,7 +207,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
     __syncwarp();
     tc::tmem_alloc(sbase + Bars::TMEM_SLOT, C::TMEM_COLS);
     tc::tmem_relinquish();
+    // The stream's next kernel may be launched now, not before: a CTA of it that held TMEM while it waits for this
+    // grid must not be in the way of this one's.
+    griddep_launch_dependents();
   }
+  griddep_wait();  // everything that is read may be the preceding kernel's
 
   // Query blocks slowest and last ones first: a prompt's first blocks have the fewest keys.
   const int split = 1 << log2_split, rank = int(blockIdx.x) & (split - 1), work = int(blockIdx.x) >> log2_split;
@@ -262,7 +266,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
     atomicOr(p.err, DEVERR_WAIT_TIMEOUT);
   };
   const uint32_t q_base = sbase + uint32_t(C::OFF_Q);
-  bool merge = false;  // this thread takes part in the cluster's merge
 
   if (row0 >= rows) {  // no query row (of any CTA of the cluster)
     tmem = meet();
@@ -467,12 +470,17 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
     const uint32_t o_tmem = lane_base + uint32_t(C::O_COL);
     float m_run = -3.0e38f, l_run = 0.f;
     bool ok = true;
+    const bool idle = row0 + warp * 32 >= rows;  // no row of this warp is one of the chunk's: whatever P is there serves
     for (int i = 0; i < steps; ++i) {
       const int sb = i & 1;
       if (__any_sync(FULL_MASK, *abort_flag != 0) ||
           !warp_wait_phase(bar(Bars::S_FULL + sb), uint32_t(i >> 1) & 1u, p.wait_ns)) {
         ok = false;
         break;
+      }
+      if (idle) {
+        if (lane == 0) mbar_arrive(bar(Bars::P_FULL + sb));
+        continue;
       }
       tc::fence_after_sync();
       const uint32_t s_tmem = lane_base + uint32_t(sb * KEYS);
@@ -556,6 +564,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
     if (ok && steps > 0)
       ok = warp_wait_phase(bar(Bars::O_DONE + ((steps - 1) & 1)), uint32_t((steps - 1) >> 1) & 1u, p.wait_ns);
     tc::fence_after_sync();
+    const bool merge = ok && split > 1;
     if (!ok) {
       if (lane == 0) fail();
     } else if (split > 1) {
@@ -580,7 +589,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
                    o[4 * u + 2], o[4 * u + 3]);
         }
       }
-      merge = true;
     } else {
       // a row that sees no key gives zeros
       const bool blind = last_key < 0 || !live;
@@ -638,13 +646,12 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
         row_again<T, D>(p, b, h, lk, q_begin + t, h * p.group + m - t * p.group, ctx + t);
       }
     }
-  }
-
-  if (split > 1) {
-    __syncwarp();
-    cluster_sync();
-    const int live_rows = min(ROWS, rows - row0), mine = merge ? (live_rows - rank + split - 1) >> log2_split : 0;
-    if (warp < C::SOFTMAX_WARPS && row0 < rows) {  // (a warp whose waits ran out has no rows, but meets the others)
+    // The cluster's merge, in the branch of the warps that have registers for it.
+    if (split > 1) {
+      __syncwarp();
+      cluster_sync();
+      const int live_rows = min(ROWS, rows - row0);
+      const int mine = merge ? (live_rows - rank + split - 1) >> log2_split : 0;  // (0: its waits ran out)
       // Row by row, the CTAs' rows dealt in turn: a row's 16-byte units over the lanes.
       constexpr int UNITS = D / 4;
       // (all threads of a row's warp take every turn, so that they can vote on it)
@@ -698,10 +705,16 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
         if (reinterpret_cast<const float*>(smem + C::OFF_AGAIN)[r] != 0.f)
           row_again<T, D>(p, b, h, lk, q_begin + t, h * p.group + m - t * p.group, ctx + t);
       }
+      __syncwarp();
+      cluster_sync();  // nothing of this CTA is read any more
     }
-    __syncwarp();
-    cluster_sync();  // nothing of this CTA is read any more
   }
+  if (split > 1 && (warp >= C::SOFTMAX_WARPS || row0 >= rows)) {  // the other warps at the cluster's barriers
+    __syncwarp();
+    cluster_sync();
+    cluster_sync();
+  }
+
   tc::fence_before_sync();
   __syncthreads();
   if (warp == C::S_WARP) {
@@ -729,18 +742,20 @@ cudaError_t launch_t(const WindowPrefillParams& p, const CUtensorMap& kmap, cons
          most_keys >= int64_t(2 * KEYS) << (log2_split + 1))
     ++log2_split;
   if ((ctas << log2_split) > 0x7fffffff) return cudaErrorInvalidValue;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1u << log2_split;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1u << log2_split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(ctas << log2_split));
   cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = log2_split > 0 ? 1 : 0;
+  cfg.numAttrs = log2_split > 0 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, fn, p, kmap, vmap, int(blocks), log2_split);
 }
 
