@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(WARPS * 32) pd_evict_select_kernel(const __gri
   extern __shared__ float s_sums[];
   griddep_launch_dependents();
   __shared__ uint2 s_range[WARPS];
-  __shared__ int s_bins[BINS];
+  __shared__ __align__(16) int s_bins[BINS];
   __shared__ int4 s_found;  // bin of the threshold, keys above it, keys in it
   __shared__ int2 s_scan[2][WARPS];
   __shared__ int s_first;
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(WARPS * 32) pd_evict_select_kernel(const __gri
   uint32_t* s_keys = reinterpret_cast<uint32_t*>(s_sums + (COPY ? n : 0));
   uint32_t low = 0xffffffffu, high = 0u;  // of the middle tokens' keys
   if constexpr (COPY) {
-#pragma unroll 4
+#pragma unroll 8
     for (int j = tid; j < n; j += THREADS) {
       const float value = w[j];
       const uint32_t k = key_of(value);
@@ -87,31 +87,51 @@ __global__ void __launch_bounds__(WARPS * 32) pd_evict_select_kernel(const __gri
   uint32_t x = 0xffffffffu;  // no token has this key: it is a NaN's pattern
   int at = 0;
   if (places > 0) {
-    low = __reduce_min_sync(FULL_MASK, low);
-    high = __reduce_max_sync(FULL_MASK, high);
-    if constexpr (WARPS > 1) {
+    // Keys low .. high hold the threshold; `need` of them stay.
+    int need = places;
+    for (bool first = true;; first = false) {
+      if (!first) {  // the range of the keys that are left
+        uint32_t a = 0xffffffffu, z = 0u;
+#pragma unroll 4
+        for (int j = lo + tid; j < hi; j += THREADS) {
+          const uint32_t k = key(j);
+          if (k - low <= high - low) {
+            a = min(a, k);
+            z = max(z, k);
+          }
+        }
+        low = a;
+        high = z;
+      }
+      low = __reduce_min_sync(FULL_MASK, low);
+      high = __reduce_max_sync(FULL_MASK, high);
       if (lane == 0) s_range[warp] = make_uint2(low, high);
+      for (int i = tid; i < BINS; i += THREADS) s_bins[i] = 0;
       __syncthreads();
       const uint2 r = s_range[lane < WARPS ? lane : 0];
       low = __reduce_min_sync(FULL_MASK, r.x);
       high = __reduce_max_sync(FULL_MASK, r.y);
-    }
-    // Keys low .. low + 2^width - 1 hold the threshold; `need` of them stay.
-    int width = 32 - __clz(high - low), need = places;
-    for (;;) {
-      const int shift = max(width - 8, 0);
-      for (int i = tid; i < BINS; i += THREADS) s_bins[i] = 0;
-      __syncthreads();
+      x = low;
+      if (low == high) {  // one key: the first of its tokens stay
+        at = need;
+        break;
+      }
+      // Bins of 2^shift from `base` on, the last one at `high`. At first an eighth of an octave each, so that the
+      // bins are many and few atomics meet; what lies 32 octaves below the largest, zeros above all, is in the lowest.
+      const int width = 32 - __clz(high - low);
+      const int shift = max((first ? min(width, 28) : width) - 8, 0);
+      const uint32_t span = uint32_t(BINS - 1) << shift;
+      const uint32_t base = high - low > span ? (high - span) >> shift << shift : low;
 #pragma unroll 4
       for (int j = lo + tid; j < hi; j += THREADS) {
-        const uint32_t k = key(j), d = k - low;  // (wraps to far above the range for a lower key)
-        if (width == 32 ? k >= low : d >> width == 0) atomicAdd(&s_bins[d >> shift], 1);
+        const uint32_t k = key(j);
+        if (k - low <= high - low) atomicAdd(&s_bins[min((max(k, base) - base) >> shift, uint32_t(BINS - 1))], 1);
       }
       __syncthreads();
       if (warp == 0) {  // lane l: bins 8 l .. 8 l + 7; the first from above with which `need` are reached
-        int c[8], sum = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += c[i] = s_bins[lane * 8 + i];
+        const int4 c0 = reinterpret_cast<const int4*>(s_bins)[lane * 2], c1 = reinterpret_cast<const int4*>(s_bins)[lane * 2 + 1];
+        const int c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+        const int sum = c0.x + c0.y + c0.z + c0.w + c1.x + c1.y + c1.z + c1.w;
         int from = sum;  // keys in this lane's bins and above
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -132,15 +152,11 @@ __global__ void __launch_bounds__(WARPS * 32) pd_evict_select_kernel(const __gri
       }
       __syncthreads();
       const int4 f = s_found;
-      low += uint32_t(f.x) << shift;
+      if (f.x < BINS - 1) high = min(high, base + (uint32_t(f.x + 1) << shift) - 1u);
+      if (f.x > 0) low = base + (uint32_t(f.x) << shift);
       need -= f.y;
-      width = shift;
       x = low;
       if (need == f.z) break;  // all of the bin stay
-      if (shift == 0) {        // its keys are one
-        at = need;
-        break;
-      }
     }
   }
   const bool exact = at == 0;
@@ -148,42 +164,55 @@ __global__ void __launch_bounds__(WARPS * 32) pd_evict_select_kernel(const __gri
 
   int32_t* order = p.order + int64_t(item) * p.keep;
   const unsigned lower = (1u << lane) - 1u;
-  auto kept = [&](int j, uint32_t k) -> bool { return j < lo || j >= hi || (exact ? k >= x : k > x); };  // but for a tie
+  const uint32_t enough = exact ? x : x + 1u;  // (x is below the largest number)
+  auto kept = [&](int j, uint32_t k) -> bool { return j < lo || j >= hi || k >= enough; };  // but for a tie
   auto is_tie = [&](int j, uint32_t k) -> bool { return !exact && k == x && j >= lo && j < hi; };
   // Token j goes to `rank`, if it stays: `before` kept tokens and `ties` at the threshold lie before its 32.
+  bool all_stay = true;  // so far in this warp
   auto place = [&](int j, float value, int before, int ties, unsigned stay_mask, unsigned tie_mask) {
-    const int tie_rank = ties + __popc(tie_mask & lower);
-    const bool stays = (stay_mask >> lane & 1u) || ((tie_mask >> lane & 1u) && tie_rank < at);
-    const int rank = before + min(ties, at) + __popc(stay_mask & lower) + min(tie_rank, at) - min(ties, at);
+    bool stays = stay_mask >> lane & 1u;
+    int rank = before + __popc(stay_mask & lower);
+    if (!exact) {
+      const int tie_rank = ties + __popc(tie_mask & lower);
+      stays = stays || ((tie_mask >> lane & 1u) && tie_rank < at);
+      rank += min(tie_rank, at);
+    }
     if (stays) {
       wo[rank] = value;
       order[rank] = j;
     }
-    const unsigned gone = __ballot_sync(FULL_MASK, j < n && !stays);
-    if (gone && lane == 0) atomicMin(&s_first, j + __ffs(gone) - 1);
+    if (all_stay) {
+      const unsigned gone = __ballot_sync(FULL_MASK, j < n && !stays);
+      if (gone) {
+        all_stay = false;
+        if (lane == 0) atomicMin(&s_first, j + __ffs(gone) - 1);
+      }
+    }
   };
   if constexpr (COPY) {
     // A warp's stretch of 32-token steps: whether they stay, a bit a step, one scan of the counts, then every
     // warp ranks its own.
     const int per = (n + THREADS - 1) / THREADS, start = warp * per * 32 + lane;
-    unsigned long long stay_bits = 0ull, tie_bits = 0ull;
+    unsigned stay_bits = 0u, tie_bits = 0u;  // (at most 32 steps: launch_select)
+#pragma unroll 4
     for (int i = 0; i < per; ++i) {
       const int j = start + i * 32;
-      if (j >= n) break;
-      const uint32_t k = s_keys[j];
-      stay_bits |= (unsigned long long)kept(j, k) << i;
-      tie_bits |= (unsigned long long)is_tie(j, k) << i;
+      if (j < n) {
+        const uint32_t k = s_keys[j];
+        stay_bits |= unsigned(kept(j, k)) << i;
+        tie_bits |= unsigned(is_tie(j, k)) << i;
+      }
     }
-    const int stay = __reduce_add_sync(FULL_MASK, __popcll(stay_bits));
-    const int tie = __reduce_add_sync(FULL_MASK, __popcll(tie_bits));
+    const int stay = __reduce_add_sync(FULL_MASK, __popc(stay_bits));
+    const int tie = __reduce_add_sync(FULL_MASK, __popc(tie_bits));
     if (lane == 0) s_scan[0][warp] = make_int2(stay, tie);
     __syncthreads();
     const int2 c = lane < warp ? s_scan[0][lane] : make_int2(0, 0);
     int before = __reduce_add_sync(FULL_MASK, c.x), ties = __reduce_add_sync(FULL_MASK, c.y);
     for (int i = 0; i < per; ++i) {
       const int j = start + i * 32;
-      const unsigned stay_mask = __ballot_sync(FULL_MASK, stay_bits >> i & 1ull);
-      const unsigned tie_mask = __ballot_sync(FULL_MASK, tie_bits >> i & 1ull);
+      const unsigned stay_mask = __ballot_sync(FULL_MASK, stay_bits >> i & 1u);
+      const unsigned tie_mask = exact ? 0u : __ballot_sync(FULL_MASK, tie_bits >> i & 1u);
       place(j, j < n ? s_sums[j] : 0.f, before, ties, stay_mask, tie_mask);
       before += __popc(stay_mask);
       ties += __popc(tie_mask);
@@ -298,7 +327,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) pd_evict_move_kernel(const __gri
 }
 
 // Rows of up to so many tokens are copied into shared memory.
-constexpr int COPY_TOKENS = 24576;
+constexpr int COPY_TOKENS = 24576;  // in keys and sums, 8 bytes a token
 
 template <int WARPS, bool COPY>
 cudaError_t select(const EvictParams& p, int64_t items, cudaStream_t stream) {
@@ -310,14 +339,15 @@ cudaError_t select(const EvictParams& p, int64_t items, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
-// Warps by the row's length: eight or so tokens a thread, 32 warps at most.
+// Warps by the row's length: eight or so tokens a thread, and half that where there are few rows.
 cudaError_t launch_select(const EvictParams& p, int64_t items, cudaStream_t stream) {
-  if (p.capacity <= 512) return select<2, true>(p, items, stream);
-  if (p.capacity <= 2048) return select<4, true>(p, items, stream);
-  if (p.capacity <= 4096) return select<8, true>(p, items, stream);
-  if (p.capacity <= 8192) return select<16, true>(p, items, stream);
-  if (p.capacity <= COPY_TOKENS) return select<32, true>(p, items, stream);
-  return select<32, false>(p, items, stream);
+  const int64_t tokens = items < 4 * int64_t(p.sms) ? int64_t(p.capacity) * 2 : p.capacity;
+  if (p.capacity > COPY_TOKENS) return select<32, false>(p, items, stream);
+  if (tokens <= 512) return select<2, true>(p, items, stream);
+  if (tokens <= 1280) return select<4, true>(p, items, stream);
+  if (tokens <= 2560) return select<8, true>(p, items, stream);
+  if (tokens <= 5120) return select<16, true>(p, items, stream);
+  return select<32, true>(p, items, stream);
 }
 
 }  // namespace
@@ -327,12 +357,13 @@ cudaError_t launch_evict(const EvictParams& p, cudaStream_t stream) {
   if (items == 0) return cudaSuccess;
   cudaError_t e = launch_select(p, items, stream);
   if (e != cudaSuccess) return e;
-  // Whole rows where there are eight CTAs for every SM; else new pages' lists are shared by CTAs, down to a
-  // chunk each, and rows moved in place are cut into slices, down to 64 bytes.
+  // New pages' lists are shared by CTAs until there are four for every SM, down to a chunk each (9 prompts in 4 layers:
+  // one or two 49.4 us, four 43.6). Rows moved in place are cut into slices, down to 64 bytes, until there are two: wider
+  // copies are worth more than more of them (one row in 28 layers: whole rows 30.0 us, 128 bytes 31.7, 64 33.3).
   int log2_slice = 2, parts = 1;
   while ((1 << log2_slice) < p.chunks) ++log2_slice;
   int64_t ctas = 2 * items;
-  const int64_t enough = 8 * int64_t(p.sms);
+  const int64_t enough = (p.fresh ? 4 : 2) * int64_t(p.sms);
   if (p.fresh) {
     parts = int(std::min((enough + ctas - 1) / ctas, int64_t(p.keep + CHUNK - 1) / CHUNK));
     ctas *= parts;
