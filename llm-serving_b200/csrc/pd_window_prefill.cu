@@ -211,6 +211,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
     // grid must not be in the way of this one's.
     griddep_launch_dependents();
   }
+  // The roles meet once, before any load: from here on each goes at its own pace (K is under way while Q is copied).
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + Bars::TMEM_SLOT);
   griddep_wait();  // everything that is read may be the preceding kernel's
 
   // Query blocks slowest and last ones first: a prompt's first blocks have the fewest keys.
@@ -245,14 +250,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
   const int all_steps = (keys.count + KEYS - 1) / KEYS;
   const int step0 = (rank * all_steps) >> log2_split, steps = (((rank + 1) * all_steps) >> log2_split) - step0;
 
-  // Every role meets here once, with its first loads already in flight; returns the TMEM address.
-  auto meet = [&]() -> uint32_t {
-    tc::fence_before_sync();
-    __syncthreads();
-    tc::fence_after_sync();
-    return *reinterpret_cast<volatile uint32_t*>(smem + Bars::TMEM_SLOT);
-  };
-  uint32_t tmem;
   auto k_addr = [&](int s) -> uint32_t { return sbase + uint32_t(C::OFF_K + s * C::KV_BYTES); };
   auto v_addr = [&](int s) -> uint32_t { return sbase + uint32_t(C::OFF_V + s * C::KV_BYTES); };
   // Where row r (a key) of 128-byte piece pc of a stage sits: 8-row groups `gstride` bytes apart, pieces
@@ -267,8 +264,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
   };
   const uint32_t q_base = sbase + uint32_t(C::OFF_Q);
 
-  if (row0 >= rows) {  // no query row (of any CTA of the cluster)
-    tmem = meet();
+  if (row0 >= rows) {
+    // no query row (of any CTA of the cluster)
   } else if (warp >= C::SOFTMAX_WARPS) {
     if constexpr (C::DEAL) regs_down<C::OTHER_REGS>();
     if (warp == C::K_WARP || warp == C::V_WARP) {
@@ -296,7 +293,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
         return token >= 0 && page < p.max_blocks ? __ldg(trow + page) : -1;
       };
       int win = window_of(0), win_next = window_of(1 << span);
-      tmem = meet();
       bool ok = true;
       int done = 0;  // steps whose copies were issued
       const uint32_t bytes = uint32_t(C::PIECES / per_box) * 128u << p.log2_box;  // of a copy
@@ -339,7 +335,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
       // ---------------------------------------------------------------- S = Q K^T
       // The whole warp runs this loop and one elected lane issues, so descriptors and addresses stay
       // uniform over the warp and no operand of an MMA is moved on its own.
-      tmem = meet();
       constexpr uint32_t IDESC_S = tc::instr_desc_f16(BF16, ROWS, KEYS, false, false);
       bool ok = lane_wait(bar(Bars::Q_FULL), 0u, p.wait_ns);
       const uint64_t q_desc = tc::smem_desc(q_base, 16u, 1024u);
@@ -369,7 +364,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
       warp_wait_phase(bar(Bars::DRAIN), 0u, DRAIN_LIMIT_NS);
     } else {
       // ---------------------------------------------------------------- O += P V
-      tmem = meet();
       constexpr uint32_t IDESC_PV = tc::instr_desc_f16(BF16, ROWS, D, false, true);
       const uint64_t v_desc = tc::smem_desc(v_addr(0), pstride, gstride);
       bool ok = true;
@@ -445,7 +439,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
         }
       }
     }
-    tmem = meet();
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (p.scale_log2 < 0.f) {  // a negative scale's sign goes into Q, so that the multiplier is never negative
       asm volatile("bar.sync 1, 128;" ::: "memory");  // the block's rows are in
