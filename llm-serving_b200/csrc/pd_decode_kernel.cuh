@@ -191,16 +191,33 @@ __device__ __forceinline__ uint32_t counter_tag(uint32_t epoch, uint32_t salt) {
 // and the plan's geometry. The layers of a decode step share both, so the first layer of a
 // step computes the split and records it per warp, and the later layers, whose lengths hash to
 // the recorded key, take it from the record (loaded in the same round trip as the lengths)
-// instead of recomputing it and then waiting on the block table. A record's key is never 0,
-// so zero-filled memory never matches.
-constexpr int STEP_REC_BYTES = 320;
-constexpr int STEP_WIN_OFF = 64;  // 64 int32 table entries (the window and the next one)
+// instead of recomputing it and then waiting on the block table. An overlapped launch may read a
+// record while the launch before it writes it (a CTA counts as past the dependency point with its
+// first warp), so the header and each lane's window entries carry the key folded with their own
+// values: a reader that sees old and new bytes together takes the record for absent and computes the
+// same split itself. Keys are odd and folds even, so zero-filled memory never matches.
+constexpr int STEP_REC_BYTES = 576;
+constexpr int STEP_WIN_OFF = 64;  // 32 lanes' table entries (the window's and the next one's) with their key, 16 bytes each
 struct StepHeader {               // bytes 0..47 of a record
   long long u0, u1;
   int b, item, tile, workers;
   int win_row, win_base;
-  unsigned long long key;
+  unsigned long long key;  // launch key ^ step_fold of the header's other 16-byte halves
 };
+
+__device__ __forceinline__ unsigned long long step_pair(uint32_t lo, uint32_t hi) { return (unsigned long long)hi << 32 | lo; }
+__device__ __forceinline__ unsigned long long step_fold(uint4 a, uint4 b, uint32_t c_lo, uint32_t c_hi) {
+  unsigned long long x = step_pair(a.x, a.y) * 0x9E3779B97F4A7C15ull + step_pair(a.z, a.w) * 0xC2B2AE3D27D4EB4Full +
+                         step_pair(b.x, b.y) * 0x165667B19E3779F9ull + step_pair(b.z, b.w) * 0xD6E8FEB86659FD93ull +
+                         step_pair(c_lo, c_hi) * 0xA0761D6478BD642Full;
+  x ^= x >> 29;
+  return x & ~1ull;
+}
+__device__ __forceinline__ unsigned long long step_fold(int win, int next) {
+  unsigned long long x = step_pair(uint32_t(win), uint32_t(next)) * 0x9E3779B97F4A7C15ull;
+  x ^= x >> 29;
+  return x & ~1ull;
+}
 
 __device__ __forceinline__ unsigned long long mix64(unsigned long long x) {  // SplitMix64 finaliser
   x ^= x >> 30;
@@ -375,11 +392,12 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
   }
 
   // A call on its own (no plan): the preceding kernel may still be writing anything that this one reads, so only
-  // the launch and the set-up above overlap it.
+  // the launch and the set-up above overlap it. (It lets the next kernel in after the wait, as every kernel here: what
+  // comes before it in the stream has then finished too, which a plan's overlapped launch relies on.)
   if constexpr (VAR != 0) {
     if (p.wait_first) {
-      griddep_launch_dependents();
       griddep_wait();
+      griddep_launch_dependents();
     }
   }
 
@@ -435,17 +453,14 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
   unsigned char* my_rec =
       use_step ? p.step_rec + (size_t(blockIdx.x) * (blockDim.x >> 5) + warp) * STEP_REC_BYTES : nullptr;
   uint4 rec_a = make_uint4(0u, 0u, 0u, 0u), rec_b = rec_a, rec_c = rec_a;
-  int rec_win0 = 0, rec_win1 = 0;
+  uint4 rec_win = make_uint4(0u, 0u, 0u, 0u);
   if (use_step) {
     if (lane == 0) {
       rec_a = ld_cg_v4(my_rec);
       rec_b = ld_cg_v4(my_rec + 16);
       rec_c = ld_cg_v4(my_rec + 32);
     }
-    if (p.step_table) {
-      rec_win0 = __ldcg(reinterpret_cast<const int*>(my_rec + STEP_WIN_OFF) + lane);
-      rec_win1 = __ldcg(reinterpret_cast<const int*>(my_rec + STEP_WIN_OFF) + 32 + lane);
-    }
+    if (p.step_table) rec_win = ld_cg_v4(my_rec + STEP_WIN_OFF + lane * 16);
   }
 
   // ---- prologue: clamp lengths, tiles per row, block-wide exclusive scan -------------
@@ -635,7 +650,9 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
   int64_t u0 = 0, u1 = 0;     // unit mode: range of units; column mode: range of real columns
   // Step cache: this warp's record holds the split of these very lengths.
   const bool cached =
-      use_step && __shfl_sync(FULL_MASK, lane == 0 && ((unsigned long long)rec_c.w << 32 | rec_c.z) == launch_key, 0);
+      use_step && __shfl_sync(FULL_MASK,
+                              lane == 0 && (step_pair(rec_c.z, rec_c.w) ^
+                                            step_fold(rec_a, rec_b, rec_c.x, rec_c.y)) == launch_key, 0);
   if (cached) {
     u0 = __shfl_sync(FULL_MASK, (long long)rec_a.y << 32 | rec_a.x, 0);
     u1 = __shfl_sync(FULL_MASK, (long long)rec_a.w << 32 | rec_a.z, 0);
@@ -679,8 +696,8 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
     }
   }
   // Records this launch's split of its warp (when it computed it): header by lane 0, the
-  // table windows the first copies used by every lane, made visible before the launch lets the
-  // next one start (enter_dependent).
+  // table windows the first copies used by every lane, before the warp passes the dependency point
+  // (enter_dependent), so that the next launch mostly finds them.
   auto write_record = [&](int rb, int ritem, int rtile, int wrow, int wbase, int wcur, int wnxt) {
     if (!use_step || cached) return;
     if (lane == 0) {
@@ -693,11 +710,14 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
       hd.workers = workers;
       hd.win_row = wrow;
       hd.win_base = wbase;
-      hd.key = launch_key;
+      hd.key = launch_key ^ step_fold(make_uint4(uint32_t(u0), uint32_t(u0 >> 32), uint32_t(u1), uint32_t(u1 >> 32)),
+                                      make_uint4(uint32_t(rb), uint32_t(ritem), uint32_t(rtile), uint32_t(workers)),
+                                      uint32_t(wrow), uint32_t(wbase));
       *reinterpret_cast<StepHeader*>(my_rec) = hd;
     }
-    reinterpret_cast<int*>(my_rec + STEP_WIN_OFF)[lane] = wcur;
-    reinterpret_cast<int*>(my_rec + STEP_WIN_OFF)[32 + lane] = wnxt;
+    const unsigned long long tag = launch_key ^ step_fold(wcur, wnxt);
+    *reinterpret_cast<uint4*>(my_rec + STEP_WIN_OFF + lane * 16) =
+        make_uint4(uint32_t(wcur), uint32_t(wnxt), uint32_t(tag), uint32_t(tag >> 32));
     __threadfence();
   };
   if (u0 >= u1) {
@@ -759,11 +779,12 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
   int win_row = -1, win_base = 0, win_cur = 0, win_nxt = 0;
   if (cached && p.step_table) {  // the recorded windows of this row's table (a fixed table)
     const int rrow = __shfl_sync(FULL_MASK, int(rec_c.x), 0);
-    if (rrow >= 0) {
+    const bool whole = (step_pair(rec_win.z, rec_win.w) ^ step_fold(int(rec_win.x), int(rec_win.y))) == launch_key;
+    if (rrow >= 0 && __all_sync(FULL_MASK, whole)) {
       win_row = rrow;
       win_base = __shfl_sync(FULL_MASK, int(rec_c.y), 0);
-      win_cur = rec_win0;
-      win_nxt = rec_win1;
+      win_cur = int(rec_win.x);
+      win_nxt = int(rec_win.y);
     }
   }
 
