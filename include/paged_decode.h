@@ -386,7 +386,8 @@ int pd_fp4_prefill(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, c
  * No reference counterpart. The pools, tables and lengths are pd_decode's.
  *
  * Window: the query at position i sees key j iff j <= i and (i - j < window or j < sinks), window >= 1,
- * sinks >= 0. Only pages that hold a visible token are looked up. Any number of q heads per kv head. */
+ * sinks >= 0. What the table names for pages without a visible token does not matter. Any number of q heads per
+ * kv head. `out` shares no memory with q. */
 
 /* Bytes of the workspace of pd_decode_window and pd_decode_weights, and of each half of
  * pd_plan_create_window's; any contents, one workspace per stream, never shared with other entry points. */
@@ -446,7 +447,8 @@ size_t pd_evict_scratch_bytes(int32_t n_layer, int32_t batch, int32_t n_kv_head,
  * new_table's pages, or of block_table's (new_table NULL: in place); shorter rows stay as they are (they are
  * copied to new_table's). weights (n_layer, B, H_kv, w_len) by strides of the first three; weights_out takes the kept
  * ones, zeros behind them (it may be weights), seqlen_out min(n, keep) (it may be seqlen). A block written for one
- * row is read or written for no other. A block id outside the pool is skipped and sets PD_DEVERR_COPY_RANGE.
+ * row is read or written for no other, and no pool is named twice. A block id outside the pool is skipped and
+ * sets PD_DEVERR_COPY_RANGE.
  * Rows of 16-byte multiples; every layer's pools have one layout. */
 int pd_evict(void* const* k_caches, void* const* v_caches, int32_t n_layer, int64_t n_blocks, int32_t block_size,
              int32_t n_kv_head, int32_t head_dim, int32_t dtype, const int64_t* k_strides, const int64_t* v_strides,

@@ -49,8 +49,8 @@ __global__ void __launch_bounds__(CLUSTER_WARPS * 32, 1)
     }
   }
   __syncwarp();
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();
 
   const int split = 1 << c.log2_split, rank = int(blockIdx.x) & (split - 1);
   const int item = int(blockIdx.x) >> c.log2_split;

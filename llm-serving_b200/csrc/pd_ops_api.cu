@@ -1,6 +1,8 @@
 // pd_ops_api.cu -- the extern "C" boundary of the head norm with rotation, the 4-bit pages, the
 // page copies and the eviction (declared in include/paged_decode.h): argument checks on the host, then the launch.
+#include <algorithm>
 #include <atomic>
+#include <vector>
 
 #include "paged_decode.h"
 #include "pd_api_internal.h"
@@ -353,6 +355,11 @@ int pd_evict(void* const* k_caches, void* const* v_caches, int32_t n_layer, int6
   for (int i = 0; i < n_layer; ++i)
     if (k_caches[i] == nullptr || v_caches[i] == nullptr || !aligned(k_caches[i], 16) || !aligned(v_caches[i], 16))
       return PD_ERR_INVALID;
+  std::vector<const void*> pools(k_caches, k_caches + n_layer);
+  pools.insert(pools.end(), v_caches, v_caches + n_layer);
+  std::sort(pools.begin(), pools.end());
+  if (std::adjacent_find(pools.begin(), pools.end()) != pools.end())
+    return api_message(PD_ERR_INVALID, "a pool is named twice, and its tokens would be moved twice");
   // no row holds more than its table: a larger budget evicts nothing either
   keep = int32_t(keep < capacity + 1 ? keep : capacity + 1);
   if (recent + sinks > keep) recent = sinks = 0;

@@ -207,9 +207,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
     __syncwarp();
     tc::tmem_alloc(sbase + Bars::TMEM_SLOT, C::TMEM_COLS);
     tc::tmem_relinquish();
-    // The stream's next kernel may be launched now, not before: a CTA of it that held TMEM while it waits for this
-    // grid must not be in the way of this one's.
-    griddep_launch_dependents();
   }
   // The roles meet once, before any load: from here on each goes at its own pace (K is under way while Q is copied).
   tc::fence_before_sync();
@@ -217,6 +214,9 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
   tc::fence_after_sync();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + Bars::TMEM_SLOT);
   griddep_wait();  // everything that is read may be the preceding kernel's
+  // The stream's next kernel may be launched now, not before: a CTA of it that held TMEM while it waits for this grid
+  // must not be in the way of this one's, and what it reads early must not be an earlier kernel's (pd_decode_kernel.cuh).
+  griddep_launch_dependents();
 
   // Query blocks slowest and last ones first: a prompt's first blocks have the fewest keys.
   const int split = 1 << log2_split, rank = int(blockIdx.x) & (split - 1), work = int(blockIdx.x) >> log2_split;

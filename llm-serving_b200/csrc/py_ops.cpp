@@ -614,13 +614,25 @@ void queries_of(const Tensor& q, const Tensor& k, const Pools& p, const char* sh
   same_device(k, "k_cache", q, "q");
 }
 
-// The result of a call: `given` (contiguous, like q) or a new tensor.
+// Whether the spans of memory from the first to the last element of a and b meet.
+bool spans_meet(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  auto end = [](const Tensor& t) {
+    int64_t last = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return static_cast<const char*>(t.const_data_ptr()) + last * t.element_size();
+  };
+  return static_cast<const char*>(a.const_data_ptr()) < end(b) && static_cast<const char*>(b.const_data_ptr()) < end(a);
+}
+
+// The result of a call: `given` (contiguous, like q, apart from it) or a new tensor.
 Tensor result_of(PyObject* given, const Tensor& q) {
   const Tensor* o = optional(given, "out");
   if (o == nullptr) return new_like(q);
   VALUE(o->sizes() == q.sizes() && o->scalar_type() == q.scalar_type() && o->device() == q.device() &&
             o->is_contiguous() && aligned16(*o),
         "out must be a contiguous, 16-byte aligned ", q.sizes(), " ", q.scalar_type(), " tensor on ", q.device());
+  VALUE(!spans_meet(*o, q), "out must not share memory with q");
   return *o;
 }
 
@@ -807,6 +819,10 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
     ks[i] = k.data_ptr();
     vs[i] = v.data_ptr();
   }
+  std::vector<void*> named(ks);
+  named.insert(named.end(), vs.begin(), vs.end());
+  std::sort(named.begin(), named.end());
+  VALUE(std::adjacent_find(named.begin(), named.end()) == named.end(), "a pool is named twice, and its tokens would be moved twice");
   const Tensor &seqlen0 = tensor(a[3], "seqlen"), &weights = tensor(a[4], "weights");
   VALUE(seqlen0.dim() == 1, "seqlen must be (B,), got shape ", seqlen0.sizes());
   VALUE(index_type(seqlen0), "seqlen must be int32 or int64, got ", seqlen0.scalar_type());
@@ -853,8 +869,8 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
     VALUE(t->size(3) == weights.size(3), "weights_out must be as long as weights, got ", t->size(3), " and ", weights.size(3));
     VALUE(t->is_contiguous() || (t->data_ptr() == weights.data_ptr() && t->strides() == weights.strides()),
           "weights_out must be contiguous, or weights itself");
-    VALUE(t->data_ptr() != weights.data_ptr() || t->strides() == weights.strides(),
-          "weights_out shares weights' memory with other strides");
+    VALUE((t->data_ptr() == weights.data_ptr() && t->strides() == weights.strides()) || !spans_meet(*t, weights),
+          "weights_out shares weights' memory, but not as weights itself");
     VALUE(disjoint_rows(*t), "weights_out rows must not overlap, got strides ", t->strides());
     sums_out = *t;
   } else {

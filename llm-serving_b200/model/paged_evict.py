@@ -14,7 +14,6 @@ Tensors on CUDA, the current stream, no host synchronisation. There is no CPU pa
 
 from __future__ import annotations
 
-
 from model import _native
 
 __all__ = ["evict_tokens", "paged_decode_weights"]
@@ -23,12 +22,13 @@ __all__ = ["evict_tokens", "paged_decode_weights"]
 def paged_decode_weights(q, k_cache, v_cache, block_table, seqlen, weights, *, scale: float | None = None, out=None,
                          workspace=None):
     """Decode one query token per row (``paged_decode``), and add to ``weights[b, g, j]``, for every token ``j``
-    below ``seqlen[b]``, its attention weight summed over the query heads of kv head ``g`` (two kernel launches).
+    below ``seqlen[b]``, its attention weight summed over the query heads of kv head ``g`` (one kernel launch for few
+    rows, else one for every 4096 rows and one for the sums).
 
     ``weights`` is float32 ``(B, H_kv, W)``, ``W`` at least the table's capacity, updated in place; what lies at
     or past a row's length is left as it is. A row's weights of one step sum to the number of query heads per
-    kv head. ``workspace`` as in :func:`model.paged_window.paged_decode_window`; a call also takes
-    4 bytes per query head and token of the table from the allocator while it runs. Other arguments and
+    kv head. ``workspace`` as in :func:`model.paged_window.paged_decode_window`; a call of more than a few rows
+    also takes 4 bytes per query head and token of the table from the allocator while it runs. Other arguments and
     types as there.
     """
     ops = _native.ops or _native.require_ops()
@@ -44,7 +44,7 @@ def evict_tokens(k_caches, v_caches, block_table, seqlen, weights, keep: int, *,
     keeps the lower ``j``, NaN counts as the smallest. The kept tokens' K and V move, in their order, to
     positions ``0 .. keep - 1`` of the row's pages, so heads of one row may hold different tokens there.
 
-    ``k_caches`` / ``v_caches``: one pool per layer, of one layout. ``weights`` float32
+    ``k_caches`` / ``v_caches``: one pool per layer, of one layout, each named once. ``weights`` float32
     ``(n_layer, B, H_kv, W)``, ``W`` at least the table's capacity. With ``new_table`` (int32 ``(B, max_blocks)``) the kept tokens go
     to its pages instead, shorter rows are copied there whole, and the old pages keep what they hold: that is
     for rows whose pages others share. A block that is written for one row must be read or written

@@ -1,8 +1,8 @@
 """Attention over a paged KV cache that sees a window: the last ``window`` tokens and the first ``sinks``.
 
 Key ``j`` is visible to the query at position ``i`` if ``j <= i`` and (``i - j < window`` or ``j < sinks``). A
-row's step then costs its window, not its length, and pages that hold no visible token are neither looked
-up nor read: their blocks may be given back (``model.paged.PagedKV(window=, sinks=)`` says which). The
+row's step then costs its window, not its length, and what a table names for pages that hold no
+visible token does not matter: their blocks may be given back (``model.paged.PagedKV(window=, sinks=)`` says which). The
 reference has no windowed attention to mirror.
 
 * :func:`paged_decode_window` -- one query token per row (``paged_decode``'s contract);

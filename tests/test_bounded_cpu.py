@@ -68,6 +68,15 @@ def test_evict_refuses(over, status):
     assert _evict(**over) == status
 
 
+def test_evict_refuses_a_pool_named_twice():
+    at = 1 << 20  # any aligned address: it is refused before anything is read
+    pools = [(ctypes.c_void_p * 2)(at, at + (1 << 16)), (ctypes.c_void_p * 2)(at + (2 << 16), at)]
+    table = ctypes.c_void_p(at)
+    status = _native.lib.pd_evict(pools[0], pools[1], 2, 8, 16, 2, 64, _native.PD_BF16, S3, S3, table, 4, 4, None, 0, 0, table,
+                                  table, table, S3, table, S3, 64, 1, 8, 2, 1, table, 1 << 20, None)
+    assert status == INVALID and b"named twice" in _native.lib.pd_last_error_string()
+
+
 def test_weights_refuse():
     f = _native.lib.pd_decode_weights
     args = lambda wlen, hkv=2: (None, 0, 0, None, None, 8, 16, S3, S3, None, 4, 4, None, None, 0, 0, wlen, None, 0, 0, 1, 2 * hkv,  # noqa: E731

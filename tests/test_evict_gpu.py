@@ -79,6 +79,26 @@ def test_weights_beside_others():
     assert torch.equal(captured, out) and torch.equal(again, third)
 
 
+@pytest.mark.parametrize("lens", [[900], [700, 0, 33] * 30])
+def test_a_wait_that_runs_out_is_reported(lens):
+    """Under the test limit every wait gives up at once: the flag is set, the kernels return, the next call is right."""
+    q, k, v, table, seqlen, w = _weights_case(lens, 8, 2, 128, 16, BF16)
+    before = w.clone()
+    limit = _native.get_wait_limit()
+    try:
+        _native.set_wait_limit(10)
+        paged_decode_weights(q, k, v, table, seqlen, w)
+        torch.cuda.synchronize()
+        assert _native.device_error(clear=True) & _native.DEVERR_WAIT_TIMEOUT
+    finally:
+        _native.set_wait_limit(limit)
+    w.copy_(before)
+    out, bound, sums, off = weights_reference(q, k, v, table, lens, w)
+    check(paged_decode_weights(q, k, v, table, seqlen, w), out, bound)
+    check(w, sums, off)
+    assert _native.device_error() == 0
+
+
 def test_weights_of_nan_past_the_row():
     lens = [100, 3]
     q, k, v, table, seqlen, w = _weights_case(lens, 4, 2, 128, 16, BF16)
@@ -287,6 +307,10 @@ def test_refusals():
     refused(match="seqlen_out", seqlen_out=seqlen.long())
     refused(match="weights_out must be", weights_out=w[..., :-1])
     refused(match="must not overlap", weights=w[:1].expand(2, -1, -1, -1), weights_out=w[:1].expand(2, -1, -1, -1))
+    room = torch.zeros(w.numel() + 4, device="cuda")
+    refused(match="not as weights itself", weights=room[:w.numel()].view(w.shape), weights_out=room[4:].view(w.shape))
+    refused(match="named twice", k_caches=[ks[0], ks[0]])
+    refused(match="named twice", v_caches=[vs[0], ks[1]])
     refused(match="int32", block_table=table.long())
     refused(RuntimeError, "requires CUDA", k_caches=[x.cpu() for x in ks], v_caches=vs)
     refused(match="seqlen is on", seqlen=seqlen.cpu())

@@ -7,7 +7,8 @@ import torch
 
 from bounded_reference import check, chunk_reference, make_pools
 from model import _native
-from model.paged_window import decode_workspace, paged_decode_window
+from model.paged_window import decode_workspace, paged_decode_window, paged_prefill_window
+from model.triton_decode import paged_decode_plan
 
 pytestmark = pytest.mark.gpu
 
@@ -147,6 +148,49 @@ def test_streams_and_graphs():
     torch.cuda.synchronize()
     for got, ref in zip([*outs, eager], want):
         assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("lens,hkv,group,d,dtype", [([900], 8, 2, 128, BF16), ([300] * 9, 2, 4, 64, F16),
+                                                    ([900, 5, 300] * 20, 8, 2, 128, BF16)])
+def test_a_wait_that_runs_out_is_reported(lens, hkv, group, d, dtype):
+    """Under the test limit every wait gives up at once: the flag is set, the kernel returns, the next call is right."""
+    case = _case(lens, hkv, group, d, 16, dtype)
+    want = paged_decode_window(*case, 700, sinks=4)
+    limit = _native.get_wait_limit()
+    try:
+        _native.set_wait_limit(10)
+        paged_decode_window(*case, 700, sinks=4)
+        torch.cuda.synchronize()
+        assert _native.device_error(clear=True) & _native.DEVERR_WAIT_TIMEOUT
+    finally:
+        _native.set_wait_limit(limit)
+    for _ in range(2):  # the workspace that the call left
+        assert torch.equal(paged_decode_window(*case, 700, sinks=4), want)
+    assert _native.device_error() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_what_a_kernel_two_back_wrote(rows):
+    """A plan whose launches overlap reads lengths and pools early: the call between it and the kernel that wrote
+    them lets it in only when that kernel is through."""
+    q, k, v, table, seqlen = _case([900] * rows, 8, 2, 128, 16, BF16)
+    other = _case([60], 8, 2, 128, 16, BF16, seed=9)
+    plan = paged_decode_plan(q, [k], [v], table, seqlen, window=300, sinks=4)
+    values = [torch.randn(v.shape, dtype=BF16, device="cuda") for _ in range(4)]
+    lens = [torch.full_like(seqlen, n) for n in (900, 333, 1, 600)]
+    want = [chunk_reference(q, k, x, table, list(range(rows + 1)), n.tolist(), 300, 4) for x, n in zip(values, lens)]
+    cu, mid = torch.tensor([0, 1], dtype=torch.int32, device="cuda"), []
+    between = [lambda: paged_decode_window(*other, 20),
+               lambda: paged_prefill_window(other[0], *other[1:4], cu, other[4], 1, 20),
+               lambda: paged_decode_window(q, k, v, table, seqlen, 300, sinks=4)]
+    for call in between:
+        for x, n, ref in zip(values, lens, want):  # nothing waits in here for the device
+            v.copy_(x)
+            seqlen.copy_(n)
+            call()
+            mid.append((plan.run(0, q, overlap=True), ref))
+    for got, ref in mid:
+        check(got, *ref)
 
 
 def test_empty_batch_and_table():

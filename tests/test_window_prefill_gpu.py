@@ -191,9 +191,11 @@ def test_empty_calls():
     assert _run((q, k, v, table[:, :0], cu, lens), 8, 0).abs().max() == 0
 
 
-def test_a_wait_that_runs_out_is_reported():
+@pytest.mark.parametrize("rows,hkv,group,d,dtype", [([(300, 900)], 4, 2, 128, BF16), ([(8, 900)], 1, 4, 64, F16),
+                                                    ([(600, 900)] * 20, 4, 4, 128, F16), ([(40, 700)], 2, 2, 256, BF16)])
+def test_a_wait_that_runs_out_is_reported(rows, hkv, group, d, dtype):
     """Under the test limit every wait gives up at once: the flag is set, the kernel returns, the next call is right."""
-    case = _case([(300, 900)], 4, 2, 128, 16, BF16)
+    case = _case(rows, hkv, group, d, 16, dtype)
     want = _run(case, 200, 4)
     limit = _native.lib.pd_get_wait_limit()
     try:
@@ -230,6 +232,7 @@ def test_refusals():
     refused(match="seqlen_k must be 1-D", seqlen_k=lens_t[None])
     refused(match="multiple of n_kv_head", q=q[:, :6])
     refused(match="out must be", out=torch.empty_like(q)[:5])
+    refused(match="share memory with q", out=q)
     refused(match="seqlen_k is on", seqlen_k=lens_t.cpu())
     refused(RuntimeError, "requires CUDA", q=q.cpu())
     refused(TypeError, max_seqlen_q="10")
