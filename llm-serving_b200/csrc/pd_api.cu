@@ -597,9 +597,11 @@ int cluster_rooms(int dev, int log2_split) {
 }
 
 // Whether a windowed or weights call takes the kernel of few rows, and how: every item's CTAs have to be on the GPU
-// at once (one to an SM), and a warp's run of tiles has to be short, as only the items' clusters stream (bf16, 8 kv
-// heads of 128: one row of 1024 tokens 6.1 us here, 15.4 by the kernel of many rows). `max_tiles` bounds a row's
-// visible tiles (the lengths are on the device).
+// at once (one to an SM), and a warp's run of tiles has to be short, as only the items' clusters stream, and shorter where
+// its scores take a stage's shared memory. bf16, 8 kv heads of 128, this kernel against the one of many rows: one row
+// of 1024 tokens 5.3 us against 15.4, with weights 7.0 / 20.0; 8 rows of 4096 (runs of 16) 24.8 / 30.3 and 35.9 / 35.4;
+// 16 of 4096 (runs of 32) 44.2 / 49.2 and 65.4 / 54.4. `max_tiles` bounds a row's visible tiles (the lengths are on the
+// device).
 bool use_cluster(const Geometry& g, int64_t batch, int n_kv_head, int64_t capacity, int window, int sinks, int dev,
                  ClusterDecode* c, int* stages) {
   const bool weights = g.variant == SCORES;
@@ -612,7 +614,7 @@ bool use_cluster(const Geometry& g, int64_t batch, int n_kv_head, int64_t capaci
   int log2_split = 0;
   while (log2_split < 3 && items <= cluster_rooms(dev, log2_split + 1) && max_tiles > (int64_t(8) << log2_split)) ++log2_split;
   const int64_t run = (max_tiles + (int64_t(8) << log2_split) - 1) / (int64_t(8) << log2_split);  // tiles of a warp
-  if (run > 32) return false;
+  if (run > (weights ? 16 : 32)) return false;
   c->log2_split = log2_split;
   c->scores_bytes = 0;
   *stages = 3;
