@@ -19,6 +19,8 @@ struct WindowPrefillParams {
   int64_t k_sb, k_sn, k_sh, v_sb, v_sn, v_sh;  // block, token, head
   int32_t total_q, max_seqlen_q;
   int32_t batch, n_kv_head, group;
+  uint32_t group_mul;  // division by group (set by the launch)
+  int32_t group_shift;
   int32_t max_blocks, capacity;
   int32_t log2_bs, log2_box;  // tokens of a block, and of a copy (window_box_tokens)
   int32_t window, sinks;

@@ -183,6 +183,13 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
   const uint32_t sbase = smem_addr(smem);
   auto bar = [&](int slot) -> uint32_t { return sbase + uint32_t(slot) * 8u; };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Bars::ABORT);
+  // Query blocks slowest and last ones first: a prompt's first blocks have the fewest keys.
+  const int split = 1 << log2_split, rank = int(blockIdx.x) & (split - 1), work = int(blockIdx.x) >> log2_split;
+  const int b = work % p.batch, pair = work / p.batch;
+  const int h = pair % p.n_kv_head;
+  const int qblock = blocks - 1 - pair / p.n_kv_head;
+  // n / group, 0 <= n < 2^31 (launch_t: group_mul is 2^group_shift / group rounded up)
+  auto tokens_of = [&](int n) -> int { return int((uint64_t(uint32_t(n)) * p.group_mul) >> p.group_shift); };
 
   if (warp == C::S_WARP) {
     if (lane == 0) {
@@ -218,12 +225,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
   // must not be in the way of this one's, and what it reads early must not be an earlier kernel's (pd_decode_kernel.cuh).
   griddep_launch_dependents();
 
-  // Query blocks slowest and last ones first: a prompt's first blocks have the fewest keys.
-  const int split = 1 << log2_split, rank = int(blockIdx.x) & (split - 1), work = int(blockIdx.x) >> log2_split;
-  const int pairs = p.batch * p.n_kv_head;
-  const int b = work % p.batch;
-  const int h = (work / p.batch) % p.n_kv_head;
-  const int qblock = blocks - 1 - work / pairs;
   const int q_begin = min(max(__ldg(p.cu_q + b), 0), p.total_q);
   const int chunk = max(min(max(__ldg(p.cu_q + b + 1), 0), p.total_q) - q_begin, 0);
   const int sq = min(chunk, p.max_seqlen_q);
@@ -237,8 +238,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
   Keys keys;
   {
     const int last = min(row0 + ROWS, rows) - 1;
-    const int end = row0 < rows ? max(ctx + last / p.group + 1, 0) : 0;  // <= lk
-    keys.first = max(ctx + row0 / p.group - p.window + 1, 0);
+    const int end = row0 < rows ? max(ctx + tokens_of(last) + 1, 0) : 0;  // <= lk
+    keys.first = max(ctx + tokens_of(row0) - p.window + 1, 0);
     const int head = (min(p.sinks, end) + box - 1) >> p.log2_box << p.log2_box;
     keys.gap = max((keys.first >> p.log2_box << p.log2_box) - head, 0);
     keys.head = keys.gap > 0 ? head : 0;
@@ -423,8 +424,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
     {
       const int u = tid % LANES;
       const int m0 = row0 + tid / LANES;
-      int mt = m0 / p.group, mh = m0 - mt * p.group;
-      const int dt = STEP / p.group, dh = STEP - dt * p.group;
+      int mt = tokens_of(m0), mh = m0 - mt * p.group;
+      const int dt = tokens_of(STEP), dh = STEP - dt * p.group;
       const T* base = reinterpret_cast<const T*>(p.q) + int64_t(q_begin) * p.q_st + int64_t(h) * p.group * p.q_sh + u * 8;
 #pragma unroll 4
       for (int rr = tid / LANES; rr < ROWS; rr += STEP) {
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
     const float mul = fmaxf(fabsf(p.scale_log2), 1.2e-38f);
     // Keys of the CTA that this row sees: below `own_sinks`, and first_key .. last_key. Rows past the chunk's
     // end take the last row's, so that they ask for no mask of their own.
-    const int at = ctx + min(n, rows - 1) / p.group;  // position
+    const int at = ctx + tokens_of(min(n, rows - 1));  // position
     const int last_key = at - keys.gap;
     const int first_key = max(at - p.window + 1 - keys.gap, keys.head);
     const int own_sinks = min(p.sinks, last_key + 1);
@@ -466,8 +467,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
     const bool idle = row0 + warp * 32 >= rows;  // no row of this warp is one of the chunk's: whatever P is there serves
     for (int i = 0; i < steps; ++i) {
       const int sb = i & 1;
-      if (__any_sync(FULL_MASK, *abort_flag != 0) ||
-          !warp_wait_phase(bar(Bars::S_FULL + sb), uint32_t(i >> 1) & 1u, p.wait_ns)) {
+      // (where another role has failed no further S comes, and this wait ends by its limit)
+      if (!warp_wait_phase(bar(Bars::S_FULL + sb), uint32_t(i >> 1) & 1u, p.wait_ns)) {
         ok = false;
         break;
       }
@@ -617,8 +618,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
       __syncwarp();
       constexpr int AT_ONCE = 32 / LANES;  // rows of a store
       const int u = lane % LANES, r0 = warp * 32 + lane / LANES, m0 = row0 + r0;
-      int mt = m0 / p.group, mh = m0 - mt * p.group;
-      const int dt = AT_ONCE / p.group, dh = AT_ONCE - dt * p.group;
+      int mt = tokens_of(m0), mh = m0 - mt * p.group;
+      const int dt = tokens_of(AT_ONCE), dh = AT_ONCE - dt * p.group;
       T* base = reinterpret_cast<T*>(p.out) + int64_t(q_begin) * p.o_st + int64_t(h) * p.group * p.o_sh + u * 8;
 #pragma unroll 4
       for (int i = 0; i < 32; i += AT_ONCE) {
@@ -633,7 +634,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
       }
       unsigned again = __ballot_sync(FULL_MASK, whole != 0.f);  // (a NaN is not 0)
       while (again != 0u) {
-        const int m = row0 + warp * 32 + __ffs(again) - 1, t = m / p.group;
+        const int m = row0 + warp * 32 + __ffs(again) - 1, t = tokens_of(m);
         again &= again - 1u;
         __syncwarp();  // this warp has stored the row
         row_again<T, D>(p, b, h, lk, q_begin + t, h * p.group + m - t * p.group, ctx + t);
@@ -680,7 +681,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
             sum.w = fmaf(f, v[k].w, sum.w);
           }
         }
-        const int n = row0 + r, t = n / p.group;
+        const int n = row0 + r, t = tokens_of(n);
         const float inv = ctx + t < 0 ? 0.f : 1.f / L;  // a row that sees no key gives zeros
         uint2 w;
         w.x = E::pack2(sum.x * inv, sum.y * inv);
@@ -694,7 +695,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");
       for (int i = warp; i < mine; i += C::SOFTMAX_WARPS) {
-        const int r = (i << log2_split) + rank, m = row0 + r, t = m / p.group;
+        const int r = (i << log2_split) + rank, m = row0 + r, t = tokens_of(m);
         if (reinterpret_cast<const float*>(smem + C::OFF_AGAIN)[r] != 0.f)
           row_again<T, D>(p, b, h, lk, q_begin + t, h * p.group + m - t * p.group, ctx + t);
       }
@@ -718,12 +719,18 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
 }
 
 template <typename T, int D>
-cudaError_t launch_t(const WindowPrefillParams& p, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
+cudaError_t launch_t(const WindowPrefillParams& p0, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
   using C = Cfg<D>;
   auto fn = pd_window_prefill_kernel<T, D>;
   static SmemRaised raised{};
   const cudaError_t err = raise_smem_limit(fn, C::SMEM, raised);
   if (err != cudaSuccess) return err;
+  WindowPrefillParams p = p0;
+  // With 2^(31 + l) / group rounded up, group <= 2^l, the product's excess stays below one part in n < 2^31.
+  int l = 0;
+  while ((int64_t(1) << l) < p.group) ++l;
+  p.group_shift = 31 + l;
+  p.group_mul = uint32_t(((uint64_t(1) << p.group_shift) + p.group - 1) / p.group);
   const int64_t rows = int64_t(p.max_seqlen_q) * p.group;
   const int64_t blocks = (rows + ROWS - 1) / ROWS;
   const int64_t ctas = blocks * p.batch * p.n_kv_head;
