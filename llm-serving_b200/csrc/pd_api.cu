@@ -585,44 +585,54 @@ int run_prepared(const Prepared& P, const CUtensorMap& kmap, const CUtensorMap& 
 }
 
 // cluster_room of a device, asked once.
-int cluster_rooms(int dev, int log2_split) {
-  static std::atomic<int> known[kMaxDevices][4];  // + 1
-  std::atomic<int>& room = known[dev][log2_split];
+int cluster_rooms(int dev, int warps, int log2_split) {
+  static std::atomic<int> known[2][kMaxDevices][4];  // + 1
+  std::atomic<int>& room = known[warps == 4][dev][log2_split];
   int n = room.load(std::memory_order_relaxed);
   if (n == 0) {
-    n = cluster_room(log2_split) + 1;
+    n = cluster_room(warps, log2_split) + 1;
     room.store(n, std::memory_order_relaxed);
   }
   return n - 1;
 }
 
 // Whether a windowed or weights call takes the kernel of few rows, and how: every item's CTAs have to be on the GPU
-// at once (one to an SM), and a warp's run of tiles has to be short, as only the items' clusters stream, and shorter where
-// its scores take a stage's shared memory. bf16, 8 kv heads of 128, this kernel against the one of many rows: one row
-// of 1024 tokens 5.3 us against 15.4, with weights 7.0 / 20.0; 8 rows of 4096 (runs of 16) 24.8 / 30.3 and 35.9 / 35.4;
-// 16 of 4096 (runs of 32) 44.2 / 49.2 and 65.4 / 54.4. `max_tiles` bounds a row's visible tiles (the lengths are on the
-// device).
+// at once, and a warp's run of tiles has to be short, as an item has no warps but its cluster's. `max_tiles` bounds a
+// row's visible tiles (the lengths are on the device).
+//
+// CTAs of eight warps, one to an SM, while items can be split between two of them, else of four, two to an SM. A warp
+// takes some 1.15 us a tile and the start 5, the kernel of many rows 11 and the same per tile over all the GPU's warps;
+// rows of uneven lengths are its better case, so it is weighed with three quarters of the tiles. bf16, 8 kv heads of
+// 128, this kernel against that one, us, windows and (weights), rows of equal length:
+//   1 row of 1024 5.2 / 15.1 (7.1 / 19.6); 8 of 4096, runs of 16, 24.9 / 30.0 (30.2 / 35.3); 10 of 2048, 16,
+//   23.7 / 22.4 (28.9 / 25.9); 32 of 512, 8, 14.5 / 19.3 (16.6 / 22.9); 32 of 1024, 16, 23.8 / 27.8 (28.3 / 33.1); 32 of
+//   2048, 32, 43.8 / 48.2 (65.4 / 54.1); of lengths 0-n: 32 of 1024 21.5 / 19.7, 32 of 2048 40.0 / 30.7.
 bool use_cluster(const Geometry& g, int64_t batch, int n_kv_head, int64_t capacity, int window, int sinks, int dev,
                  ClusterDecode* c, int* stages) {
   const bool weights = g.variant == SCORES;
   if (!g.mma || g.variant == PLAIN || (weights && g.n_gchunks != 1)) return false;
   const int64_t items = batch * n_kv_head * g.n_gchunks;
-  if (items < 1 || items > sm_count(dev)) return false;
+  if (items < 1 || items > cluster_rooms(dev, 4, 0)) return false;
   int64_t keys = capacity;
   if (g.variant == WINDOW) keys = std::min(keys, int64_t(window) + sinks + 2 * g.tile);
   const int64_t max_tiles = (keys + g.tile - 1) / g.tile;
+  const int warps = items <= cluster_rooms(dev, 8, 1) ? 8 : 4;
   int log2_split = 0;
-  while (log2_split < 3 && items <= cluster_rooms(dev, log2_split + 1) && max_tiles > (int64_t(8) << log2_split)) ++log2_split;
-  const int64_t run = (max_tiles + (int64_t(8) << log2_split) - 1) / (int64_t(8) << log2_split);  // tiles of a warp
+  while (log2_split < 3 && items <= cluster_rooms(dev, warps, log2_split + 1) && max_tiles > (int64_t(warps) << log2_split))
+    ++log2_split;
+  const int64_t run = (max_tiles + (int64_t(warps) << log2_split) - 1) / (int64_t(warps) << log2_split);  // tiles of a warp
   if (run > (weights ? 16 : 32)) return false;
+  if (warps == 4 && run > 7 + items * max_tiles * 3 / (4 * 8 * int64_t(sm_count(dev)))) return false;
+  c->warps = warps;
   c->log2_split = log2_split;
   c->scores_bytes = 0;
   *stages = 3;
   if (weights) {
-    const int64_t bytes = 8 * run * g.tile * g.gt * 4;
-    if (bytes > 65536) return false;
+    const int64_t bytes = warps * run * g.tile * g.gt * 4;
+    const int64_t room = cluster_smem(warps, g.gt, 8 << g.d_index) - 1024 - bytes;
+    *stages = room >= int64_t(3) * warps * g.stage_bytes ? 3 : 2;
+    if (room < int64_t(*stages) * warps * g.stage_bytes) return false;
     c->scores_bytes = int32_t(bytes);
-    *stages = 2;
   }
   return true;
 }

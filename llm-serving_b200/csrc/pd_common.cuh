@@ -502,7 +502,14 @@ struct DecodeParams {
 };
 
 // What the decode of few rows (pd_decode_cluster.cuh) takes beside DecodeParams.
+// Dynamic shared memory that a CTA of `warps` (8: one on an SM, 4: two) of the few rows' kernel may have, next to its
+// static arrays.
+constexpr int cluster_smem(int warps, int gt, int head_dim) {
+  return 233472 * warps / 8 - 1024 - (gt * head_dim * 4 + 1024);
+}
+
 struct ClusterDecode {
+  int32_t warps;         // of a CTA
   int32_t log2_split;    // CTAs of an item's cluster
   int32_t scores_bytes;  // shared memory for the scores of a CTA's warps (weights)
   float* weights;        // row b, kv head h, token j at b * w_sb + h * w_sh + j

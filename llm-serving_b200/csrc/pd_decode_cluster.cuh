@@ -10,22 +10,22 @@
 // (one q-head chunk per kv head, so that a sum has one writer).
 //
 // Bound by latency: length, block ids, tiles, merge, each a round trip; every warp's first loads go out before it
-// waits for anything.
+// waits for anything. One row, 8 kv heads of 128, a window of 1024: 6.2 us, of which 4 are its 4 MB's round trips and
+// 2 the merge (0.65 would move the bytes); with weights over 700 tokens 7.0. 61 rows of 2 kv heads of 256, windows of
+// 777: 23.3 us, 95 MB at 4.1 TB/s: the longest rows' runs of 13 tiles a warp.
 #pragma once
 
 #include "pd_decode_kernel.cuh"
 
 namespace pd {
 
-constexpr int CLUSTER_WARPS = 8;
-
-template <typename T, int D, int GT, bool LOG>
-__global__ void __launch_bounds__(CLUSTER_WARPS * 32, 1)
+// W warps a CTA: eight of one CTA on an SM, or four of two, so that more items run at once.
+template <typename T, int D, int GT, bool LOG, int W>
+__global__ void __launch_bounds__(W * 32, 8 / W)
     pd_decode_cluster_kernel(const __grid_constant__ DecodeParams p, const __grid_constant__ ClusterDecode c,
                              const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using C = DecodeCfg<T, D, GT>;
   using E = Elem<T>;
-  constexpr int W = CLUSTER_WARPS;
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ float s_m[W][GT], s_l[W][GT];           // the warps'
   __shared__ __align__(16) float s_cta[2 * GT];      // the CTA's m, then l
@@ -245,15 +245,15 @@ __global__ void __launch_bounds__(CLUSTER_WARPS * 32, 1)
   if (split > 1) cluster_sync();  // nothing of this CTA is read any more
 }
 
-template <typename T, int D, int GT, bool LOG>
-cudaError_t launch_cluster(const DecodeParams& p, const ClusterDecode& c, const CUtensorMap& kmap, const CUtensorMap& vmap,
-                           int items, cudaStream_t stream) {
-  auto fn = pd_decode_cluster_kernel<T, D, GT, LOG>;
-  constexpr int MOST = MAX_DYNAMIC_SMEM - 16384;  // less the static arrays
+template <typename T, int D, int GT, bool LOG, int W>
+cudaError_t launch_cluster_w(const DecodeParams& p, const ClusterDecode& c, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                             int items, cudaStream_t stream) {
+  auto fn = pd_decode_cluster_kernel<T, D, GT, LOG, W>;
+  constexpr int MOST = cluster_smem(W, GT, D);
   static SmemRaised raised{};
   const cudaError_t err = raise_smem_limit(fn, MOST, raised);
   if (err != cudaSuccess) return err;
-  const size_t smem = size_t(c.scores_bytes) + 1024 + size_t(CLUSTER_WARPS) * p.stages * DecodeCfg<T, D, GT>::STAGE_BYTES;
+  const size_t smem = size_t(c.scores_bytes) + 1024 + size_t(W) * p.stages * DecodeCfg<T, D, GT>::STAGE_BYTES;
   if (smem > size_t(MOST)) return cudaErrorInvalidValue;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -264,7 +264,7 @@ cudaError_t launch_cluster(const DecodeParams& p, const ClusterDecode& c, const 
   attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(items) << c.log2_split);
-  cfg.blockDim = dim3(CLUSTER_WARPS * 32);
+  cfg.blockDim = dim3(W * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -272,12 +272,19 @@ cudaError_t launch_cluster(const DecodeParams& p, const ClusterDecode& c, const 
   return cudaLaunchKernelEx(&cfg, fn, p, c, kmap, vmap);
 }
 
-// Clusters of 2^log2_split CTAs of this kernel that the current device runs at once (a cluster stays in one of its
-// groups of multiprocessors: of eight CTAs, 15 clusters on 148), 0 where it cannot be asked.
-template <typename T>
+template <typename T, int D, int GT, bool LOG>
+cudaError_t launch_cluster(const DecodeParams& p, const ClusterDecode& c, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                           int items, cudaStream_t stream) {
+  return c.warps == 4 ? launch_cluster_w<T, D, GT, LOG, 4>(p, c, kmap, vmap, items, stream)
+                      : launch_cluster_w<T, D, GT, LOG, 8>(p, c, kmap, vmap, items, stream);
+}
+
+// Clusters of 2^log2_split CTAs of W warps that the current device runs at once (a cluster stays in one of its
+// groups of multiprocessors: of eight CTAs of eight warps, 15 clusters on 148), 0 where it cannot be asked.
+template <typename T, int W>
 int cluster_room_of(int log2_split) {
-  auto fn = pd_decode_cluster_kernel<T, 128, 2, false>;
-  constexpr int SMEM = MAX_DYNAMIC_SMEM - 16384;
+  auto fn = pd_decode_cluster_kernel<T, 128, 2, false, W>;
+  constexpr int SMEM = cluster_smem(W, 2, 128);
   static SmemRaised raised{};
   if (raise_smem_limit(fn, SMEM, raised) != cudaSuccess) return 0;
   cudaLaunchAttribute attr[1];
@@ -287,7 +294,7 @@ int cluster_room_of(int log2_split) {
   attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(1u << log2_split);
-  cfg.blockDim = dim3(CLUSTER_WARPS * 32);
+  cfg.blockDim = dim3(W * 32);
   cfg.dynamicSmemBytes = SMEM;
   cfg.attrs = attr;
   cfg.numAttrs = 1;

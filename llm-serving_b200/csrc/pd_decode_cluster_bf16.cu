@@ -17,6 +17,8 @@ ClusterLaunchFn cluster_launcher_bf16(bool weights, int d_index, int gt_index) {
   return kClusterTable[weights ? 1 : 0][d_index - 3][gt_index];
 }
 
-int cluster_room(int log2_split) { return cluster_room_of<__nv_bfloat16>(log2_split); }
+int cluster_room(int warps, int log2_split) {
+  return warps == 4 ? cluster_room_of<__nv_bfloat16, 4>(log2_split) : cluster_room_of<__nv_bfloat16, 8>(log2_split);
+}
 
 }  // namespace pd

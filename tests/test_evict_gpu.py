@@ -35,7 +35,7 @@ def test_weights(dtype, hkv, group, d, bs):
     assert _native.device_error() == 0
 
 
-@pytest.mark.parametrize("rows,length", [(1, 5000), (40, 3000), (150, 300)])
+@pytest.mark.parametrize("rows,length", [(1, 5000), (40, 3000), (150, 300), (12, 900), (24, 400), (35, 700)])
 def test_weights_of_many_and_long_rows(rows, length):
     gen = torch.Generator().manual_seed(rows)
     lens = torch.randint(0, length + 1, (rows,), generator=gen).tolist()
@@ -79,7 +79,7 @@ def test_weights_beside_others():
     assert torch.equal(captured, out) and torch.equal(again, third)
 
 
-@pytest.mark.parametrize("lens", [[900], [700, 0, 33] * 30])
+@pytest.mark.parametrize("lens", [[900], [300, 0] * 12, [700, 0, 33] * 30])
 def test_a_wait_that_runs_out_is_reported(lens):
     """Under the test limit every wait gives up at once: the flag is set, the kernels return, the next call is right."""
     q, k, v, table, seqlen, w = _weights_case(lens, 8, 2, 128, 16, BF16)

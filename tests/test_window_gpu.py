@@ -48,7 +48,8 @@ def test_heads_and_blocks(dtype, hkv, group, d, bs):
     _check([0, 700, 3], hkv, group, d, bs, dtype, 300, 0, seed=2)
 
 
-@pytest.mark.parametrize("rows,length,window,sinks", [(1, 5000, 1024, 4), (1, 5000, 3, 0), (40, 3000, 700, 9), (150, 300, 64, 1)])
+@pytest.mark.parametrize("rows,length,window,sinks", [(1, 5000, 1024, 4), (1, 5000, 3, 0), (40, 3000, 700, 9), (150, 300, 64, 1),
+                                                       (12, 1000, 500, 4), (24, 400, 1 << 20, 0), (33, 700, 400, 20)])
 def test_long_and_many(rows, length, window, sinks):
     gen = torch.Generator().manual_seed(rows)
     lens = torch.randint(0, length + 1, (rows,), generator=gen).tolist()
@@ -150,7 +151,7 @@ def test_streams_and_graphs():
         assert torch.equal(got, ref)
 
 
-@pytest.mark.parametrize("lens,hkv,group,d,dtype", [([900], 8, 2, 128, BF16), ([300] * 9, 2, 4, 64, F16),
+@pytest.mark.parametrize("lens,hkv,group,d,dtype", [([900], 8, 2, 128, BF16), ([300] * 9, 2, 4, 64, F16), ([300, 0] * 12, 8, 2, 128, BF16),
                                                     ([900, 5, 300] * 20, 8, 2, 128, BF16)])
 def test_a_wait_that_runs_out_is_reported(lens, hkv, group, d, dtype):
     """Under the test limit every wait gives up at once: the flag is set, the kernel returns, the next call is right."""
