@@ -604,8 +604,8 @@ int cluster_rooms(int dev, int warps, int log2_split) {
 // takes some 1.15 us a tile and the start 5, the kernel of many rows 11 and the same per tile over all the GPU's warps;
 // rows of uneven lengths are its better case, so it is weighed with three quarters of the tiles. bf16, 8 kv heads of
 // 128, this kernel against that one, us, windows and (weights), rows of equal length:
-//   1 row of 1024 5.2 / 15.1 (7.1 / 19.6); 8 of 4096, runs of 16, 24.9 / 30.0 (30.2 / 35.3); 10 of 2048, 16,
-//   23.7 / 22.4 (28.9 / 25.9); 32 of 512, 8, 14.5 / 19.3 (16.6 / 22.9); 32 of 1024, 16, 23.8 / 27.8 (28.3 / 33.1); 32 of
+//   1 row of 1024 5.2 / 15.1 (7.3 / 19.6); 8 of 4096, runs of 16, 24.9 / 30.0 (28.6 / 35.3); 10 of 2048, 16,
+//   23.7 / 22.4 (28.9 / 25.9); 32 of 512, 8, 14.4 / 19.3 (16.2 / 22.9); 32 of 1024, 16, 23.8 / 27.8 (26.8 / 33.1); 32 of
 //   2048, 32, 43.8 / 48.2 (65.4 / 54.1); of lengths 0-n: 32 of 1024 21.5 / 19.7, 32 of 2048 40.0 / 30.7.
 bool use_cluster(const Geometry& g, int64_t batch, int n_kv_head, int64_t capacity, int window, int sinks, int dev,
                  ClusterDecode* c, int* stages) {
@@ -621,7 +621,6 @@ bool use_cluster(const Geometry& g, int64_t batch, int n_kv_head, int64_t capaci
   while (log2_split < 3 && items <= cluster_rooms(dev, warps, log2_split + 1) && max_tiles > (int64_t(warps) << log2_split))
     ++log2_split;
   const int64_t run = (max_tiles + (int64_t(warps) << log2_split) - 1) / (int64_t(warps) << log2_split);  // tiles of a warp
-  if (run > (weights ? 16 : 32)) return false;
   if (warps == 4 && run > 7 + items * max_tiles * 3 / (4 * 8 * int64_t(sm_count(dev)))) return false;
   c->warps = warps;
   c->log2_split = log2_split;
@@ -634,6 +633,7 @@ bool use_cluster(const Geometry& g, int64_t batch, int n_kv_head, int64_t capaci
     if (room < int64_t(*stages) * warps * g.stage_bytes) return false;
     c->scores_bytes = int32_t(bytes);
   }
+  if (run > (*stages == 3 ? 32 : 16)) return false;
   return true;
 }
 

@@ -141,6 +141,21 @@ __global__ void __launch_bounds__(W * 32, 8 / W)
     }
   }
 
+  // The sums that this warp's tokens have so far, the first ones under way while the pieces meet.
+  constexpr int AHEAD = 4;
+  float* const sums = LOG ? c.weights + int64_t(b) * c.w_sb + int64_t(h) * c.w_sh : nullptr;
+  float old[AHEAD];
+  auto load_old = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (i0 + u * 32 >= n * C::TILE) break;
+      const int i = i0 + u * 32 + lane;
+      const int j = i < n * C::TILE ? tile_token(i >> C::LOG_TILE) + (i & (C::TILE - 1)) : len;
+      old[u] = j < len ? sums[j] : 0.f;
+    }
+  };
+  if constexpr (LOG) load_old(0);
+
   // ---- the warps' pieces, in their own stages; a warp without tiles has m = -inf and no accumulators
   float* const piece = reinterpret_cast<float*>(my_stages);
   if (n > 0 && ok) {
@@ -231,15 +246,35 @@ __global__ void __launch_bounds__(W * 32, 8 / W)
       s_final[1][tid] = 1.f / l;
     }
     __syncthreads();
-    float* w = c.weights + int64_t(b) * c.w_sb + int64_t(h) * c.w_sh;
-    for (int i = lane; ok && i < n * C::TILE; i += 32) {
-      const int j = tile_token(i >> C::LOG_TILE) + (i & (C::TILE - 1));
-      if (j >= len) continue;
-      float sum = 0.f;
+    float m_of[GT], inv_of[GT];
 #pragma unroll
-      for (int q = 0; q < GT; ++q)
-        if (q < heads) sum = fmaf(exp2f(my_scores[i * GT + q] - s_final[0][q]), s_final[1][q], sum);
-      w[j] += sum;
+    for (int q = 0; q < GT; ++q) {
+      m_of[q] = q < heads ? s_final[0][q] : 0.f;
+      inv_of[q] = q < heads ? s_final[1][q] : 0.f;
+    }
+    for (int i0 = 0; ok && i0 < n * C::TILE; i0 += 32 * AHEAD) {
+      if (i0 > 0) load_old(i0);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (i0 + u * 32 >= n * C::TILE) break;
+        const int i = i0 + u * 32 + lane;
+        const int j = i < n * C::TILE ? tile_token(i >> C::LOG_TILE) + (i & (C::TILE - 1)) : len;
+        if (j >= len) continue;
+        float s[GT];
+        if constexpr (GT >= 4) {
+#pragma unroll
+          for (int q = 0; q < GT; q += 4) *reinterpret_cast<float4*>(s + q) = *reinterpret_cast<const float4*>(my_scores + i * GT + q);
+        } else if constexpr (GT == 2) {
+          *reinterpret_cast<float2*>(s) = *reinterpret_cast<const float2*>(my_scores + i * GT);
+        } else {
+          s[0] = my_scores[i];
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int q = 0; q < GT; ++q)
+          if (q < heads) sum = fmaf(exp2f(s[q] - m_of[q]), inv_of[q], sum);
+        sums[j] = old[u] + sum;
+      }
     }
   }
   if (split > 1) cluster_sync();  // nothing of this CTA is read any more
