@@ -95,6 +95,37 @@ def test_windowed_prompts_and_steps(captured, hkv, group, d):
     assert _native.device_error() == 0
 
 
+@pytest.mark.parametrize("seed", range(6))
+def test_captured_layers_that_overlap(seed):
+    """Every step of overlapped captured layers, each of which may read the split that the layer before it is still
+    recording."""
+    gen = torch.Generator().manual_seed(seed)
+    layers, bs, hkv, heads, d, window, sinks, steps = 3, 16, 2, 8, 256, 50, 5, 40
+    prompts = [130, 3, 60]
+    pool = _pool(layers, 64, hkv, d, heads)
+    manager = BlockManager(64, bs)
+    tables = [manager.reserve(-(-(n + steps) // bs)) for n in prompts]
+    width = max(len(t) for t in tables)
+    table = torch.tensor([t + [0] * (width - len(t)) for t in tables], dtype=torch.int32).cuda()
+    slots = torch.tensor([tables[b][t // bs] * bs + t % bs for b, n in enumerate(prompts) for t in range(n)]).cuda()
+    for layer in range(layers):
+        pool.write_slots(layer, slots, _rand(gen, len(slots), hkv, d), _rand(gen, len(slots), hkv, d))
+    kv = PagedKV(pool, tables, prompts, rope_len=1000, n_head=heads, window=window, sinks=sinks)
+    shape = (layers, len(prompts), hkv, 1, d)
+    q, k, v = _rand(gen, layers, len(prompts), heads, 1, d), _rand(gen, *shape), _rand(gen, *shape)
+    graph = PagedStepGraph(kv, q, k, v)
+    for step in range(steps):
+        for x in (q, k, v):
+            x.copy_(_rand(gen, *x.shape))
+        out = graph.replay()
+        lens = [n + step + 1 for n in prompts]
+        for layer in range(layers):
+            want, bound = chunk_reference(q[layer, :, :, 0], pool.keys[layer], pool.values[layer], table,
+                                          list(range(len(prompts) + 1)), lens, window, sinks)
+            check(out[layer][:, :, 0], want, bound)
+    assert _native.device_error() == 0
+
+
 @pytest.mark.parametrize("captured", [False, True])
 def test_steps_with_weights_and_evictions(captured):
     """Rows of different lengths, several layers, a budget that they pass again and again: cache, weights and
