@@ -56,6 +56,7 @@ SOURCES = [
     "pd_weights.cu",
     "pd_decode_cluster_bf16.cu",
     "pd_decode_cluster_f16.cu",
+    "pd_decode_cluster_f32.cu",
     "pd_prefill.cu",
     "pd_prefill_tc.cu",
     "pd_ops_api.cu",

@@ -607,10 +607,10 @@ int cluster_rooms(int dev, int warps, int log2_split) {
 //   1 row of 1024 5.2 / 15.1 (7.3 / 19.6); 8 of 4096, runs of 16, 24.9 / 30.0 (28.6 / 35.3); 10 of 2048, 16,
 //   23.7 / 22.4 (28.9 / 25.9); 32 of 512, 8, 14.4 / 19.3 (16.2 / 22.9); 32 of 1024, 16, 23.8 / 27.8 (26.8 / 33.1); 32 of
 //   2048, 32, 43.8 / 48.2 (65.4 / 54.1); of lengths 0-n: 32 of 1024 21.5 / 19.7, 32 of 2048 40.0 / 30.7.
-bool use_cluster(const Geometry& g, int64_t batch, int n_kv_head, int64_t capacity, int window, int sinks, int dev,
+bool use_cluster(const Geometry& g, bool fp32, int64_t batch, int n_kv_head, int64_t capacity, int window, int sinks, int dev,
                  ClusterDecode* c, int* stages) {
   const bool weights = g.variant == SCORES;
-  if (!g.mma || g.variant == PLAIN || (weights && g.n_gchunks != 1)) return false;
+  if (!(g.mma || (fp32 && g.d_index >= 3)) || g.variant == PLAIN || (weights && g.n_gchunks != 1)) return false;
   const int64_t items = batch * n_kv_head * g.n_gchunks;
   if (items < 1 || items > cluster_rooms(dev, 4, 0)) return false;
   int64_t keys = capacity;
@@ -621,7 +621,7 @@ bool use_cluster(const Geometry& g, int64_t batch, int n_kv_head, int64_t capaci
   while (log2_split < 3 && items <= cluster_rooms(dev, warps, log2_split + 1) && max_tiles > (int64_t(warps) << log2_split))
     ++log2_split;
   const int64_t run = (max_tiles + (int64_t(warps) << log2_split) - 1) / (int64_t(warps) << log2_split);  // tiles of a warp
-  if (warps == 4 && run > 7 + items * max_tiles * 3 / (4 * 8 * int64_t(sm_count(dev)))) return false;
+  if (warps == 4 && !(fp32 && weights) && run > 7 + items * max_tiles * 3 / (4 * 8 * int64_t(sm_count(dev)))) return false;
   c->warps = warps;
   c->log2_split = log2_split;
   c->scores_bytes = 0;
@@ -634,6 +634,10 @@ bool use_cluster(const Geometry& g, int64_t batch, int n_kv_head, int64_t capaci
     c->scores_bytes = int32_t(bytes);
   }
   if (run > (*stages == 3 ? 32 : 16)) return false;
+  // fp32 tiles take longer by their scores (4 us for 64 of them), the kernel of many rows too, with weights more so: 4
+  // rows of 4096 on 8 heads of 128, 2 to a group, 33.8 / 35.4 (39.8 / 66.2); 12 rows on 3 heads of 64, 5 to a group, of 1024
+  // 20.0 / 29.0, of 4096 67.6 / 44.1; weights of 12 rows of 1024, runs of 16 of four warps, 36.9 / 51.1; with few items it is at its worst (4 rows of 4096, one head of 128, 39.4 / 92.5).
+  if (fp32 && run * g.gt * std::min(8, g.tile) > (weights ? 512 : 256) * (items <= 8 ? 2 : 1)) return false;
   return true;
 }
 
@@ -644,7 +648,7 @@ bool is_small(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim
   if (batch < 1 || max_blocks < 1 || window < (variant == WINDOW ? 1 : 0) || sinks < 0) return false;
   if (geometry(n_head, n_kv_head, head_dim, block_size, dtype, variant, &g) != PD_OK || current_device(&dev) != PD_OK)
     return false;
-  return use_cluster(g, batch, n_kv_head, int64_t(max_blocks) * block_size, window, sinks, dev, c, stages);
+  return use_cluster(g, dtype == PD_F32, batch, n_kv_head, int64_t(max_blocks) * block_size, window, sinks, dev, c, stages);
 }
 
 int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache, const void* v_cache,
@@ -689,8 +693,9 @@ int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache
     p.stages = stages;
     p.wait_ns = g_wait_limit_ns.load(std::memory_order_relaxed);
     const bool weights = variant == SCORES;
-    const ClusterLaunchFn fn = dtype == PD_BF16 ? cluster_launcher_bf16(weights, P.g.d_index, P.g.gt_index)
-                                                : cluster_launcher_f16(weights, P.g.d_index, P.g.gt_index);
+    const ClusterLaunchFn fn = dtype == PD_F32    ? cluster_launcher_f32(weights, P.g.d_index, P.g.gt_index)
+                               : dtype == PD_BF16 ? cluster_launcher_bf16(weights, P.g.d_index, P.g.gt_index)
+                                                  : cluster_launcher_f16(weights, P.g.d_index, P.g.gt_index);
     const cudaError_t e =
         fn(p, c, kmap, vmap, batch * n_kv_head * P.g.n_gchunks, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(e, "decode launch");

@@ -1,10 +1,10 @@
-// pd_decode_cluster.cuh -- paged GQA decode of few rows for sm_100a: windows and attention weights, bf16 / fp16,
-// head_dim 64..256, blocks of at least 8 tokens.
+// pd_decode_cluster.cuh -- paged GQA decode of few rows for sm_100a: windows and attention weights, head_dim 64..256;
+// bf16 / fp16 in blocks of at least 8 tokens, fp32 in any.
 //
 // The function of pd_decode_kernel.cuh's variants where that kernel's start costs more than its work: with so few
 // (row, kv head, q-head chunk) items that all their CTAs run at once, nothing has to be dealt. A cluster of `split` CTAs
 // takes one item and each of its warps an even run of the row's visible tiles (VisibleTiles), through a TMA
-// ring of its own into the tensor-core consumer of pd_decode_mma.cuh. The warps' (m, l, acc) meet in shared memory
+// ring of its own into the tensor-core consumer of pd_decode_mma.cuh (fp32: pd_decode_fma.cuh). The warps' (m, l, acc) meet in shared memory
 // and the CTAs' in distributed shared memory: no workspace, no counter, no second pass over global memory. With
 // weights (LOG) the scores wait in shared memory until the row's m and l are known, and are added in the same launch
 // (one q-head chunk per kv head, so that a sum has one writer).
@@ -15,9 +15,22 @@
 // 777: 23.3 us, 95 MB at 4.1 TB/s: the longest rows' runs of 13 tiles a warp.
 #pragma once
 
+#include "pd_decode_fma.cuh"
 #include "pd_decode_kernel.cuh"
 
 namespace pd {
+
+// Tile math: tensor cores for 16-bit K/V, multiply-adds for fp32; scores and normalisers that a lane holds.
+template <typename T, int D, int GT>
+struct ClusterMath {
+  using W = MmaWorker<T, D, GT>;
+  static constexpr int R = MmaCfg<T, D, GT>::R, L = 2;
+};
+template <int D, int GT>
+struct ClusterMath<float, D, GT> {
+  using W = FmaWorker<D, GT>;
+  static constexpr int R = W::R, L = GT;
+};
 
 // W warps a CTA: eight of one CTA on an SM, or four of two, so that more items run at once.
 template <typename T, int D, int GT, bool LOG, int W>
@@ -93,18 +106,24 @@ __global__ void __launch_bounds__(W * 32, 8 / W)
       const int blk = __shfl_sync(FULL_MASK, win, ((k << log2_nbox) + j) & 31);
       if (lane == 0) {
         const int off = (tok0 + (j << p.log2_box)) & (p.block_size - 1);
-        tma_load_5d_hint(kdst + j * box_bytes, &kmap, full, 0, off, h, 0, blk, kv_policy);
-        tma_load_5d_hint(kdst + uint32_t(C::TILE_BYTES) + j * box_bytes, &vmap, full, 0, off, h, 0, blk, kv_policy);
+        const uint32_t at = kdst + j * box_bytes;
+        if constexpr (sizeof(T) == 4) {
+          tma_load_4d_hint(at, &kmap, full, 0, h, off, blk, kv_policy);
+          tma_load_4d_hint(at + uint32_t(C::TILE_BYTES), &vmap, full, 0, h, off, blk, kv_policy);
+        } else {
+          tma_load_5d_hint(at, &kmap, full, 0, off, h, 0, blk, kv_policy);
+          tma_load_5d_hint(at + uint32_t(C::TILE_BYTES), &vmap, full, 0, off, h, 0, blk, kv_policy);
+        }
       }
     }
   };
   int issued = 0;
   for (; issued < min(n, S); ++issued) issue(issued, issued);
-  MmaWorker<T, D, GT> mw;
+  using M = ClusterMath<T, D, GT>;
+  typename M::W mw;
   mw.init(lane, p.box_tokens, p.log2_box);
   mw.start(reinterpret_cast<const T*>(p.q) + int64_t(b) * p.q_sb, p.q_sh, hq0, heads);
 
-  using M = MmaCfg<T, D, GT>;
   bool ok = true;
   if (n > 0) {
     float sc_cur[M::R], sc_nxt[M::R];
@@ -159,7 +178,7 @@ __global__ void __launch_bounds__(W * 32, 8 / W)
   // ---- the warps' pieces, in their own stages; a warp without tiles has m = -inf and no accumulators
   float* const piece = reinterpret_cast<float*>(my_stages);
   if (n > 0 && ok) {
-    float lt[2];
+    float lt[M::L];
     mw.total_l(lt);
     mw.store_ml(s_m[warp], s_l[warp], lt);
     mw.store_acc(piece);
@@ -229,10 +248,15 @@ __global__ void __launch_bounds__(W * 32, 8 / W)
       }
     }
     const float inv = 1.f / fmaxf(l, 1.f);
-    uint2 o;
-    o.x = E::pack2(a.x * inv, a.y * inv);
-    o.y = E::pack2(a.z * inv, a.w * inv);
-    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + int64_t(b) * p.o_sb + int64_t(hq0 + hd) * p.o_sh + i % GPH * 4) = o;
+    T* const out = reinterpret_cast<T*>(p.out) + int64_t(b) * p.o_sb + int64_t(hq0 + hd) * p.o_sh + i % GPH * 4;
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(out) = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+    } else {
+      uint2 o;
+      o.x = E::pack2(a.x * inv, a.y * inv);
+      o.y = E::pack2(a.z * inv, a.w * inv);
+      *reinterpret_cast<uint2*>(out) = o;
+    }
   }
   if constexpr (LOG) {
     if (tid < heads) {

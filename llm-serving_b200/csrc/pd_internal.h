@@ -26,6 +26,7 @@ DecodeLaunchFn decode_launcher_var_bf16(int d_index, int gt_index);
 // The same for few rows, all of whose CTAs run at once (pd_decode_cluster.cuh).
 ClusterLaunchFn cluster_launcher_f16(bool weights, int d_index, int gt_index);
 ClusterLaunchFn cluster_launcher_bf16(bool weights, int d_index, int gt_index);
+ClusterLaunchFn cluster_launcher_f32(bool weights, int d_index, int gt_index);
 int cluster_room(int warps, int log2_split);  // its clusters of 2^log2_split CTAs that the current device runs at once
 
 // weights[b][h][j] += the sum over the group of exp2(score - m) / l (pd_weights.cu).
