@@ -9,7 +9,8 @@ import torch
 from bounded_reference import check, chunk_reference, evict_reference, weights_reference
 from model import _native
 from model.paged import PagedKV, PagedPool
-from model.paged_window import paged_prefill_window
+from model.paged_evict import evict_tokens, paged_decode_weights
+from model.paged_window import paged_decode_window, paged_prefill_window
 from serve.block_manager import BlockManager
 from serve.graph import PagedStepGraph
 
@@ -187,6 +188,41 @@ def test_steps_with_weights_and_evictions(captured):
             lens = [min(n, keep) for n in lens]
             assert kv.pos.tolist() == lens == kv._host_pos
     assert evictions >= 3 and kv.evicted.tolist() == kv._host_evicted
+    assert _native.device_error() == 0
+
+
+def test_blocks_past_32_bit_offsets():
+    """Pools of more than 2^31 elements give what small ones with the same blocks give, bit for bit."""
+    gen = torch.Generator().manual_seed(4)
+    hkv, group, d, bs, few, many = 8, 2, 128, 16, 96, (1 << 17) + 1000  # 16,384 elements a block
+    lens = [700, 1, 333]
+    small = [_rand(gen, few, bs, hkv, d) for _ in range(2)]
+    big = [torch.empty(many, bs, hkv, d, dtype=small[0].dtype, device="cuda") for _ in range(2)]
+    at = many - few
+    for x, y in zip(big, small):
+        x[at:].copy_(y)
+    ids = torch.randperm(few, generator=gen)
+    width, tables, cursor = -(-max(lens) // bs), torch.zeros(len(lens), -(-max(lens) // bs), dtype=torch.int32), 0
+    for row, n in enumerate(lens):
+        pages = -(-n // bs)
+        tables[row, :pages] = ids[cursor:cursor + pages]
+        cursor += pages
+    tables = tables.cuda()
+    seqlen = torch.tensor(lens, dtype=torch.int32).cuda()
+    q = _rand(gen, 40, hkv * group, d)
+    cu = torch.tensor([0, 30, 31, 40], dtype=torch.int32).cuda()
+    weights = torch.rand(1, len(lens), hkv, width * bs, generator=gen).cuda()
+    results = []
+    for (k, v), table in ((small, tables), (big, tables + at)):
+        w = weights[0].clone()
+        results.append([paged_decode_window(q[:3], k, v, table, seqlen, 200, sinks=4),
+                        paged_prefill_window(q, k, v, table, cu, seqlen, 30, 200, sinks=4),
+                        paged_decode_weights(q[:3], k, v, table, seqlen, w), w,
+                        *evict_tokens([k], [v], table, seqlen, weights, 128, recent=16, sinks=4)])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    for x, y in zip(big, small):
+        assert torch.equal(x[at:], y)
     assert _native.device_error() == 0
 
 
