@@ -8,6 +8,7 @@ import torch
 from bounded_reference import check, evict_reference, make_pools, weights_reference
 from model import _native
 from model.paged_evict import evict_tokens, paged_decode_weights
+from model.paged_window import paged_decode_window
 
 pytestmark = pytest.mark.gpu
 
@@ -47,6 +48,44 @@ def test_weights_of_many_and_long_rows(rows, length):
         out, bound, sums, off = weights_reference(q, k, v, table, lens, w)
         check(paged_decode_weights(q, k, v, table, seqlen, w), out, bound)
         check(w, sums, off)
+
+
+@pytest.mark.parametrize("rows", [9000, 70000])
+def test_more_rows_than_a_launch_takes(rows):
+    """One block a row: decode over a window and with weights in several launches, and eviction of every row."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    d, bs, group, blocks = 64, 16, 2, 300
+    k, v = (torch.randn(blocks, bs, 1, d, generator=gen, device="cuda").to(BF16) for _ in range(2))
+    table = torch.randint(0, blocks, (rows, 1), generator=gen, device="cuda", dtype=torch.int32)
+    lens = torch.randint(0, bs + 1, (rows,), generator=gen, device="cuda", dtype=torch.int32)
+    q = torch.randn(rows, group, d, generator=gen, device="cuda").to(BF16)
+    w = torch.zeros(rows, 1, bs, device="cuda")
+    j = torch.arange(bs, device="cuda")
+    s = torch.einsum("bhd,bjd->bhj", q.double(), k[table[:, 0].long(), :, 0].double()) * d ** -0.5
+    vv = v[table[:, 0].long(), :, 0].double()
+    size = float(torch.einsum("bhd,bjd->bhj", q.abs().double(), k[table[:, 0].long(), :, 0].abs().double()).max()) * d ** -0.5
+    rel = 2.0 ** -16 + 2.0 ** -20 + 2 * (d + 4) * 2.0 ** -24 * size + 2 * bs * 2.0 ** -24
+    for window in (None, 5):
+        seen = (j < lens[:, None]) & (j >= (lens[:, None] - window if window else 0))
+        p = s.masked_fill(~seen[:, None], float("-inf")).softmax(-1).nan_to_num(0.0)
+        out = paged_decode_weights(q, k, v, table, lens, w) if window is None else paged_decode_window(q, k, v, table, lens, 5)
+        check(out, torch.einsum("bhj,bjd->bhd", p, vv), rel * torch.einsum("bhj,bjd->bhd", p, vv.abs()))
+        if window is None:
+            check(w[:, 0], p.sum(1), rel * p.sum(1))
+    # every row its own block
+    own = torch.arange(rows, device="cuda", dtype=torch.int32)[:, None]
+    kk, vv = (torch.randn(rows, bs, 1, d, generator=gen, device="cuda").to(BF16) for _ in range(2))
+    sums = torch.rand(1, rows, 1, bs, generator=gen, device="cuda")
+    old = kk.clone()
+    left, kept = evict_tokens([kk], [vv], own, lens, sums, 6, recent=1, sinks=1)
+    assert torch.equal(left, lens.clamp(max=6))
+    cut = lens > 6
+    middle = sums[0, :, 0].masked_fill((j < 1) | (j >= lens[:, None] - 1), -1.0)
+    places = middle[cut].topk(4, -1).indices.sort(-1).values
+    places = torch.cat((torch.zeros_like(places[:, :1]), places, lens[cut, None].long() - 1), 1)
+    assert torch.equal(kept[0, cut, 0, :6], sums[0, cut, 0].gather(1, places))
+    assert torch.equal(kk[cut, :6, 0], old[cut, :, 0].gather(1, places[..., None].expand(-1, -1, d)))
+    assert torch.equal(kk[~cut], old[~cut]) and _native.device_error() == 0
 
 
 def test_weights_beside_others():
