@@ -449,7 +449,7 @@ size_t pd_evict_scratch_bytes(int32_t n_layer, int32_t batch, int32_t n_kv_head,
  * ones, zeros behind them (it may be weights), seqlen_out min(n, keep) (it may be seqlen). A block written for one
  * row is read or written for no other, and no pool is named twice. A block id outside the pool is skipped and
  * sets PD_DEVERR_COPY_RANGE.
- * Rows of 16-byte multiples; every layer's pools have one layout. */
+ * Rows of 16-byte multiples, at most 4096 bytes; every layer's pools have one layout. */
 int pd_evict(void* const* k_caches, void* const* v_caches, int32_t n_layer, int64_t n_blocks, int32_t block_size,
              int32_t n_kv_head, int32_t head_dim, int32_t dtype, const int64_t* k_strides, const int64_t* v_strides,
              const int32_t* block_table, int64_t bt_stride, int32_t max_blocks, const int32_t* new_table,

@@ -248,6 +248,7 @@ __global__ void __launch_bounds__(WARPS * 32) pd_evict_select_kernel(const __gri
 constexpr int MOVE_THREADS = 256;
 constexpr int AHEAD = 4;             // rows of a thread in a stretch
 constexpr int CHUNK = MOVE_THREADS;  // rows whose places are looked up at a time
+static_assert(EVICT_UNITS <= MOVE_THREADS, "every unit of a slice has a thread, so that a step is a row or more");
 
 // `parts` CTAs share the list of one (layer, row, kv head)'s K or V (new pages only: nothing that is written is
 // read), each of them in slices of 2^log2_slice 16-byte units, at least 4, so that a stretch is at most a chunk.
@@ -359,6 +360,7 @@ cudaError_t launch_select(const EvictParams& p, int64_t items, cudaStream_t stre
 cudaError_t launch_evict(const EvictParams& p, cudaStream_t stream) {
   const int64_t items = int64_t(p.layers) * p.batch * p.n_kv_head;
   if (items == 0) return cudaSuccess;
+  if (p.chunks > EVICT_UNITS) return cudaErrorInvalidValue;
   cudaError_t e = launch_select(p, items, stream);
   if (e != cudaSuccess) return e;
   // New pages' lists are shared by CTAs until there are four for every SM, down to a chunk each (9 prompts in 4 layers:

@@ -6,6 +6,7 @@
 namespace pd {
 
 constexpr int EVICT_LAYERS = 64;  // layers of one launch: their pool pointers travel in the parameters
+constexpr int EVICT_UNITS = 256;  // most 16-byte units of a row: the move gives each a thread of a CTA
 
 struct EvictParams {
   void* k[EVICT_LAYERS];

@@ -340,7 +340,7 @@ int pd_evict(void* const* k_caches, void* const* v_caches, int32_t n_layer, int6
   if (capacity > (int64_t(1) << 30) || int64_t(new_max_blocks) * block_size > (int64_t(1) << 30)) return PD_ERR_INVALID;
   if (w_len < capacity || bt_stride < max_blocks) return PD_ERR_INVALID;
   const int es = elem_size(dtype);
-  if (head_dim * es % 16 != 0) return PD_ERR_UNSUPPORTED;
+  if (head_dim > EVICT_UNITS * 16 / es || head_dim * es % 16 != 0) return PD_ERR_UNSUPPORTED;
   if (n_layer == 0 || batch == 0) return PD_OK;
   if (k_caches == nullptr || v_caches == nullptr || k_strides == nullptr || v_strides == nullptr ||
       w_strides == nullptr || wo_strides == nullptr || seqlen == nullptr || seqlen_out == nullptr ||
