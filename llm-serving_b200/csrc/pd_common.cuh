@@ -284,6 +284,17 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
+// ------------------------------------------------------------------ softmax
+// Where a running maximum starts: the lowest number, not -inf. A run of tokens whose scores are all -inf then has
+// weights exp2(-inf - start) = 0, where -inf - -inf would be a NaN, and one whose scores are all NaN (no NaN
+// raises a maximum) keeps a number, so that a merge does not take it for a piece without tokens: only that has m = -inf.
+constexpr float MAX_START = -3.402823466e38f;
+
+// What a row's accumulators are multiplied with at the end. The token at the maximum has weight 1, so l is 1 or more,
+// unless every score is -inf: then l is 0 and the result 0 / 0, as the softmax has it. A row without tokens has m = -inf
+// and zeros.
+__device__ __forceinline__ float normaliser(float m, float l) { return m == -INFINITY ? 0.f : 1.f / l; }
+
 // ------------------------------------------------------------------ element conversion
 // A "chunk" is 16 bytes of one row: 8 bf16/fp16 or 4 fp32 elements.
 

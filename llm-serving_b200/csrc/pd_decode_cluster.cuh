@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(W * 32, 8 / W)
         a.w = fmaf(f, x[r].w, a.w);
       }
     }
-    const float inv = 1.f / fmaxf(l, 1.f);
+    const float inv = normaliser(m, l);
     T* const out = reinterpret_cast<T*>(p.out) + int64_t(b) * p.o_sb + int64_t(hq0 + hd) * p.o_sh + i % GPH * 4;
     if constexpr (sizeof(T) == 4) {
       *reinterpret_cast<float4*>(out) = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);

@@ -35,7 +35,7 @@ struct FmaWorker {
   __device__ __forceinline__ void start(const float* qrow, int64_t q_sh, int hq0, int heads) {
 #pragma unroll
     for (int g = 0; g < GT; ++g) {
-      m_run[g] = -INFINITY;
+      m_run[g] = MAX_START;
       l_run[g] = 0.f;
 #pragma unroll
       for (int c = 0; c < CPL; ++c) {

@@ -1056,7 +1056,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
         }
 #pragma unroll
         for (int g = 0; g < GT; ++g) {
-          const float mn = fmaxf(m_run[g], tmax[g]);  // finite: the tile has a live row
+          const float mn = fmaxf(m_run[g], tmax[g]);  // (never -inf: MAX_START)
           const float alpha = exp2f(m_run[g] - mn);
           m_run[g] = mn;
           l_run[g] *= alpha;
@@ -1152,7 +1152,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
             raw = __ldg(reinterpret_cast<const uint4*>(qrow + int64_t(hq + g) * p.q_sh + (cc * C::LPR + pl) * C::EPC));
           E::unpack_pairs(raw, &qf[g][cc * (C::EPC / 2)]);
         }
-        m_run[g] = -INFINITY;
+        m_run[g] = MAX_START;
         l_run[g] = 0.f;
 #pragma unroll
         for (int e = 0; e < C::PPL; ++e) acc[g][e] = make_float2(0.f, 0.f);
@@ -1341,7 +1341,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
           float f[GT];
 #pragma unroll
           for (int g = 0; g < GT; ++g) {
-            f[g] = mj[j][g] == -INFINITY ? 0.f : exp2f(mj[j][g] - Mn[g]);
+            f[g] = exp2f(mj[j][g] - Mn[g]);  // (a piece has tokens: its m is MAX_START or more)
             L[g] = fmaf(f[g], lj[j][g], L[g]);
           }
 #pragma unroll
@@ -1371,7 +1371,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
         } else if (VAR && g >= mheads) {
           continue;
         } else if (p.mode == 0) {
-          const float inv = 1.f / fmaxf(pick(L, g), 1.f);
+          const float inv = normaliser(pick(M, g), pick(L, g));
           T* o = reinterpret_cast<T*>(p.out) + int64_t(mb) * p.o_sb + int64_t(mhq0 + g) * p.o_sh + col;
           o[0] = E::from_float(a[t].x * inv);
           o[1] = E::from_float(a[t].y * inv);
@@ -1570,7 +1570,7 @@ __device__ __forceinline__ uint32_t decode_body(const DecodeParams& p, const CUt
 #pragma unroll
               for (int g = 0; g < GT; ++g) {
                 if (VAR && g >= heads_of(cur.gc)) break;
-                const float inv = 1.f / fmaxf(l_tot[g], 1.f);
+                const float inv = normaliser(m_run[g], l_tot[g]);
 #pragma unroll
                 for (int c = 0; c < C::CPL; ++c) {
                   float o[C::EPC];

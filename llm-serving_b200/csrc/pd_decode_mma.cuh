@@ -109,7 +109,7 @@ struct MmaWorker {
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      m_run[e] = -INFINITY;
+      m_run[e] = MAX_START;
       l_run[e] = 0.f;
     }
 #pragma unroll
@@ -173,7 +173,7 @@ struct MmaWorker {
       float alpha[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float mn = fmaxf(m_run[e], t[e]);  // finite: the tile has a live row
+        const float mn = fmaxf(m_run[e], t[e]);  // (never -inf: MAX_START)
         alpha[e] = exp2f(m_run[e] - mn);
         m_run[e] = mn;
         l_run[e] *= alpha[e];
@@ -287,8 +287,7 @@ struct MmaWorker {
   // Each (d, head) pair is transposed to (head, d) pairs so that a lane stores 4 bytes of one
   // head row.
   __device__ __forceinline__ void store_out(T* out_h0, int64_t o_sh, const float (&l_tot)[2], int heads) const {
-    const float inv0 = 1.f / fmaxf(l_tot[0], 1.f);
-    const float inv1 = 1.f / fmaxf(l_tot[1], 1.f);
+    const float inv0 = normaliser(m_run[0], l_tot[0]), inv1 = normaliser(m_run[1], l_tot[1]);
     T* dst = out_h0 + int64_t(g < heads ? g : 0) * o_sh + 2 * c;
 #pragma unroll
     for (int dm = 0; dm < M::DM; ++dm) {

@@ -5,7 +5,7 @@
 // the part (-inf when the part saw no token), l = sum exp2(s - m), acc = sum exp2(s - m) v.
 // Output: out[b, h] = sum_p 2^(m_p - M) acc_p / max(sum_p 2^(m_p - M) l_p, 1), M = max_p m_p,
 // i.e. the reference's acc / max(l, 1) (model/triton_decode.py:639) over the union of the
-// parts; a row whose parts are all empty decodes to zeros. One warp per (row, head), lanes
+// parts; a row whose parts are all empty decodes to zeros, one whose scores are all -inf to NaN. One warp per (row, head), lanes
 // over head_dim in float4 steps; the partials are a few hundred KB, so this is launch-bound.
 #include "pd_internal.h"
 
@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(256) pd_merge_kernel(const MergeParams p) {
     L += p.l[i * p.ml_stride + pair] * exp2f(mi - M);
   }
   for (int o = 16; o >= 1; o >>= 1) L += __shfl_xor_sync(FULL_MASK, L, o);
-  const float inv = 1.f / fmaxf(L, 1.f);
+  const float inv = 1.f / (L == 0.f ? 0.f : fmaxf(L, 1.f));  // l = 0 with a maximum: every score is -inf, 0 / 0
   for (int d = lane * 4; d < p.head_dim; d += 128) {
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i = 0; i < p.n_parts; ++i) {
