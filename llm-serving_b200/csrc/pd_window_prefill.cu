@@ -124,7 +124,7 @@ __device__ __noinline__ void row_again(const WindowPrefillParams& p, int b, int 
   const T* q = reinterpret_cast<const T*>(p.q) + int64_t(token) * p.q_st + int64_t(head) * p.q_sh;
   const int32_t* trow = p.table + int64_t(b) * p.bt_stride;
   const int first = max(at - p.window + 1, 0), sinks = min(p.sinks, first), count = sinks + max(at + 1 - first, 0);
-  float m = -INFINITY, l = 0.f, acc[PER];
+  float m = MAX_START, l = 0.f, acc[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) acc[e] = 0.f;
   for (int i0 = 0; i0 < count; i0 += 32) {
@@ -150,7 +150,7 @@ __device__ __noinline__ void row_again(const WindowPrefillParams& p, int b, int 
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
     const float m_new = fmaxf(m, top), alpha = m == m_new ? 1.f : exp2f(m - m_new);
-    const float w = i < count ? exp2f(s - m_new) : 0.f;
+    const float w = i < count ? exp2f(s - m_new) : 0.f;  // (m_new is never -inf: scores of -inf have weight 0)
     m = m_new;
     l = fmaf(l, alpha, w);  // a lane's own sum
 #pragma unroll
