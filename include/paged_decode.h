@@ -444,7 +444,7 @@ size_t pd_evict_scratch_bytes(int32_t n_layer, int32_t batch, int32_t n_kv_head,
 /* Per (layer, row, kv head) of n = seqlen[b] > keep tokens: the first `sinks` and the last `recent` stay
  * (sinks + recent <= keep), and of the others those with the keep - sinks - recent largest weights (a tie keeps
  * the lower index; NaN is the smallest). The kept tokens' K and V take, in order, positions 0 .. keep - 1 of
- * new_table's pages, or of block_table's (new_table NULL: in place); shorter rows stay as they are (they are
+ * new_table's pages, or of block_table's (new_table NULL: in place; block_table itself is refused); shorter rows stay as they are (they are
  * copied to new_table's). weights (n_layer, B, H_kv, w_len) by strides of the first three; weights_out takes the kept
  * ones, zeros behind them (it may be weights), seqlen_out min(n, keep) (it may be seqlen). A block written for one
  * row is read or written for no other, and no pool is named twice. A block id outside the pool is skipped and

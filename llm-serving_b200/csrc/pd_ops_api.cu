@@ -350,6 +350,16 @@ int pd_evict(void* const* k_caches, void* const* v_caches, int32_t n_layer, int6
   if (new_table != nullptr &&
       (nbt_stride < new_max_blocks || int64_t(new_max_blocks) * block_size < (keep < capacity ? keep : capacity)))
     return PD_ERR_INVALID;
+  // A row's own pages as its new ones: rows moved to new pages are moved by several CTAs in any order, which would read
+  // what others have written. (Equal block ids elsewhere in the tables are on the device.)
+  if (new_table != nullptr) {
+    const int64_t apart = (reinterpret_cast<intptr_t>(new_table) - reinterpret_cast<intptr_t>(block_table)) / 4;
+    for (int64_t b = 0; b < (nbt_stride == bt_stride ? 1 : batch); ++b) {
+      const int64_t at = apart + b * (nbt_stride - bt_stride);
+      if (at < max_blocks && at > -int64_t(new_max_blocks))
+        return api_message(PD_ERR_INVALID, "new_table is a row's own block_table (NULL evicts in place)");
+    }
+  }
   for (int i = 0; i < 3; ++i)
     if (k_strides[i] * es % 16 != 0 || v_strides[i] * es % 16 != 0) return PD_ERR_INVALID;
   for (int i = 0; i < n_layer; ++i)

@@ -850,6 +850,8 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int keep = all_fit ? int(capacity) + 1 : int(keep0);
   Tensor fresh;
   if (const Tensor* t = optional(a[8], "new_table")) {
+    VALUE(t->numel() == 0 || t->const_data_ptr() != tensor(a[2], "block_table").const_data_ptr(),
+          "new_table is block_table itself (without it tokens move within their own pages)");
     fresh = table_of(*t, "new_table", rows, k0, "the pools");
     VALUE(fresh.size(1) * p.block_size >= std::min<int64_t>(keep, capacity), "new_table holds ", fresh.size(1) * p.block_size,
           " tokens, but rows may keep ", std::min<int64_t>(keep, capacity));

@@ -49,7 +49,7 @@ def evict_tokens(k_caches, v_caches, block_table, seqlen, weights, keep: int, *,
     to its pages instead, shorter rows are copied there whole, and the old pages keep what they hold: that is
     for rows whose pages others share. A block that is written for one row must be read or written
     for no other: without ``new_table`` rows share no blocks, and its blocks are distinct and in no old table
-    (nothing on the host can check that without waiting for the device).
+    (nothing on the host can check that without waiting for the device; ``block_table`` itself is refused).
 
     Returns ``(seqlen, weights)``: int32 ``min(n, keep)`` and the kept tokens' weights in their new places,
     zeros behind them; new tensors, or ``seqlen_out`` / ``weights_out``, which may be the inputs themselves.
