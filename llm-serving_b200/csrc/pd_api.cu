@@ -715,6 +715,20 @@ size_t workspace_bytes(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t
   if (current_device(&dev) != PD_OK) return 0;
   Launch L;
   if (launch_shape(dev, batch, g, &L) != PD_OK) return 0;
+  if (variant == PLAIN) return workspace_layout(batch, n_kv_head, g, head_dim, L).total;
+  // The variants' is for calls of fewer rows too, and a launch of many rows that is halved until its arrays fit takes
+  // fewer of them than a smaller batch that fits whole: as many rows as any call of up to `batch` gives one launch.
+  int lo = L.rows_per_launch, hi = std::min(std::max(batch, 1), 4096);
+  while (lo < hi) {
+    const int mid = lo + (hi - lo + 1) / 2;
+    Launch M;
+    if (launch_shape(dev, mid, g, &M) == PD_OK && M.rows_per_launch == mid) {
+      lo = mid;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  L.rows_per_launch = lo;
   return workspace_layout(batch, n_kv_head, g, head_dim, L).total;
 }
 
