@@ -117,8 +117,8 @@ int pd_decode(const void* q, int64_t q_sb, int64_t q_sh,
  * itself performs no allocation of any kind. Its first call on a device, with that device
  * current, looks the array's device address up (cudaGetSymbolAddress) and caches it; make
  * that first call before capturing a stream. Shapes whose scratch need exceeds the array
- * (pd_decode_workspace_bytes(...) > PD_NOALLOC_SCRATCH_BYTES, e.g. head_dim 256 with 8 q
- * heads per kv head) are rejected with PD_ERR_WORKSPACE and a message in
+ * (pd_decode_workspace_bytes(...) without a plan's step records, some 0.7 MB of it, above
+ * PD_NOALLOC_SCRATCH_BYTES, e.g. head_dim 256 with 8 q heads per kv head) are rejected with PD_ERR_WORKSPACE and a message in
  * pd_last_error_string(); use pd_decode with a workspace for those.
  *
  * The array keeps whatever the previous call left and starts out zero-filled; neither needs

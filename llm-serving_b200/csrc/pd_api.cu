@@ -382,7 +382,7 @@ int prepare(Prepared* P, int64_t n_blocks, int32_t block_size, const int32_t* bl
             int64_t bt_stride, int32_t max_blocks, const int32_t* seqlen, int32_t batch,
             int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype, float scale_log2,
             void* workspace, size_t workspace_bytes, Variant variant = PLAIN, int32_t window = 0,
-            int32_t sinks = 0, bool needs_workspace = true) {
+            int32_t sinks = 0, bool needs_workspace = true, bool records = true) {
   if (batch < 0 || max_blocks < 0 || n_blocks < 1) return PD_ERR_INVALID;
   if (variant == WINDOW && (window < 1 || sinks < 0)) return PD_ERR_INVALID;
   int st = geometry(n_head, n_kv_head, head_dim, block_size, dtype, variant, &P->g);
@@ -395,7 +395,8 @@ int prepare(Prepared* P, int64_t n_blocks, int32_t block_size, const int32_t* bl
   if (st != PD_OK) return st;
   P->ws = workspace_layout(batch, n_kv_head, P->g, head_dim, P->L);
   if (batch > 0) {
-    if (needs_workspace && (workspace == nullptr || workspace_bytes < P->ws.total)) {
+    // The step records, which come last, are a plan's: a call that has no room for them (`records` false) needs none.
+    if (needs_workspace && (workspace == nullptr || workspace_bytes < (records ? P->ws.total : P->ws.step_off))) {
       g_last_ws_need = P->ws.total;
       snprintf(g_last_error, sizeof(g_last_error),
                "workspace of %zu bytes is smaller than the %zu bytes this shape needs", workspace_bytes,
@@ -658,7 +659,8 @@ int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache
                   float* pm, float* pl, float* pacc, int mode, int32_t batch, int32_t n_head,
                   int32_t n_kv_head, int32_t head_dim, int32_t dtype, float scale_log2,
                   void* workspace, size_t workspace_bytes, void* stream, Variant variant = PLAIN, int32_t window = 0,
-                  int32_t sinks = 0, float* scores = nullptr, ClusterDecode* cluster = nullptr, bool* done = nullptr) {
+                  int32_t sinks = 0, float* scores = nullptr, ClusterDecode* cluster = nullptr, bool* done = nullptr,
+                  bool records = true) {
   if (k_strides == nullptr || v_strides == nullptr) return PD_ERR_INVALID;
   Prepared P;
   ClusterDecode c = cluster != nullptr ? *cluster : ClusterDecode{};
@@ -668,7 +670,7 @@ int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache
                                    &c, &stages))
     small = true;
   int st = prepare(&P, n_blocks, block_size, block_table, bt_stride, max_blocks, seqlen, batch, n_head, n_kv_head, head_dim,
-                   dtype, scale_log2, workspace, workspace_bytes, variant, window, sinks, !small);
+                   dtype, scale_log2, workspace, workspace_bytes, variant, window, sinks, !small, records);
   if (st != PD_OK) return st;
   if (batch == 0) return PD_OK;
   if (check_rows(q, q_sb, q_sh, dtype) != PD_OK) return PD_ERR_INVALID;
@@ -1476,12 +1478,13 @@ int pd_decode_noalloc(const void* q, int64_t q_sb, int64_t q_sh, const void* k_c
   void* scratch = nullptr;
   int st = noalloc_scratch(&scratch);
   if (st != PD_OK) return st;
-  // The size check is the one pd_decode makes against its workspace, done by the same prepare()
-  // that lays the scratch out, so the refusal always matches the layout actually used.
+  // The size check is the one pd_decode makes against its workspace, but for the step records that a plan keeps
+  // there, done by the same prepare() that lays the scratch out, so the refusal always matches the layout actually
+  // used. (The message names what pd_decode asks for.)
   st = decode_common(q, q_sb, q_sh, k_cache, v_cache, n_blocks, block_size, k_strides, v_strides,
                      block_table, bt_stride, max_blocks, seqlen, out, o_sb, o_sh, nullptr, nullptr,
                      nullptr, 0, batch, n_head, n_kv_head, head_dim, dtype, scale_log2, scratch,
-                     size_t(PD_NOALLOC_SCRATCH_BYTES), stream);
+                     size_t(PD_NOALLOC_SCRATCH_BYTES), stream, PLAIN, 0, 0, nullptr, nullptr, nullptr, false);
   if (st == PD_ERR_WORKSPACE)
     snprintf(g_last_error, sizeof(g_last_error),
              "pd_decode_noalloc: this shape needs %zu bytes of scratch but the built-in scratch array "
