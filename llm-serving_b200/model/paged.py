@@ -37,8 +37,6 @@ from __future__ import annotations
 import torch
 
 from model import _native
-from model.paged_evict import evict_tokens, paged_decode_weights
-from model.paged_window import decode_workspace
 from model.triton_decode import TRITON_AVAILABLE, _raise_first, window_rules
 
 __all__ = ["PagedPool", "PagedKV"]
@@ -377,6 +375,8 @@ class PagedKV:
         self.weights: torch.Tensor | None = None
         if track_weights:
             self.weights = torch.zeros(self.n_layer, n_rows, self.n_kv_head, width * pool.block_size, device=self.device)
+            from model.paged_window import decode_workspace
+
             self._weights_workspace = decode_workspace(n_rows, n_head, self.n_kv_head, self.head_dim, pool._keys[0])
 
     # ---------------------------------------------------------------- step hooks
@@ -531,6 +531,8 @@ class PagedKV:
         return plan.run(layer, q3, out=out3).unsqueeze(2)
 
     def _attend_weights(self, layer: int, q3: torch.Tensor, weights: torch.Tensor, out3=None) -> torch.Tensor:
+        from model.paged_evict import paged_decode_weights
+
         return paged_decode_weights(q3, self.pool._keys[layer], self.pool._values[layer], self._block_table_tensor,
                                     self._seqlen, weights, scale=1.0 / (self.head_dim ** 0.5), out=out3,
                                     workspace=self._weights_workspace)
@@ -553,6 +555,8 @@ class PagedKV:
         self.pool.flush()
         if max(self._host_pos) <= keep:
             return
+        from model.paged_evict import evict_tokens
+
         left, _ = evict_tokens(self.pool._keys, self.pool._values, self._block_table_tensor, self.pos, self.weights, keep,
                                recent=recent, sinks=sinks, weights_out=self.weights)
         self.evicted.add_(self.pos - left)
