@@ -540,14 +540,16 @@ class PagedKV:
     def evict(self, keep: int, *, recent: int = 0, sinks: int = 0) -> None:
         """Cut every row above ``keep`` cached tokens down to ``keep``, in every layer and in place, by the attention
         weights so far (``track_weights``): :func:`model.paged_evict.evict_tokens`. Between steps (after
-        :meth:`advance`). The rows' cache positions fall, their sequence positions (:attr:`position`) go on; captured
-        steps stay valid. Rows must not share blocks."""
+        :meth:`advance`), never inside a capture. The rows' cache positions fall, their sequence positions
+        (:attr:`position`) go on; captured steps stay valid. Rows must not share blocks."""
         if self.weights is None:
             raise RuntimeError("PagedKV.evict() needs a container that keeps attention weights (track_weights=True)")
         if not self._rows_disjoint:
             raise ValueError("PagedKV.evict() moves tokens in place, but rows of this container share blocks")
         if self._step_written or self._seqlen_ready:
             raise RuntimeError("PagedKV.evict() inside a step: call it after advance()")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("PagedKV.evict() inside a capture: a graph would move tokens that the container does not know of")
         if any(isinstance(x, bool) or not isinstance(x, int) for x in (keep, recent, sinks)):
             raise ValueError(f"keep, recent and sinks must be ints, got {keep!r}, {recent!r}, {sinks!r}")
         if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
