@@ -642,14 +642,14 @@ bool use_cluster(const Geometry& g, bool fp32, int64_t batch, int n_kv_head, int
   return true;
 }
 
+// `g`: the geometry that a call of few rows takes.
 bool is_small(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype, int32_t block_size,
-              int32_t max_blocks, Variant variant, int32_t window, int32_t sinks, ClusterDecode* c, int* stages) {
-  Geometry g;
+              int32_t max_blocks, Variant variant, int32_t window, int32_t sinks, Geometry* g, ClusterDecode* c, int* stages) {
   int dev = 0;
   if (batch < 1 || max_blocks < 1 || window < (variant == WINDOW ? 1 : 0) || sinks < 0) return false;
-  if (geometry(n_head, n_kv_head, head_dim, block_size, dtype, variant, &g) != PD_OK || current_device(&dev) != PD_OK)
+  if (geometry(n_head, n_kv_head, head_dim, block_size, dtype, variant, g) != PD_OK || current_device(&dev) != PD_OK)
     return false;
-  return use_cluster(g, dtype == PD_F32, batch, n_kv_head, int64_t(max_blocks) * block_size, window, sinks, dev, c, stages);
+  return use_cluster(*g, dtype == PD_F32, batch, n_kv_head, int64_t(max_blocks) * block_size, window, sinks, dev, c, stages);
 }
 
 int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache, const void* v_cache,
@@ -663,15 +663,18 @@ int decode_common(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache
                   bool records = true) {
   if (k_strides == nullptr || v_strides == nullptr) return PD_ERR_INVALID;
   Prepared P;
+  // Whether the rows are few is decided here, once: another thread may change the decode mode meanwhile.
   ClusterDecode c = cluster != nullptr ? *cluster : ClusterDecode{};
+  Geometry few;
   int stages = 0;
-  bool small = false;
-  if (variant != PLAIN && is_small(batch, n_head, n_kv_head, head_dim, dtype, block_size, max_blocks, variant, window, sinks,
-                                   &c, &stages))
-    small = true;
+  const bool small = variant != PLAIN && is_small(batch, n_head, n_kv_head, head_dim, dtype, block_size, max_blocks, variant,
+                                                  window, sinks, &few, &c, &stages);
+  if (variant == SCORES && !small && scores == nullptr && batch > 0 && max_blocks > 0)
+    return api_message(PD_ERR_WORKSPACE, "scratch is smaller than pd_decode_weights_scratch_bytes");
   int st = prepare(&P, n_blocks, block_size, block_table, bt_stride, max_blocks, seqlen, batch, n_head, n_kv_head, head_dim,
                    dtype, scale_log2, workspace, workspace_bytes, variant, window, sinks, !small, records);
   if (st != PD_OK) return st;
+  if (small) P.g = few;
   if (batch == 0) return PD_OK;
   if (check_rows(q, q_sb, q_sh, dtype) != PD_OK) return PD_ERR_INVALID;
   if (mode == 0 && check_rows(out, o_sb, o_sh, dtype) != PD_OK) return PD_ERR_INVALID;
@@ -869,10 +872,11 @@ size_t pd_decode_workspace_bytes(int32_t batch, int32_t n_head, int32_t n_kv_hea
 
 int32_t pd_decode_window_small(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim, int32_t dtype,
                                int32_t block_size, int32_t max_blocks, int32_t window, int32_t sinks) {
+  Geometry g;
   ClusterDecode c;
   int stages;
   return is_small(batch, n_head, n_kv_head, head_dim, dtype, block_size, max_blocks, window > 0 ? WINDOW : SCORES, window,
-                  sinks, &c, &stages);
+                  sinks, &g, &c, &stages);
 }
 
 size_t pd_decode_window_workspace_bytes(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim,
@@ -919,14 +923,11 @@ int pd_decode_weights(const void* q, int64_t q_sb, int64_t q_sh, const void* k_c
                       void* stream) {
   if (w_len < int64_t(max_blocks) * block_size) return PD_ERR_INVALID;
   if (n_kv_head > 65535) return PD_ERR_UNSUPPORTED;  // a grid's second dimension
-  if (batch > 0 && max_blocks > 0) {
-    if (weights == nullptr) return PD_ERR_INVALID;
-    if ((scratch == nullptr || !aligned16(scratch) ||
-         scratch_bytes < pd_decode_weights_scratch_bytes(batch, n_head, max_blocks, block_size)) &&
-        !pd_decode_window_small(batch, n_head, n_kv_head, head_dim, dtype, block_size, max_blocks, 0, 0))
-      return api_message(PD_ERR_WORKSPACE, "scratch is smaller than pd_decode_weights_scratch_bytes");
-  }
-  float* m = static_cast<float*>(scratch);
+  if (batch > 0 && max_blocks > 0 && weights == nullptr) return PD_ERR_INVALID;
+  // (too little of it is none: enough for few rows, and refused for more)
+  const bool enough = scratch != nullptr && aligned16(scratch) &&
+                      scratch_bytes >= pd_decode_weights_scratch_bytes(batch, n_head, max_blocks, block_size);
+  float* m = enough ? static_cast<float*>(scratch) : nullptr;
   float* l = m == nullptr ? nullptr : m + int64_t(batch) * n_head;
   float* scores =
       m == nullptr ? nullptr : reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + round_up(size_t(batch) * n_head * 8, 256));
