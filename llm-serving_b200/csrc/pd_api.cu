@@ -5,6 +5,7 @@
 // pd_append.cu and pd_merge.cu.
 #include <atomic>
 #include <cstdio>
+#include <exception>
 #include <mutex>
 #include <new>
 #include <vector>
@@ -808,10 +809,15 @@ static int plan_create(pd_plan** plan, int32_t n_layer, const void* const* k_cac
     h->k_strides[i] = k_strides[i];
     h->v_strides[i] = v_strides[i];
   }
-  h->kmaps.resize(n_layer);
-  h->vmaps.resize(n_layer);
-  h->k_pools.resize(n_layer);
-  h->v_pools.resize(n_layer);
+  try {
+    h->kmaps.resize(n_layer);
+    h->vmaps.resize(n_layer);
+    h->k_pools.resize(n_layer);
+    h->v_pools.resize(n_layer);
+  } catch (const std::exception&) {
+    delete h;
+    return api_message(PD_ERR_INVALID, "no host memory for that many layers");
+  }
   for (int layer = 0; layer < n_layer; ++layer) {
     h->k_pools[layer] = const_cast<void*>(k_caches[layer]);
     h->v_pools[layer] = const_cast<void*>(v_caches[layer]);

@@ -2,6 +2,7 @@
 // page copies and the eviction (declared in include/paged_decode.h): argument checks on the host, then the launch.
 #include <algorithm>
 #include <atomic>
+#include <exception>
 #include <vector>
 
 #include "paged_decode.h"
@@ -365,7 +366,13 @@ int pd_evict(void* const* k_caches, void* const* v_caches, int32_t n_layer, int6
   for (int i = 0; i < n_layer; ++i)
     if (k_caches[i] == nullptr || v_caches[i] == nullptr || !aligned(k_caches[i], 16) || !aligned(v_caches[i], 16))
       return PD_ERR_INVALID;
-  std::vector<const void*> pools(k_caches, k_caches + n_layer);
+  std::vector<const void*> pools;
+  try {
+    pools.reserve(2 * size_t(n_layer));
+  } catch (const std::exception&) {
+    return api_message(PD_ERR_INVALID, "no host memory for that many layers");
+  }
+  pools.insert(pools.end(), k_caches, k_caches + n_layer);
   pools.insert(pools.end(), v_caches, v_caches + n_layer);
   std::sort(pools.begin(), pools.end());
   if (std::adjacent_find(pools.begin(), pools.end()) != pools.end())
