@@ -88,7 +88,9 @@ int pd_device_error(unsigned int* bits, int clear);
  *     still usable as is.
  *
  * Row b, head h reads only the first ceil(seqlen[b] / block_size) table entries;
- * zero-length rows produce exact zeros (model/triton_decode.py:639).
+ * zero-length rows produce exact zeros (model/triton_decode.py:639). A NaN score makes its (row, head) NaN, one of -inf
+ * has weight 0, and a row of nothing but -inf gives NaN. A block of one head needs a multiple of 128 bytes
+ * (PD_ERR_UNSUPPORTED otherwise).
  */
 size_t pd_decode_workspace_bytes(int32_t batch, int32_t n_head, int32_t n_kv_head,
                                  int32_t head_dim, int32_t dtype);
@@ -389,7 +391,7 @@ int pd_fp4_prefill(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, c
  * sinks >= 0. What the table names for pages without a visible token does not matter. Any number of q heads per
  * kv head. `out` shares no memory with q. */
 
-/* Bytes of the workspace of pd_decode_window and pd_decode_weights, and of each half of
+/* Bytes of the workspace of pd_decode_window and pd_decode_weights for up to `batch` rows, and of each half of
  * pd_plan_create_window's; any contents, one workspace per stream, never shared with other entry points. */
 size_t pd_decode_window_workspace_bytes(int32_t batch, int32_t n_head, int32_t n_kv_head, int32_t head_dim,
                                         int32_t dtype);
@@ -408,8 +410,8 @@ int pd_decode_window(const void* q, int64_t q_sb, int64_t q_sh, const void* k_ca
                      void* workspace, size_t workspace_bytes, void* stream);
 
 /* pd_prefill where each query sees its window: token t of row b's S = cu[b + 1] - cu[b] packed ones sits at
- * position seqlen_k[b] - S + t. total_q bounds the packed tensor; a loose max_seqlen_q costs nothing. A block id
- * outside the pool reads zeros. fp16 / bf16, head_dim 64, 128 or 256, block_size >= 8. */
+ * position seqlen_k[b] - S + t. total_q bounds the packed tensor; max_seqlen_q is at least the longest chunk and sizes
+ * the launch (a loose one costs time, no more). A block id outside the pool reads zeros. fp16 / bf16, head_dim 64, 128 or 256, block_size >= 8. */
 int pd_prefill_window(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, const void* k_cache,
                       const void* v_cache, int64_t n_blocks, int32_t block_size, const int64_t* k_strides,
                       const int64_t* v_strides, const int32_t* block_table, int64_t bt_stride, int32_t max_blocks,

@@ -512,13 +512,13 @@ struct DecodeParams {
   int32_t wait_first;  // variants: wait for the preceding kernel before anything is read (programmatic launch)
 };
 
-// What the decode of few rows (pd_decode_cluster.cuh) takes beside DecodeParams.
 // Dynamic shared memory that a CTA of `warps` (8: one on an SM, 4: two) of the few rows' kernel may have, next to its
 // static arrays.
 constexpr int cluster_smem(int warps, int gt, int head_dim) {
   return 233472 * warps / 8 - 1024 - (gt * head_dim * 4 + 1024);
 }
 
+// What the decode of few rows (pd_decode_cluster.cuh) takes beside DecodeParams.
 struct ClusterDecode {
   int32_t warps;         // of a CTA
   int32_t log2_split;    // CTAs of an item's cluster

@@ -10,9 +10,10 @@
 // (one q-head chunk per kv head, so that a sum has one writer).
 //
 // Bound by latency: length, block ids, tiles, merge, each a round trip; every warp's first loads go out before it
-// waits for anything. One row, 8 kv heads of 128, a window of 1024: 6.2 us, of which 4 are its 4 MB's round trips and
-// 2 the merge (0.65 would move the bytes); with weights over 700 tokens 7.0. 61 rows of 2 kv heads of 256, windows of
-// 777: 23.3 us, 95 MB at 4.1 TB/s: the longest rows' runs of 13 tiles a warp.
+// waits for anything. One row, 8 kv heads of 128, a window of 1024: 6.2 us in a graph of such calls, of which 4 are its
+// 4 MB's round trips and 2 the merge (0.65 would move the bytes), 7.4 launched one by one; with weights over 700 tokens
+// 7.7 either way. 61 rows of 2 kv heads of 256, windows of 777: 23.4 and 24.4 us, 95 MB at 4.1 TB/s: the longest rows'
+// runs of 13 tiles a warp.
 #pragma once
 
 #include "pd_decode_fma.cuh"

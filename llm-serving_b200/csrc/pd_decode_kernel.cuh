@@ -43,7 +43,7 @@
 //    between them, so the split, its cache and the merge work on them as on a shorter row, and no
 //    hidden page is looked up or read but for the tokens that share a tile with a visible one; bit 1,
 //    every score and the rows' (m, l) are stored for the attention weights (pd_decode_weights). 32 rows of
-//    1500-8192 tokens, 16 heads on 8 of 128, bf16, window 2048 and 16 sinks: 49.6 us, 41.3 at the rate of a
+//    1500-8192 tokens, 16 heads on 8 of 128, bf16, window 2048 and 16 sinks: 49.7 us, 41.3 at the rate of a
 //    copy; 38 us of it stream at 7.0 TB/s.
 //  * Every mbarrier wait is bounded (1 s of %globaltimer). On expiry the warp records
 //    DEVERR_WAIT_TIMEOUT, drains its in-flight copies (bounded again) and returns.

@@ -1,4 +1,4 @@
-// pd_tile.cuh -- what the tcgen05 attention kernels with two alternating query blocks share: bounded waits,
+// pd_tile.cuh -- what the tcgen05 attention kernels of 4-bit pages and of windows share: bounded waits,
 // register splits, packed fp32 arithmetic, TMEM stores and shared-memory accesses.
 #pragma once
 

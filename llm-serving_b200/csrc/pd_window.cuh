@@ -22,7 +22,7 @@ struct WindowPrefillParams {
   uint32_t group_mul;  // division by group (set by the launch)
   int32_t group_shift;
   int32_t max_blocks, capacity;
-  int32_t log2_bs, log2_box;  // tokens of a block, and of a copy (window_box_tokens)
+  int32_t log2_bs, log2_box;  // tokens of a block, and of a copy: min(block, WINDOW_BOX)
   int32_t window, sinks;
   int32_t grouped;  // pool maps: a copy is 8-token groups of all pieces, or one piece
   int32_t sms;

@@ -26,10 +26,14 @@
 //    own rounding. The factor 2^7, which the sums carry too, keeps fp16 weights down to 2^-21 normal numbers.
 //  * With few blocks a cluster of `split` CTAs shares one block's steps. Each leaves its O, m and l in shared memory,
 //    and every one merges a share of the rows from all of them.
-//  * Measured (bf16, 16 heads on 8 of 128, window 1024): 4 prompts of 4096 tokens 180 us, 0.6 of the rate that its three
-//    products a step allow (P V twice); inside the steps the tensor pipe is busy 0.9 of the time, a CTA's start and end, which
-//    its neighbour on the SM covers in part, are a quarter of its clocks. With S of 128 keys at a time, which leaves one
-//    CTA an SM, 204 us. 16 chunks of 1-8 tokens 18.0 us, latency: 9.1 would move the bytes.
+//  * Measured (bf16, 16 heads on 8 of 128, window 1024): 4 prompts of 4096 tokens 175-180 us in a burst, 0.6 of the rate
+//    that its three products a step allow (P V twice), and 209 call after call, under the power cap; inside the steps the
+//    tensor pipe is busy 0.9 of the time, a CTA's start and end, which its neighbour on the SM covers in part, are a
+//    quarter of its clocks. With S of 128 keys at a time, which leaves one CTA an SM, 204 us in a burst. 16 chunks of 1-8
+//    tokens 17.9 us, latency: 9.1 would move the bytes.
+//  * The grid is the longest chunk's blocks times rows and kv heads: blocks past a shorter chunk start and leave, and what
+//    they take of the GPU is not left for clusters. One prompt of 4096 beside 60 rows of one token is 271 us, the
+//    prompt alone 49 and the others 54.
 //  * Every wait is bounded; a role whose wait runs out records DEVERR_WAIT_TIMEOUT and raises the CTA's abort
 //    flag, every role then leaves its loop, copies and MMAs in flight are waited for, and the CTA frees its TMEM. All
 //    threads reach the cluster's two barriers on every path.
