@@ -411,7 +411,8 @@ int pd_decode_window(const void* q, int64_t q_sb, int64_t q_sh, const void* k_ca
 
 /* pd_prefill where each query sees its window: token t of row b's S = cu[b + 1] - cu[b] packed ones sits at
  * position seqlen_k[b] - S + t. total_q bounds the packed tensor; max_seqlen_q is at least the longest chunk and sizes
- * the launch (a loose one costs time, no more). A block id outside the pool reads zeros. fp16 / bf16, head_dim 64, 128 or 256, block_size >= 8. */
+ * the launch (a loose one costs time; PD_ERR_UNSUPPORTED above 2^31 CTAs: ceil(max_seqlen_q * group / 128) a row and
+ * kv head). A block id outside the pool reads zeros. fp16 / bf16, head_dim 64, 128 or 256, block_size >= 8. */
 int pd_prefill_window(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh, const void* k_cache,
                       const void* v_cache, int64_t n_blocks, int32_t block_size, const int64_t* k_strides,
                       const int64_t* v_strides, const int32_t* block_table, int64_t bt_stride, int32_t max_blocks,
@@ -451,7 +452,7 @@ size_t pd_evict_scratch_bytes(int32_t n_layer, int32_t batch, int32_t n_kv_head,
  * ones, zeros behind them (it may be weights), seqlen_out min(n, keep) (it may be seqlen). A block written for one
  * row is read or written for no other, and no pool is named twice. A block id outside the pool is skipped and
  * sets PD_DEVERR_COPY_RANGE.
- * Rows of 16-byte multiples, at most 4096 bytes; every layer's pools have one layout. */
+ * batch * n_kv_head at most 131071. Rows of 16-byte multiples, at most 4096 bytes; every layer's pools have one layout. */
 int pd_evict(void* const* k_caches, void* const* v_caches, int32_t n_layer, int64_t n_blocks, int32_t block_size,
              int32_t n_kv_head, int32_t head_dim, int32_t dtype, const int64_t* k_strides, const int64_t* v_strides,
              const int32_t* block_table, int64_t bt_stride, int32_t max_blocks, const int32_t* new_table,

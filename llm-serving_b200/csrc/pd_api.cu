@@ -1064,6 +1064,10 @@ int pd_prefill_window(const void* q, int64_t total_q, int64_t q_st, int64_t q_sh
   if (cu_seqlens_q == nullptr || seqlen_k == nullptr || (block_table == nullptr && max_blocks > 0))
     return PD_ERR_INVALID;
   if (check_rows(q, q_st, q_sh, dtype) != PD_OK || check_rows(out, o_st, o_sh, dtype) != PD_OK) return PD_ERR_INVALID;
+  // a CTA for every block of the longest chunk's query rows, of every row and kv head
+  const int64_t blocks = (int64_t(max_seqlen_q) * (n_head / n_kv_head) + WINDOW_ROWS - 1) / WINDOW_ROWS;
+  if (blocks > 0x7fffffff / n_kv_head / batch)
+    return api_message(PD_ERR_UNSUPPORTED, "max_seqlen_q asks for more CTAs than a launch has: a tighter bound, or fewer rows");
   int dev = 0;
   if (current_device(&dev) != PD_OK) return PD_ERR_CUDA;
   WindowPrefillParams p{};

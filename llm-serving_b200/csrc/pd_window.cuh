@@ -31,7 +31,8 @@ struct WindowPrefillParams {
   unsigned long long wait_ns;
 };
 
-constexpr int WINDOW_BOX = 16;  // most tokens of a copy
+constexpr int WINDOW_BOX = 16;    // most tokens of a copy
+constexpr int WINDOW_ROWS = 128;  // query rows of a block (the MMA's M)
 
 cudaError_t launch_window_prefill(const WindowPrefillParams& p, const CUtensorMap& kmap, const CUtensorMap& vmap,
                                   int dtype, int head_dim, cudaStream_t stream);

@@ -50,7 +50,7 @@ namespace pd {
 
 namespace {
 
-constexpr int ROWS = 128;  // query rows of a block (the MMA's M)
+constexpr int ROWS = WINDOW_ROWS;
 constexpr int KEYS = 64;   // keys of a softmax step (the S MMA's N)
 constexpr float P_SHIFT = 7.f, HEADROOM = 8.f;
 

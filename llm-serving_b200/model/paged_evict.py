@@ -44,7 +44,7 @@ def evict_tokens(k_caches, v_caches, block_table, seqlen, weights, keep: int, *,
     keeps the lower ``j``, NaN counts as the smallest. The kept tokens' K and V move, in their order, to
     positions ``0 .. keep - 1`` of the row's pages, so heads of one row may hold different tokens there.
 
-    ``k_caches`` / ``v_caches``: one pool per layer, of one layout, each named once. ``weights`` float32
+    ``k_caches`` / ``v_caches``: one pool per layer, of one layout, each named once; up to 131,071 (row, kv head) pairs. ``weights`` float32
     ``(n_layer, B, H_kv, W)``, ``W`` at least the table's capacity. With ``new_table`` (int32 ``(B, max_blocks)``) the kept tokens go
     to its pages instead, shorter rows are copied there whole, and the old pages keep what they hold: that is
     for rows whose pages others share. A block that is written for one row must be read or written
