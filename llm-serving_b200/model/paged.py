@@ -295,7 +295,9 @@ class PagedKV:
     Two ways to bound a row, which the reference does not have: with ``window`` (and ``sinks``) every step sees the
     last ``window`` tokens and the first ``sinks`` only, :meth:`hidden_blocks` names the blocks that are out of
     sight for good; with ``track_weights`` the steps add up each cached token's attention weight in
-    :attr:`weights`, by which :meth:`evict` cuts rows down to a budget.
+    :attr:`weights`, by which :meth:`evict` cuts rows down to a budget. A container built anew for rows that go on
+    (others joined or left, a table grew) is told how many of their tokens were ``evicted``
+    (``old.evicted.tolist()``), so that :attr:`position` goes on, and its owner copies their rows of :attr:`weights`.
     """
 
     decode_container = True
@@ -304,10 +306,12 @@ class PagedKV:
     def __init__(self, pool: PagedPool, block_tables, lengths, *, rope_len: int, seats=None,
                  n_head: int | None = None, check_bounds: bool = True, fuse_append: bool = True,
                  overlap_layers: bool = True, window: int | None = None, sinks: int = 0,
-                 track_weights: bool = False) -> None:
+                 track_weights: bool = False, evicted=None) -> None:
         _raise_first(window_rules(window, sinks))
         if track_weights and window is not None:
             raise ValueError("a container keeps attention weights (track_weights) or a window, not both")
+        if evicted is not None and not track_weights:
+            raise ValueError("evicted tokens are those of a container that keeps attention weights (track_weights=True)")
         lengths = [int(n) for n in lengths]
         rope_len = int(rope_len)
         seats = list(range(len(block_tables))) if seats is None else list(seats)
@@ -315,6 +319,12 @@ class PagedKV:
             if violated:
                 raise error(message())
         n_head = pool.n_kv_head if n_head is None else int(n_head)
+        evicted = [0] * len(lengths) if evicted is None else [int(n) for n in evicted]
+        if len(evicted) != len(lengths) or any(n < 0 for n in evicted):
+            raise ValueError(f"evicted must be one count of at least 0 per row ({len(lengths)}), got {evicted}")
+        for row, (n, e) in enumerate(zip(lengths, evicted)):
+            if n + e > rope_len:
+                raise IndexError(f"row {row}: length {n} and {e} evicted tokens exceed the run's position bound {rope_len}")
 
         self.pool = pool
         self.n_layer = pool.n_layer
@@ -368,8 +378,8 @@ class PagedKV:
         self.window, self.sinks = window, int(sinks)
         # Tokens of each row that were evicted: its next token sits that much further on in its sequence than in
         # the cache.
-        self.evicted = torch.zeros(n_rows, dtype=torch.long, device=self.device)
-        self._host_evicted = [0] * n_rows
+        self.evicted = torch.tensor(evicted, dtype=torch.long, device=self.device)
+        self._host_evicted = evicted
         #: (n_layer, rows, n_kv_head, table capacity) float32 with ``track_weights``: every cached token's attention
         #: weights so far, summed over the steps and over the query heads of a kv head.
         self.weights: torch.Tensor | None = None
