@@ -8,8 +8,8 @@ reference has no windowed attention to mirror.
 * :func:`paged_decode_window` -- one query token per row (``paged_decode``'s contract);
 * :func:`paged_prefill_window` -- a chunk of query tokens per row (``paged_prefill``'s contract).
 
-Tensors on CUDA, the current stream, no host synchronisation: ``seqlen`` is never read on the host, lengths are
-clamped to the table's capacity on the device. Rows of length 0 give zeros; a block id outside the pool reads
+Tensors on CUDA, the current stream, no host synchronisation: ``seqlen`` is never read on the host, lengths (int32, or
+int64 that fit it) are clamped to the table's capacity on the device. Rows of length 0 give zeros; a block id outside the pool reads
 zeros. Pools need a unit head_dim stride and strides of 16-byte multiples (any contiguous pool has them). There
 is no CPU path and no fallback.
 """
