@@ -252,7 +252,8 @@ void pd_plan_destroy(pd_plan* plan);
  * start at m_parts + p * ml_part_stride (resp. l_parts), its acc at acc_parts +
  * p * acc_part_stride, each (B, H[, D]) contiguous -- into out = sum_p 2^(m_p-M) acc_p /
  * max(sum_p 2^(m_p-M) l_p, 1) with M = max_p m_p, which is the reference's normalisation
- * acc / max(l, 1) (model/triton_decode.py:639) applied to the union of the parts.
+ * acc / max(l, 1) (model/triton_decode.py:639) applied to the union of the parts. (l is 0 beside an m above -inf
+ * where every score of a part is -inf; a row of such parts alone merges to NaN.)
  */
 int pd_decode_partials(const void* q, int64_t q_sb, int64_t q_sh,
                        const void* k_cache, const void* v_cache, int64_t n_blocks,

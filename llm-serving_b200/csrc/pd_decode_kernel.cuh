@@ -4,7 +4,7 @@
 // query head h, out[b, h] = softmax(q[b, h] . K^T * scale) V over the first seqlen[b]
 // logical tokens of the row, token t living at pool block block_table[b, t / bs], slot
 // t % bs. Scores are formed in fp32 and scaled by scale * log2(e) so the online softmax
-// uses exp2; the result is acc / max(l, 1), which makes a zero-length row exactly zero.
+// uses exp2; the result is acc / l (normaliser), a zero-length row's exactly zero.
 //
 // How (B200 design, not the reference's):
 //  * Work unit = one KV tile of TILE tokens of one (row, kv head, q-head chunk) item;
